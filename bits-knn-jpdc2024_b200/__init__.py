@@ -24,6 +24,7 @@ ERR_UNSUPPORTED_MODE = 7
 ERR_COMM = 8
 SHARDED_ID_BYTES = 128
 
+F32, F16, BF16 = 0, 1, 2  # enum bitsknn_dtype
 L2_EXACT, L2_PARTIAL, L2_TF32, L2_BF16 = 0, 1, 2, 3
 STATIC_SCRATCH_BYTES = 8 << 20  # BITSKNN_STATIC_SCRATCH_BYTES
 
@@ -32,6 +33,22 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _ptr = ctypes.c_void_p
 _sz = ctypes.c_size_t
+
+
+class _CacheStruct(ctypes.Structure):
+    """bitsknn_cache_t"""
+    _fields_ = [("d_keys", _ptr), ("d_values", _ptr), ("d_key_scales", _ptr), ("d_value_scales", _ptr), ("pages", _i64),
+                ("page_stride", _i64), ("heads", ctypes.c_int32), ("page_rows", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class _BatchStruct(ctypes.Structure):
+    """bitsknn_cache_batch_t"""
+    _fields_ = [("d_table", _ptr), ("table_ld", _i64), ("table_pages", _i64), ("d_lengths", _ptr), ("d_starts", _ptr),
+                ("requests", _i64), ("tokens", _i64)]
+
+
+_cache_p = ctypes.POINTER(_CacheStruct)
+_batch_p = ctypes.POINTER(_BatchStruct)
 SIGNATURES = {
     "bitsknn_version": (_int, []),
     "bitsknn_last_error_string": (ctypes.c_char_p, []),
@@ -66,6 +83,15 @@ SIGNATURES = {
     "bitsknn_transpose": (_int, [_ptr, _i64, _i64, _ptr, _ptr]),
     "bitsknn_l2": (_int, [_ptr, _ptr, _i64, _i64, _int, _int, _ptr, _i64, _ptr, _sz, _ptr]),
     "bitsknn_fused_workspace_bytes": (_sz, [_i64, _i64, _int, _int, _int]),
+    "bitsknn_cache_plan": (_int, [_ptr, _ptr, _i64, _int, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _ptr,
+                                  _ptr]),
+    "bitsknn_cache_append": (_int, [_cache_p, _ptr, _ptr, _int, _i64, _i64, _ptr, _i64, _ptr]),
+    "bitsknn_cache_distance": (_int, [_cache_p, _batch_p, _ptr, _int, _i64, _int, _ptr, _i64, _i64, _ptr]),
+    "bitsknn_cache_attend_workspace_bytes": (_sz, [_cache_p, _int]),
+    "bitsknn_cache_attend": (_int, [_cache_p, _batch_p, _ptr, _int, _i64, _int, ctypes.c_float, _ptr, _i64, _ptr, _ptr,
+                                    _sz, _ptr]),
+    "bitsknn_cache_attend_selected": (_int, [_cache_p, _batch_p, _ptr, _int, _i64, _int, _ptr, _i64, _int,
+                                             ctypes.c_float, _ptr, _i64, _ptr, _ptr, _sz, _ptr]),
     "bitsknn_fused": (_int, [_ptr, _ptr, _i64, _i64, _int, _int, _int, ctypes.c_int32, _ptr, _ptr, _ptr, _sz, _ptr]),
 }
 
@@ -157,7 +183,7 @@ def _device_check(t, dtype, name):
         raise ValueError(f"{name} must be a CUDA tensor (the library has no CPU path)")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}")
-    if t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
 
 
@@ -333,6 +359,185 @@ def fused(points, queries, k, mode=L2_PARTIAL, index_base=0, out=None, workspace
     _check(lib().bitsknn_fused(_p(points), _p(queries), n, q, dim, k, mode, index_base, _p(out[0]), _p(out[1]),
                                _p(workspace), 0 if workspace is None else workspace.numel(), _stream()))
     return out
+
+
+# ---- search in a paged cache of keys and values held in 8 bits ---------------------------------
+class Cache:
+    """Keys and values as e4m3 codes in pages: uint8 (pages, heads, page_rows, dim) CUDA tensors and float32
+    (pages, heads) scales.  Holds the tensors; pages may lie apart (stride of the first dimension)."""
+
+    def __init__(self, keys, values, key_scales, value_scales):
+        import torch
+        for t, name in ((keys, "keys"), (values, "values")):
+            _device_check(t, torch.uint8, name)
+        for t, name in ((key_scales, "key_scales"), (value_scales, "value_scales")):
+            _device_check(t, torch.float32, name)
+        if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
+            raise ValueError("keys and values must be (pages, heads, page_rows, dim) tensors of the same strides")
+        pages, heads, rows, dim = keys.shape
+        if keys.stride()[1:] != (rows * dim, dim, 1):
+            raise ValueError("a page must be contiguous")
+        if any(tuple(s.shape) != (pages, heads) or not s.is_contiguous() for s in (key_scales, value_scales)):
+            raise ValueError("scales must be contiguous (pages, heads) tensors")
+        if any(t.device != keys.device for t in (values, key_scales, value_scales)):
+            raise ValueError("the cache's tensors must be on one device")
+        self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
+        self.pages, self.heads, self.page_rows, self.dim = pages, heads, rows, dim
+        self.device = keys.device
+        stride = keys.stride(0) if pages > 1 else heads * rows * dim
+        self.struct = _CacheStruct(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+                                   pages, stride, heads, rows, dim)
+
+    @classmethod
+    def empty(cls, pages, heads, page_rows, dim, device="cuda"):
+        """A cache without content; its pages are to be appended to from their first row."""
+        import torch
+        shape = (pages, heads, page_rows, dim)
+        return cls(torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device),
+                   torch.zeros(shape[:2], dtype=torch.float32, device=device),
+                   torch.zeros(shape[:2], dtype=torch.float32, device=device))
+
+
+def _on_device(device, *tensors):
+    import torch
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {device}, which is not the current device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+
+
+def _vectors(t, name, heads=None, dim=None):
+    """(dtype code, elements between tokens) of a (tokens, heads, dim) tensor of vectors."""
+    import torch
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    if not t.is_cuda or t.dim() != 3:
+        raise ValueError(f"{name} must be a (tokens, heads, dim) CUDA tensor (the library has no CPU path)")
+    if (heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, which does not fit the cache")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+        raise ValueError(f"{name} must be contiguous in its last two dimensions")
+    return code, t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
+
+
+def _cache_batch(table, lengths, starts, tokens):
+    import torch
+    _device_check(table, torch.int32, "table")
+    _device_check(lengths, torch.int32, "lengths")
+    _device_check(starts, torch.int32, "starts")
+    requests = lengths.shape[0]
+    if table.dim() != 2 or table.shape[0] != requests or (starts is not None and starts.shape[0] != requests + 1):
+        raise ValueError("table must be (requests, pages), lengths (requests,), starts (requests + 1,)")
+    ld = table.stride(0) if requests > 1 else table.shape[1]
+    return _BatchStruct(table.data_ptr(), ld, table.shape[1], lengths.data_ptr(),
+                        None if starts is None else starts.data_ptr(), requests, tokens)
+
+
+def cache_plan(lengths, new, free_pages, table, page_rows, max_tokens, out=None):
+    """Places for `new` tokens of every request: writes the new pages into `table` and returns
+    (starts, new_lengths, slots, counts); counts = (tokens, pages taken, tokens without a place)."""
+    import torch
+    for t, name in ((lengths, "lengths"), (new, "new"), (free_pages, "free_pages"), (table, "table")):
+        _device_check(t, torch.int32, name)
+    _on_device(lengths.device, new, free_pages, table)
+    requests = lengths.shape[0]
+    if new.shape[0] != requests or table.dim() != 2 or table.shape[0] != requests:
+        raise ValueError("lengths and new must be (requests,), table (requests, pages)")
+    if out is None:
+        i32 = dict(dtype=torch.int32, device=lengths.device)
+        out = (torch.empty(requests + 1, **i32), torch.empty(requests, **i32),
+               torch.empty(max_tokens, dtype=torch.int64, device=lengths.device), torch.empty(3, **i32))
+    ld = table.stride(0) if requests > 1 else table.shape[1]
+    _check(lib().bitsknn_cache_plan(_p(lengths), _p(new), requests, page_rows, _p(free_pages), free_pages.shape[0],
+                                    _p(table), ld, table.shape[1], _p(out[0]), _p(out[1]), _p(out[2]), max_tokens,
+                                    _p(out[3]), _stream()))
+    return out
+
+
+def cache_append(cache, keys, values, slots):
+    """Quantises (tokens, heads, dim) keys and values into the cache at `slots` (int64, from cache_plan)."""
+    import torch
+    code, key_stride = _vectors(keys, "keys", cache.heads, cache.dim)
+    value_code, value_stride = _vectors(values, "values", cache.heads, cache.dim)
+    _device_check(slots, torch.int64, "slots")
+    _on_device(cache.device, keys, values, slots)
+    tokens = keys.shape[0]
+    if value_code != code or values.shape[0] != tokens or slots.shape[0] < tokens:
+        raise ValueError("keys and values must agree in type and tokens, and every token needs a slot")
+    _check(lib().bitsknn_cache_append(cache.struct, _p(keys), _p(values), code, key_stride, value_stride, _p(slots),
+                                      tokens, _stream()))
+
+
+def cache_distance(cache, queries, lengths, table, n, starts=None, out=None):
+    """(tokens * heads, n) float32 distances for `select`: minus the largest inner product over a head's queries."""
+    import torch
+    code, stride = _vectors(queries, "queries", None, cache.dim)
+    _on_device(cache.device, queries, lengths, table, starts)
+    tokens, query_heads, _ = queries.shape
+    batch = _cache_batch(table, lengths, starts, tokens)
+    if out is None:
+        out = torch.empty((tokens * cache.heads, n), dtype=torch.float32, device=cache.device)
+    _device_check(out, torch.float32, "out")
+    if out.shape[0] < tokens * cache.heads or out.shape[1] < n:
+        raise ValueError("out must have tokens * heads rows of n distances")
+    ld = out.stride(0) if out.shape[0] > 1 else out.shape[1]
+    _check(lib().bitsknn_cache_distance(cache.struct, batch, _p(queries), code, stride, query_heads, _p(out), ld, n,
+                                        _stream()))
+    return out
+
+
+def cache_attend_workspace_bytes(cache, query_heads):
+    return int(lib().bitsknn_cache_attend_workspace_bytes(cache.struct, query_heads))
+
+
+def _attend_buffers(cache, queries, out, lse, workspace):
+    import torch
+    if out is None:
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=queries.device)
+    elif out.shape != queries.shape or out.dtype != queries.dtype:
+        raise ValueError("out must have the queries' shape and type")
+    if lse is None:
+        lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=queries.device)
+    elif lse.shape != queries.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous (tokens, query_heads) float32 tensor")
+    if workspace is None:
+        workspace = torch.empty(cache_attend_workspace_bytes(cache, queries.shape[1]), dtype=torch.uint8,
+                                device=queries.device)
+    _on_device(cache.device, queries, out, lse, workspace)
+    return out, lse, workspace
+
+
+def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
+    """Attention of (tokens, query_heads, dim) queries over everything cached: (out, lse)."""
+    code, stride = _vectors(queries, "queries", None, cache.dim)
+    out, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
+    _on_device(cache.device, lengths, table, starts)
+    batch = _cache_batch(table, lengths, starts, queries.shape[0])
+    _check(lib().bitsknn_cache_attend(cache.struct, batch, _p(queries), code, stride, queries.shape[1], scale, _p(out),
+                                      _vectors(out, "out", None, cache.dim)[1], _p(lse), _p(workspace), workspace.numel(),
+                                      _stream()))
+    return out, lse
+
+
+def cache_attend_selected(cache, queries, idx, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
+    """Attention over listed positions: idx (tokens * heads, k) int32, as `select` returns them.  (out, lse)."""
+    import torch
+    code, stride = _vectors(queries, "queries", None, cache.dim)
+    _device_check(idx, torch.int32, "idx")
+    tokens = queries.shape[0]
+    if idx.dim() != 2 or idx.shape[0] != tokens * cache.heads:
+        raise ValueError("idx must be (tokens * heads, k)")
+    out, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
+    _on_device(cache.device, idx, lengths, table, starts)
+    batch = _cache_batch(table, lengths, starts, tokens)
+    k = idx.shape[1]
+    _check(lib().bitsknn_cache_attend_selected(cache.struct, batch, _p(queries), code, stride, queries.shape[1], _p(idx),
+                                               idx.stride(0) if idx.shape[0] > 1 else k, k, scale, _p(out),
+                                               _vectors(out, "out", None, cache.dim)[1], _p(lse), _p(workspace),
+                                               workspace.numel(), _stream()))
+    return out, lse
 
 
 # ---- database-sharded search (one handle per GPU; NCCL inside the library) --------------------

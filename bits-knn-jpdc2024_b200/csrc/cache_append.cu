@@ -1,0 +1,357 @@
+// cache_append: new keys and values are quantised into the paged 8-bit cache.
+#include <algorithm>
+
+#include "cache.cuh"
+
+namespace bitsknn
+{
+
+namespace
+{
+
+constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_HELD = 8; // vectors of 8 numbers a thread keeps between the two passes
+
+struct append_args
+{
+    cache::view c;
+    const void* src[2]; // keys, values
+    int64_t stride[2];  // elements between tokens
+    const int64_t* slots;
+    int tokens;
+    int window;         // tokens per block
+    int dim;
+    int dtype;
+};
+
+struct vec8
+{
+    float v[8];
+};
+
+__device__ __forceinline__ vec8 load8(const void* src, int64_t at, int dtype)
+{
+    vec8 r;
+    if (dtype == BITSKNN_F32)
+    {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at);
+        const float4 x = __ldg(p);
+        const float4 y = __ldg(p + 1);
+        r.v[0] = x.x, r.v[1] = x.y, r.v[2] = x.z, r.v[3] = x.w;
+        r.v[4] = y.x, r.v[5] = y.y, r.v[6] = y.z, r.v[7] = y.w;
+        return r;
+    }
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at));
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        if (dtype == BITSKNN_BF16)
+        {
+            r.v[2 * i] = __uint_as_float(w[i] << 16);
+            r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000U);
+        }
+        else
+        {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            r.v[2 * i] = f.x;
+            r.v[2 * i + 1] = f.y;
+        }
+    }
+    return r;
+}
+
+// Smallest power of two s in [2^E_MIN, 2^E_MAX] with amax <= 448 s.  448 = 1.75 * 2^8, so the
+// exponent is that of amax less 8, and one more if its fraction is above 1.75.
+__device__ __forceinline__ float scale_of(float amax)
+{
+    const uint32_t bits = __float_as_uint(amax);
+    const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffU) > 0x600000U ? 1 : 0);
+    return cache::pow2_int(min(max(e, cache::E_MIN), cache::E_MAX)); // subnormal amax: far below the border
+}
+
+// One block = one window of tokens, one head, keys or values (gridDim = windows x heads x 2).  It
+// serves the pages whose first token lies in its window, run after run: a run is the longest
+// stretch of tokens of one page with ascending rows.  Two passes over a run: the largest finite
+// entry (block maximum), then rounding; what fits into APPEND_HELD vectors per thread stays in
+// registers between them (128 rows of 64 numbers, 64 rows of 128), the rest is read again from L2.
+// A page has one scale per head, which is why a run belongs to one block and why a later token
+// that needs a larger scale re-rounds the rows in front of it: with powers of two that only
+// costs bits at the subnormal end, code * 2^(old - new) is exact for every other code.
+template <int DTYPE>
+__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const append_args a)
+{
+    __shared__ float s_top[APPEND_THREADS / 32];
+    const int t = threadIdx.x;
+    const int lane = t & 31;
+    const int head = blockIdx.y;
+    const int which = blockIdx.z;
+    const void* src = a.src[which];
+    const int64_t stride = a.stride[which];
+    uint8_t* const codes = which == 0 ? a.c.keys : a.c.values;
+    float* const scales = which == 0 ? a.c.key_scales : a.c.value_scales;
+    const int vecs = a.dim >> 3; // vectors per row
+    // w / vecs == (w * vec_magic) >> 16 for w < 2^13, the most vectors a run can have (256 rows of 32)
+    const int vec_magic = (65536 + vecs - 1) / vecs;
+    const int rows_mask = (1 << a.c.page_shift) - 1;
+    const int first_token = blockIdx.x * a.window;
+    int end_token = min(first_token + a.window, a.tokens);
+    auto page_of = [&](int64_t slot) -> int64_t {
+        const int64_t p = slot < 0 ? -1 : slot >> a.c.page_shift;
+        return p < a.c.pages ? p : -1;
+    };
+    // first token in [from, limit) that has a place on a page other than `but`, else `limit`; every
+    // warp looks for itself, 128 slots at a time
+    auto find = [&](int from, int limit, int64_t but) {
+        for (; from < limit; from += 128)
+        {
+            int64_t s[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+            {
+                const int j = from + x * 32 + lane;
+                s[x] = j < limit ? a.slots[j] : -1;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+            {
+                const int64_t p = page_of(s[x]);
+                const unsigned hit = __ballot_sync(FULL_MASK, p >= 0 && p != but);
+                if (hit != 0)
+                {
+                    return from + x * 32 + __ffs(hit) - 1;
+                }
+            }
+        }
+        return limit;
+    };
+    int i = find(first_token, end_token, -1);
+    if (i < end_token && first_token > 0)
+    {
+        // a page whose tokens reach into the window from the left is served by an earlier block
+        int64_t before = -1;
+        for (int j = first_token - 1; j >= 0 && before < 0; j -= 32)
+        {
+            const int64_t p = j - lane >= 0 ? page_of(a.slots[j - lane]) : -1;
+            const unsigned hit = __ballot_sync(FULL_MASK, p >= 0);
+            before = hit != 0 ? __shfl_sync(FULL_MASK, p, __ffs(hit) - 1) : -1;
+        }
+        i = find(i, end_token, before);
+    }
+    while (i < end_token)
+    {
+        const int64_t slot0 = a.slots[i];
+        const int64_t page = page_of(slot0);
+        // length of the run: every warp finds it for itself
+        int64_t last = slot0;
+        int run = 1;
+        bool more = true;
+        while (more)
+        {
+            const int j = i + run + lane;
+            const int64_t s = j < a.tokens ? a.slots[j] : -1;
+            int64_t left = __shfl_up_sync(FULL_MASK, s, 1);
+            left = lane == 0 ? last : left;
+            const unsigned stop = __ballot_sync(FULL_MASK, page_of(s) != page || s <= left);
+            const int n = stop == 0 ? 32 : __ffs(stop) - 1;
+            last = __shfl_sync(FULL_MASK, s, 31);
+            run += n;
+            more = stop == 0;
+        }
+        const int offset0 = static_cast<int>(slot0) & rows_mask;
+        const int64_t base = page * a.c.page_stride + (static_cast<int64_t>(head) << a.c.page_shift) * a.dim;
+        const int work = run * vecs;
+        vec8 held[APPEND_HELD];
+        float top = 0.0F;
+        auto fetch = [&](int w) {
+            const int row = (w * vec_magic) >> 16;
+            const int part = w - row * vecs;
+            return load8(src, (i + row) * stride + static_cast<int64_t>(head) * a.dim + part * 8, DTYPE);
+        };
+        auto look = [&](const vec8& x) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                const float v = fabsf(x.v[e]);
+                top = v < INFINITY ? fmaxf(top, v) : top; // NaN and the infinities set no scale
+            }
+        };
+#pragma unroll
+        for (int h = 0; h < APPEND_HELD; ++h)
+        {
+            const int w = t + h * APPEND_THREADS;
+            if (w < work)
+            {
+                held[h] = fetch(w);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < APPEND_HELD; ++h)
+        {
+            if (t + h * APPEND_THREADS < work)
+            {
+                look(held[h]);
+            }
+        }
+        for (int w = t + APPEND_HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
+        {
+            look(fetch(w));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+        {
+            top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+        }
+        if (lane == 0)
+        {
+            s_top[t >> 5] = top;
+        }
+        float* const scale_at = scales + page * a.c.heads + head;
+        const float stored = offset0 == 0 ? 0.0F : *scale_at;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < APPEND_THREADS / 32; ++w)
+        {
+            top = fmaxf(top, s_top[w]);
+        }
+        // a page that is begun forgets the scale of its former owner; one that is continued keeps
+        // at least its own (anything but a positive number in range counts as the smallest)
+        const float old = stored > 0.0F && stored <= cache::pow2_int(cache::E_MAX) ? stored : cache::pow2_int(cache::E_MIN);
+        const float scale = fmaxf(scale_of(top), old);
+        const float inverse = 1.0F / scale;
+        auto store = [&](int w, const vec8& x) {
+            const int row = (w * vec_magic) >> 16;
+            const int part = w - row * vecs;
+            const int64_t at = base + static_cast<int64_t>(static_cast<int>(a.slots[i + row]) & rows_mask) * a.dim + part * 8;
+            uint2 out;
+            out.x = cache::codes_of_floats(x.v[0] * inverse, x.v[1] * inverse) |
+                    cache::codes_of_floats(x.v[2] * inverse, x.v[3] * inverse) << 16;
+            out.y = cache::codes_of_floats(x.v[4] * inverse, x.v[5] * inverse) |
+                    cache::codes_of_floats(x.v[6] * inverse, x.v[7] * inverse) << 16;
+            *reinterpret_cast<uint2*>(codes + at) = out;
+        };
+#pragma unroll
+        for (int h = 0; h < APPEND_HELD; ++h)
+        {
+            const int w = t + h * APPEND_THREADS;
+            if (w < work)
+            {
+                store(w, held[h]);
+            }
+        }
+        for (int w = t + APPEND_HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
+        {
+            store(w, fetch(w));
+        }
+        if (offset0 > 0 && scale > old)
+        {
+            const float shrink = old / scale;
+            const int words = offset0 * a.dim >> 2;
+            for (int w = t; w < words; w += APPEND_THREADS)
+            {
+                uint32_t* const p = reinterpret_cast<uint32_t*>(codes + base) + w;
+                const uint32_t c = *p;
+                const uint32_t lo = cache::half2_of_codes(c & 0xffffU);
+                const uint32_t hi = cache::half2_of_codes(c >> 16);
+                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                *p = cache::codes_of_floats(x.x * shrink, x.y * shrink) |
+                     cache::codes_of_floats(y.x * shrink, y.y * shrink) << 16;
+            }
+        }
+        __syncthreads(); // the next run may continue this page
+        if (t == 0)
+        {
+            *scale_at = scale;
+        }
+        __syncthreads();
+        i += run;
+        if (i < end_token)
+        {
+            i = find(i, end_token, -1);
+        }
+        if (i >= end_token)
+        {
+            // the page may go on behind the window, with rows that do not ascend
+            i = find(i, a.tokens, -1);
+            if (i == a.tokens || page_of(a.slots[i]) != page)
+            {
+                return;
+            }
+            end_token = i + 1;
+        }
+    }
+}
+
+} // namespace
+
+} // namespace bitsknn
+
+extern "C" int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_new_keys, const void* d_new_values,
+                                    int dtype, int64_t key_stride, int64_t value_stride, const int64_t* d_slots,
+                                    int64_t tokens, bitsknn_stream_t stream)
+{
+    using namespace bitsknn;
+    append_args a{};
+    const int rc = check_cache(cache, &a.c);
+    if (rc != BITSKNN_OK)
+    {
+        return rc;
+    }
+    if (dtype != BITSKNN_F32 && dtype != BITSKNN_F16 && dtype != BITSKNN_BF16)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED_MODE, "dtype %d: only F32, F16 and BF16", dtype);
+    }
+    if (tokens < 0 || tokens > 0x7ffffffe)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "invalid token count %lld", static_cast<long long>(tokens));
+    }
+    const int64_t dense = static_cast<int64_t>(cache->heads) * cache->dim;
+    key_stride = key_stride == 0 ? dense : key_stride;
+    value_stride = value_stride == 0 ? dense : value_stride;
+    const int64_t unit = dtype == BITSKNN_F32 ? 4 : 8; // elements in 16 bytes
+    if (key_stride < dense || value_stride < dense || key_stride % unit != 0 || value_stride % unit != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "strides %lld and %lld between tokens: at least %lld and a multiple of %lld",
+                    static_cast<long long>(key_stride), static_cast<long long>(value_stride),
+                    static_cast<long long>(dense), static_cast<long long>(unit));
+    }
+    if (tokens == 0)
+    {
+        return BITSKNN_OK;
+    }
+    if (d_new_keys == nullptr || d_new_values == nullptr || d_slots == nullptr)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "null pointer argument");
+    }
+    if (((reinterpret_cast<uintptr_t>(d_new_keys) | reinterpret_cast<uintptr_t>(d_new_values)) & 15) != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "misaligned vectors: 16-byte alignment needed");
+    }
+    a.src[0] = d_new_keys;
+    a.src[1] = d_new_values;
+    a.stride[0] = key_stride;
+    a.stride[1] = value_stride;
+    a.slots = d_slots;
+    a.tokens = static_cast<int>(tokens);
+    a.dim = cache->dim;
+    a.dtype = dtype;
+    // few tokens: one block for each, so that the runs of a decode step (one token long) run side by
+    // side; many: windows, so that the grid stays at some sixteen blocks per SM
+    const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(device_sm_count()) * 16 / (2 * cache->heads));
+    a.window = static_cast<int>((tokens + target - 1) / target);
+    const int64_t windows = (tokens + a.window - 1) / a.window;
+    const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(cache->heads), 2U);
+    auto s = static_cast<cudaStream_t>(stream);
+    {
+        kernel_scope scope("cache_append_kernel", s);
+        switch (dtype)
+        {
+        case BITSKNN_F32: cache_append_kernel<BITSKNN_F32><<<grid, APPEND_THREADS, 0, s>>>(a); break;
+        case BITSKNN_F16: cache_append_kernel<BITSKNN_F16><<<grid, APPEND_THREADS, 0, s>>>(a); break;
+        default: cache_append_kernel<BITSKNN_BF16><<<grid, APPEND_THREADS, 0, s>>>(a); break;
+        }
+    }
+    BITSKNN_CUDA_TRY(cudaGetLastError());
+    return BITSKNN_OK;
+}

@@ -1,0 +1,956 @@
+// cache_attend, cache_attend_selected: attention over a paged 8-bit cache, over all positions a token
+// sees or over a list of them.
+//
+// Mathematics.  For a query column with logits (base 2) t_j = scale * log2(e) * <q, code_j> * ks_j,
+// the weights are w_j = 2^(t_j + log2(vs_j) - m): the value scale rides on the logit, so that the
+// second product multiplies weights with bare codes, and m is the running maximum of t_j + log2(vs_j).
+// The denominator sums w_j / vs_j = 2^(t_j - m), in the same units, so out = sum w_j code_j / sum w_j / vs_j
+// needs no scale at all.  One pass: when m grows, what was summed is multiplied by 2^(m_old - m_new).
+// Logits, maxima and sums are FP32.  Weights are rounded to halves (11 bits, the codes are exact
+// halves): the reference point m is kept 7 binary orders below the half range's 2^7 ... 2^15, so a
+// weight of 2^-31 of the largest is still not lost, which 10^5 positions of little weight need.
+#include <algorithm>
+
+#include "cache.cuh"
+
+namespace bitsknn
+{
+
+namespace
+{
+
+using namespace cache;
+
+constexpr float WEIGHT_BIAS = 7.0F;  // the weight of the reference point is 2^7
+constexpr float WEIGHT_SLACK = 8.0F; // a logit may pass the reference point by 8 (weight 2^15) before it moves
+constexpr float LOG2_E = 1.4426950408889634F;
+constexpr float LN_2 = 0.6931471805599453F;
+
+struct attend_args
+{
+    view c;
+    batch b;
+    const void* queries;
+    int dtype;
+    int64_t query_stride;
+    int group;
+    float scale;      // times log2(e)
+    void* out;
+    int64_t out_stride;
+    float* lse;
+    const int32_t* idx; // selected: lists
+    int64_t ld_idx;
+    int k;
+    float* part_o;    // [2 * blocks][columns][DIM]
+    float2* part_ml;  // [2 * blocks][columns]
+    int4* joins;      // [blocks]
+    int* join_end;    // [blocks]
+};
+
+// What the stream of a block works on: one block of query columns of a request and head.
+struct item
+{
+    int request;
+    int first_token; // packed token of column 0 of the request (selected: the token)
+    int head;
+    int column0;
+    int columns;     // columns of the request (selected: of the token) in total
+    int64_t begin;   // first tile
+    int64_t end;
+};
+
+template <int DIM, int NB>
+struct attend_smem
+{
+    static constexpr int COLS = 8 * NB;
+    static constexpr int SCALES = 2 * SUB * PITCH<DIM>; // offset of the scales in a stage
+    static constexpr int STAGE = SCALES + 2 * SUB * 4;
+    static constexpr int FIT = 18432 / STAGE;
+    static constexpr int STAGES = FIT < 3 ? (NB > 3 ? NB : 3) : FIT > 8 ? 8 : (FIT < NB ? NB : FIT);
+    static constexpr int IMAGE = NB * 16 * DIM;
+    static constexpr int SMALL = COLS * (4 + 4 + WARPS * 8); // undo, visible, per-warp (m, l)
+    static constexpr int BYTES = IMAGE + SMALL + WARPS * STAGES * STAGE;
+    static constexpr int BY_SMEM = 227 * 1024 / (BYTES + 1024);
+    static constexpr int BY_REGS = NB * DIM <= 128 ? 4 : NB * DIM <= 256 ? 3 : 2;
+    static constexpr int BLOCKS = BY_SMEM < BY_REGS ? BY_SMEM : BY_REGS; // per SM
+    static_assert(BLOCKS >= 1, "shared memory");
+    static_assert(WARPS * STAGES * STAGE >= WARPS * COLS * DIM * 4, "the stages hold the warps' sums at the end");
+};
+
+__device__ __forceinline__ void store_out(void* out, int64_t at, float v, int dtype)
+{
+    if (dtype == BITSKNN_F16)
+    {
+        static_cast<__half*>(out)[at] = __float2half_rn(v);
+    }
+    else
+    {
+        static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+    }
+}
+
+// ---- tiles of the requests -------------------------------------------------------------------
+// All tiles of all items lie on one axis: requests in order, within a request heads, within a
+// head blocks of columns, within a block its tiles of 64 positions (at least one, which writes
+// the zeros of a row that sees nothing).  Block c of the grid takes the c-th equal share, so a
+// long request is spread over many blocks and short ones fill up the others.
+template <int COLS>
+__device__ __forceinline__ int tiles_of_block(const attend_args& a, const request& q, int column0)
+{
+    const int last = min(column0 + COLS, q.count * a.group) - 1;
+    return max((visible_of(a.b, q, last / a.group) + TILE - 1) / TILE, 1);
+}
+
+template <int COLS>
+__device__ __forceinline__ int64_t tiles_of_head(const attend_args& a, const request& q)
+{
+    int64_t sum = 0;
+    for (int col = 0; col < q.count * a.group; col += COLS)
+    {
+        sum += tiles_of_block<COLS>(a, q, col);
+    }
+    return sum;
+}
+
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* words)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        v += __shfl_xor_sync(FULL_MASK, v, o);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0)
+    {
+        words[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    int64_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+    {
+        sum += words[w];
+    }
+    return sum;
+}
+
+// The request that holds tile `at`, and the first tile of that request.
+template <int COLS>
+__device__ __forceinline__ int find_request(const attend_args& a, int64_t at, int64_t* first, int64_t* words, int* found)
+{
+    int64_t before = 0;
+    for (int base = 0; base < a.b.requests; base += THREADS)
+    {
+        const int r = base + threadIdx.x;
+        const int64_t mine = r < a.b.requests ? tiles_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads : 0;
+        int64_t upto = mine;
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const int64_t x = __shfl_up_sync(FULL_MASK, upto, o);
+            upto += lane >= o ? x : 0;
+        }
+        __syncthreads();
+        if (lane == 31)
+        {
+            words[threadIdx.x >> 5] = upto;
+        }
+        if (threadIdx.x == 0)
+        {
+            *found = -1;
+        }
+        __syncthreads();
+        int64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+        {
+            upto += w < static_cast<int>(threadIdx.x >> 5) ? words[w] : 0;
+            all += words[w];
+        }
+        const int64_t start = before + upto - mine;
+        __syncthreads();
+        if (at >= start && at < start + mine)
+        {
+            *found = r;
+            words[0] = start;
+        }
+        __syncthreads();
+        if (*found >= 0)
+        {
+            *first = words[0];
+            return *found;
+        }
+        before += all;
+    }
+    return -1; // not reached: `at` lies below the total
+}
+
+// ---- the kernel ------------------------------------------------------------------------------------
+// Four warps, each streaming its own 16-position subtiles (position tile * 64 + warp * 16)
+// through shared memory with asynchronous copies, without a block barrier in the loop: cached
+// rows are the 16 rows of the matrix step, query columns its 8 columns, so eight query heads cost
+// one conversion and one product, and scores come out with two positions of two columns per
+// thread, which the 8 x 8 transposition turns into the operand of the second product.
+//   scores  S^T = K Q^T   rows = positions  (operand: key codes as halves)
+//   output  O^T = V^T P^T rows = dims       (operand: value codes, read transposed as pairs of
+//                                            dims; the pairs are split when they become halves)
+// The four warps' sums are joined in shared memory when an item ends, those of several blocks by
+// cache_join_kernel.  Bound by the bytes of the cache (HBM) while the columns are few.
+template <int DIM, int NB, bool SELECTED>
+__global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_attend_kernel(const attend_args a)
+{
+    using smem = attend_smem<DIM, NB>;
+    constexpr int COLS = smem::COLS;
+    constexpr int STAGES = smem::STAGES;
+    extern __shared__ __align__(16) unsigned char shared[];
+    __shared__ int64_t s_words[WARPS];
+    __shared__ int s_found;
+    uint32_t* const image = reinterpret_cast<uint32_t*>(shared);
+    float* const undo = reinterpret_cast<float*>(shared + smem::IMAGE);
+    int* const visible = reinterpret_cast<int*>(undo + COLS);
+    float2* const warp_ml = reinterpret_cast<float2*>(visible + COLS);
+    unsigned char* const stages = shared + smem::IMAGE + smem::SMALL;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    unsigned char* const mine = stages + warp * STAGES * smem::STAGE;
+    const int rows_mask = (1 << a.c.page_shift) - 1;
+    const int c = (lane & 3) * 2;             // this thread's columns: c, c + 1 of every block of 8
+    const int row_lo = row_order(lane >> 2);  // its rows: row_lo, row_lo + 8
+
+    // this block's share of the tiles, and the item it begins in
+    const int list_tiles = SELECTED ? (a.k + TILE - 1) / TILE : 0;
+    const int list_blocks = SELECTED ? (a.group + COLS - 1) / COLS : 0;
+    int64_t total;
+    if constexpr (SELECTED)
+    {
+        total = static_cast<int64_t>(a.b.tokens) * a.c.heads * list_blocks * list_tiles;
+    }
+    else
+    {
+        int64_t sum = 0;
+        for (int r = threadIdx.x; r < a.b.requests; r += THREADS)
+        {
+            sum += tiles_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads;
+        }
+        total = block_sum(sum, s_words);
+    }
+    if (threadIdx.x == 0)
+    {
+        a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total); // those that get a tile at all
+    if (blockIdx.x >= blocks)
+    {
+        return;
+    }
+    int64_t at = blockIdx.x * total / blocks;
+    const int64_t share_end = (blockIdx.x + 1) * total / blocks;
+    item it{};
+    if constexpr (SELECTED)
+    {
+        const int64_t n = at / list_tiles;
+        it.begin = n * list_tiles;
+        it.end = it.begin + list_tiles;
+        it.column0 = static_cast<int>(n % list_blocks) * COLS;
+        it.head = static_cast<int>(n / list_blocks % a.c.heads);
+        it.first_token = static_cast<int>(n / list_blocks / a.c.heads);
+        it.columns = a.group;
+    }
+    else
+    {
+        int64_t first = 0;
+        it.request = find_request<COLS>(a, at, &first, s_words, &s_found);
+        const request q = request_of(a.b, it.request);
+        const int64_t per_head = tiles_of_head<COLS>(a, q);
+        it.head = static_cast<int>((at - first) / per_head);
+        it.begin = first + it.head * per_head;
+        it.first_token = q.first;
+        it.columns = q.count * a.group;
+        it.end = it.begin + tiles_of_block<COLS>(a, q, 0);
+        while (at >= it.end)
+        {
+            it.column0 += COLS;
+            it.begin = it.end;
+            it.end += tiles_of_block<COLS>(a, q, it.column0);
+        }
+    }
+
+    while (true)
+    {
+        const int64_t seg_end = min(it.end, share_end);
+        bool live = true;
+        request q;
+        if constexpr (SELECTED)
+        {
+            it.request = owner_of(a.b, it.first_token);
+            live = it.request >= 0; // tokens behind the last request are not touched
+        }
+        if (live)
+        {
+            q = request_of(a.b, it.request);
+            // ---- columns ----
+            __syncthreads();
+            for (int col = warp; col < COLS; col += WARPS)
+            {
+                const int g = it.column0 + col;
+                const bool real = g < it.columns;
+                const int i = g / a.group;
+                const int64_t from = static_cast<int64_t>(it.first_token + i) * a.query_stride +
+                                     static_cast<int64_t>(it.head * a.group + g % a.group) * DIM;
+                const float f = pack_column<DIM, NB>(image, col, real ? a.queries : nullptr, from, a.dtype);
+                if (lane == 0)
+                {
+                    undo[col] = f * a.scale;
+                    const int token = SELECTED ? it.first_token - q.first : i;
+                    visible[col] = real ? visible_of(a.b, q, token) : 0;
+                }
+            }
+            __syncthreads();
+            const int last = min(it.column0 + COLS, it.columns) - 1 - it.column0;
+            const int furthest = visible[last];
+            const int nearest = visible[0]; // columns of a block see ever more positions
+            const int32_t* const table = a.b.table + it.request * a.b.table_ld;
+            const int32_t* list = nullptr;
+            if constexpr (SELECTED)
+            {
+                list = a.idx + (static_cast<int64_t>(it.first_token) * a.c.heads + it.head) * a.ld_idx;
+            }
+            const int first_tile = static_cast<int>(at - it.begin);
+            const int count = static_cast<int>(seg_end - at);
+            const int row_end = SELECTED ? a.k : furthest; // rows behind it are zero
+            auto row_of = [&](int j) { return (first_tile + j) * TILE + warp * SUB; };
+
+            // ---- the stream ----
+            // page of subtile j (dense), or position and page of this lane's list entry (selected),
+            // fetched one subtile (entries: two) ahead of the copies that need it
+            int next_page = -1;
+            int next_pos = -1;
+            int later_pos = -1;
+            auto entry = [&](int j) {
+                const int e = row_of(j) + lane;
+                int p = lane < SUB && j < count && e < a.k ? list[e] : -1;
+                return p < furthest ? p : -1;
+            };
+            auto page_at = [&](int pos) {
+                const int p = pos >= 0 ? table[pos >> a.c.page_shift] : -1;
+                return p < a.c.pages ? p : -1;
+            };
+            if constexpr (SELECTED)
+            {
+                next_pos = entry(0);
+                next_page = page_at(next_pos);
+                later_pos = entry(1);
+            }
+            else
+            {
+                next_page = page_at(row_of(0) < furthest ? row_of(0) : -1);
+            }
+            auto issue = [&](int j) {
+                if (j < count)
+                {
+                    const uint32_t dst = ptx::smem_addr(mine + (j % STAGES) * smem::STAGE);
+                    constexpr int PARTS = DIM / 16;
+                    const int page = next_page;
+                    const int safe = max(page, 0);
+                    if constexpr (SELECTED)
+                    {
+                        int64_t from = -1;
+                        if (page >= 0)
+                        {
+                            from = page * a.c.page_stride +
+                                   ((static_cast<int64_t>(it.head) << a.c.page_shift) + (next_pos & rows_mask)) * DIM;
+                        }
+                        const uint32_t there = page >= 0 ? 4U : 0U;
+                        next_pos = later_pos;
+                        next_page = page_at(next_pos);
+                        later_pos = entry(j + 2);
+#pragma unroll
+                        for (int x = 0; x < DIM / 32; ++x)
+                        {
+                            const int e = lane + x * 32;
+                            const int row = e / PARTS;
+                            const int64_t f = __shfl_sync(FULL_MASK, from, row);
+                            const int64_t g = max(f, static_cast<int64_t>(0)) + (e % PARTS) * 16;
+                            const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
+                            copy16(to, a.c.keys + g, f >= 0 ? 16U : 0U);
+                            copy16(to + SUB * PITCH<DIM>, a.c.values + g, f >= 0 ? 16U : 0U);
+                        }
+                        if (lane < SUB)
+                        {
+                            const int64_t s = static_cast<int64_t>(safe) * a.c.heads + it.head;
+                            copy4(dst + smem::SCALES + lane * 4, a.c.key_scales + s, there);
+                            copy4(dst + smem::SCALES + SUB * 4 + lane * 4, a.c.value_scales + s, there);
+                        }
+                    }
+                    else
+                    {
+                        const int pos = row_of(j);
+                        const int there = page < 0 ? 0 : min(SUB, furthest - pos);
+                        next_page = page_at(j + 1 < count && row_of(j + 1) < furthest ? row_of(j + 1) : -1);
+                        const int64_t from = safe * a.c.page_stride +
+                                             ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
+#pragma unroll
+                        for (int x = 0; x < DIM / 32; ++x)
+                        {
+                            const int e = lane + x * 32;
+                            const int row = e / PARTS;
+                            const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
+                            copy16(to, a.c.keys + from + e * 16, row < there ? 16U : 0U);
+                            copy16(to + SUB * PITCH<DIM>, a.c.values + from + e * 16, row < there ? 16U : 0U);
+                        }
+                        const float* scales = lane < SUB ? a.c.key_scales : a.c.value_scales;
+                        copy4(dst + smem::SCALES + lane * 4, scales + static_cast<int64_t>(safe) * a.c.heads + it.head,
+                              (lane & (SUB - 1)) < there ? 4U : 0U);
+                    }
+                }
+                copy_commit();
+            };
+
+            float o[DIM / 16][NB][4];
+            float m[NB][2];
+            float l[NB][2];
+            float f[NB][2];
+            int see[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+            {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                {
+                    m[nb][x] = -INFINITY;
+                    l[nb][x] = 0.0F;
+                    f[nb][x] = undo[nb * 8 + c + x];
+                    see[nb][x] = SELECTED ? 0x7fffffff : visible[nb * 8 + c + x];
+                }
+#pragma unroll
+                for (int g = 0; g < DIM / 16; ++g)
+                {
+                    o[g][nb][0] = o[g][nb][1] = o[g][nb][2] = o[g][nb][3] = 0.0F;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < STAGES - 1; ++j)
+            {
+                issue(j);
+            }
+            for (int j = 0; j < count; ++j)
+            {
+                copy_wait<STAGES - 2>();
+                __syncwarp();
+                const int pos = row_of(j);
+                if (pos < row_end)
+                {
+                    const unsigned char* const stage = mine + (j % STAGES) * smem::STAGE;
+                    const float* const scales = reinterpret_cast<const float*>(stage + smem::SCALES);
+                    float s[NB][4];
+                    score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
+                    const float ks_lo = scales[row_lo];
+                    const float ks_hi = scales[row_lo + 8];
+                    // value scales at the border of their range and beyond would leave that of the sums
+                    const float vs_lo = fminf(fmaxf(scales[SUB + row_lo], pow2_int(E_MIN)), pow2_int(E_MAX));
+                    const float vs_hi = fminf(fmaxf(scales[SUB + row_lo + 8], pow2_int(E_MIN)), pow2_int(E_MAX));
+                    const float lv_lo = log2_fast(vs_lo);
+                    const float lv_hi = log2_fast(vs_hi);
+                    // absent rows were copied as zeros, scale included; others are seen below `see`
+                    const int at_lo = ks_lo != 0.0F ? pos + row_lo : 0x7fffffff;
+                    const int at_hi = ks_hi != 0.0F ? pos + row_lo + 8 : 0x7fffffff;
+                    bool raise = false;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                    {
+                        s[nb][0] = at_lo < see[nb][0] ? fmaf(s[nb][0], f[nb][0] * ks_lo, lv_lo) : -INFINITY;
+                        s[nb][1] = at_lo < see[nb][1] ? fmaf(s[nb][1], f[nb][1] * ks_lo, lv_lo) : -INFINITY;
+                        s[nb][2] = at_hi < see[nb][0] ? fmaf(s[nb][2], f[nb][0] * ks_hi, lv_hi) : -INFINITY;
+                        s[nb][3] = at_hi < see[nb][1] ? fmaf(s[nb][3], f[nb][1] * ks_hi, lv_hi) : -INFINITY;
+                        raise |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + WEIGHT_SLACK;
+                        raise |= fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + WEIGHT_SLACK;
+                    }
+                    if (__any_sync(FULL_MASK, raise))
+                    {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                        {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                            {
+                                float top = fmaxf(s[nb][x], s[nb][2 + x]);
+#pragma unroll
+                                for (int w = 4; w < 32; w <<= 1)
+                                {
+                                    top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, w));
+                                }
+                                top = fmaxf(top, m[nb][x]);
+                                const float keep = m[nb][x] == -INFINITY ? 0.0F : exp2_fast(m[nb][x] - top);
+                                m[nb][x] = top;
+                                l[nb][x] *= keep;
+#pragma unroll
+                                for (int g = 0; g < DIM / 16; ++g)
+                                {
+                                    o[g][nb][x] *= keep;
+                                    o[g][nb][2 + x] *= keep;
+                                }
+                            }
+                        }
+                    }
+                    uint32_t w_lo[NB];
+                    uint32_t w_hi[NB];
+                    const float iv_lo = __fdividef(1.0F, vs_lo);
+                    const float iv_hi = __fdividef(1.0F, vs_hi);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                    {
+                        const float b0 = WEIGHT_BIAS - (m[nb][0] == -INFINITY ? 0.0F : m[nb][0]);
+                        const float b1 = WEIGHT_BIAS - (m[nb][1] == -INFINITY ? 0.0F : m[nb][1]);
+                        const float p0 = exp2_fast(s[nb][0] + b0);
+                        const float p1 = exp2_fast(s[nb][1] + b1);
+                        const float p2 = exp2_fast(s[nb][2] + b0);
+                        const float p3 = exp2_fast(s[nb][3] + b1);
+                        l[nb][0] = fmaf(p0, iv_lo, fmaf(p2, iv_hi, l[nb][0]));
+                        l[nb][1] = fmaf(p1, iv_lo, fmaf(p3, iv_hi, l[nb][1]));
+                        w_lo[nb] = transpose_8x8(pack_half2(p0, p1));
+                        w_hi[nb] = transpose_8x8(pack_half2(p2, p3));
+                    }
+                    // A NaN code times a weight of zero would spoil the columns that do not see its row.
+                    // Only rows that some columns see and others do not can do that (rows nobody sees
+                    // were copied as zeros); if such a subtile holds one, the codes are cleaned, and a
+                    // second product of indicators finds the outputs that the NaN belongs to.
+                    const unsigned char* const vrows = stage + SUB * PITCH<DIM>;
+                    bool nan_here = false;
+                    if (!SELECTED && nearest < furthest && pos + SUB > nearest)
+                    {
+                        for (int e = lane; e < SUB * DIM / 4; e += 32)
+                        {
+                            const uint32_t w =
+                                *reinterpret_cast<const uint32_t*>(vrows + (e * 4 / DIM) * PITCH<DIM> + e * 4 % DIM);
+                            nan_here |= (((w & 0x7f7f7f7fU) + 0x01010101U) & 0x80808080U) != 0;
+                        }
+                        nan_here = __any_sync(FULL_MASK, nan_here);
+                    }
+                    const uint32_t vaddr = ptx::smem_addr(vrows) +
+                                           (((lane >> 3) & 1) * 8 + row_order(lane & 7)) * PITCH<DIM> + (lane >> 4) * 16;
+                    if (!nan_here)
+                    {
+#pragma unroll
+                        for (int g = 0; g < DIM / 16; g += 2)
+                        {
+                            uint32_t r[4];
+                            ldmatrix_x4_trans(r, vaddr + g * 16);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                            {
+                                const uint32_t u = __byte_perm(r[2 * x], 0, 0x3120);
+                                const uint32_t v = __byte_perm(r[2 * x + 1], 0, 0x3120);
+                                const uint32_t a0 = half2_of_codes(u & 0xffffU);
+                                const uint32_t a1 = half2_of_codes(u >> 16);
+                                const uint32_t a2 = half2_of_codes(v & 0xffffU);
+                                const uint32_t a3 = half2_of_codes(v >> 16);
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+                                {
+                                    mma_16816(o[g + x][nb], a0, a1, a2, a3, w_lo[nb], w_hi[nb]);
+                                }
+                            }
+                        }
+                    }
+                    else
+                    {
+                        uint32_t one_lo[NB];
+                        uint32_t one_hi[NB];
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                        {
+                            one_lo[nb] = transpose_8x8(pack_half2(at_lo < see[nb][0] ? 1.0F : 0.0F, at_lo < see[nb][1] ? 1.0F : 0.0F));
+                            one_hi[nb] = transpose_8x8(pack_half2(at_hi < see[nb][0] ? 1.0F : 0.0F, at_hi < see[nb][1] ? 1.0F : 0.0F));
+                        }
+#pragma unroll
+                        for (int g = 0; g < DIM / 16; g += 2)
+                        {
+                            uint32_t r[4];
+                            ldmatrix_x4_trans(r, vaddr + g * 16);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                            {
+                                const uint32_t u = __byte_perm(r[2 * x], 0, 0x3120);
+                                const uint32_t v = __byte_perm(r[2 * x + 1], 0, 0x3120);
+                                uint32_t h[4] = {half2_of_codes(u & 0xffffU), half2_of_codes(u >> 16),
+                                                 half2_of_codes(v & 0xffffU), half2_of_codes(v >> 16)};
+                                uint32_t is[4];
+#pragma unroll
+                                for (int y = 0; y < 4; ++y)
+                                {
+                                    // a half is NaN above 0x7c00 (codes give no infinities)
+                                    const uint32_t low = (h[y] & 0x7fffU) > 0x7c00U ? 0xffffU : 0U;
+                                    const uint32_t high = (h[y] & 0x7fff0000U) > 0x7c000000U ? 0xffff0000U : 0U;
+                                    is[y] = (low | high) & 0x3c003c00U; // ones
+                                    h[y] &= ~(low | high);
+                                }
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+                                {
+                                    float hits[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+                                    mma_16816(hits, is[0], is[1], is[2], is[3], one_lo[nb], one_hi[nb]);
+                                    mma_16816(o[g + x][nb], h[0], h[1], h[2], h[3], w_lo[nb], w_hi[nb]);
+#pragma unroll
+                                    for (int y = 0; y < 4; ++y)
+                                    {
+                                        o[g + x][nb][y] = hits[y] > 0.0F ? NAN : o[g + x][nb][y];
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                issue(j + STAGES - 1);
+            }
+            copy_wait<0>();
+
+            // ---- the four warps' sums ----
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+            {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                {
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1)
+                    {
+                        l[nb][x] += __shfl_xor_sync(FULL_MASK, l[nb][x], w);
+                    }
+                    if (lane < 4)
+                    {
+                        warp_ml[warp * COLS + nb * 8 + c + x] = make_float2(m[nb][x], l[nb][x]);
+                    }
+                }
+            }
+            __syncthreads(); // every warp's stream has ended: the stages are free
+            float* const sums = reinterpret_cast<float*>(stages);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+            {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                {
+                    const int col = nb * 8 + c + x;
+                    float top = warp_ml[col].x;
+#pragma unroll
+                    for (int w = 1; w < WARPS; ++w)
+                    {
+                        top = fmaxf(top, warp_ml[w * COLS + col].x);
+                    }
+                    const float keep = m[nb][x] == -INFINITY ? (l[nb][x] == 0.0F ? 0.0F : 1.0F) : exp2_fast(m[nb][x] - top);
+                    float* const to = sums + (warp * COLS + col) * DIM + (lane >> 2) * 2;
+#pragma unroll
+                    for (int g = 0; g < DIM / 16; ++g)
+                    {
+                        *reinterpret_cast<float2*>(to + g * 16) = make_float2(o[g][nb][x] * keep, o[g][nb][2 + x] * keep);
+                    }
+                }
+            }
+            __syncthreads();
+            const bool whole = at == it.begin && seg_end == it.end;
+            // part 1 of a block: an item that begins in it and ends in another one; part 0: one that began before
+            const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at == it.begin ? 1 : 0);
+            for (int e = threadIdx.x; e < COLS * DIM; e += THREADS)
+            {
+                const int col = e / DIM;
+                const int d = e % DIM;
+                const int g = it.column0 + col;
+                if (g >= it.columns)
+                {
+                    break;
+                }
+                float top = warp_ml[col].x;
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w)
+                {
+                    top = fmaxf(top, warp_ml[w * COLS + col].x);
+                }
+                float sum = 0.0F;
+                float den = 0.0F;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w)
+                {
+                    const float2 ml = warp_ml[w * COLS + col];
+                    sum += sums[(w * COLS + col) * DIM + d];
+                    den += ml.x == -INFINITY ? ml.y : ml.y * exp2_fast(ml.x - top);
+                }
+                if (whole)
+                {
+                    const int64_t token = it.first_token + g / a.group;
+                    const int qhead = it.head * a.group + g % a.group;
+                    store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + d,
+                              den == 0.0F ? 0.0F : sum / den, a.dtype);
+                    if (d == 0 && a.lse != nullptr)
+                    {
+                        a.lse[token * a.group * a.c.heads + qhead] =
+                            den == 0.0F ? -INFINITY : (top - WEIGHT_BIAS + log2f(den)) * LN_2;
+                    }
+                }
+                else
+                {
+                    a.part_o[(part * COLS + col) * DIM + d] = sum;
+                    if (d == 0)
+                    {
+                        a.part_ml[part * COLS + col] = make_float2(top, den);
+                    }
+                }
+            }
+            if (at == it.begin && !whole && threadIdx.x == 0)
+            {
+                // the block of the item's last tile: blocks begin at floor(c * total / blocks)
+                a.joins[blockIdx.x] = make_int4(it.first_token, it.head, it.column0, it.columns);
+                a.join_end[blockIdx.x] = static_cast<int>(((it.end * blocks) - 1) / total);
+            }
+        }
+        // ---- the next item ----
+        at = seg_end;
+        if (at >= share_end)
+        {
+            return;
+        }
+        it.begin = it.end;
+        it.column0 += COLS;
+        if constexpr (SELECTED)
+        {
+            it.end += list_tiles;
+            if (it.column0 >= it.columns)
+            {
+                it.column0 = 0;
+                if (++it.head == a.c.heads)
+                {
+                    it.head = 0;
+                    ++it.first_token;
+                }
+            }
+        }
+        else
+        {
+            if (it.column0 >= it.columns)
+            {
+                it.column0 = 0;
+                if (++it.head == a.c.heads)
+                {
+                    it.head = 0;
+                    do
+                    {
+                        ++it.request; // requests without tokens have no tiles; `at` < total, so one follows
+                        q = request_of(a.b, it.request);
+                    } while (q.count == 0);
+                    it.first_token = q.first;
+                    it.columns = q.count * a.group;
+                }
+            }
+            it.end = it.begin + tiles_of_block<COLS>(a, q, it.column0);
+        }
+    }
+}
+
+// Joins the parts of items that several blocks worked on: block c looks after the item that begins
+// in block c of the main kernel and ends in a later one, whose parts are part 1 of block c and
+// part 0 of the blocks up to its last.  Always in that order, so results do not depend on timing.
+template <int DIM, int COLS>
+__global__ void __launch_bounds__(THREADS) cache_join_kernel(const attend_args a)
+{
+    const int4 join = a.joins[blockIdx.x];
+    const int columns = min(COLS, join.w - join.z);
+    if (columns <= 0)
+    {
+        return;
+    }
+    const int64_t first = 2 * static_cast<int64_t>(blockIdx.x) + 1;
+    const int more = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x);
+    for (int e = blockIdx.y * THREADS + threadIdx.x; e < columns * DIM; e += gridDim.y * THREADS)
+    {
+        const int col = e / DIM;
+        const int d = e % DIM;
+        auto part = [&](int i) { return first + (i == 0 ? 0 : 2 * i - 1); };
+        float top = -INFINITY;
+        for (int i = 0; i <= more; ++i)
+        {
+            top = fmaxf(top, a.part_ml[part(i) * COLS + col].x);
+        }
+        float sum = 0.0F;
+        float den = 0.0F;
+#pragma unroll 4
+        for (int i = 0; i <= more; ++i)
+        {
+            const float2 ml = a.part_ml[part(i) * COLS + col];
+            const float keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
+            sum = fmaf(keep, a.part_o[(part(i) * COLS + col) * DIM + d], sum);
+            den = fmaf(keep, ml.y, den);
+        }
+        const int g = join.z + col;
+        const int64_t token = join.x + g / a.group;
+        const int qhead = join.y * a.group + g % a.group;
+        store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + d, den == 0.0F ? 0.0F : sum / den,
+                  a.dtype);
+        if (d == 0 && a.lse != nullptr)
+        {
+            a.lse[token * a.group * a.c.heads + qhead] =
+                den == 0.0F ? -INFINITY : (top - WEIGHT_BIAS + log2f(den)) * LN_2;
+        }
+    }
+}
+
+constexpr size_t JOIN_BYTES = sizeof(int4) + sizeof(int);
+
+template <int DIM, int NB>
+size_t workspace_of()
+{
+    const size_t blocks = static_cast<size_t>(device_sm_count()) * attend_smem<DIM, NB>::BLOCKS;
+    return blocks * (2 * 8 * NB * (DIM * sizeof(float) + sizeof(float2)) + JOIN_BYTES) + 256;
+}
+
+// Most columns a block can take: the sums of 8 NB columns take NB * DIM / 4 registers of a thread.
+constexpr int most_columns(int dim) { return dim <= 128 ? 4 : 2; }
+
+template <int DIM, int NB, bool SELECTED>
+int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaStream_t stream)
+{
+    using smem = attend_smem<DIM, NB>;
+    const int blocks = device_sm_count() * smem::BLOCKS;
+    if (workspace_bytes < workspace_of<DIM, NB>())
+    {
+        return fail(BITSKNN_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes,
+                    workspace_of<DIM, NB>());
+    }
+    a.joins = static_cast<int4*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.joins + blocks);
+    a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(blocks) * 2 * smem::COLS);
+    a.join_end = reinterpret_cast<int*>(a.part_o + static_cast<size_t>(blocks) * 2 * smem::COLS * DIM);
+    auto kernel = cache_attend_kernel<DIM, NB, SELECTED>;
+    BITSKNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem::BYTES));
+    {
+        kernel_scope scope("cache_attend_kernel", stream);
+        kernel<<<blocks, THREADS, smem::BYTES, stream>>>(a);
+    }
+    BITSKNN_CUDA_TRY(cudaGetLastError());
+    cache_join_kernel<DIM, smem::COLS><<<dim3(blocks, 4), THREADS, 0, stream>>>(a);
+    BITSKNN_CUDA_TRY(cudaGetLastError());
+    return BITSKNN_OK;
+}
+
+int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries, int dtype,
+           int64_t query_stride, int query_heads, bool selected, const int32_t* d_idx, int64_t ld_idx, int k, float scale,
+           void* d_out, int64_t out_stride, float* d_lse, void* d_workspace, size_t workspace_bytes,
+           bitsknn_stream_t stream)
+{
+    attend_args a{};
+    int rc = check_cache(cache, &a.c);
+    if (rc != BITSKNN_OK || (rc = check_cache_batch(batch, cache->page_rows, &a.b)) != BITSKNN_OK)
+    {
+        return rc;
+    }
+    if (selected && k < 1)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED_K, "Unsupported k value: %d", k);
+    }
+    if (selected && ld_idx < k)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "ld_idx=%lld is smaller than k=%d", static_cast<long long>(ld_idx), k);
+    }
+    const bool empty = batch->tokens == 0 || batch->requests == 0;
+    rc = check_cache_queries(empty && d_queries == nullptr ? cache->d_keys : d_queries, dtype, &query_stride, query_heads,
+                             cache->heads, cache->dim);
+    if (rc != BITSKNN_OK)
+    {
+        return rc;
+    }
+    const int64_t dense = static_cast<int64_t>(query_heads) * cache->dim;
+    out_stride = out_stride == 0 ? dense : out_stride;
+    if (out_stride < dense)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "out_stride=%lld: at least %lld", static_cast<long long>(out_stride),
+                    static_cast<long long>(dense));
+    }
+    if (empty)
+    {
+        return BITSKNN_OK;
+    }
+    if (d_out == nullptr || (selected && d_idx == nullptr) || d_workspace == nullptr)
+    {
+        return fail(d_workspace == nullptr && d_out != nullptr ? BITSKNN_ERR_WORKSPACE : BITSKNN_ERR_INVALID_ARGUMENT,
+                    "null pointer argument");
+    }
+    if ((reinterpret_cast<uintptr_t>(d_workspace) & 255) != 0 || (reinterpret_cast<uintptr_t>(d_out) & 1) != 0 ||
+        ((reinterpret_cast<uintptr_t>(d_lse) | reinterpret_cast<uintptr_t>(d_idx)) & 3) != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "misaligned pointer (workspace 256 bytes, out 2, lse and idx 4)");
+    }
+    a.queries = d_queries;
+    a.dtype = dtype;
+    a.query_stride = query_stride;
+    a.group = query_heads / cache->heads;
+    a.scale = scale * LOG2_E;
+    a.out = d_out;
+    a.out_stride = out_stride;
+    a.lse = d_lse;
+    a.idx = d_idx;
+    a.ld_idx = ld_idx;
+    a.k = k;
+    // columns that share a stream of the cache: the query heads of a token, times the tokens a request
+    // has on average when the whole cache is attended to
+    const int64_t per_request = selected ? 1 : (batch->tokens + batch->requests - 1) / batch->requests;
+    const int64_t want = std::min<int64_t>(a.group * per_request, 8 * most_columns(cache->dim));
+    auto s = static_cast<cudaStream_t>(stream);
+    return dispatch_cache_dim(cache->dim, [&](auto dim) {
+        constexpr int DIM = decltype(dim)::value;
+        if constexpr (most_columns(DIM) == 4)
+        {
+            if (want > 16)
+            {
+                return selected ? launch_attend<DIM, 4, true>(a, d_workspace, workspace_bytes, s)
+                                : launch_attend<DIM, 4, false>(a, d_workspace, workspace_bytes, s);
+            }
+        }
+        if (want > 8)
+        {
+            return selected ? launch_attend<DIM, 2, true>(a, d_workspace, workspace_bytes, s)
+                            : launch_attend<DIM, 2, false>(a, d_workspace, workspace_bytes, s);
+        }
+        return selected ? launch_attend<DIM, 1, true>(a, d_workspace, workspace_bytes, s)
+                        : launch_attend<DIM, 1, false>(a, d_workspace, workspace_bytes, s);
+    });
+}
+
+} // namespace
+
+} // namespace bitsknn
+
+extern "C" size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* cache, int query_heads)
+{
+    using namespace bitsknn;
+    cache::view v;
+    if (check_cache(cache, &v) != BITSKNN_OK || query_heads < 1)
+    {
+        return 0;
+    }
+    size_t bytes = 0;
+    dispatch_cache_dim(cache->dim, [&](auto dim) {
+        constexpr int DIM = decltype(dim)::value;
+        bytes = std::max({workspace_of<DIM, 1>(), workspace_of<DIM, 2>(), workspace_of<DIM, most_columns(DIM)>()});
+        return BITSKNN_OK;
+    });
+    return bytes;
+}
+
+extern "C" int bitsknn_cache_attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch,
+                                    const void* d_queries, int dtype, int64_t query_stride, int query_heads, float scale,
+                                    void* d_out, int64_t out_stride, float* d_lse, void* d_workspace,
+                                    size_t workspace_bytes, bitsknn_stream_t stream)
+{
+    return bitsknn::attend(cache, batch, d_queries, dtype, query_stride, query_heads, false, nullptr, 0, 0, scale, d_out,
+                           out_stride, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+extern "C" int bitsknn_cache_attend_selected(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch,
+                                             const void* d_queries, int dtype, int64_t query_stride, int query_heads,
+                                             const int32_t* d_idx, int64_t ld_idx, int k, float scale, void* d_out,
+                                             int64_t out_stride, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                                             bitsknn_stream_t stream)
+{
+    return bitsknn::attend(cache, batch, d_queries, dtype, query_stride, query_heads, true, d_idx, ld_idx, k, scale, d_out,
+                           out_stride, d_lse, d_workspace, workspace_bytes, stream);
+}

@@ -106,7 +106,8 @@ const char* bitsknn_tuning_key(int index);
  * with CUDA events on the launching stream while the knob "profile.kernel_events" is 1 (the
  * role of the reference's cuda_event pairs, include/bits/cuda_event.hpp:63-68, moved from the
  * transfers to the kernels).  Names: "select_kernel", "merge_kernel", "rerank_kernel",
- * "l2_fp32_kernel", "l2_tc_kernel", "fused_kernel", "fused_tiled_kernel", "fused_tc_kernel".
+ * "l2_fp32_kernel", "l2_tc_kernel", "fused_kernel", "fused_tiled_kernel", "fused_tc_kernel",
+ * "cache_append_kernel", "cache_distance_kernel", "cache_attend_kernel".
  * Synchronises on that launch's end.  INVALID_ARGUMENT if no timed launch of that name exists. */
 int bitsknn_kernel_ms(const char* kernel, float* ms);
 
@@ -322,6 +323,134 @@ int bitsknn_sharded_search_fused(bitsknn_sharded_t* handle, const float* d_point
                                  size_t fused_workspace_bytes, void* d_workspace, size_t workspace_bytes,
                                  bitsknn_stream_t stream);
 int bitsknn_sharded_drain(bitsknn_sharded_t* handle, bitsknn_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Search in a paged cache of keys and values held in 8 bits (no counterpart in the reference).
+ *
+ * For a database that is not a float32 matrix but grows row by row on the GPU, for many requests
+ * at once: the keys and values of an attention layer.  cache_plan gives the new rows of every
+ * request their places, cache_append quantises and stores them, cache_distance writes the
+ * distance matrix bitsknn_select takes, and cache_attend_selected consumes the index lists that
+ * come back: the softmax-weighted sum of the values at the k nearest keys.  cache_attend is the
+ * sum over the whole cache.
+ *
+ * Layout.  A page holds `page_rows` consecutive positions of one request for every head:
+ *   d_keys, d_values   e4m3 codes (1 byte) [pages][heads][page_rows][dim]; page p starts
+ *                      p * page_stride codes behind the base; bases 16-byte aligned
+ *   d_key_scales, d_value_scales   float32[pages][heads]; a number is code * scale.  The append
+ *                      writes powers of two in [2^-60, 2^60]; a reader takes any finite positive
+ *                      scale in that range and moves value scales outside it to its border
+ *   page_rows          16, 32, 64, 128 or 256
+ *   dim                32, 64, 96, 128, 192 or 256 (BITSKNN_ERR_UNSUPPORTED_DIM otherwise)
+ *   page_stride        0 = heads * page_rows * dim, else a multiple of 16 at least as large
+ *
+ * Batch.  Request r owns row r of the block table: entry j is the page of its positions
+ * [j * page_rows, (j + 1) * page_rows), an entry outside [0, pages) is an absent page whose
+ * positions nobody sees.  Its query tokens are the rows [d_starts[r], d_starts[r + 1]) of the
+ * packed token arrays (d_starts == NULL: one token per request, `tokens` == `requests`).
+ * d_lengths[r] counts its cached positions INCLUDING those tokens, so token i of m sees the
+ * positions below d_lengths[r] - m + i + 1.  Rows of outputs behind the last request's tokens are
+ * left as they were.  Lengths beyond the table's table_pages * page_rows are cut there.
+ *
+ * Query vectors: BITSKNN_F16 or BITSKNN_BF16, [tokens][query_heads][dim] with `query_stride`
+ * elements between tokens (0 = query_heads * dim); query head j belongs to cache head
+ * j / (query_heads / heads).  16-byte aligned, stride a multiple of 8.
+ * --------------------------------------------------------------------------------------- */
+enum bitsknn_dtype
+{
+    BITSKNN_F32 = 0,
+    BITSKNN_F16 = 1,
+    BITSKNN_BF16 = 2
+};
+
+typedef struct bitsknn_cache
+{
+    void* d_keys;
+    void* d_values;
+    float* d_key_scales;
+    float* d_value_scales;
+    int64_t pages;
+    int64_t page_stride;
+    int32_t heads;
+    int32_t page_rows;
+    int32_t dim;
+} bitsknn_cache_t;
+
+typedef struct bitsknn_cache_batch
+{
+    const int32_t* d_table; /* int32[requests][table_ld], table_ld >= table_pages */
+    int64_t table_ld;
+    int64_t table_pages;
+    const int32_t* d_lengths; /* int32[requests] */
+    const int32_t* d_starts;  /* int32[requests + 1], ascending, or NULL */
+    int64_t requests;
+    int64_t tokens;
+} bitsknn_cache_batch_t;
+
+/* Block tables and slot maps from request lengths, in one launch.  Request r holds d_lengths[r]
+ * positions and gets d_new[r] more (negative counts as 0); the pages it needs beyond the
+ * ceil(d_lengths[r] / page_rows) it has are taken from the front of d_free_pages in request order.
+ *   d_table        int32[requests][table_ld]: entries of the new pages are written, others kept
+ *   d_starts       int32[requests + 1] out: sums of d_new (the batch's d_starts)
+ *   d_new_lengths  int32[requests] out: d_lengths + d_new (the batch's d_lengths); not d_lengths itself
+ *   d_slots        int64[max_tokens] out: page * page_rows + row of every new token, -1 behind the
+ *                  last one and for a token that got no place (free list or table row exhausted,
+ *                  or its page is absent from the table).  More than max_tokens tokens: the first
+ *                  max_tokens slots are written
+ *   d_counts       int32[3] out: new tokens, pages asked of the free list, tokens for which the
+ *                  free list or the table row was too short (0: the plan holds)
+ * The sum of d_new must stay below 2^31. */
+int bitsknn_cache_plan(const int32_t* d_lengths, const int32_t* d_new, int64_t requests, int page_rows,
+                       const int32_t* d_free_pages, int64_t free_count, int32_t* d_table, int64_t table_ld,
+                       int64_t table_pages, int32_t* d_starts, int32_t* d_new_lengths, int64_t* d_slots,
+                       int64_t max_tokens, int32_t* d_counts, bitsknn_stream_t stream);
+
+/* Quantises new keys and values ([tokens][heads][dim] of `dtype`, any of the three; key_stride /
+ * value_stride elements between tokens, 0 = heads * dim; 16-byte aligned rows) into the cache at
+ * d_slots (int64[tokens], as cache_plan writes them; a slot outside the cache is skipped).
+ * Per page and head the scale is the smallest power of two under which the page's largest new
+ * finite entry stays within 448, and at least the page's scale unless row 0 of the page is among
+ * the new rows (a page that is begun).  When it grows, the rows in front of the new ones are
+ * re-rounded to it.  Rounding is to nearest, ties to even; what lies beyond 448 * 2^60 (and the
+ * infinities) saturates; NaN is kept.
+ * The tokens of one page must follow one another in d_slots (skipped slots may lie between).  Slots that do not ascend inside a page
+ * act like appends one after the other.  Calls that write the same page must not overlap. */
+int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_new_keys, const void* d_new_values, int dtype,
+                         int64_t key_stride, int64_t value_stride, const int64_t* d_slots, int64_t tokens,
+                         bitsknn_stream_t stream);
+
+/* Distances of every token to the cached keys of its request, per cache head:
+ *   d_dist[token * heads + h][j] = - max over the head's query heads of <query, key j>
+ * for the positions j < n that the token sees, +inf for the others below n.  A smaller value is a
+ * nearer key, so bitsknn_select(d_dist, ld, ..., tokens * heads, n, k, ...) lists the k keys with
+ * the largest inner products.  NaN products give NaN distances, which are never selected.
+ * float32[tokens * heads][ld], ld >= n, 4-byte aligned. */
+int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries,
+                           int dtype, int64_t query_stride, int query_heads, float* d_dist, int64_t ld, int64_t n,
+                           bitsknn_stream_t stream);
+
+/* Attention over the cache: for every token and query head
+ *   out = sum_j p_j value_j / sum_j p_j,   p_j = exp(scale * <query, key_j>),
+ * over the positions j the token sees; zeros (and lse = -inf) if there are none.
+ *   d_out   [tokens][query_heads][dim] of `dtype`, out_stride elements between tokens (0 = dense)
+ *   d_lse   optional float32[tokens][query_heads]: ln sum_j p_j (joins results over shards)
+ * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the batch; its
+ * contents on entry do not matter.  Calls that can overlap need workspaces of their own. */
+size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* cache, int query_heads);
+int bitsknn_cache_attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries,
+                         int dtype, int64_t query_stride, int query_heads, float scale, void* d_out,
+                         int64_t out_stride, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                         bitsknn_stream_t stream);
+
+/* The same sums over listed positions only: d_idx[token * heads + h][0 ... k), int32 with ld_idx
+ * entries between rows, as bitsknn_select writes them (any order).  Entries that the token does
+ * not see -- negative, behind its last position, padding, on an absent page -- are skipped; an
+ * entry that is listed twice counts twice.  k >= 1. */
+int bitsknn_cache_attend_selected(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch,
+                                  const void* d_queries, int dtype, int64_t query_stride, int query_heads,
+                                  const int32_t* d_idx, int64_t ld_idx, int k, float scale, void* d_out,
+                                  int64_t out_stride, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                                  bitsknn_stream_t stream);
 
 #ifdef __cplusplus
 }
