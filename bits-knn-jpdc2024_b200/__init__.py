@@ -393,9 +393,28 @@ class Cache:
         """A cache without content; its pages are to be appended to from their first row."""
         import torch
         shape = (pages, heads, page_rows, dim)
-        return cls(torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device),
-                   torch.zeros(shape[:2], dtype=torch.float32, device=device),
-                   torch.zeros(shape[:2], dtype=torch.float32, device=device))
+        codes = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+    def batch(self, queries, lengths, table, starts):
+        """(bitsknn_cache_batch_t, dtype code, elements between tokens) of a call's arguments.  These wrappers run once
+        per layer and step: they look at every argument once and keep nothing between calls."""
+        import torch
+        if queries.dim() != 3 or queries.shape[2] != self.dim:
+            raise ValueError(f"queries have shape {tuple(queries.shape)}, which does not fit the cache")
+        code, stride = _vectors(queries, "queries")
+        if lengths.dtype is not torch.int32 or table.dtype is not torch.int32:
+            raise ValueError("lengths and table must be torch.int32")
+        tokens, (requests, pages), (ld, inner) = queries.shape[0], table.shape, table.stride()
+        if lengths.shape != (requests,) or (inner != 1 and pages > 1) or (requests > 1 and lengths.stride(0) != 1):
+            raise ValueError("table must be (requests, pages) and lengths (requests,), contiguous in the last dimension")
+        if starts is not None and (starts.dtype is not torch.int32 or starts.shape != (requests + 1,)
+                                   or (requests > 0 and starts.stride(0) != 1)):
+            raise ValueError("starts must be a contiguous (requests + 1,) torch.int32 tensor")
+        _on_device(self.device, queries, lengths, table, starts)
+        return _BatchStruct(table.data_ptr(), ld if requests > 1 else pages, pages, lengths.data_ptr(),
+                            None if starts is None else starts.data_ptr(), requests, tokens), code, stride
 
 
 def _on_device(device, *tensors):
@@ -404,87 +423,79 @@ def _on_device(device, *tensors):
         raise ValueError(f"the tensors are on {device}, which is not the current device")
     for t in tensors:
         if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
+            raise ValueError(f"tensors on {device} and {t.device} (the library has no CPU path)")
 
 
-def _vectors(t, name, heads=None, dim=None):
+def _vectors(t, name):
     """(dtype code, elements between tokens) of a (tokens, heads, dim) tensor of vectors."""
     import torch
-    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    dtype = t.dtype
+    code = BF16 if dtype is torch.bfloat16 else F16 if dtype is torch.float16 else F32 if dtype is torch.float32 else None
     if code is None:
         raise ValueError(f"{name} must be float32, float16 or bfloat16")
-    if not t.is_cuda or t.dim() != 3:
-        raise ValueError(f"{name} must be a (tokens, heads, dim) CUDA tensor (the library has no CPU path)")
-    if (heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, which does not fit the cache")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+    tokens, heads, dim = t.shape
+    outer, middle, inner = t.stride()
+    if inner != 1 or (heads > 1 and middle != dim):
         raise ValueError(f"{name} must be contiguous in its last two dimensions")
-    return code, t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
-
-
-def _cache_batch(table, lengths, starts, tokens):
-    import torch
-    _device_check(table, torch.int32, "table")
-    _device_check(lengths, torch.int32, "lengths")
-    _device_check(starts, torch.int32, "starts")
-    requests = lengths.shape[0]
-    if table.dim() != 2 or table.shape[0] != requests or (starts is not None and starts.shape[0] != requests + 1):
-        raise ValueError("table must be (requests, pages), lengths (requests,), starts (requests + 1,)")
-    ld = table.stride(0) if requests > 1 else table.shape[1]
-    return _BatchStruct(table.data_ptr(), ld, table.shape[1], lengths.data_ptr(),
-                        None if starts is None else starts.data_ptr(), requests, tokens)
+    return code, outer if tokens > 1 else heads * dim
 
 
 def cache_plan(lengths, new, free_pages, table, page_rows, max_tokens, out=None):
     """Places for `new` tokens of every request: writes the new pages into `table` and returns
     (starts, new_lengths, slots, counts); counts = (tokens, pages taken, tokens without a place)."""
     import torch
+    int32, device = torch.int32, lengths.device
     for t, name in ((lengths, "lengths"), (new, "new"), (free_pages, "free_pages"), (table, "table")):
-        _device_check(t, torch.int32, name)
-    _on_device(lengths.device, new, free_pages, table)
-    requests = lengths.shape[0]
-    if new.shape[0] != requests or table.dim() != 2 or table.shape[0] != requests:
+        if not t.is_cuda or t.dtype is not int32:
+            raise ValueError(f"{name} must be a torch.int32 CUDA tensor (the library has no CPU path)")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} must be contiguous in its last dimension")
+    _on_device(device, new, free_pages, table)
+    requests, pages = table.shape
+    if lengths.shape != (requests,) or new.shape != (requests,) or free_pages.dim() != 1:
         raise ValueError("lengths and new must be (requests,), table (requests, pages)")
     if out is None:
-        i32 = dict(dtype=torch.int32, device=lengths.device)
-        out = (torch.empty(requests + 1, **i32), torch.empty(requests, **i32),
-               torch.empty(max_tokens, dtype=torch.int64, device=lengths.device), torch.empty(3, **i32))
-    ld = table.stride(0) if requests > 1 else table.shape[1]
-    _check(lib().bitsknn_cache_plan(_p(lengths), _p(new), requests, page_rows, _p(free_pages), free_pages.shape[0],
-                                    _p(table), ld, table.shape[1], _p(out[0]), _p(out[1]), _p(out[2]), max_tokens,
-                                    _p(out[3]), _stream()))
+        out = (torch.empty(requests + 1, dtype=int32, device=device), torch.empty(requests, dtype=int32, device=device),
+               torch.empty(max_tokens, dtype=torch.int64, device=device), torch.empty(3, dtype=int32, device=device))
+    _check(lib().bitsknn_cache_plan(lengths.data_ptr(), new.data_ptr(), requests, page_rows, free_pages.data_ptr(),
+                                    free_pages.shape[0], table.data_ptr(), table.stride(0) if requests > 1 else pages, pages,
+                                    out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), max_tokens,
+                                    out[3].data_ptr(), _stream()))
     return out
 
 
 def cache_append(cache, keys, values, slots):
     """Quantises (tokens, heads, dim) keys and values into the cache at `slots` (int64, from cache_plan)."""
     import torch
-    code, key_stride = _vectors(keys, "keys", cache.heads, cache.dim)
-    value_code, value_stride = _vectors(values, "values", cache.heads, cache.dim)
-    _device_check(slots, torch.int64, "slots")
+    shape = keys.shape
+    if values.shape != shape or len(shape) != 3 or shape[1] != cache.heads or shape[2] != cache.dim:
+        raise ValueError(f"keys {tuple(shape)} and values {tuple(values.shape)} do not fit the cache")
+    code, key_stride = _vectors(keys, "keys")
+    value_code, value_stride = _vectors(values, "values")
+    tokens = shape[0]
+    if value_code != code or slots.dtype is not torch.int64 or slots.dim() != 1 or slots.shape[0] < tokens:
+        raise ValueError("keys and values must agree in type, and every token needs an int64 slot")
+    if tokens > 1 and slots.stride(0) != 1:
+        raise ValueError("slots must be contiguous in its last dimension")
     _on_device(cache.device, keys, values, slots)
-    tokens = keys.shape[0]
-    if value_code != code or values.shape[0] != tokens or slots.shape[0] < tokens:
-        raise ValueError("keys and values must agree in type and tokens, and every token needs a slot")
-    _check(lib().bitsknn_cache_append(cache.struct, _p(keys), _p(values), code, key_stride, value_stride, _p(slots),
-                                      tokens, _stream()))
+    _check(lib().bitsknn_cache_append(cache.struct, keys.data_ptr(), values.data_ptr(), code, key_stride, value_stride,
+                                      slots.data_ptr(), tokens, _stream()))
 
 
 def cache_distance(cache, queries, lengths, table, n, starts=None, out=None):
     """(tokens * heads, n) float32 distances for `select`: minus the largest inner product over a head's queries."""
     import torch
-    code, stride = _vectors(queries, "queries", None, cache.dim)
-    _on_device(cache.device, queries, lengths, table, starts)
-    tokens, query_heads, _ = queries.shape
-    batch = _cache_batch(table, lengths, starts, tokens)
+    batch, code, stride = cache.batch(queries, lengths, table, starts)
+    rows = queries.shape[0] * cache.heads
     if out is None:
-        out = torch.empty((tokens * cache.heads, n), dtype=torch.float32, device=cache.device)
-    _device_check(out, torch.float32, "out")
-    if out.shape[0] < tokens * cache.heads or out.shape[1] < n:
-        raise ValueError("out must have tokens * heads rows of n distances")
-    ld = out.stride(0) if out.shape[0] > 1 else out.shape[1]
-    _check(lib().bitsknn_cache_distance(cache.struct, batch, _p(queries), code, stride, query_heads, _p(out), ld, n,
-                                        _stream()))
+        out = torch.empty((rows, n), dtype=torch.float32, device=cache.device)
+    else:
+        _device_check(out, torch.float32, "out")
+        _on_device(cache.device, out)
+        if out.dim() != 2 or out.shape[0] < rows or out.shape[1] < n:
+            raise ValueError("out must have tokens * heads rows of n distances")
+    _check(lib().bitsknn_cache_distance(cache.struct, batch, queries.data_ptr(), code, stride, queries.shape[1],
+                                        out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1], n, _stream()))
     return out
 
 
@@ -494,49 +505,53 @@ def cache_attend_workspace_bytes(cache, query_heads):
 
 def _attend_buffers(cache, queries, out, lse, workspace):
     import torch
+    shape, device = queries.shape, cache.device
+    stride = 0
     if out is None:
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=queries.device)
-    elif out.shape != queries.shape or out.dtype != queries.dtype:
+        out = torch.empty(shape, dtype=queries.dtype, device=device)
+    elif out.shape != shape or out.dtype is not queries.dtype:
         raise ValueError("out must have the queries' shape and type")
+    else:
+        _on_device(device, out)
+        stride = _vectors(out, "out")[1]
     if lse is None:
-        lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=queries.device)
-    elif lse.shape != queries.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=device)
+    elif lse.shape != shape[:2] or lse.dtype is not torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous (tokens, query_heads) float32 tensor")
+    else:
+        _on_device(device, lse)
     if workspace is None:
-        workspace = torch.empty(cache_attend_workspace_bytes(cache, queries.shape[1]), dtype=torch.uint8,
-                                device=queries.device)
-    _on_device(cache.device, queries, out, lse, workspace)
-    return out, lse, workspace
+        workspace = torch.empty(cache_attend_workspace_bytes(cache, shape[1]), dtype=torch.uint8, device=device)
+    elif workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor on the cache's device")
+    return out, stride, lse, workspace
 
 
 def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
     """Attention of (tokens, query_heads, dim) queries over everything cached: (out, lse)."""
-    code, stride = _vectors(queries, "queries", None, cache.dim)
-    out, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
-    _on_device(cache.device, lengths, table, starts)
-    batch = _cache_batch(table, lengths, starts, queries.shape[0])
-    _check(lib().bitsknn_cache_attend(cache.struct, batch, _p(queries), code, stride, queries.shape[1], scale, _p(out),
-                                      _vectors(out, "out", None, cache.dim)[1], _p(lse), _p(workspace), workspace.numel(),
-                                      _stream()))
+    batch, code, stride = cache.batch(queries, lengths, table, starts)
+    out, out_stride, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
+    _check(lib().bitsknn_cache_attend(cache.struct, batch, queries.data_ptr(), code, stride, queries.shape[1], scale,
+                                      out.data_ptr(), out_stride, lse.data_ptr(), workspace.data_ptr(),
+                                      workspace.numel(), _stream()))
     return out, lse
 
 
 def cache_attend_selected(cache, queries, idx, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
     """Attention over listed positions: idx (tokens * heads, k) int32, as `select` returns them.  (out, lse)."""
     import torch
-    code, stride = _vectors(queries, "queries", None, cache.dim)
-    _device_check(idx, torch.int32, "idx")
-    tokens = queries.shape[0]
-    if idx.dim() != 2 or idx.shape[0] != tokens * cache.heads:
+    batch, code, stride = cache.batch(queries, lengths, table, starts)
+    if idx.dim() != 2 or idx.shape[0] != queries.shape[0] * cache.heads:
         raise ValueError("idx must be (tokens * heads, k)")
-    out, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
-    _on_device(cache.device, idx, lengths, table, starts)
-    batch = _cache_batch(table, lengths, starts, tokens)
-    k = idx.shape[1]
-    _check(lib().bitsknn_cache_attend_selected(cache.struct, batch, _p(queries), code, stride, queries.shape[1], _p(idx),
-                                               idx.stride(0) if idx.shape[0] > 1 else k, k, scale, _p(out),
-                                               _vectors(out, "out", None, cache.dim)[1], _p(lse), _p(workspace),
-                                               workspace.numel(), _stream()))
+    rows, k = idx.shape
+    if idx.dtype is not torch.int32 or (k > 1 and idx.stride(1) != 1):
+        raise ValueError("idx must be torch.int32, contiguous in its last dimension")
+    _on_device(cache.device, idx)
+    out, out_stride, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
+    _check(lib().bitsknn_cache_attend_selected(cache.struct, batch, queries.data_ptr(), code, stride, queries.shape[1],
+                                               idx.data_ptr(), idx.stride(0) if rows > 1 else k, k, scale, out.data_ptr(),
+                                               out_stride, lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                               _stream()))
     return out, lse
 
 

@@ -6,6 +6,7 @@
 // bits, no infinities, 0x7f / 0xff = NaN) times the scale of its page and head.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -25,6 +26,27 @@ constexpr int SUB = 16;              // cached rows a warp handles at a time
 constexpr int TILE = WARPS * SUB;    // cached rows a block handles at a time
 constexpr int E_MIN = -60;           // exponents of the scales the append kernel writes
 constexpr int E_MAX = 60;
+
+// Devices on which a kernel's attributes have been set (they hold for the life of the context; a
+// device beyond the 64th is set up at every call).
+struct device_set
+{
+    std::atomic<uint64_t> bits{0};
+
+    bool contains_current() const
+    {
+        int device = 64;
+        return cudaGetDevice(&device) == cudaSuccess && device < 64 && ((bits.load() >> device) & 1) != 0;
+    }
+    void add_current()
+    {
+        int device = 64;
+        if (cudaGetDevice(&device) == cudaSuccess && device < 64)
+        {
+            bits.fetch_or(1ULL << device);
+        }
+    }
+};
 
 // Device view of bitsknn_cache_t (strides resolved).
 struct view
@@ -109,12 +131,13 @@ __device__ __forceinline__ int owner_of(const batch& b, int token)
 }
 
 // ---- number formats ------------------------------------------------------------------------
-// Two codes (low byte first) to two halves; exact, every e4m3 number is a half.
-__device__ __forceinline__ uint32_t half2_of_codes(uint32_t codes16)
+// The four codes of a word to halves, bytes 0, 1 to `lo` and bytes 2, 3 to `hi`; exact, every e4m3
+// number is a half.
+__device__ __forceinline__ void halves_of_codes(uint32_t w, uint32_t& lo, uint32_t& hi)
 {
-    uint32_t out;
-    asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(out) : "r"(codes16));
-    return out;
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
 }
 
 // Two floats to two codes (`lo` in the low byte): nearest, ties to even, saturating at 448; NaN -> 0x7f.
@@ -155,6 +178,11 @@ __device__ __forceinline__ float load_float(const void* p, int64_t i, int dtype)
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t bytes)
@@ -272,21 +300,23 @@ __device__ __forceinline__ void score_rows(float (&s)[NB][4], const unsigned cha
     const int c = lane & 3;
     const unsigned char* low = rows + row_order(lane >> 2) * PITCH<DIM>;
     const unsigned char* high = low + 8 * PITCH<DIM>;
+    // two sums, for even and odd steps, so that a step does not wait for the one before it
+    float odd[NB][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
     {
         s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.0F;
+        odd[nb][0] = odd[nb][1] = odd[nb][2] = odd[nb][3] = 0.0F;
     }
     auto step = [&](int kstep, uint32_t a, uint32_t b) {
-        const uint32_t a0 = half2_of_codes(a & 0xffffU);
-        const uint32_t a2 = half2_of_codes(a >> 16);
-        const uint32_t a1 = half2_of_codes(b & 0xffffU);
-        const uint32_t a3 = half2_of_codes(b >> 16);
+        uint32_t a0, a1, a2, a3;
+        halves_of_codes(a, a0, a2);
+        halves_of_codes(b, a1, a3);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
         {
             const uint2 q = image[(kstep * NB + nb) * 32 + lane];
-            mma_16816(s[nb], a0, a1, a2, a3, q.x, q.y);
+            mma_16816((kstep & 1) != 0 ? odd[nb] : s[nb], a0, a1, a2, a3, q.x, q.y);
         }
     };
 #pragma unroll
@@ -305,6 +335,15 @@ __device__ __forceinline__ void score_rows(float (&s)[NB][4], const unsigned cha
         const uint2 y = *reinterpret_cast<const uint2*>(high + FULL * 64 + c * 8);
         step(FULL * 4 + 0, x.x, y.x);
         step(FULL * 4 + 1, x.y, y.y);
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            s[nb][i] += odd[nb][i];
+        }
     }
 }
 

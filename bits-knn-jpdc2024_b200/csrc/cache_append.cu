@@ -10,7 +10,6 @@ namespace
 {
 
 constexpr int APPEND_THREADS = 128;
-constexpr int APPEND_HELD = 8; // vectors of 8 numbers a thread keeps between the two passes
 
 struct append_args
 {
@@ -24,41 +23,57 @@ struct append_args
     int dtype;
 };
 
-struct vec8
+// Eight numbers as they lie in memory (one 16-byte word, two for FP32), and as floats.
+template <int DTYPE>
+struct raw8
 {
-    float v[8];
+    uint4 w[DTYPE == BITSKNN_F32 ? 2 : 1];
 };
 
-__device__ __forceinline__ vec8 load8(const void* src, int64_t at, int dtype)
+template <int DTYPE>
+__device__ __forceinline__ raw8<DTYPE> load8(const void* src, int64_t at)
 {
-    vec8 r;
-    if (dtype == BITSKNN_F32)
+    raw8<DTYPE> r;
+    if constexpr (DTYPE == BITSKNN_F32)
     {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at);
-        const float4 x = __ldg(p);
-        const float4 y = __ldg(p + 1);
-        r.v[0] = x.x, r.v[1] = x.y, r.v[2] = x.z, r.v[3] = x.w;
-        r.v[4] = y.x, r.v[5] = y.y, r.v[6] = y.z, r.v[7] = y.w;
-        return r;
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(src) + at);
+        r.w[0] = __ldg(p);
+        r.w[1] = __ldg(p + 1);
     }
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at));
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
+    else
     {
-        if (dtype == BITSKNN_BF16)
-        {
-            r.v[2 * i] = __uint_as_float(w[i] << 16);
-            r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000U);
-        }
-        else
-        {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            r.v[2 * i] = f.x;
-            r.v[2 * i + 1] = f.y;
-        }
+        r.w[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at));
     }
     return r;
+}
+
+template <int DTYPE>
+__device__ __forceinline__ void floats_of(const raw8<DTYPE>& r, float (&v)[8])
+{
+#pragma unroll
+    for (int i = 0; i < (DTYPE == BITSKNN_F32 ? 2 : 1); ++i)
+    {
+        const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            if constexpr (DTYPE == BITSKNN_F32)
+            {
+                v[4 * i + j] = __uint_as_float(w[j]);
+            }
+            else if constexpr (DTYPE == BITSKNN_BF16)
+            {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000U);
+            }
+            else
+            {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+        }
+    }
 }
 
 // Smallest power of two s in [2^E_MIN, 2^E_MAX] with amax <= 448 s.  448 = 1.75 * 2^8, so the
@@ -73,14 +88,15 @@ __device__ __forceinline__ float scale_of(float amax)
 // One block = one window of tokens, one head, keys or values (gridDim = windows x heads x 2).  It
 // serves the pages whose first token lies in its window, run after run: a run is the longest
 // stretch of tokens of one page with ascending rows.  Two passes over a run: the largest finite
-// entry (block maximum), then rounding; what fits into APPEND_HELD vectors per thread stays in
-// registers between them (128 rows of 64 numbers, 64 rows of 128), the rest is read again from L2.
+// entry (block maximum), then rounding; what fits into HELD vectors per thread stays in
+// registers between them (64 rows of 128 halves, 32 of 128 floats), the rest is read again from L2.
 // A page has one scale per head, which is why a run belongs to one block and why a later token
 // that needs a larger scale re-rounds the rows in front of it: with powers of two that only
 // costs bits at the subnormal end, code * 2^(old - new) is exact for every other code.
 template <int DTYPE>
-__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const append_args a)
+__global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const append_args a)
 {
+    constexpr int HELD = DTYPE == BITSKNN_F32 ? 4 : 8; // vectors of 8 numbers a thread keeps between the passes
     __shared__ float s_top[APPEND_THREADS / 32];
     const int t = threadIdx.x;
     const int lane = t & 31;
@@ -161,23 +177,25 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const appe
         const int offset0 = static_cast<int>(slot0) & rows_mask;
         const int64_t base = page * a.c.page_stride + (static_cast<int64_t>(head) << a.c.page_shift) * a.dim;
         const int work = run * vecs;
-        vec8 held[APPEND_HELD];
+        raw8<DTYPE> held[HELD];
         float top = 0.0F;
         auto fetch = [&](int w) {
             const int row = (w * vec_magic) >> 16;
             const int part = w - row * vecs;
-            return load8(src, (i + row) * stride + static_cast<int64_t>(head) * a.dim + part * 8, DTYPE);
+            return load8<DTYPE>(src, (i + row) * stride + static_cast<int64_t>(head) * a.dim + part * 8);
         };
-        auto look = [&](const vec8& x) {
+        auto look = [&](const raw8<DTYPE>& x) {
+            float f[8];
+            floats_of<DTYPE>(x, f);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                const float v = fabsf(x.v[e]);
+                const float v = fabsf(f[e]);
                 top = v < INFINITY ? fmaxf(top, v) : top; // NaN and the infinities set no scale
             }
         };
 #pragma unroll
-        for (int h = 0; h < APPEND_HELD; ++h)
+        for (int h = 0; h < HELD; ++h)
         {
             const int w = t + h * APPEND_THREADS;
             if (w < work)
@@ -186,14 +204,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const appe
             }
         }
 #pragma unroll
-        for (int h = 0; h < APPEND_HELD; ++h)
+        for (int h = 0; h < HELD; ++h)
         {
             if (t + h * APPEND_THREADS < work)
             {
                 look(held[h]);
             }
         }
-        for (int w = t + APPEND_HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
+        for (int w = t + HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
         {
             look(fetch(w));
         }
@@ -219,19 +237,21 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const appe
         const float old = stored > 0.0F && stored <= cache::pow2_int(cache::E_MAX) ? stored : cache::pow2_int(cache::E_MIN);
         const float scale = fmaxf(scale_of(top), old);
         const float inverse = 1.0F / scale;
-        auto store = [&](int w, const vec8& x) {
+        auto store = [&](int w, const raw8<DTYPE>& x) {
+            float f[8];
+            floats_of<DTYPE>(x, f);
             const int row = (w * vec_magic) >> 16;
             const int part = w - row * vecs;
             const int64_t at = base + static_cast<int64_t>(static_cast<int>(a.slots[i + row]) & rows_mask) * a.dim + part * 8;
             uint2 out;
-            out.x = cache::codes_of_floats(x.v[0] * inverse, x.v[1] * inverse) |
-                    cache::codes_of_floats(x.v[2] * inverse, x.v[3] * inverse) << 16;
-            out.y = cache::codes_of_floats(x.v[4] * inverse, x.v[5] * inverse) |
-                    cache::codes_of_floats(x.v[6] * inverse, x.v[7] * inverse) << 16;
+            out.x = cache::codes_of_floats(f[0] * inverse, f[1] * inverse) |
+                    cache::codes_of_floats(f[2] * inverse, f[3] * inverse) << 16;
+            out.y = cache::codes_of_floats(f[4] * inverse, f[5] * inverse) |
+                    cache::codes_of_floats(f[6] * inverse, f[7] * inverse) << 16;
             *reinterpret_cast<uint2*>(codes + at) = out;
         };
 #pragma unroll
-        for (int h = 0; h < APPEND_HELD; ++h)
+        for (int h = 0; h < HELD; ++h)
         {
             const int w = t + h * APPEND_THREADS;
             if (w < work)
@@ -239,7 +259,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const appe
                 store(w, held[h]);
             }
         }
-        for (int w = t + APPEND_HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
+        for (int w = t + HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
         {
             store(w, fetch(w));
         }
@@ -251,8 +271,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const appe
             {
                 uint32_t* const p = reinterpret_cast<uint32_t*>(codes + base) + w;
                 const uint32_t c = *p;
-                const uint32_t lo = cache::half2_of_codes(c & 0xffffU);
-                const uint32_t hi = cache::half2_of_codes(c >> 16);
+                uint32_t lo, hi;
+                cache::halves_of_codes(c, lo, hi);
                 const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
                 const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 *p = cache::codes_of_floats(x.x * shrink, x.y * shrink) |

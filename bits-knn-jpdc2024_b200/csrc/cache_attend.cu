@@ -55,7 +55,7 @@ struct item
     int head;
     int column0;
     int columns;     // columns of the request (selected: of the token) in total
-    int64_t begin;   // first tile
+    int64_t begin;   // where it lies on the axis of the work
     int64_t end;
 };
 
@@ -89,25 +89,28 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, float v, int dt
     }
 }
 
-// ---- tiles of the requests -------------------------------------------------------------------
-// All tiles of all items lie on one axis: requests in order, within a request heads, within a
-// head blocks of columns, within a block its tiles of 64 positions (at least one, which writes
-// the zeros of a row that sees nothing).  Block c of the grid takes the c-th equal share, so a
-// long request is spread over many blocks and short ones fill up the others.
+// ---- shares of the work ----------------------------------------------------------------------
+// All items lie on one axis: requests in order, within a request heads, within a head blocks of
+// columns.  An item covers ITEM_COST units for its beginning and end (packing the queries, filling
+// the pipeline, joining the warps: about as long as three tiles) and one unit for each of its tiles
+// of 64 positions.  Block c of the grid takes the c-th equal share of the axis, so a long request
+// is spread over many blocks and short ones fill up the others.
+constexpr int ITEM_COST = 3;
+
 template <int COLS>
-__device__ __forceinline__ int tiles_of_block(const attend_args& a, const request& q, int column0)
+__device__ __forceinline__ int units_of_block(const attend_args& a, const request& q, int column0)
 {
     const int last = min(column0 + COLS, q.count * a.group) - 1;
-    return max((visible_of(a.b, q, last / a.group) + TILE - 1) / TILE, 1);
+    return (visible_of(a.b, q, last / a.group) + TILE - 1) / TILE + ITEM_COST;
 }
 
 template <int COLS>
-__device__ __forceinline__ int64_t tiles_of_head(const attend_args& a, const request& q)
+__device__ __forceinline__ int64_t units_of_head(const attend_args& a, const request& q)
 {
     int64_t sum = 0;
     for (int col = 0; col < q.count * a.group; col += COLS)
     {
-        sum += tiles_of_block<COLS>(a, q, col);
+        sum += units_of_block<COLS>(a, q, col);
     }
     return sum;
 }
@@ -134,7 +137,7 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* words)
     return sum;
 }
 
-// The request that holds tile `at`, and the first tile of that request.
+// The request that holds unit `at`, and the first unit of that request.
 template <int COLS>
 __device__ __forceinline__ int find_request(const attend_args& a, int64_t at, int64_t* first, int64_t* words, int* found)
 {
@@ -142,7 +145,7 @@ __device__ __forceinline__ int find_request(const attend_args& a, int64_t at, in
     for (int base = 0; base < a.b.requests; base += THREADS)
     {
         const int r = base + threadIdx.x;
-        const int64_t mine = r < a.b.requests ? tiles_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads : 0;
+        const int64_t mine = r < a.b.requests ? units_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads : 0;
         int64_t upto = mine;
         const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -218,28 +221,29 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
     const int c = (lane & 3) * 2;             // this thread's columns: c, c + 1 of every block of 8
     const int row_lo = row_order(lane >> 2);  // its rows: row_lo, row_lo + 8
 
-    // this block's share of the tiles, and the item it begins in
-    const int list_tiles = SELECTED ? (a.k + TILE - 1) / TILE : 0;
+    // this block's share, and the item it begins in
+    const int list_units = SELECTED ? (a.k + TILE - 1) / TILE + ITEM_COST : 0;
     const int list_blocks = SELECTED ? (a.group + COLS - 1) / COLS : 0;
     int64_t total;
     if constexpr (SELECTED)
     {
-        total = static_cast<int64_t>(a.b.tokens) * a.c.heads * list_blocks * list_tiles;
+        total = static_cast<int64_t>(a.b.tokens) * a.c.heads * list_blocks * list_units;
     }
     else
     {
         int64_t sum = 0;
         for (int r = threadIdx.x; r < a.b.requests; r += THREADS)
         {
-            sum += tiles_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads;
+            sum += units_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads;
         }
         total = block_sum(sum, s_words);
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0)
     {
         a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
-    const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total); // those that get a tile at all
+    const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total); // those that get a share at all
     if (blockIdx.x >= blocks)
     {
         return;
@@ -249,9 +253,9 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
     item it{};
     if constexpr (SELECTED)
     {
-        const int64_t n = at / list_tiles;
-        it.begin = n * list_tiles;
-        it.end = it.begin + list_tiles;
+        const int64_t n = at / list_units;
+        it.begin = n * list_units;
+        it.end = it.begin + list_units;
         it.column0 = static_cast<int>(n % list_blocks) * COLS;
         it.head = static_cast<int>(n / list_blocks % a.c.heads);
         it.first_token = static_cast<int>(n / list_blocks / a.c.heads);
@@ -262,17 +266,17 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
         int64_t first = 0;
         it.request = find_request<COLS>(a, at, &first, s_words, &s_found);
         const request q = request_of(a.b, it.request);
-        const int64_t per_head = tiles_of_head<COLS>(a, q);
+        const int64_t per_head = units_of_head<COLS>(a, q);
         it.head = static_cast<int>((at - first) / per_head);
         it.begin = first + it.head * per_head;
         it.first_token = q.first;
         it.columns = q.count * a.group;
-        it.end = it.begin + tiles_of_block<COLS>(a, q, 0);
+        it.end = it.begin + units_of_block<COLS>(a, q, 0);
         while (at >= it.end)
         {
             it.column0 += COLS;
             it.begin = it.end;
-            it.end += tiles_of_block<COLS>(a, q, it.column0);
+            it.end += units_of_block<COLS>(a, q, it.column0);
         }
     }
 
@@ -316,8 +320,9 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
             {
                 list = a.idx + (static_cast<int64_t>(it.first_token) * a.c.heads + it.head) * a.ld_idx;
             }
-            const int first_tile = static_cast<int>(at - it.begin);
-            const int count = static_cast<int>(seg_end - at);
+            // tiles of the share; none if it ends within the units of the item's beginning
+            const int first_tile = max(static_cast<int>(at - it.begin) - ITEM_COST, 0);
+            const int count = max(static_cast<int>(seg_end - it.begin) - ITEM_COST, 0) - first_tile;
             const int row_end = SELECTED ? a.k : furthest; // rows behind it are zero
             auto row_of = [&](int j) { return (first_tile + j) * TILE + warp * SUB; };
 
@@ -388,20 +393,40 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                         const int pos = row_of(j);
                         const int there = page < 0 ? 0 : min(SUB, furthest - pos);
                         next_page = page_at(j + 1 < count && row_of(j + 1) < furthest ? row_of(j + 1) : -1);
-                        const int64_t from = safe * a.c.page_stride +
+                        // a subtile lies within one page: its rows are contiguous and share a scale
+                        const int64_t from = safe * a.c.page_stride + lane * 16 +
                                              ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
-#pragma unroll
-                        for (int x = 0; x < DIM / 32; ++x)
+                        const uint8_t* const k_from = a.c.keys + from;
+                        const uint8_t* const v_from = a.c.values + from;
+                        if (there == SUB)
                         {
-                            const int e = lane + x * 32;
-                            const int row = e / PARTS;
-                            const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
-                            copy16(to, a.c.keys + from + e * 16, row < there ? 16U : 0U);
-                            copy16(to + SUB * PITCH<DIM>, a.c.values + from + e * 16, row < there ? 16U : 0U);
+#pragma unroll
+                            for (int x = 0; x < DIM / 32; ++x)
+                            {
+                                const int e = lane + x * 32;
+                                const uint32_t to = dst + e / PARTS * PITCH<DIM> + (e % PARTS) * 16;
+                                copy16(to, k_from + x * 512);
+                                copy16(to + SUB * PITCH<DIM>, v_from + x * 512);
+                            }
                         }
-                        const float* scales = lane < SUB ? a.c.key_scales : a.c.value_scales;
-                        copy4(dst + smem::SCALES + lane * 4, scales + static_cast<int64_t>(safe) * a.c.heads + it.head,
-                              (lane & (SUB - 1)) < there ? 4U : 0U);
+                        else
+                        {
+#pragma unroll
+                            for (int x = 0; x < DIM / 32; ++x)
+                            {
+                                const int e = lane + x * 32;
+                                const int row = e / PARTS;
+                                const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
+                                copy16(to, k_from + x * 512, row < there ? 16U : 0U);
+                                copy16(to + SUB * PITCH<DIM>, v_from + x * 512, row < there ? 16U : 0U);
+                            }
+                        }
+                        if (lane < 2)
+                        {
+                            const float* scales = lane == 0 ? a.c.key_scales : a.c.value_scales;
+                            copy4(dst + smem::SCALES + lane * 4, scales + static_cast<int64_t>(safe) * a.c.heads + it.head,
+                                  page < 0 ? 0U : 4U);
+                        }
                     }
                 }
                 copy_commit();
@@ -445,24 +470,40 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     const float* const scales = reinterpret_cast<const float*>(stage + smem::SCALES);
                     float s[NB][4];
                     score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
-                    const float ks_lo = scales[row_lo];
-                    const float ks_hi = scales[row_lo + 8];
                     // value scales at the border of their range and beyond would leave that of the sums
-                    const float vs_lo = fminf(fmaxf(scales[SUB + row_lo], pow2_int(E_MIN)), pow2_int(E_MAX));
-                    const float vs_hi = fminf(fmaxf(scales[SUB + row_lo + 8], pow2_int(E_MIN)), pow2_int(E_MAX));
+                    auto fit = [](float vs) { return fminf(fmaxf(vs, pow2_int(E_MIN)), pow2_int(E_MAX)); };
+                    const float ks_lo = SELECTED ? scales[row_lo] : scales[0];
+                    const float ks_hi = SELECTED ? scales[row_lo + 8] : ks_lo;
+                    const float vs_lo = fit(SELECTED ? scales[SUB + row_lo] : scales[1]);
+                    const float vs_hi = SELECTED ? fit(scales[SUB + row_lo + 8]) : vs_lo;
                     const float lv_lo = log2_fast(vs_lo);
-                    const float lv_hi = log2_fast(vs_hi);
+                    const float lv_hi = SELECTED ? log2_fast(vs_hi) : lv_lo;
                     // absent rows were copied as zeros, scale included; others are seen below `see`
                     const int at_lo = ks_lo != 0.0F ? pos + row_lo : 0x7fffffff;
                     const int at_hi = ks_hi != 0.0F ? pos + row_lo + 8 : 0x7fffffff;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                    {
+                        s[nb][0] = fmaf(s[nb][0], f[nb][0] * ks_lo, lv_lo);
+                        s[nb][1] = fmaf(s[nb][1], f[nb][1] * ks_lo, lv_lo);
+                        s[nb][2] = fmaf(s[nb][2], f[nb][0] * ks_hi, lv_hi);
+                        s[nb][3] = fmaf(s[nb][3], f[nb][1] * ks_hi, lv_hi);
+                    }
+                    if (SELECTED || ks_lo == 0.0F || pos + SUB > nearest)
+                    {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                        {
+                            s[nb][0] = at_lo < see[nb][0] ? s[nb][0] : -INFINITY;
+                            s[nb][1] = at_lo < see[nb][1] ? s[nb][1] : -INFINITY;
+                            s[nb][2] = at_hi < see[nb][0] ? s[nb][2] : -INFINITY;
+                            s[nb][3] = at_hi < see[nb][1] ? s[nb][3] : -INFINITY;
+                        }
+                    }
                     bool raise = false;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
-                        s[nb][0] = at_lo < see[nb][0] ? fmaf(s[nb][0], f[nb][0] * ks_lo, lv_lo) : -INFINITY;
-                        s[nb][1] = at_lo < see[nb][1] ? fmaf(s[nb][1], f[nb][1] * ks_lo, lv_lo) : -INFINITY;
-                        s[nb][2] = at_hi < see[nb][0] ? fmaf(s[nb][2], f[nb][0] * ks_hi, lv_hi) : -INFINITY;
-                        s[nb][3] = at_hi < see[nb][1] ? fmaf(s[nb][3], f[nb][1] * ks_hi, lv_hi) : -INFINITY;
                         raise |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + WEIGHT_SLACK;
                         raise |= fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + WEIGHT_SLACK;
                     }
@@ -496,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     uint32_t w_lo[NB];
                     uint32_t w_hi[NB];
                     const float iv_lo = __fdividef(1.0F, vs_lo);
-                    const float iv_hi = __fdividef(1.0F, vs_hi);
+                    const float iv_hi = SELECTED ? __fdividef(1.0F, vs_hi) : iv_lo;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
@@ -506,8 +547,16 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                         const float p1 = exp2_fast(s[nb][1] + b1);
                         const float p2 = exp2_fast(s[nb][2] + b0);
                         const float p3 = exp2_fast(s[nb][3] + b1);
-                        l[nb][0] = fmaf(p0, iv_lo, fmaf(p2, iv_hi, l[nb][0]));
-                        l[nb][1] = fmaf(p1, iv_lo, fmaf(p3, iv_hi, l[nb][1]));
+                        if constexpr (SELECTED)
+                        {
+                            l[nb][0] = fmaf(p0, iv_lo, fmaf(p2, iv_hi, l[nb][0]));
+                            l[nb][1] = fmaf(p1, iv_lo, fmaf(p3, iv_hi, l[nb][1]));
+                        }
+                        else
+                        {
+                            l[nb][0] = fmaf(p0 + p2, iv_lo, l[nb][0]);
+                            l[nb][1] = fmaf(p1 + p3, iv_lo, l[nb][1]);
+                        }
                         w_lo[nb] = transpose_8x8(pack_half2(p0, p1));
                         w_hi[nb] = transpose_8x8(pack_half2(p2, p3));
                     }
@@ -541,10 +590,9 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                             {
                                 const uint32_t u = __byte_perm(r[2 * x], 0, 0x3120);
                                 const uint32_t v = __byte_perm(r[2 * x + 1], 0, 0x3120);
-                                const uint32_t a0 = half2_of_codes(u & 0xffffU);
-                                const uint32_t a1 = half2_of_codes(u >> 16);
-                                const uint32_t a2 = half2_of_codes(v & 0xffffU);
-                                const uint32_t a3 = half2_of_codes(v >> 16);
+                                uint32_t a0, a1, a2, a3;
+                                halves_of_codes(u, a0, a1);
+                                halves_of_codes(v, a2, a3);
 #pragma unroll
                                 for (int nb = 0; nb < NB; ++nb)
                                 {
@@ -573,8 +621,9 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                             {
                                 const uint32_t u = __byte_perm(r[2 * x], 0, 0x3120);
                                 const uint32_t v = __byte_perm(r[2 * x + 1], 0, 0x3120);
-                                uint32_t h[4] = {half2_of_codes(u & 0xffffU), half2_of_codes(u >> 16),
-                                                 half2_of_codes(v & 0xffffU), half2_of_codes(v >> 16)};
+                                uint32_t h[4];
+                                halves_of_codes(u, h[0], h[1]);
+                                halves_of_codes(v, h[2], h[3]);
                                 uint32_t is[4];
 #pragma unroll
                                 for (int y = 0; y < 4; ++y)
@@ -699,7 +748,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
             }
             if (at == it.begin && !whole && threadIdx.x == 0)
             {
-                // the block of the item's last tile: blocks begin at floor(c * total / blocks)
+                // the block of the item's last unit: blocks begin at floor(c * total / blocks)
                 a.joins[blockIdx.x] = make_int4(it.first_token, it.head, it.column0, it.columns);
                 a.join_end[blockIdx.x] = static_cast<int>(((it.end * blocks) - 1) / total);
             }
@@ -714,7 +763,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
         it.column0 += COLS;
         if constexpr (SELECTED)
         {
-            it.end += list_tiles;
+            it.end += list_units;
             if (it.column0 >= it.columns)
             {
                 it.column0 = 0;
@@ -735,14 +784,14 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     it.head = 0;
                     do
                     {
-                        ++it.request; // requests without tokens have no tiles; `at` < total, so one follows
+                        ++it.request; // requests without tokens have no units; `at` < total, so one follows
                         q = request_of(a.b, it.request);
                     } while (q.count == 0);
                     it.first_token = q.first;
                     it.columns = q.count * a.group;
                 }
             }
-            it.end = it.begin + tiles_of_block<COLS>(a, q, it.column0);
+            it.end = it.begin + units_of_block<COLS>(a, q, it.column0);
         }
     }
 }
@@ -750,47 +799,79 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
 // Joins the parts of items that several blocks worked on: block c looks after the item that begins
 // in block c of the main kernel and ends in a later one, whose parts are part 1 of block c and
 // part 0 of the blocks up to its last.  Always in that order, so results do not depend on timing.
+// One warp per column; launched while the main kernel still runs (griddepcontrol), so that its
+// own launch takes no time.
 template <int DIM, int COLS>
-__global__ void __launch_bounds__(THREADS) cache_join_kernel(const attend_args a)
+__global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
 {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 join = a.joins[blockIdx.x];
-    const int columns = min(COLS, join.w - join.z);
-    if (columns <= 0)
+    const int col = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (col >= join.w - join.z)
     {
         return;
     }
     const int64_t first = 2 * static_cast<int64_t>(blockIdx.x) + 1;
-    const int more = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x);
-    for (int e = blockIdx.y * THREADS + threadIdx.x; e < columns * DIM; e += gridDim.y * THREADS)
+    const int parts = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x) + 1;
+    auto part = [&](int i) { return (first + (i == 0 ? 0 : 2 * i - 1)) * COLS + col; };
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32)
     {
-        const int col = e / DIM;
-        const int d = e % DIM;
-        auto part = [&](int i) { return first + (i == 0 ? 0 : 2 * i - 1); };
-        float top = -INFINITY;
-        for (int i = 0; i <= more; ++i)
+        top = fmaxf(top, a.part_ml[part(i)].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+    }
+    constexpr int PER = DIM / 32;
+    float sum[PER];
+#pragma unroll
+    for (int x = 0; x < PER; ++x)
+    {
+        sum[x] = 0.0F;
+    }
+    float den = 0.0F;
+    for (int base = 0; base < parts; base += 32)
+    {
+        float keep = 0.0F;
+        if (base + lane < parts)
         {
-            top = fmaxf(top, a.part_ml[part(i) * COLS + col].x);
-        }
-        float sum = 0.0F;
-        float den = 0.0F;
-#pragma unroll 4
-        for (int i = 0; i <= more; ++i)
-        {
-            const float2 ml = a.part_ml[part(i) * COLS + col];
-            const float keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
-            sum = fmaf(keep, a.part_o[(part(i) * COLS + col) * DIM + d], sum);
+            const float2 ml = a.part_ml[part(base + lane)];
+            keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
             den = fmaf(keep, ml.y, den);
         }
-        const int g = join.z + col;
-        const int64_t token = join.x + g / a.group;
-        const int qhead = join.y * a.group + g % a.group;
-        store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + d, den == 0.0F ? 0.0F : sum / den,
-                  a.dtype);
-        if (d == 0 && a.lse != nullptr)
+        const int here = min(parts - base, 32);
+#pragma unroll 4
+        for (int i = 0; i < here; ++i)
         {
-            a.lse[token * a.group * a.c.heads + qhead] =
-                den == 0.0F ? -INFINITY : (top - WEIGHT_BIAS + log2f(den)) * LN_2;
+            const float f = __shfl_sync(FULL_MASK, keep, i);
+            const float* from = a.part_o + part(base + i) * DIM + lane;
+#pragma unroll
+            for (int x = 0; x < PER; ++x)
+            {
+                sum[x] = fmaf(f, from[x * 32], sum[x]);
+            }
         }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        den += __shfl_xor_sync(FULL_MASK, den, o);
+    }
+    const int g = join.z + col;
+    const int64_t token = join.x + g / a.group;
+    const int qhead = join.y * a.group + g % a.group;
+#pragma unroll
+    for (int x = 0; x < PER; ++x)
+    {
+        store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + x * 32 + lane,
+                  den == 0.0F ? 0.0F : sum[x] / den, a.dtype);
+    }
+    if (lane == 0 && a.lse != nullptr)
+    {
+        a.lse[token * a.group * a.c.heads + qhead] = den == 0.0F ? -INFINITY : (top - WEIGHT_BIAS + log2f(den)) * LN_2;
     }
 }
 
@@ -821,14 +902,27 @@ int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaSt
     a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(blocks) * 2 * smem::COLS);
     a.join_end = reinterpret_cast<int*>(a.part_o + static_cast<size_t>(blocks) * 2 * smem::COLS * DIM);
     auto kernel = cache_attend_kernel<DIM, NB, SELECTED>;
-    BITSKNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem::BYTES));
+    static cache::device_set prepared;
+    if (!prepared.contains_current())
+    {
+        BITSKNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem::BYTES));
+        prepared.add_current();
+    }
     {
         kernel_scope scope("cache_attend_kernel", stream);
         kernel<<<blocks, THREADS, smem::BYTES, stream>>>(a);
     }
     BITSKNN_CUDA_TRY(cudaGetLastError());
-    cache_join_kernel<DIM, smem::COLS><<<dim3(blocks, 4), THREADS, 0, stream>>>(a);
-    BITSKNN_CUDA_TRY(cudaGetLastError());
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks, NB);
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    BITSKNN_CUDA_TRY(cudaLaunchKernelEx(&config, cache_join_kernel<DIM, smem::COLS>, a));
     return BITSKNN_OK;
 }
 

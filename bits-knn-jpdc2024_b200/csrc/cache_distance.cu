@@ -39,7 +39,7 @@ __device__ __forceinline__ float max_nan(float a, float b)
 template <int DIM, int NB>
 struct distance_smem
 {
-    static constexpr int STAGE = SUB * PITCH<DIM> + SUB * 4;
+    static constexpr int STAGE = SUB * PITCH<DIM> + 16; // rows and their scale
     static constexpr int SCRATCH = 8 * NB * (SUB + 1) * 4;
     static constexpr int IMAGE = NB * 16 * DIM; // 8 NB columns of DIM halves
     static constexpr int BYTES = IMAGE + 8 * NB * 4 + WARPS * (DIST_STAGES * STAGE + SCRATCH);
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
         const request q = request_of(a.b, r);
         const int many = max(static_cast<int>(min(token_end, static_cast<int64_t>(q.first) + q.count)) - token, 1);
         const int furthest = min(visible_of(a.b, q, token + many - 1 - q.first), a.n);
+        const int64_t nearest = static_cast<int64_t>(q.length) - q.count + (token - q.first) + 1; // token i sees i more
         const int32_t* table = a.b.table + r * a.b.table_ld;
         const int columns = many * a.group;
         // blocks of columns: one, unless a head has more query heads than a block has columns
@@ -103,6 +104,13 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                 }
             }
             __syncthreads();
+            float factor[NB][2]; // of this thread's columns
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+            {
+                factor[nb][0] = undo[nb * 8 + (lane & 3) * 2];
+                factor[nb][1] = undo[nb * 8 + (lane & 3) * 2 + 1];
+            }
             const int first = begin / SUB + warp;
             const int count = end > first * SUB ? ((end - 1) / SUB - first) / WARPS + 1 : 0;
             const int loaded = furthest > first * SUB ? min(count, ((furthest - 1) / SUB - first) / WARPS + 1) : 0;
@@ -121,19 +129,33 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                     const uint32_t dst = ptx::smem_addr(mine + (j % DIST_STAGES) * smem::STAGE);
                     const int safe = max(page, 0);
                     const uint8_t* src = a.c.keys + safe * a.c.page_stride +
-                                         ((static_cast<int64_t>(head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
+                                         ((static_cast<int64_t>(head) << a.c.page_shift) + (pos & rows_mask)) * DIM +
+                                         lane * 16;
+                    // a subtile lies within one page: its rows are contiguous and share a scale
                     constexpr int PARTS = DIM / 16;
+                    if (there == SUB)
+                    {
 #pragma unroll
-                    for (int x = 0; x < DIM / 32; ++x)
-                    {
-                        const int e = lane + x * 32;
-                        const int row = e / PARTS;
-                        copy16(dst + row * PITCH<DIM> + (e % PARTS) * 16, src + e * 16, row < there ? 16U : 0U);
+                        for (int x = 0; x < DIM / 32; ++x)
+                        {
+                            const int e = lane + x * 32;
+                            copy16(dst + e / PARTS * PITCH<DIM> + (e % PARTS) * 16, src + x * 512);
+                        }
                     }
-                    if (lane < SUB)
+                    else
                     {
-                        copy4(dst + SUB * PITCH<DIM> + lane * 4,
-                              a.c.key_scales + static_cast<int64_t>(safe) * a.c.heads + head, lane < there ? 4U : 0U);
+#pragma unroll
+                        for (int x = 0; x < DIM / 32; ++x)
+                        {
+                            const int e = lane + x * 32;
+                            const int row = e / PARTS;
+                            copy16(dst + row * PITCH<DIM> + (e % PARTS) * 16, src + x * 512, row < there ? 16U : 0U);
+                        }
+                    }
+                    if (lane == 0)
+                    {
+                        copy4(dst + SUB * PITCH<DIM>, a.c.key_scales + static_cast<int64_t>(safe) * a.c.heads + head,
+                              page < 0 ? 0U : 4U);
                     }
                 }
                 copy_commit();
@@ -143,57 +165,74 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
             {
                 issue(j);
             }
+            const int row = lane & (SUB - 1);
+            const int half = lane >> 4;
+            const int cols = min(columns - col0, 8 * NB);
+            float* const only = a.dist + (static_cast<int64_t>(token) * a.c.heads + head) * a.ld;
             for (int j = 0; j < count; ++j)
             {
                 const int pos = (first + j * WARPS) * SUB;
                 copy_wait<DIST_STAGES - 2>();
                 __syncwarp();
+                float ks = 0.0F; // that of an absent page was copied as zero
                 if (j < loaded)
                 {
                     const unsigned char* stage = mine + (j % DIST_STAGES) * smem::STAGE;
+                    ks = *reinterpret_cast<const float*>(stage + SUB * PITCH<DIM>);
                     float s[NB][4];
                     score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
-                    const int row = row_order(lane >> 2);
-                    const int c = (lane & 3) * 2;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
-                        float* out = scratch + (nb * 8 + c) * (SUB + 1) + row;
-                        out[0] = s[nb][0] * undo[nb * 8 + c];
-                        out[SUB + 1] = s[nb][1] * undo[nb * 8 + c + 1];
-                        out[8] = s[nb][2] * undo[nb * 8 + c];
-                        out[SUB + 1 + 8] = s[nb][3] * undo[nb * 8 + c + 1];
+                        float* out = scratch + (nb * 8 + (lane & 3) * 2) * (SUB + 1) + row_order(lane >> 2);
+                        out[0] = s[nb][0] * factor[nb][0];
+                        out[SUB + 1] = s[nb][1] * factor[nb][1];
+                        out[8] = s[nb][2] * factor[nb][0];
+                        out[SUB + 1 + 8] = s[nb][3] * factor[nb][1];
                     }
                 }
                 __syncwarp();
-                const int row = lane & (SUB - 1);
-                // the scale of an absent position was copied as zero
-                const float ks = j < loaded ? reinterpret_cast<const float*>(mine + (j % DIST_STAGES) * smem::STAGE +
-                                                                             SUB * PITCH<DIM>)[row]
-                                            : 0.0F;
-                const int last = (min(columns, col0 + 8 * NB) - 1) / a.group;
-                for (int i = col0 / a.group + (lane >> 4); i <= last; i += 2)
+                if (many == 1)
                 {
-                    const int g0 = max(i * a.group, col0);
-                    const int g1 = min((i + 1) * a.group, min(columns, col0 + 8 * NB));
-                    float d = INFINITY;
-                    if (j < loaded && ks != 0.0F && pos + row < visible_of(a.b, q, token + i - q.first))
+                    // all columns are one token's: the two halves of the warp share them
+                    float best = half < cols ? scratch[half * (SUB + 1) + row] : -INFINITY;
+#pragma unroll 4
+                    for (int g = half + 2; g < cols; g += 2)
                     {
-                        float best = scratch[(g0 - col0) * (SUB + 1) + row];
+                        best = max_nan(best, scratch[g * (SUB + 1) + row]);
+                    }
+                    best = max_nan(best, __shfl_xor_sync(FULL_MASK, best, 16));
+                    float d = ks != 0.0F && pos + row < furthest ? -(best * ks) : INFINITY;
+                    if (half == 0 && pos + row < end)
+                    {
+                        if (col0 > 0) // the head's first columns were in an earlier block
+                        {
+                            d = -max_nan(-d, -only[pos + row]);
+                        }
+                        only[pos + row] = d;
+                    }
+                }
+                else
+                {
+                    for (int i = col0 / a.group + half; i * a.group < col0 + cols; i += 2)
+                    {
+                        const int g0 = max(i * a.group, col0) - col0;
+                        const int g1 = min((i + 1) * a.group - col0, cols);
+                        float best = scratch[g0 * (SUB + 1) + row];
                         for (int g = g0 + 1; g < g1; ++g)
                         {
-                            best = max_nan(best, scratch[(g - col0) * (SUB + 1) + row]);
+                            best = max_nan(best, scratch[g * (SUB + 1) + row]);
                         }
-                        d = -(best * ks);
-                    }
-                    if (pos + row < end)
-                    {
-                        float* out = a.dist + (static_cast<int64_t>(token + i) * a.c.heads + head) * a.ld + pos + row;
-                        if (g0 != i * a.group) // the head's first columns were in an earlier block
+                        float d = ks != 0.0F && pos + row < nearest + i ? -(best * ks) : INFINITY;
+                        if (pos + row < end)
                         {
-                            d = -max_nan(-d, -*out);
+                            float* out = only + static_cast<int64_t>(i) * a.c.heads * a.ld + pos + row;
+                            if (g0 + col0 != i * a.group)
+                            {
+                                d = -max_nan(-d, -*out);
+                            }
+                            *out = d;
                         }
-                        *out = d;
                     }
                 }
                 __syncwarp();
@@ -210,7 +249,13 @@ int launch_distance(const distance_args& a, int64_t blocks, cudaStream_t stream)
 {
     constexpr int bytes = distance_smem<DIM, NB>::BYTES;
     static_assert(bytes <= 227 * 1024, "shared memory");
-    BITSKNN_CUDA_TRY(cudaFuncSetAttribute(cache_distance_kernel<DIM, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    static cache::device_set prepared;
+    if (!prepared.contains_current())
+    {
+        BITSKNN_CUDA_TRY(
+            cudaFuncSetAttribute(cache_distance_kernel<DIM, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        prepared.add_current();
+    }
     {
         kernel_scope scope("cache_distance_kernel", stream);
         cache_distance_kernel<DIM, NB><<<static_cast<unsigned>(blocks), THREADS, bytes, stream>>>(a);

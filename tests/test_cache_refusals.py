@@ -149,6 +149,6 @@ def test_python_layer_refuses_tensors_that_do_not_fit(bk):
     with pytest.raises(ValueError, match="CUDA tensor"):
         bk.Cache(codes, codes, torch.zeros(2, 1), torch.zeros(2, 1))
     with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
-        bk._vectors(torch.zeros(1, 1, 32, dtype=torch.int32), "queries", 1, 32)
+        bk._vectors(torch.zeros(1, 1, 32, dtype=torch.int32), "queries")
     with pytest.raises(ValueError, match="CUDA tensor"):
         bk.cache_plan(torch.zeros(1, dtype=torch.int32), None, None, None, 16, 1)
