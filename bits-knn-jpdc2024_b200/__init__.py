@@ -35,20 +35,20 @@ _ptr = ctypes.c_void_p
 _sz = ctypes.c_size_t
 
 
-class _CacheStruct(ctypes.Structure):
+class CacheStruct(ctypes.Structure):
     """bitsknn_cache_t"""
     _fields_ = [("d_keys", _ptr), ("d_values", _ptr), ("d_key_scales", _ptr), ("d_value_scales", _ptr), ("pages", _i64),
                 ("page_stride", _i64), ("heads", ctypes.c_int32), ("page_rows", ctypes.c_int32), ("dim", ctypes.c_int32)]
 
 
-class _BatchStruct(ctypes.Structure):
+class BatchStruct(ctypes.Structure):
     """bitsknn_cache_batch_t"""
     _fields_ = [("d_table", _ptr), ("table_ld", _i64), ("table_pages", _i64), ("d_lengths", _ptr), ("d_starts", _ptr),
                 ("requests", _i64), ("tokens", _i64)]
 
 
-_cache_p = ctypes.POINTER(_CacheStruct)
-_batch_p = ctypes.POINTER(_BatchStruct)
+_cache_p = ctypes.POINTER(CacheStruct)
+_batch_p = ctypes.POINTER(BatchStruct)
 SIGNATURES = {
     "bitsknn_version": (_int, []),
     "bitsknn_last_error_string": (ctypes.c_char_p, []),
@@ -361,200 +361,6 @@ def fused(points, queries, k, mode=L2_PARTIAL, index_base=0, out=None, workspace
     return out
 
 
-# ---- search in a paged cache of keys and values held in 8 bits ---------------------------------
-class Cache:
-    """Keys and values as e4m3 codes in pages: uint8 (pages, heads, page_rows, dim) CUDA tensors and float32
-    (pages, heads) scales.  Holds the tensors; pages may lie apart (stride of the first dimension)."""
-
-    def __init__(self, keys, values, key_scales, value_scales):
-        import torch
-        for t, name in ((keys, "keys"), (values, "values")):
-            _device_check(t, torch.uint8, name)
-        for t, name in ((key_scales, "key_scales"), (value_scales, "value_scales")):
-            _device_check(t, torch.float32, name)
-        if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
-            raise ValueError("keys and values must be (pages, heads, page_rows, dim) tensors of the same strides")
-        pages, heads, rows, dim = keys.shape
-        if keys.stride()[1:] != (rows * dim, dim, 1):
-            raise ValueError("a page must be contiguous")
-        if any(tuple(s.shape) != (pages, heads) or not s.is_contiguous() for s in (key_scales, value_scales)):
-            raise ValueError("scales must be contiguous (pages, heads) tensors")
-        if any(t.device != keys.device for t in (values, key_scales, value_scales)):
-            raise ValueError("the cache's tensors must be on one device")
-        self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
-        self.pages, self.heads, self.page_rows, self.dim = pages, heads, rows, dim
-        self.device = keys.device
-        stride = keys.stride(0) if pages > 1 else heads * rows * dim
-        self.struct = _CacheStruct(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-                                   pages, stride, heads, rows, dim)
-
-    @classmethod
-    def empty(cls, pages, heads, page_rows, dim, device="cuda"):
-        """A cache without content; its pages are to be appended to from their first row."""
-        import torch
-        shape = (pages, heads, page_rows, dim)
-        codes = [torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2)]
-        scales = [torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)]
-        return cls(*codes, *scales)
-
-    def batch(self, queries, lengths, table, starts):
-        """(bitsknn_cache_batch_t, dtype code, elements between tokens) of a call's arguments.  These wrappers run once
-        per layer and step: they look at every argument once and keep nothing between calls."""
-        import torch
-        if queries.dim() != 3 or queries.shape[2] != self.dim:
-            raise ValueError(f"queries have shape {tuple(queries.shape)}, which does not fit the cache")
-        code, stride = _vectors(queries, "queries")
-        if lengths.dtype is not torch.int32 or table.dtype is not torch.int32:
-            raise ValueError("lengths and table must be torch.int32")
-        tokens, (requests, pages), (ld, inner) = queries.shape[0], table.shape, table.stride()
-        if lengths.shape != (requests,) or (inner != 1 and pages > 1) or (requests > 1 and lengths.stride(0) != 1):
-            raise ValueError("table must be (requests, pages) and lengths (requests,), contiguous in the last dimension")
-        if starts is not None and (starts.dtype is not torch.int32 or starts.shape != (requests + 1,)
-                                   or (requests > 0 and starts.stride(0) != 1)):
-            raise ValueError("starts must be a contiguous (requests + 1,) torch.int32 tensor")
-        _on_device(self.device, queries, lengths, table, starts)
-        return _BatchStruct(table.data_ptr(), ld if requests > 1 else pages, pages, lengths.data_ptr(),
-                            None if starts is None else starts.data_ptr(), requests, tokens), code, stride
-
-
-def _on_device(device, *tensors):
-    import torch
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {device}, which is not the current device")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device} (the library has no CPU path)")
-
-
-def _vectors(t, name):
-    """(dtype code, elements between tokens) of a (tokens, heads, dim) tensor of vectors."""
-    import torch
-    dtype = t.dtype
-    code = BF16 if dtype is torch.bfloat16 else F16 if dtype is torch.float16 else F32 if dtype is torch.float32 else None
-    if code is None:
-        raise ValueError(f"{name} must be float32, float16 or bfloat16")
-    tokens, heads, dim = t.shape
-    outer, middle, inner = t.stride()
-    if inner != 1 or (heads > 1 and middle != dim):
-        raise ValueError(f"{name} must be contiguous in its last two dimensions")
-    return code, outer if tokens > 1 else heads * dim
-
-
-def cache_plan(lengths, new, free_pages, table, page_rows, max_tokens, out=None):
-    """Places for `new` tokens of every request: writes the new pages into `table` and returns
-    (starts, new_lengths, slots, counts); counts = (tokens, pages taken, tokens without a place)."""
-    import torch
-    int32, device = torch.int32, lengths.device
-    for t, name in ((lengths, "lengths"), (new, "new"), (free_pages, "free_pages"), (table, "table")):
-        if not t.is_cuda or t.dtype is not int32:
-            raise ValueError(f"{name} must be a torch.int32 CUDA tensor (the library has no CPU path)")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{name} must be contiguous in its last dimension")
-    _on_device(device, new, free_pages, table)
-    requests, pages = table.shape
-    if lengths.shape != (requests,) or new.shape != (requests,) or free_pages.dim() != 1:
-        raise ValueError("lengths and new must be (requests,), table (requests, pages)")
-    if out is None:
-        out = (torch.empty(requests + 1, dtype=int32, device=device), torch.empty(requests, dtype=int32, device=device),
-               torch.empty(max_tokens, dtype=torch.int64, device=device), torch.empty(3, dtype=int32, device=device))
-    _check(lib().bitsknn_cache_plan(lengths.data_ptr(), new.data_ptr(), requests, page_rows, free_pages.data_ptr(),
-                                    free_pages.shape[0], table.data_ptr(), table.stride(0) if requests > 1 else pages, pages,
-                                    out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), max_tokens,
-                                    out[3].data_ptr(), _stream()))
-    return out
-
-
-def cache_append(cache, keys, values, slots):
-    """Quantises (tokens, heads, dim) keys and values into the cache at `slots` (int64, from cache_plan)."""
-    import torch
-    shape = keys.shape
-    if values.shape != shape or len(shape) != 3 or shape[1] != cache.heads or shape[2] != cache.dim:
-        raise ValueError(f"keys {tuple(shape)} and values {tuple(values.shape)} do not fit the cache")
-    code, key_stride = _vectors(keys, "keys")
-    value_code, value_stride = _vectors(values, "values")
-    tokens = shape[0]
-    if value_code != code or slots.dtype is not torch.int64 or slots.dim() != 1 or slots.shape[0] < tokens:
-        raise ValueError("keys and values must agree in type, and every token needs an int64 slot")
-    if tokens > 1 and slots.stride(0) != 1:
-        raise ValueError("slots must be contiguous in its last dimension")
-    _on_device(cache.device, keys, values, slots)
-    _check(lib().bitsknn_cache_append(cache.struct, keys.data_ptr(), values.data_ptr(), code, key_stride, value_stride,
-                                      slots.data_ptr(), tokens, _stream()))
-
-
-def cache_distance(cache, queries, lengths, table, n, starts=None, out=None):
-    """(tokens * heads, n) float32 distances for `select`: minus the largest inner product over a head's queries."""
-    import torch
-    batch, code, stride = cache.batch(queries, lengths, table, starts)
-    rows = queries.shape[0] * cache.heads
-    if out is None:
-        out = torch.empty((rows, n), dtype=torch.float32, device=cache.device)
-    else:
-        _device_check(out, torch.float32, "out")
-        _on_device(cache.device, out)
-        if out.dim() != 2 or out.shape[0] < rows or out.shape[1] < n:
-            raise ValueError("out must have tokens * heads rows of n distances")
-    _check(lib().bitsknn_cache_distance(cache.struct, batch, queries.data_ptr(), code, stride, queries.shape[1],
-                                        out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1], n, _stream()))
-    return out
-
-
-def cache_attend_workspace_bytes(cache, query_heads):
-    return int(lib().bitsknn_cache_attend_workspace_bytes(cache.struct, query_heads))
-
-
-def _attend_buffers(cache, queries, out, lse, workspace):
-    import torch
-    shape, device = queries.shape, cache.device
-    stride = 0
-    if out is None:
-        out = torch.empty(shape, dtype=queries.dtype, device=device)
-    elif out.shape != shape or out.dtype is not queries.dtype:
-        raise ValueError("out must have the queries' shape and type")
-    else:
-        _on_device(device, out)
-        stride = _vectors(out, "out")[1]
-    if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=device)
-    elif lse.shape != shape[:2] or lse.dtype is not torch.float32 or not lse.is_contiguous():
-        raise ValueError("lse must be a contiguous (tokens, query_heads) float32 tensor")
-    else:
-        _on_device(device, lse)
-    if workspace is None:
-        workspace = torch.empty(cache_attend_workspace_bytes(cache, shape[1]), dtype=torch.uint8, device=device)
-    elif workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous():
-        raise ValueError("workspace must be a contiguous uint8 tensor on the cache's device")
-    return out, stride, lse, workspace
-
-
-def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
-    """Attention of (tokens, query_heads, dim) queries over everything cached: (out, lse)."""
-    batch, code, stride = cache.batch(queries, lengths, table, starts)
-    out, out_stride, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
-    _check(lib().bitsknn_cache_attend(cache.struct, batch, queries.data_ptr(), code, stride, queries.shape[1], scale,
-                                      out.data_ptr(), out_stride, lse.data_ptr(), workspace.data_ptr(),
-                                      workspace.numel(), _stream()))
-    return out, lse
-
-
-def cache_attend_selected(cache, queries, idx, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
-    """Attention over listed positions: idx (tokens * heads, k) int32, as `select` returns them.  (out, lse)."""
-    import torch
-    batch, code, stride = cache.batch(queries, lengths, table, starts)
-    if idx.dim() != 2 or idx.shape[0] != queries.shape[0] * cache.heads:
-        raise ValueError("idx must be (tokens * heads, k)")
-    rows, k = idx.shape
-    if idx.dtype is not torch.int32 or (k > 1 and idx.stride(1) != 1):
-        raise ValueError("idx must be torch.int32, contiguous in its last dimension")
-    _on_device(cache.device, idx)
-    out, out_stride, lse, workspace = _attend_buffers(cache, queries, out, lse, workspace)
-    _check(lib().bitsknn_cache_attend_selected(cache.struct, batch, queries.data_ptr(), code, stride, queries.shape[1],
-                                               idx.data_ptr(), idx.stride(0) if rows > 1 else k, k, scale, out.data_ptr(),
-                                               out_stride, lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                                               _stream()))
-    return out, lse
-
-
 # ---- database-sharded search (one handle per GPU; NCCL inside the library) --------------------
 def sharded_unique_id():
     """An NCCL unique id (bytes) made on the calling rank; distribute it to the other ranks."""
@@ -620,3 +426,17 @@ def sharded_fused(handle, points, queries, k, shard_begin, workspace, mode=L2_PA
 
 def sharded_drain(handle):
     _check(lib().bitsknn_sharded_drain(handle, _stream()))
+
+
+# ---- search in a paged cache of keys and values held in 8 bits: cache.py, loaded when first used ----
+_CACHE_NAMES = ("Cache", "cache_plan", "cache_append", "cache_distance", "cache_attend_workspace_bytes", "cache_attend",
+                "cache_attend_selected")
+
+
+def __getattr__(name):
+    if name not in _CACHE_NAMES:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import cache as module
+    for n in _CACHE_NAMES:
+        globals()[n] = getattr(module, n)
+    return globals()[name]

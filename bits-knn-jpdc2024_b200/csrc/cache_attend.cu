@@ -826,6 +826,11 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
         top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
     }
     constexpr int PER = DIM / 32;
+    constexpr int VEC = PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1; // numbers per load
+    struct alignas(4 * VEC) vec
+    {
+        float v[VEC];
+    };
     float sum[PER];
 #pragma unroll
     for (int x = 0; x < PER; ++x)
@@ -843,15 +848,20 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
             den = fmaf(keep, ml.y, den);
         }
         const int here = min(parts - base, 32);
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < here; ++i)
         {
             const float f = __shfl_sync(FULL_MASK, keep, i);
-            const float* from = a.part_o + part(base + i) * DIM + lane;
+            const vec* from = reinterpret_cast<const vec*>(a.part_o + part(base + i) * DIM) + lane;
 #pragma unroll
-            for (int x = 0; x < PER; ++x)
+            for (int x = 0; x < PER / VEC; ++x)
             {
-                sum[x] = fmaf(f, from[x * 32], sum[x]);
+                const vec w = from[x * 32];
+#pragma unroll
+                for (int y = 0; y < VEC; ++y)
+                {
+                    sum[x * VEC + y] = fmaf(f, w.v[y], sum[x * VEC + y]);
+                }
             }
         }
     }
@@ -866,7 +876,8 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
 #pragma unroll
     for (int x = 0; x < PER; ++x)
     {
-        store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + x * 32 + lane,
+        const int d = (x / VEC * 32 + lane) * VEC + x % VEC;
+        store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + d,
                   den == 0.0F ? 0.0F : sum[x] / den, a.dtype);
     }
     if (lane == 0 && a.lse != nullptr)

@@ -10,13 +10,13 @@ def cache_struct(bk, **over):
     fields = dict(d_keys=FAKE, d_values=FAKE, d_key_scales=FAKE, d_value_scales=FAKE, pages=4, page_stride=0, heads=2,
                   page_rows=16, dim=64)
     fields.update(over)
-    return bk._CacheStruct(*(fields[name] for name, _ in bk._CacheStruct._fields_))
+    return bk.CacheStruct(*(fields[name] for name, _ in bk.CacheStruct._fields_))
 
 
 def batch_struct(bk, **over):
     fields = dict(d_table=FAKE, table_ld=4, table_pages=4, d_lengths=FAKE, d_starts=None, requests=3, tokens=3)
     fields.update(over)
-    return bk._BatchStruct(*(fields[name] for name, _ in bk._BatchStruct._fields_))
+    return bk.BatchStruct(*(fields[name] for name, _ in bk.BatchStruct._fields_))
 
 
 def attend(bk, cache=None, batch=None, queries=FAKE, dtype=None, stride=0, query_heads=4, out=FAKE, out_stride=0,
@@ -148,7 +148,5 @@ def test_python_layer_refuses_tensors_that_do_not_fit(bk):
     codes = torch.zeros((2, 1, 16, 32), dtype=torch.uint8)
     with pytest.raises(ValueError, match="CUDA tensor"):
         bk.Cache(codes, codes, torch.zeros(2, 1), torch.zeros(2, 1))
-    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
-        bk._vectors(torch.zeros(1, 1, 32, dtype=torch.int32), "queries")
     with pytest.raises(ValueError, match="CUDA tensor"):
         bk.cache_plan(torch.zeros(1, dtype=torch.int32), None, None, None, 16, 1)
