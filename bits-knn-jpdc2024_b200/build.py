@@ -21,7 +21,8 @@ OBJ_DIR = LIB_DIR / "obj"
 LIB = LIB_DIR / "libbitsknn.so"
 
 SOURCES = ["abi.cu", "select.cu", "ablation.cu", "merge.cu", "sharded.cu", "l2.cu", "l2_tc.cu", "fused.cu", "fused_tiled.cu", "fused_tc.cu",
-           "cache_plan.cu", "cache_append.cu", "cache_distance.cu", "cache_attend.cu"]
+           "cache_plan.cu", "cache_append.cu", "cache_distance.cu", "cache_attend.cu",
+           "cache_attend_tc.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

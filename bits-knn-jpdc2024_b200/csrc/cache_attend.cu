@@ -1,17 +1,8 @@
 // cache_attend, cache_attend_selected: attention over a paged 8-bit cache, over all positions a token
 // sees or over a list of them.
-//
-// Mathematics.  For a query column with logits (base 2) t_j = scale * log2(e) * <q, code_j> * ks_j,
-// the weights are w_j = 2^(t_j + log2(vs_j) - m): the value scale rides on the logit, so that the
-// second product multiplies weights with bare codes, and m is the running maximum of t_j + log2(vs_j).
-// The denominator sums w_j / vs_j = 2^(t_j - m), in the same units, so out = sum w_j code_j / sum w_j / vs_j
-// needs no scale at all.  One pass: when m grows, what was summed is multiplied by 2^(m_old - m_new).
-// Logits, maxima and sums are FP32.  Weights are rounded to halves (11 bits, the codes are exact
-// halves): the reference point m is kept 7 binary orders below the half range's 2^7 ... 2^15, so a
-// weight of 2^-31 of the largest is still not lost, which 10^5 positions of little weight need.
 #include <algorithm>
 
-#include "cache.cuh"
+#include "cache_attend.cuh"
 
 namespace bitsknn
 {
@@ -19,50 +10,12 @@ namespace bitsknn
 namespace
 {
 
-using namespace cache;
-
-constexpr float WEIGHT_BIAS = 7.0F;  // the weight of the reference point is 2^7
-constexpr float WEIGHT_SLACK = 8.0F; // a logit may pass the reference point by 8 (weight 2^15) before it moves
-constexpr float LOG2_E = 1.4426950408889634F;
-constexpr float LN_2 = 0.6931471805599453F;
-
-struct attend_args
-{
-    view c;
-    batch b;
-    const void* queries;
-    int dtype;
-    int64_t query_stride;
-    int group;
-    float scale;      // times log2(e)
-    void* out;
-    int64_t out_stride;
-    float* lse;
-    const int32_t* idx; // selected: lists
-    int64_t ld_idx;
-    int k;
-    float* part_o;    // [2 * blocks][columns][DIM]
-    float2* part_ml;  // [2 * blocks][columns]
-    int4* joins;      // [blocks]
-    int* join_end;    // [blocks]
-};
-
-// What the stream of a block works on: one block of query columns of a request and head.
-struct item
-{
-    int request;
-    int first_token; // packed token of column 0 of the request (selected: the token)
-    int head;
-    int column0;
-    int columns;     // columns of the request (selected: of the token) in total
-    int64_t begin;   // where it lies on the axis of the work
-    int64_t end;
-};
-
 template <int DIM, int NB>
 struct attend_smem
 {
     static constexpr int COLS = 8 * NB;
+    static constexpr int ROWS = TILE;
+    static constexpr int COST = 3; // an item's beginning and end take about as long as three tiles
     static constexpr int SCALES = 2 * SUB * PITCH<DIM>; // offset of the scales in a stage
     static constexpr int STAGE = SCALES + 2 * SUB * 4;
     static constexpr int FIT = 18432 / STAGE;
@@ -76,118 +29,6 @@ struct attend_smem
     static_assert(BLOCKS >= 1, "shared memory");
     static_assert(WARPS * STAGES * STAGE >= WARPS * COLS * DIM * 4, "the stages hold the warps' sums at the end");
 };
-
-__device__ __forceinline__ void store_out(void* out, int64_t at, float v, int dtype)
-{
-    if (dtype == BITSKNN_F16)
-    {
-        static_cast<__half*>(out)[at] = __float2half_rn(v);
-    }
-    else
-    {
-        static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-    }
-}
-
-// ---- shares of the work ----------------------------------------------------------------------
-// All items lie on one axis: requests in order, within a request heads, within a head blocks of
-// columns.  An item covers ITEM_COST units for its beginning and end (packing the queries, filling
-// the pipeline, joining the warps: about as long as three tiles) and one unit for each of its tiles
-// of 64 positions.  Block c of the grid takes the c-th equal share of the axis, so a long request
-// is spread over many blocks and short ones fill up the others.
-constexpr int ITEM_COST = 3;
-
-template <int COLS>
-__device__ __forceinline__ int units_of_block(const attend_args& a, const request& q, int column0)
-{
-    const int last = min(column0 + COLS, q.count * a.group) - 1;
-    return (visible_of(a.b, q, last / a.group) + TILE - 1) / TILE + ITEM_COST;
-}
-
-template <int COLS>
-__device__ __forceinline__ int64_t units_of_head(const attend_args& a, const request& q)
-{
-    int64_t sum = 0;
-    for (int col = 0; col < q.count * a.group; col += COLS)
-    {
-        sum += units_of_block<COLS>(a, q, col);
-    }
-    return sum;
-}
-
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* words)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-    {
-        v += __shfl_xor_sync(FULL_MASK, v, o);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0)
-    {
-        words[threadIdx.x >> 5] = v;
-    }
-    __syncthreads();
-    int64_t sum = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-    {
-        sum += words[w];
-    }
-    return sum;
-}
-
-// The request that holds unit `at`, and the first unit of that request.
-template <int COLS>
-__device__ __forceinline__ int find_request(const attend_args& a, int64_t at, int64_t* first, int64_t* words, int* found)
-{
-    int64_t before = 0;
-    for (int base = 0; base < a.b.requests; base += THREADS)
-    {
-        const int r = base + threadIdx.x;
-        const int64_t mine = r < a.b.requests ? units_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads : 0;
-        int64_t upto = mine;
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-        {
-            const int64_t x = __shfl_up_sync(FULL_MASK, upto, o);
-            upto += lane >= o ? x : 0;
-        }
-        __syncthreads();
-        if (lane == 31)
-        {
-            words[threadIdx.x >> 5] = upto;
-        }
-        if (threadIdx.x == 0)
-        {
-            *found = -1;
-        }
-        __syncthreads();
-        int64_t all = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-        {
-            upto += w < static_cast<int>(threadIdx.x >> 5) ? words[w] : 0;
-            all += words[w];
-        }
-        const int64_t start = before + upto - mine;
-        __syncthreads();
-        if (at >= start && at < start + mine)
-        {
-            *found = r;
-            words[0] = start;
-        }
-        __syncthreads();
-        if (*found >= 0)
-        {
-            *first = words[0];
-            return *found;
-        }
-        before += all;
-    }
-    return -1; // not reached: `at` lies below the total
-}
 
 // ---- the kernel ------------------------------------------------------------------------------------
 // Four warps, each streaming its own 16-position subtiles (position tile * 64 + warp * 16)
@@ -222,7 +63,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
     const int row_lo = row_order(lane >> 2);  // its rows: row_lo, row_lo + 8
 
     // this block's share, and the item it begins in
-    const int list_units = SELECTED ? (a.k + TILE - 1) / TILE + ITEM_COST : 0;
+    const int list_units = SELECTED ? (a.k + TILE - 1) / TILE + smem::COST : 0;
     const int list_blocks = SELECTED ? (a.group + COLS - 1) / COLS : 0;
     int64_t total;
     if constexpr (SELECTED)
@@ -234,9 +75,9 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
         int64_t sum = 0;
         for (int r = threadIdx.x; r < a.b.requests; r += THREADS)
         {
-            sum += units_of_head<COLS>(a, request_of(a.b, r)) * a.c.heads;
+            sum += units_of_head<smem>(a, request_of(a.b, r)) * a.c.heads;
         }
-        total = block_sum(sum, s_words);
+        total = block_sum<WARPS>(sum, s_words);
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0)
@@ -264,19 +105,19 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
     else
     {
         int64_t first = 0;
-        it.request = find_request<COLS>(a, at, &first, s_words, &s_found);
+        it.request = find_request<smem, WARPS>(a, at, &first, s_words, &s_found);
         const request q = request_of(a.b, it.request);
-        const int64_t per_head = units_of_head<COLS>(a, q);
+        const int64_t per_head = units_of_head<smem>(a, q);
         it.head = static_cast<int>((at - first) / per_head);
         it.begin = first + it.head * per_head;
         it.first_token = q.first;
         it.columns = q.count * a.group;
-        it.end = it.begin + units_of_block<COLS>(a, q, 0);
+        it.end = it.begin + units_of_block<smem>(a, q, 0);
         while (at >= it.end)
         {
             it.column0 += COLS;
             it.begin = it.end;
-            it.end += units_of_block<COLS>(a, q, it.column0);
+            it.end += units_of_block<smem>(a, q, it.column0);
         }
     }
 
@@ -321,8 +162,8 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                 list = a.idx + (static_cast<int64_t>(it.first_token) * a.c.heads + it.head) * a.ld_idx;
             }
             // tiles of the share; none if it ends within the units of the item's beginning
-            const int first_tile = max(static_cast<int>(at - it.begin) - ITEM_COST, 0);
-            const int count = max(static_cast<int>(seg_end - it.begin) - ITEM_COST, 0) - first_tile;
+            const int first_tile = max(static_cast<int>(at - it.begin) - smem::COST, 0);
+            const int count = max(static_cast<int>(seg_end - it.begin) - smem::COST, 0) - first_tile;
             const int row_end = SELECTED ? a.k : furthest; // rows behind it are zero
             auto row_of = [&](int j) { return (first_tile + j) * TILE + warp * SUB; };
 
@@ -791,109 +632,19 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     it.columns = q.count * a.group;
                 }
             }
-            it.end = it.begin + units_of_block<COLS>(a, q, it.column0);
+            it.end = it.begin + units_of_block<smem>(a, q, it.column0);
         }
     }
 }
-
-// Joins the parts of items that several blocks worked on: block c looks after the item that begins
-// in block c of the main kernel and ends in a later one, whose parts are part 1 of block c and
-// part 0 of the blocks up to its last.  Always in that order, so results do not depend on timing.
-// One warp per column; launched while the main kernel still runs (griddepcontrol), so that its
-// own launch takes no time.
-template <int DIM, int COLS>
-__global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
-{
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 join = a.joins[blockIdx.x];
-    const int col = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (col >= join.w - join.z)
-    {
-        return;
-    }
-    const int64_t first = 2 * static_cast<int64_t>(blockIdx.x) + 1;
-    const int parts = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x) + 1;
-    auto part = [&](int i) { return (first + (i == 0 ? 0 : 2 * i - 1)) * COLS + col; };
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32)
-    {
-        top = fmaxf(top, a.part_ml[part(i)].x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-    {
-        top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
-    }
-    constexpr int PER = DIM / 32;
-    constexpr int VEC = PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1; // numbers per load
-    struct alignas(4 * VEC) vec
-    {
-        float v[VEC];
-    };
-    float sum[PER];
-#pragma unroll
-    for (int x = 0; x < PER; ++x)
-    {
-        sum[x] = 0.0F;
-    }
-    float den = 0.0F;
-    for (int base = 0; base < parts; base += 32)
-    {
-        float keep = 0.0F;
-        if (base + lane < parts)
-        {
-            const float2 ml = a.part_ml[part(base + lane)];
-            keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
-            den = fmaf(keep, ml.y, den);
-        }
-        const int here = min(parts - base, 32);
-#pragma unroll 8
-        for (int i = 0; i < here; ++i)
-        {
-            const float f = __shfl_sync(FULL_MASK, keep, i);
-            const vec* from = reinterpret_cast<const vec*>(a.part_o + part(base + i) * DIM) + lane;
-#pragma unroll
-            for (int x = 0; x < PER / VEC; ++x)
-            {
-                const vec w = from[x * 32];
-#pragma unroll
-                for (int y = 0; y < VEC; ++y)
-                {
-                    sum[x * VEC + y] = fmaf(f, w.v[y], sum[x * VEC + y]);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-    {
-        den += __shfl_xor_sync(FULL_MASK, den, o);
-    }
-    const int g = join.z + col;
-    const int64_t token = join.x + g / a.group;
-    const int qhead = join.y * a.group + g % a.group;
-#pragma unroll
-    for (int x = 0; x < PER; ++x)
-    {
-        const int d = (x / VEC * 32 + lane) * VEC + x % VEC;
-        store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + d,
-                  den == 0.0F ? 0.0F : sum[x] / den, a.dtype);
-    }
-    if (lane == 0 && a.lse != nullptr)
-    {
-        a.lse[token * a.group * a.c.heads + qhead] = den == 0.0F ? -INFINITY : (top - WEIGHT_BIAS + log2f(den)) * LN_2;
-    }
-}
-
-constexpr size_t JOIN_BYTES = sizeof(int4) + sizeof(int);
 
 template <int DIM, int NB>
-size_t workspace_of()
+int blocks_of()
 {
-    const size_t blocks = static_cast<size_t>(device_sm_count()) * attend_smem<DIM, NB>::BLOCKS;
-    return blocks * (2 * 8 * NB * (DIM * sizeof(float) + sizeof(float2)) + JOIN_BYTES) + 256;
+    return device_sm_count() * attend_smem<DIM, NB>::BLOCKS;
 }
+
+// From this many query columns per request and head on the tensor-memory kernel takes over.
+constexpr int TC_COLUMNS = 64;
 
 // Most columns a block can take: the sums of 8 NB columns take NB * DIM / 4 registers of a thread.
 constexpr int most_columns(int dim) { return dim <= 128 ? 4 : 2; }
@@ -902,16 +653,12 @@ template <int DIM, int NB, bool SELECTED>
 int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaStream_t stream)
 {
     using smem = attend_smem<DIM, NB>;
-    const int blocks = device_sm_count() * smem::BLOCKS;
-    if (workspace_bytes < workspace_of<DIM, NB>())
+    const int blocks = blocks_of<DIM, NB>();
+    const int rc = place_parts<DIM, smem::COLS>(a, blocks, workspace, workspace_bytes);
+    if (rc != BITSKNN_OK)
     {
-        return fail(BITSKNN_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes,
-                    workspace_of<DIM, NB>());
+        return rc;
     }
-    a.joins = static_cast<int4*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.joins + blocks);
-    a.part_o = reinterpret_cast<float*>(a.part_ml + static_cast<size_t>(blocks) * 2 * smem::COLS);
-    a.join_end = reinterpret_cast<int*>(a.part_o + static_cast<size_t>(blocks) * 2 * smem::COLS * DIM);
     auto kernel = cache_attend_kernel<DIM, NB, SELECTED>;
     static cache::device_set prepared;
     if (!prepared.contains_current())
@@ -924,17 +671,7 @@ int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaSt
         kernel<<<blocks, THREADS, smem::BYTES, stream>>>(a);
     }
     BITSKNN_CUDA_TRY(cudaGetLastError());
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(blocks, NB);
-    config.blockDim = dim3(256);
-    config.stream = stream;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    BITSKNN_CUDA_TRY(cudaLaunchKernelEx(&config, cache_join_kernel<DIM, smem::COLS>, a));
-    return BITSKNN_OK;
+    return launch_join<DIM, smem::COLS>(a, blocks, stream);
 }
 
 int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries, int dtype,
@@ -998,8 +735,12 @@ int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, con
     // columns that share a stream of the cache: the query heads of a token, times the tokens a request
     // has on average when the whole cache is attended to
     const int64_t per_request = selected ? 1 : (batch->tokens + batch->requests - 1) / batch->requests;
-    const int64_t want = std::min<int64_t>(a.group * per_request, 8 * most_columns(cache->dim));
+    const int64_t want = a.group * per_request;
     auto s = static_cast<cudaStream_t>(stream);
+    if (!selected && want >= TC_COLUMNS)
+    {
+        return launch_attend_tc(cache->dim, a, d_workspace, workspace_bytes, s);
+    }
     return dispatch_cache_dim(cache->dim, [&](auto dim) {
         constexpr int DIM = decltype(dim)::value;
         if constexpr (most_columns(DIM) == 4)
@@ -1035,7 +776,9 @@ extern "C" size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* ca
     size_t bytes = 0;
     dispatch_cache_dim(cache->dim, [&](auto dim) {
         constexpr int DIM = decltype(dim)::value;
-        bytes = std::max({workspace_of<DIM, 1>(), workspace_of<DIM, 2>(), workspace_of<DIM, most_columns(DIM)>()});
+        constexpr int MOST = most_columns(DIM);
+        bytes = std::max({parts_bytes<DIM, 8>(blocks_of<DIM, 1>()), parts_bytes<DIM, 16>(blocks_of<DIM, 2>()),
+                          parts_bytes<DIM, 8 * MOST>(blocks_of<DIM, MOST>()), attend_tc_workspace_bytes(DIM)});
         return BITSKNN_OK;
     });
     return bytes;

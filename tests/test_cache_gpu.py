@@ -191,7 +191,7 @@ class Plain:
                 k, v = k[use], v[use]
                 for g in range(h * self.group, (h + 1) * self.group):
                     s = scale * (k @ q[t, g])
-                    d = scale * self.dim * 2 * U * (np.abs(k) @ np.abs(q[t, g])).max()
+                    d = abs(scale) * self.dim * 2 * U * (np.abs(k) @ np.abs(q[t, g])).max()
                     p = np.exp(s - s.max())
                     n = len(use)
                     out[t, g] = (p @ v) / p.sum()
@@ -689,3 +689,67 @@ def test_python_layer_refuses(bk, cuda):
         bk.cache_append(p.cache, torch.zeros((2, 1, 128), dtype=torch.float16, device="cuda")[:, :, ::2],
                         torch.zeros((2, 1, 64), dtype=torch.float16, device="cuda"),
                         torch.zeros(2, dtype=torch.int64, device="cuda"))
+
+
+# ---- many query columns: the tensor-memory kernel ------------------------------------------------------------
+@pytest.mark.parametrize("lengths, news, heads, group, dim, page_rows, dtype", [
+    ([64], [64], 1, 1, 128, 16, torch.bfloat16),
+    ([128], [128], 1, 2, 128, 64, torch.float16),                       # two full query tiles
+    ([300], [200], 1, 4, 64, 16, torch.bfloat16),
+    ([517], [100], 2, 3, 32, 32, torch.float16),
+    ([450], [129], 1, 2, 96, 128, torch.bfloat16),
+    ([333], [70], 1, 5, 192, 16, torch.float16),
+    ([290], [131], 1, 1, 256, 256, torch.bfloat16),
+    ([1000, 3, 0, 260], [90, 3, 0, 200], 2, 4, 128, 32, torch.bfloat16),  # ragged: few rows and none beside many
+    ([100], [150], 1, 3, 128, 16, torch.float16),                       # rows that see nothing
+    ([129, 4000], [65, 64], 1, 8, 64, 16, torch.bfloat16),
+    ([3000], [300], 1, 2, 128, 64, torch.float16),                      # parts of several blocks
+    ([2000], [64], 1, 16, 256, 32, torch.bfloat16),
+])
+def test_attend_many_columns(bk, cuda, lengths, news, heads, group, dim, page_rows, dtype):
+    p = Plain(bk, lengths, news, heads, group, dim, page_rows, dtype, seed=dim + heads).upload()
+    scale = 1 / math.sqrt(dim)
+    want, lse, tol, lse_tol = p.plain_attend(scale)
+    out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, scale, starts=p.d_starts)
+    bk.device_status()
+    check(out, want, tol, "out")
+    check(got_lse, lse, lse_tol, "lse")
+    again, _ = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, scale, starts=p.d_starts)
+    assert torch.equal(out, again)
+
+
+def test_attend_many_columns_special(bk, cuda):
+    """Absent pages, a negative scale, infinite queries, odd strides, one call after the other."""
+    p = Plain(bk, [400, 90], [100, 80], 1, 4, 128, 16, torch.bfloat16, seed=31, page_pad=32)
+    p.table[0, 3], p.table[0, 20], p.table[1, 0] = -1, 10 ** 7, -5
+    p.upload()
+    want, lse, tol, lse_tol = p.plain_attend(-0.05)
+    wide = torch.full((182, 5, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, -0.05, starts=p.d_starts, out=wide[:180, :4])
+    check(out, want, tol, "out")
+    check(got_lse, lse, lse_tol, "lse")
+    assert bool((wide[180:] == 7).all()) and bool((wide[:, 4] == 7).all())
+    odd = torch.full((180 * 4 * 128 + 1,), 7.0, dtype=torch.bfloat16, device="cuda")[1:].view(180, 4, 128)   # 2-byte aligned
+    bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, -0.05, starts=p.d_starts, out=odd)
+    assert torch.equal(odd, out)
+    clean = out.clone()
+    p.d_queries[5, 2, 7], p.d_queries[150, 0, 0] = math.inf, math.nan
+    out, _ = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, -0.05, starts=p.d_starts)
+    bad = out.isnan().all(dim=2)
+    assert bad.sum() == 2 and bool(bad[5, 2]) and bool(bad[150, 0])
+    assert torch.equal(out[~bad], clean[~bad])
+    bk.device_status()
+
+
+def test_attend_sharp_rows_move_the_reference(bk, cuda):
+    """Keys that grow along the cache: the running maximum rises tile after tile, and what was summed is scaled."""
+    p = Plain(bk, [1500], [64], 1, 4, 128, 64, torch.float16, seed=33, spread=0.0)
+    for r, page in enumerate(p.table[0, :24]):
+        p.scales["k"][page, 0] *= 2.0 ** (r / 4 // 1)
+    p.upload()
+    want, lse, tol, lse_tol = p.plain_attend(0.02)
+    out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.02, starts=p.d_starts)
+    check(out, want, tol, "out")
+    check(got_lse, lse, lse_tol, "lse")
+    one = bk.cache_attend(p.cache, p.d_queries[-1:], p.d_lengths, p.d_table, 0.02)[0]
+    check(one, want[-1:], tol[-1:], "decode")
