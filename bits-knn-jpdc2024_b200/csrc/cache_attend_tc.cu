@@ -11,31 +11,38 @@ namespace bitsknn
 namespace
 {
 
-constexpr int TC_GROUPS = 4;  // scale slots: positions in flight between a conversion and its softmax
-constexpr int TC_THREADS = 14 * 32;
+constexpr int TC_THREADS = 16 * 32; // warps 14 and 15 only complete the warpgroup of the issuers
 constexpr int CONVERTERS = 128;
+constexpr int RING = 8;             // scale slots (tiles) and first-NaN slots (items): see cache_attend_tc_kernel
+// Registers of a thread after the split of the 512 x 128 the block is launched with: two warpgroups of
+// softmax, one of converters, one of issuers: 256 * 168 + 128 * 112 + 128 * 56 = 64512 of 65536.
+constexpr int SOFTMAX_REGISTERS = 168;
+constexpr int CONVERT_REGISTERS = 112;
+constexpr int ISSUE_REGISTERS = 56;
 
-// One block: NQ tiles of 128 query rows against tiles of ROWS positions.  Rows of 192 and 256 numbers
-// leave tensor memory (512 columns: scores + sums) for one query tile only, and shared memory for tiles
-// of 64 positions.
+// One block: NQ tiles of 128 query rows against tiles of 64 positions.  Tensor memory (512 columns)
+// holds two score tiles per query tile, so that the next scores are computed while a softmax runs, and
+// the sums; rows of 192 and 256 numbers leave room for one query tile only.
 template <int DIM>
 struct tc_shape
 {
     static constexpr int NQ = DIM <= 128 ? 2 : 1;
     static constexpr int COLS = 128 * NQ;
-    static constexpr int ROWS = DIM <= 128 ? 128 : 64;
-    static constexpr int COST = 2;               // an item's beginning and end, in tiles
+    static constexpr int ROWS = 64;
+    static constexpr int COST = 4;               // an item's beginning and end, in tiles
     static constexpr int BLK = (DIM + 63) / 64;  // 128-byte blocks of 64 halves per row
     static constexpr int Q_BYTES = BLK * 128 * 128;
     static constexpr int KV_BYTES = BLK * ROWS * 128;
+    static constexpr int STAGES = DIM <= 128 ? 4 : DIM <= 192 ? 3 : 2; // of keys, and of values
     static constexpr int GROUPS = ROWS / 16;
-    static constexpr int O_COL = NQ * ROWS;      // tensor memory: scores of the query tiles, then their sums
+    static constexpr int O_COL = NQ * 2 * ROWS;  // tensor memory: two score tiles per query tile, then the sums
     static constexpr int USED_COLS = O_COL + NQ * DIM;
-    static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
-    static constexpr int TAIL = TC_GROUPS * GROUPS * 16 + DIM * 4 + 15 * 8 + 8; // scales, first NaN, barriers, tmem slot
-    static constexpr int BYTES = NQ * Q_BYTES + 4 * KV_BYTES + TAIL + 1024;
+    static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
+    static constexpr int TAIL = RING * GROUPS * 16 + RING * DIM * 4 + 32 * 8; // scales, first NaN, barriers
+    static constexpr int BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + TAIL + 1024;
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(BYTES <= 227 * 1024, "shared memory");
+    static_assert(RING >= STAGES + 2, "scale slots");
 };
 
 // D[tmem] (+)= A[tmem] * B[smem], halves, FP32 sums; issued by one thread.
@@ -47,15 +54,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
                  "}\n" ::"r"(d_tmem),
                  "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1U : 0U)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&v)[16])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
 
@@ -98,165 +96,208 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Largest logit of a row of 64 scores, 16 scores to a scale; with CUT only columns below `limit` count.
+template <bool CUT>
+__device__ __forceinline__ float row_top(const uint32_t (&s)[2][32], const float4* scales, float factor, int limit)
+{
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+    {
+        const float4 k = scales[g];
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            v[i] = __uint_as_float(s[g / 2][g % 2 * 16 + i]);
+            if constexpr (CUT)
+            {
+                v[i] = g * 16 + i < limit ? v[i] : -INFINITY;
+            }
+        }
+        float a = fmaxf(fmaxf(v[0], v[1]), v[2]);
+        float b = fmaxf(fmaxf(v[3], v[4]), v[5]);
+        a = fmaxf(fmaxf(a, v[6]), v[7]);
+        b = fmaxf(fmaxf(b, v[8]), v[9]);
+        a = fmaxf(fmaxf(a, v[10]), v[11]);
+        b = fmaxf(fmaxf(b, v[12]), v[13]);
+        const float most = fmaxf(fmaxf(fmaxf(a, b), v[14]), v[15]);
+        // an absent page has the logarithm -inf
+        top = fmaxf(top, most == -INFINITY ? most : fmaf(most, factor * k.x, k.y));
+    }
+    return top;
+}
+
+// Scores to weights 2^(logit + bias) as halves; returns l plus the row's share of the denominator.
+template <bool CUT>
+__device__ __forceinline__ float row_weights(const uint32_t (&s)[2][32], uint32_t (&p)[32], const float4* scales,
+                                             float factor, float bias, int limit, float l)
+{
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+    {
+        const float4 k = scales[g];
+        const float f = factor * k.x;
+        const float add = k.y + bias;
+        float even = 0.0F;
+        float odd = 0.0F;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2)
+        {
+            float x = exp2_fast(fmaf(__uint_as_float(s[g / 2][g % 2 * 16 + i]), f, add));
+            float y = exp2_fast(fmaf(__uint_as_float(s[g / 2][g % 2 * 16 + i + 1]), f, add));
+            if constexpr (CUT)
+            {
+                x = g * 16 + i < limit ? x : 0.0F;
+                y = g * 16 + i + 1 < limit ? y : 0.0F;
+            }
+            even += x;
+            odd += y;
+            p[g * 8 + i / 2] = pack_half2(x, y);
+        }
+        l = fmaf(even + odd, k.z, l);
+    }
+    return l;
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int N>
+__device__ __forceinline__ void fewer_registers()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // A wait of a whole warp: its threads go on, or give up, together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity)
 {
     return __all_sync(FULL_MASK, ptx::mbar_wait_bounded_spin(bar, parity)) != 0;
 }
 
-// Warps 0-3 and 4-7: softmax of query tile 0 and 1, one thread per row.  Warps 8-11: converters, codes
-// to halves.  Warps 12 and 13: one thread each issues the products of a query tile.
-//
-// A tile of ROWS positions goes round like this.  The converters bring 16 codes per thread and load
-// from the cache a tile ahead, turn them into halves and store them in the swizzled layout the tensor
-// cores read (two stages each of keys and values).  S = Q K^T lands in tensor memory; a softmax thread
-// reads its row twice (maximum, then weights; the row's 128 scores would not fit its registers) and
-// writes the weights as halves over the scores; O += P V takes them from there as its first
-// operand, and the values as they lie, contiguous along the outputs.  While one query tile is with its
-// softmax warps the tensor cores work for the other one.  The two issuing threads do not wait for one
-// another (a thread is held while its products run).  O stays in tensor memory; it is touched
-// only when a row's reference point has to move by more than 2^8 (rarely after the first tile).
-//
-// Bound by the exponentials (16 per clock and SM: 2048 clocks for 256 rows x 128 positions) and the
-// tensor cores (4 products of 128 x 128 x 128: about 2300 clocks) alike.
+// First position of a dimension with a NaN among the tiles that only some rows of item number `items`
+// see wholly, as an offset (below 1024: a block's columns span at most 256 tokens) from the first
+// of these tiles.  The key grows with the item and towards earlier positions, so a maximum keeps
+// the first one and what an item before has left needs no clearing.
+__device__ __forceinline__ uint32_t nan_key(uint32_t items, int offset) { return (items + 1) << 10 | (1023U - offset); }
+
+// A block's walk over its share: every role goes through the same items for itself.
+template <class SHAPE>
+struct walk
+{
+    item it;
+    request q;
+    int64_t at;        // of the axis
+    int64_t share_end;
+
+    __device__ __forceinline__ int64_t segment_end() const { return min(it.end, share_end); }
+    __device__ __forceinline__ int first_tile() const { return max(static_cast<int>(at - it.begin) - SHAPE::COST, 0); }
+    // tiles of the share; none if it ends within the units of the item's beginning
+    __device__ __forceinline__ int count() const
+    {
+        return max(static_cast<int>(segment_end() - it.begin) - SHAPE::COST, 0) - first_tile();
+    }
+    __device__ __forceinline__ int query_tiles() const { return it.columns - it.column0 > 128 ? SHAPE::NQ : 1; }
+    __device__ __forceinline__ int last_column() const { return min(it.column0 + SHAPE::COLS, it.columns) - 1; }
+    __device__ __forceinline__ bool next(const attend_args& a)
+    {
+        at = segment_end();
+        if (at >= share_end)
+        {
+            return false;
+        }
+        it.begin = it.end;
+        it.column0 += SHAPE::COLS;
+        if (it.column0 >= it.columns)
+        {
+            it.column0 = 0;
+            if (++it.head == a.c.heads)
+            {
+                it.head = 0;
+                do
+                {
+                    ++it.request; // requests without tokens have no units; `at` < total, so one follows
+                    q = request_of(a.b, it.request);
+                } while (q.count == 0);
+                it.first_token = q.first;
+                it.columns = q.count * a.group;
+            }
+        }
+        it.end = it.begin + units_of_block<SHAPE>(a, q, it.column0);
+        return true;
+    }
+};
+
+// Barriers and buffers of a block in shared memory.
+struct tc_state
+{
+    unsigned char* q_tiles;
+    unsigned char* k_tiles;
+    unsigned char* v_tiles;
+    float4* scales;     // [RING][GROUPS]: key scale, log2 of the value scale, its inverse
+    uint32_t* first_nan; // [RING][DIM]: nan_key
+    uint64_t* k_full;   // [STAGES]
+    uint64_t* k_empty;
+    uint64_t* v_full;
+    uint64_t* v_empty;
+    uint64_t* s_full;   // [query tile][score tile]
+    uint64_t* p_full;   // [query tile][score tile]
+    uint64_t* o_done;   // [query tile]
+    uint64_t* q_full;   // [query tile]
+};
+
+// ================= softmax: one thread per query row =================
 template <int DIM>
-__global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)
+__device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem)
 {
     using shape = tc_shape<DIM>;
-    constexpr int NQ = shape::NQ;
-    constexpr int ROWS = shape::ROWS;
-    constexpr int GROUPS = shape::GROUPS;
-    constexpr int PARTS = DIM / 16;                        // 16-code pieces per row
-    constexpr int PIECES = ROWS * PARTS / CONVERTERS;      // per converter thread and tile
-    static_assert(ROWS * PARTS % CONVERTERS == 0, "pieces");
-    extern __shared__ unsigned char raw[];
-    unsigned char* const base = raw + ((1024U - (ptx::smem_addr(raw) & 1023U)) & 1023U);
-    unsigned char* const q_tiles = base;
-    unsigned char* const k_tiles = base + NQ * shape::Q_BYTES;
-    unsigned char* const v_tiles = k_tiles + 2 * shape::KV_BYTES;
-    float4* const scales = reinterpret_cast<float4*>(v_tiles + 2 * shape::KV_BYTES); // [TC_GROUPS][GROUPS]: ks, lv, 1 / vs
-    int* const first_nan = reinterpret_cast<int*>(scales + TC_GROUPS * GROUPS);      // [DIM]
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(first_nan + DIM);
-    uint64_t* const k_full = bars;        // [2]
-    uint64_t* const k_empty = bars + 2;   // [2]
-    uint64_t* const v_full = bars + 4;    // [2]
-    uint64_t* const v_empty = bars + 6;   // [2]
-    uint64_t* const s_full = bars + 8;    // [2] per query tile
-    uint64_t* const p_full = bars + 10;   // [2]
-    uint64_t* const o_done = bars + 12;   // [2]
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
-    __shared__ int64_t s_words[TC_THREADS / 32];
-    __shared__ int s_found;
     const int t = threadIdx.x;
-    const int warp = t >> 5;
-    const int lane = t & 31;
-    const int rows_mask = (1 << a.c.page_shift) - 1;
-
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (t == 0)
+    const int my_tile = t >> 7;
+    const uint32_t lane_base = static_cast<uint32_t>(((t >> 5) & 3) * 32) << 16;
+    const uint32_t s_base = tmem + lane_base + my_tile * 2 * shape::ROWS;
+    const uint32_t o_addr = tmem + lane_base + shape::O_COL + my_tile * DIM;
+    uint32_t kv_tiles = 0; // tiles of the block so far
+    uint32_t s_tiles = 0;  // and those of this query tile
+    uint32_t items = 0;    // items with tiles
+    do
     {
-        a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-        for (int i = 0; i < 2; ++i)
+        const int count = w.count();
+        if (my_tile < w.query_tiles())
         {
-            ptx::mbar_init(&k_full[i], CONVERTERS);
-            ptx::mbar_init(&v_full[i], CONVERTERS);
-            ptx::mbar_init(&k_empty[i], NQ);
-            ptx::mbar_init(&v_empty[i], NQ);
-            ptx::mbar_init(&s_full[i], 2); // the products' commit, and the issuing thread itself: what it has
-            ptx::mbar_init(&p_full[i], 128);
-            ptx::mbar_init(&o_done[i], 2); // seen of the converters (scales, NaN) is then seen by the softmax
-        }
-        ptx::mbar_init_fence();
-    }
-    if (warp == 0)
-    {
-        tc::tmem_alloc(tmem_slot, shape::TMEM_COLS);
-    }
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
-
-    int64_t sum = 0;
-    for (int r = t; r < a.b.requests; r += TC_THREADS)
-    {
-        sum += units_of_head<shape>(a, request_of(a.b, r)) * a.c.heads;
-    }
-    const int64_t total = block_sum<TC_THREADS / 32>(sum, s_words);
-    const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total);
-    bool fine = true; // no wait of this thread has expired
-    if (blockIdx.x < blocks)
-    {
-        int64_t at = blockIdx.x * total / blocks;
-        const int64_t share_end = (blockIdx.x + 1) * total / blocks;
-        item it{};
-        int64_t first = 0;
-        it.request = find_request<shape, TC_THREADS / 32>(a, at, &first, s_words, &s_found);
-        request q = request_of(a.b, it.request);
-        const int64_t per_head = units_of_head<shape>(a, q);
-        it.head = static_cast<int>((at - first) / per_head);
-        it.begin = first + it.head * per_head;
-        it.first_token = q.first;
-        it.columns = q.count * a.group;
-        it.end = it.begin + units_of_block<shape>(a, q, 0);
-        while (at >= it.end)
-        {
-            it.column0 += shape::COLS;
-            it.begin = it.end;
-            it.end += units_of_block<shape>(a, q, it.column0);
-        }
-        uint32_t kv_tiles = 0; // tiles of keys and values this block has gone through
-        uint32_t s_tiles = 0;  // and those of this warp's query tile
-        while (true)
-        {
-            const int64_t seg_end = min(it.end, share_end);
-            const int first_tile = max(static_cast<int>(at - it.begin) - shape::COST, 0);
-            const int count = max(static_cast<int>(seg_end - it.begin) - shape::COST, 0) - first_tile;
-            const int last_col = min(it.column0 + shape::COLS, it.columns) - 1;
-            const int furthest = visible_of(a.b, q, last_col / a.group);
-            const int nearest = visible_of(a.b, q, it.column0 / a.group);
-            const bool whole = at == it.begin && seg_end == it.end;
-            const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at == it.begin ? 1 : 0);
-            const int tiles = it.columns - it.column0 > 128 ? NQ : 1; // query tiles with real rows
-            const int my_tile = warp < 8 ? warp >> 2 : warp - 12;     // softmax warps and issuers
-            // ---- query rows: one softmax thread each ----
-            const int col = it.column0 + t; // of softmax threads
-            const bool softmax = warp < 8 && my_tile < tiles;
-            const bool real = softmax && col < it.columns;
+            const int col = w.it.column0 + t;
+            const bool real = col < w.it.columns;
             const int token = col / a.group;
-            const int qhead = it.head * a.group + col % a.group;
+            const int qhead = w.it.head * a.group + col % a.group;
+            const int64_t row_token = w.it.first_token + token;
+            const int see = real ? visible_of(a.b, w.q, token) : 0;
             float factor = 0.0F;
-            int see = 0;
-            if (softmax)
+            if (count > 0)
             {
-                const uint32_t to = ptx::smem_addr(q_tiles + my_tile * shape::Q_BYTES);
-                const int row = t & 127;
-                uint4 v[DIM / 8];
-                float top = 0.0F;
-                const uint4* from = reinterpret_cast<const uint4*>(
+                // the products that read the query tile's rows before are done: o_done was waited for
+                const uint32_t to = ptx::smem_addr(st.q_tiles + my_tile * shape::Q_BYTES);
+                const uint4* const from = reinterpret_cast<const uint4*>(
                     static_cast<const uint16_t*>(a.queries) +
-                    (real ? static_cast<int64_t>(it.first_token + token) * a.query_stride + static_cast<int64_t>(qhead) * DIM
-                          : 0));
-                auto floats = [&](uint32_t w) {
+                    (real ? row_token * a.query_stride + static_cast<int64_t>(qhead) * DIM : 0));
+                auto floats = [&](uint32_t x) {
                     if (a.dtype == BITSKNN_BF16)
                     {
-                        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000U));
+                        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000U));
                     }
-                    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+                    return __half22float2(*reinterpret_cast<const __half2*>(&x));
                 };
-#pragma unroll
+                float top = 0.0F;
+#pragma unroll 8
                 for (int i = 0; i < DIM / 8; ++i)
                 {
-                    v[i] = real ? __ldg(from + i) : make_uint4(0U, 0U, 0U, 0U);
-                }
-#pragma unroll
-                for (int i = 0; i < DIM / 8; ++i)
-                {
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                    const uint4 v = real ? __ldg(from + i) : make_uint4(0U, 0U, 0U, 0U);
+                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                     {
-                        const float2 f = floats(w[j]);
+                        const float2 f = floats(x[j]);
                         top = fabsf(f.x) < INFINITY ? fmaxf(top, fabsf(f.x)) : top;
                         top = fabsf(f.y) < INFINITY ? fmaxf(top, fabsf(f.y)) : top;
                     }
@@ -267,195 +308,131 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
                 const int shift = top > 0.0F ? min(max(14 - e, -126), 126) : 0;
                 const float up = a.scale < 0.0F ? -pow2_int(shift) : pow2_int(shift);
                 factor = pow2_int(-shift) * fabsf(a.scale);
-#pragma unroll
+#pragma unroll 8
                 for (int i = 0; i < DIM / 8; ++i)
                 {
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                    const uint4 v = real ? __ldg(from + i) : make_uint4(0U, 0U, 0U, 0U);
+                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
                     uint32_t h[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                     {
-                        const float2 f = floats(w[j]);
+                        const float2 f = floats(x[j]);
                         h[j] = pack_half2(f.x * up, f.y * up);
                     }
-                    st_shared16(to + tile_byte(row, i, 128), h[0], h[1], h[2], h[3]);
+                    st_shared16(to + tile_byte(t & 127, i, 128), h[0], h[1], h[2], h[3]);
                 }
-                see = real ? visible_of(a.b, q, token) : 0;
                 fence_async_proxy();
+                tc::mbar_arrive(&st.q_full[my_tile]);
             }
-            for (int d = t; d < DIM; d += TC_THREADS)
+            const int nearest = visible_of(a.b, w.q, min(w.it.column0 + my_tile * 128, w.last_column()) / a.group);
+            float m = -INFINITY;
+            float l = 0.0F;
+            for (int j = 0; j < count; ++j, ++s_tiles)
             {
-                first_nan[d] = 0x7fffffff;
-            }
-            __syncthreads();
-
-            if (warp < 8)
-            {
-                // ================= softmax =================
-                const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-                const uint32_t s_addr = tmem + lane_base + my_tile * ROWS;
-                const uint32_t o_addr = tmem + lane_base + shape::O_COL + my_tile * DIM;
-                const int tile_nearest = visible_of(a.b, q, min(it.column0 + my_tile * 128, last_col) / a.group);
-                float m = -INFINITY;
-                float l = 0.0F;
-                for (int j = 0; j < count && softmax && fine; ++j)
+                const uint32_t buffer = s_tiles & 1;
+                const uint32_t phase = (s_tiles >> 1) & 1U;
+                const uint32_t s_addr = s_base + buffer * shape::ROWS;
+                if (!warp_wait(&st.s_full[my_tile * 2 + buffer], phase))
                 {
-                    const uint32_t n = kv_tiles + j;
-                    fine = warp_wait(&s_full[my_tile], s_tiles & 1U);
-                    if (!fine)
-                    {
-                        break;
-                    }
-                    ++s_tiles;
-                    tc::fence_after_sync();
-                    const int pos = (first_tile + j) * ROWS;
-                    const float4* const sc = scales + (n % TC_GROUPS) * GROUPS;
-                    const bool cut = pos + ROWS > tile_nearest;
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < ROWS; c += 32)
-                    {
-                        uint32_t s[32];
-                        tc::tmem_ld_32x32(s_addr + c, s);
-                        tc::tmem_ld_wait();
-#pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                        {
-                            const float4 k = sc[c / 16 + g];
-                            float most = -INFINITY;
-                            if (!cut)
-                            {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i)
-                                {
-                                    most = fmaxf(most, __uint_as_float(s[g * 16 + i]));
-                                }
-                            }
-                            else
-                            {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i)
-                                {
-                                    most = pos + c + g * 16 + i < see ? fmaxf(most, __uint_as_float(s[g * 16 + i])) : most;
-                                }
-                            }
-                            // an absent page has lv = -inf
-                            top = fmaxf(top, most == -INFINITY ? most : fmaf(most, factor * k.x, k.y));
-                        }
-                    }
-                    if (__any_sync(FULL_MASK, top > m + WEIGHT_SLACK))
-                    {
-                        const float raised = fmaxf(top, m);
-                        const float keep = m == -INFINITY ? 0.0F : exp2_fast(m - raised);
-                        m = raised;
-                        l *= keep;
-                        if (j > 0)
-                        {
-                            // the product before this one has to be through with the sums
-                            fine = warp_wait(&o_done[my_tile], s_tiles & 1U);
-                            if (!fine)
-                            {
-                                break;
-                            }
-                            tc::fence_after_sync();
-#pragma unroll 1
-                            for (int c = 0; c < DIM; c += 32)
-                            {
-                                uint32_t o[32];
-                                tc::tmem_ld_32x32(o_addr + c, o);
-                                tc::tmem_ld_wait();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                {
-                                    o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                                }
-                                tmem_st_32(o_addr + c, o);
-                            }
-                        }
-                    }
-                    const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
-#pragma unroll
-                    for (int c = 0; c < ROWS; c += 32)
-                    {
-                        uint32_t s[32];
-                        tc::tmem_ld_32x32(s_addr + c, s);
-                        tc::tmem_ld_wait();
-                        uint32_t p[16];
-#pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                        {
-                            const float4 k = sc[c / 16 + g];
-                            const float f = factor * k.x;
-                            const float add = k.y + bias;
-                            float part_sum = 0.0F;
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2)
-                            {
-                                float x = exp2_fast(fmaf(__uint_as_float(s[g * 16 + i]), f, add));
-                                float y = exp2_fast(fmaf(__uint_as_float(s[g * 16 + i + 1]), f, add));
-                                if (cut)
-                                {
-                                    x = pos + c + g * 16 + i < see ? x : 0.0F;
-                                    y = pos + c + g * 16 + i + 1 < see ? y : 0.0F;
-                                }
-                                part_sum += x + y;
-                                p[g * 8 + i / 2] = pack_half2(x, y);
-                            }
-                            l = fmaf(part_sum, k.z, l);
-                        }
-                        // weights of columns c ... c + 31 take the place of scores c / 2 ..., read before
-                        tmem_st_16(s_addr + c / 2, p);
-                    }
-                    tmem_st_wait();
-                    tc::fence_before_sync();
-                    tc::mbar_arrive(&p_full[my_tile]);
+                    return false;
                 }
-                // ---- results of the rows ----
-                if (softmax && fine && count > 0)
+                tc::fence_after_sync();
+                const int pos = (w.first_tile() + j) * shape::ROWS;
+                const float4* const scales = st.scales + ((kv_tiles + j) % RING) * shape::GROUPS;
+                const bool cut = pos + shape::ROWS > nearest;
+                uint32_t s[2][32];
+                tc::tmem_ld_32x32(s_addr, s[0]);
+                tc::tmem_ld_32x32(s_addr + 32, s[1]);
+                tc::tmem_ld_wait();
+                const float top =
+                    cut ? row_top<true>(s, scales, factor, see - pos) : row_top<false>(s, scales, factor, 0);
+                if (__any_sync(FULL_MASK, top > m + WEIGHT_SLACK))
                 {
-                    fine = warp_wait(&o_done[my_tile], (s_tiles - 1) & 1U);
-                    tc::fence_after_sync();
-                }
-                if (softmax && fine)
-                {
-                    const float inverse = l == 0.0F ? 0.0F : 1.0F / l;
-                    const int64_t row_token = it.first_token + token;
-                    const int64_t out_at = row_token * a.out_stride + static_cast<int64_t>(qhead) * DIM;
-                    const bool aligned = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * 2)) & 15) == 0;
-                    float* const part_row = a.part_o + (part * shape::COLS + t) * DIM;
-#pragma unroll 1
-                    for (int c = 0; c < DIM; c += 32)
+                    const float raised = fmaxf(top, m);
+                    const float keep = m == -INFINITY ? 0.0F : exp2_fast(m - raised);
+                    m = raised;
+                    l *= keep;
+                    if (j > 0)
                     {
-                        uint32_t o[32];
-                        __syncwarp();
-                        if (count > 0)
+                        // the product before this one has to be through with the sums
+                        if (!warp_wait(&st.o_done[my_tile], (s_tiles - 1) & 1U))
                         {
+                            return false;
+                        }
+                        tc::fence_after_sync();
+#pragma unroll 1
+                        for (int c = 0; c < DIM; c += 32)
+                        {
+                            uint32_t o[32];
                             tc::tmem_ld_32x32(o_addr + c, o);
                             tc::tmem_ld_wait();
-                        }
-                        if (!real)
-                        {
-                            continue;
-                        }
-                        float v[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                        {
-                            v[i] = count > 0 ? __uint_as_float(o[i]) : 0.0F;
-                            v[i] = first_nan[c + i] < see ? NAN : v[i];
-                        }
-                        if (!whole)
-                        {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4)
+                            for (int i = 0; i < 32; ++i)
                             {
-                                *reinterpret_cast<float4*>(part_row + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                                o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
                             }
-                            continue;
+                            tmem_st_32(o_addr + c, o);
                         }
-                        // l = 0: nothing was seen; NaN in l makes the row NaN
-                        auto result = [&](float x) { return l == 0.0F ? 0.0F : x * inverse; };
-                        auto pair = [&](float x, float y) {
+                    }
+                }
+                const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
+                uint32_t p[32];
+                l = cut ? row_weights<true>(s, p, scales, factor, bias, see - pos, l)
+                        : row_weights<false>(s, p, scales, factor, bias, 0, l);
+                tmem_st_32(s_addr, p); // over the scores
+                tmem_st_wait();
+                tc::fence_before_sync();
+                tc::mbar_arrive(&st.p_full[my_tile * 2 + buffer]);
+            }
+            // ---- the row's result ----
+            if (count > 0 && !warp_wait(&st.o_done[my_tile], (s_tiles - 1) & 1U))
+            {
+                return false;
+            }
+            tc::fence_after_sync();
+            const bool whole = w.at == w.it.begin && w.segment_end() == w.it.end;
+            const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (w.at == w.it.begin ? 1 : 0);
+            const uint32_t* const first_nan = st.first_nan + (items % RING) * DIM;
+            // a key of this item at least as large stands for a position below `see`
+            const int cut_base = visible_of(a.b, w.q, w.it.column0 / a.group) / shape::ROWS * shape::ROWS;
+            const uint32_t seen_nan = see > cut_base ? nan_key(items, see - 1 - cut_base) : 0xffffffffU;
+            const float inverse = l == 0.0F ? 0.0F : 1.0F / l;
+            uint16_t* const out =
+                static_cast<uint16_t*>(a.out) + row_token * a.out_stride + static_cast<int64_t>(qhead) * DIM;
+            const bool aligned =
+                ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * 2)) & 15) == 0;
+            float* const part_row = a.part_o + (part * shape::COLS + t) * DIM;
+#pragma unroll 1
+            for (int c = 0; c < DIM; c += 32)
+            {
+                uint32_t o[32];
+                __syncwarp();
+                if (count > 0)
+                {
+                    tc::tmem_ld_32x32(o_addr + c, o);
+                    tc::tmem_ld_wait();
+                }
+                if (real)
+                {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                    {
+                        o[i] = count > 0 ? (first_nan[c + i] >= seen_nan ? 0x7fc00000U : o[i]) : 0U;
+                    }
+                    if (!whole)
+                    {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                        {
+                            *reinterpret_cast<uint4*>(part_row + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                    else
+                    {
+                        // l = 0: nothing was seen; a NaN in l makes the row NaN
+                        auto result = [&](uint32_t x) { return l == 0.0F ? 0.0F : __uint_as_float(x) * inverse; };
+                        auto pair = [&](uint32_t x, uint32_t y) {
                             if (a.dtype == BITSKNN_BF16)
                             {
                                 const __nv_bfloat162 b = __floats2bfloat162_rn(result(x), result(y));
@@ -463,271 +440,473 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
                             }
                             return pack_half2(result(x), result(y));
                         };
-                        uint16_t* const out = static_cast<uint16_t*>(a.out) + out_at + c;
 #pragma unroll
                         for (int i = 0; i < 32; i += 8)
                         {
-                            const uint4 w = make_uint4(pair(v[i], v[i + 1]), pair(v[i + 2], v[i + 3]),
-                                                       pair(v[i + 4], v[i + 5]), pair(v[i + 6], v[i + 7]));
+                            const uint32_t x[4] = {pair(o[i], o[i + 1]), pair(o[i + 2], o[i + 3]), pair(o[i + 4], o[i + 5]),
+                                                   pair(o[i + 6], o[i + 7])};
                             if (aligned)
                             {
-                                *reinterpret_cast<uint4*>(out + i) = w;
+                                *reinterpret_cast<uint4*>(out + c + i) = make_uint4(x[0], x[1], x[2], x[3]);
                             }
                             else
                             {
-                                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                                 for (int y = 0; y < 8; ++y)
                                 {
-                                    out[i + y] = static_cast<uint16_t>(x[y >> 1] >> (16 * (y & 1)));
+                                    out[c + i + y] = static_cast<uint16_t>(x[y >> 1] >> (16 * (y & 1)));
                                 }
                             }
                         }
                     }
-                    if (real && !whole)
-                    {
-                        a.part_ml[part * shape::COLS + t] = make_float2(m, l);
-                    }
-                    if (real && whole && a.lse != nullptr)
-                    {
-                        a.lse[row_token * a.group * a.c.heads + qhead] =
-                            l == 0.0F ? -INFINITY : (m - WEIGHT_BIAS + log2f(l)) * LN_2;
-                    }
-                    tc::fence_before_sync();
                 }
             }
-            else if (warp < 12)
+            __syncwarp();
+            if (real && !whole)
             {
-                // ================= converters =================
-                const int me = t - 8 * 32;
-                const int32_t* const table = a.b.table + it.request * a.b.table_ld;
-                auto page_of = [&](int j) { // page of this lane's 16 positions of tile j
-                    const int pos = (first_tile + j) * ROWS + lane * 16;
-                    const int p = lane < GROUPS && j < count && pos < furthest ? table[pos >> a.c.page_shift] : -1;
-                    return p < a.c.pages ? p : -1;
-                };
-                auto load = [&](uint4 (&r)[PIECES], const uint8_t* codes, int j, int page) {
+                a.part_ml[part * shape::COLS + t] = make_float2(m, l);
+            }
+            if (real && whole && a.lse != nullptr)
+            {
+                a.lse[row_token * a.group * a.c.heads + qhead] =
+                    l == 0.0F ? -INFINITY : (m - WEIGHT_BIAS + log2f(l)) * LN_2;
+            }
+            tc::fence_before_sync();
+        }
+        kv_tiles += count;
+        items += count > 0 ? 1 : 0;
+    } while (w.next(a));
+    return true;
+}
+
+// ================= converters: codes from the cache to halves in shared memory =================
+template <int DIM>
+__device__ __forceinline__ bool convert_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w)
+{
+    using shape = tc_shape<DIM>;
+    constexpr int BLK = shape::BLK;
+    constexpr int ROWS = shape::ROWS;
+    constexpr int SLABS = ROWS / 32;     // rows a thread serves: one of every 32
+    constexpr int PIECES = SLABS * BLK;  // 16-code pieces of a thread and tile
+    constexpr int AHEAD = 32 / shape::GROUPS; // tiles whose pages a warp looks up at a time, one lane per 16 positions
+    const int lane = threadIdx.x & 31;
+    const int warp = (threadIdx.x >> 5) - 8;
+    const int rows_mask = (1 << a.c.page_shift) - 1;
+    // A warp's load covers 8 rows of 4 pieces (64 codes): its 8 rows lie within one page, and its
+    // two 16-byte stores per piece reach eight different granules in every phase (two rows, four even or
+    // four odd chunks, moved apart by the swizzle).
+    const int piece = lane & 3;
+    const int row0 = warp * 8 + (lane >> 2);
+    const uint32_t first_half = tile_byte(row0, piece * 2, ROWS);
+    const uint32_t second_half = tile_byte(row0, piece * 2 + 1, ROWS);
+    uint32_t n = 0; // tiles so far
+    uint32_t items = 0;
+    do
+    {
+        const int count = w.count();
+        if (count == 0)
+        {
+            continue;
+        }
+        const int first_tile = w.first_tile();
+        const int furthest = visible_of(a.b, w.q, w.last_column() / a.group);
+        const int nearest = visible_of(a.b, w.q, w.it.column0 / a.group);
+        const int32_t* const table = a.b.table + w.it.request * a.b.table_ld;
+        uint32_t* const first_nan = st.first_nan + (items % RING) * DIM;
+        const int cut_base = nearest / ROWS * ROWS;
+        auto pages_from = [&](int j) { // page of this lane's 16 positions, AHEAD tiles from tile j on
+            const int pos = (first_tile + j) * ROWS + lane * 16;
+            const int p = j < count && pos < furthest ? table[pos >> a.c.page_shift] : -1;
+            return p < a.c.pages ? p : -1;
+        };
+        int page_now = pages_from(0);
+        int page_next = pages_from(AHEAD);
+        auto scales_of = [&](int page, float& ks, float& vs) {
+            ks = page < 0 ? 0.0F : a.c.key_scales[static_cast<int64_t>(page) * a.c.heads + w.it.head];
+            vs = page < 0 ? 1.0F : a.c.value_scales[static_cast<int64_t>(page) * a.c.heads + w.it.head];
+        };
+        float ks_now = 0.0F, vs_now = 1.0F, ks_next = 0.0F, vs_next = 1.0F;
+        if (warp == 0)
+        {
+            scales_of(page_now, ks_now, vs_now);
+        }
+        int base = 0; // first tile of page_now
+        auto load = [&](uint4 (&r)[PIECES], const uint8_t* codes, int j) {
+            const int pages = j - base < AHEAD ? page_now : page_next;
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i)
+            for (int i = 0; i < SLABS; ++i)
+            {
+                const int pos = (first_tile + j) * ROWS + i * 32 + row0;
+                const int p = __shfl_sync(FULL_MASK, pages, (j % AHEAD) * shape::GROUPS + i * 2 + (warp >> 1));
+                const uint8_t* const from = codes + max(p, 0) * a.c.page_stride +
+                                            ((static_cast<int64_t>(w.it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM +
+                                            piece * 16;
+                const bool there = j < count && p >= 0 && pos < furthest;
+#pragma unroll
+                for (int b = 0; b < BLK; ++b)
+                {
+                    r[i * BLK + b] = make_uint4(0U, 0U, 0U, 0U);
+                    if (there && (DIM % 64 == 0 || b * 64 + piece * 16 < DIM))
                     {
-                        const int e = me + i * CONVERTERS;
-                        const int row = e / PARTS;
-                        const int p = __shfl_sync(FULL_MASK, page, row >> 4);
-                        const int pos = (first_tile + j) * ROWS + row;
-                        r[i] = make_uint4(0U, 0U, 0U, 0U);
-                        if (p >= 0 && pos < furthest)
-                        {
-                            r[i] = __ldg(reinterpret_cast<const uint4*>(
-                                codes + p * a.c.page_stride +
-                                ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM +
-                                (e % PARTS) * 16));
-                        }
+                        r[i * BLK + b] = __ldg(reinterpret_cast<const uint4*>(from + b * 64));
                     }
-                };
-                auto store = [&](const uint4 (&r)[PIECES], unsigned char* tile) {
-                    const uint32_t to = ptx::smem_addr(tile);
+                }
+            }
+        };
+        auto store = [&](const uint4 (&r)[PIECES], unsigned char* tile) {
+            const uint32_t to = ptx::smem_addr(tile);
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i)
+            for (int i = 0; i < SLABS; ++i)
+            {
+#pragma unroll
+                for (int b = 0; b < BLK; ++b)
+                {
+                    const uint4 x = r[i * BLK + b];
+                    const uint32_t at_row = to + b * ROWS * 128 + i * 32 * 128;
+                    uint32_t h[8];
+                    halves_of_codes(x.x, h[0], h[1]);
+                    halves_of_codes(x.y, h[2], h[3]);
+                    halves_of_codes(x.z, h[4], h[5]);
+                    halves_of_codes(x.w, h[6], h[7]);
+                    st_shared16(at_row + first_half, h[0], h[1], h[2], h[3]);
+                    st_shared16(at_row + second_half, h[4], h[5], h[6], h[7]);
+                }
+            }
+        };
+        // A NaN code times a weight of zero would spoil the rows that do not see its position.  In
+        // tiles that only some rows see wholly the NaN are taken out of the values and the first position
+        // of each dimension that had one is kept: a row is NaN there if it sees it.
+        auto clean = [&](uint4 (&r)[PIECES], int j) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+            {
+                uint32_t x[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                {
+                    const uint32_t hit = ((x[y] & 0x7f7f7f7fU) + 0x01010101U) & 0x80808080U;
+                    if (hit != 0)
                     {
-                        const int e = me + i * CONVERTERS;
-                        const int row = e / PARTS;
-                        const int chunk = (e % PARTS) * 2;
-                        uint32_t h[8];
-                        halves_of_codes(r[i].x, h[0], h[1]);
-                        halves_of_codes(r[i].y, h[2], h[3]);
-                        halves_of_codes(r[i].z, h[4], h[5]);
-                        halves_of_codes(r[i].w, h[6], h[7]);
-                        // lanes whose block of 64 halves is odd store their second half first: the eight
-                        // lanes of a phase then reach eight different granules
-                        const bool turn = ((chunk >> 3) & 1) != 0;
-                        st_shared16(to + tile_byte(row, chunk + (turn ? 1 : 0), ROWS), turn ? h[4] : h[0], turn ? h[5] : h[1],
-                                    turn ? h[6] : h[2], turn ? h[7] : h[3]);
-                        st_shared16(to + tile_byte(row, chunk + (turn ? 0 : 1), ROWS), turn ? h[0] : h[4], turn ? h[1] : h[5],
-                                    turn ? h[2] : h[6], turn ? h[3] : h[7]);
-                    }
-                };
-                // A NaN code times a weight of zero would spoil the rows that do not see its position.  In
-                // tiles that only some rows see wholly the NaN are taken out of the values and the first
-                // position of each dimension that had one is kept: a row is NaN there if it sees it.
-                auto clean = [&](uint4 (&r)[PIECES], int j) {
-#pragma unroll
-                    for (int i = 0; i < PIECES; ++i)
-                    {
-                        uint32_t* const w = reinterpret_cast<uint32_t*>(&r[i]);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
+                        const int d = i % BLK * 64 + piece * 16 + y * 4;
+                        const int pos = (first_tile + j) * ROWS + i / BLK * 32 + row0;
+#pragma unroll 1
+                        for (int z = 0; z < 4; ++z)
                         {
-                            const uint32_t hit = ((w[x] & 0x7f7f7f7fU) + 0x01010101U) & 0x80808080U;
-                            if (hit != 0)
+                            if ((hit >> (8 * z + 7)) & 1U)
                             {
-                                const int e = me + i * CONVERTERS;
-                                for (int y = 0; y < 4; ++y)
-                                {
-                                    if ((hit >> (8 * y + 7)) & 1U)
-                                    {
-                                        atomicMin(&first_nan[(e % PARTS) * 16 + x * 4 + y],
-                                                  (first_tile + j) * ROWS + e / PARTS);
-                                        w[x] &= ~(0xffU << (8 * y));
-                                    }
-                                }
+                                atomicMax(&first_nan[d + z], nan_key(items, pos - cut_base));
+                                x[y] &= ~(0xffU << (8 * z));
                             }
                         }
                     }
-                };
-                uint4 rk[PIECES];
-                uint4 rv[PIECES];
-                int page = page_of(0);
-                int next = page_of(1);
-                load(rk, a.c.keys, 0, page);
-                load(rv, a.c.values, 0, page);
-                for (int j = 0; j < count; ++j)
-                {
-                    const uint32_t n = kv_tiles + j;
-                    const uint32_t stage = n & 1;
-                    const uint32_t phase = (n >> 1) & 1U;
-                    float ks = 0.0F;
-                    float vs = 1.0F;
-                    if (warp == 8 && page >= 0)
-                    {
-                        ks = a.c.key_scales[static_cast<int64_t>(page) * a.c.heads + it.head];
-                        vs = a.c.value_scales[static_cast<int64_t>(page) * a.c.heads + it.head];
-                    }
-                    fine = warp_wait(&k_empty[stage], phase ^ 1U);
-                    if (!fine)
-                    {
-                        break;
-                    }
-                    store(rk, k_tiles + stage * shape::KV_BYTES);
-                    if (warp == 8 && lane < GROUPS)
-                    {
-                        vs = fminf(fmaxf(vs, pow2_int(E_MIN)), pow2_int(E_MAX));
-                        scales[(n % TC_GROUPS) * GROUPS + lane] =
-                            make_float4(ks, ks == 0.0F ? -INFINITY : log2_fast(vs), __fdividef(1.0F, vs), 0.0F);
-                    }
-                    fence_async_proxy();
-                    tc::mbar_arrive(&k_full[stage]);
-                    load(rk, a.c.keys, j + 1, next);
-                    fine = warp_wait(&v_empty[stage], phase ^ 1U);
-                    if (!fine)
-                    {
-                        break;
-                    }
-                    if (nearest < furthest && (first_tile + j + 1) * ROWS > nearest)
-                    {
-                        clean(rv, j);
-                    }
-                    store(rv, v_tiles + stage * shape::KV_BYTES);
-                    fence_async_proxy();
-                    tc::mbar_arrive(&v_full[stage]);
-                    load(rv, a.c.values, j + 1, next);
-                    page = next;
-                    next = page_of(j + 2);
                 }
+                r[i] = make_uint4(x[0], x[1], x[2], x[3]);
             }
-            else if (my_tile < NQ && lane == 0)
+        };
+        uint4 rk[PIECES];
+        uint4 rv[PIECES];
+        load(rk, a.c.keys, 0);
+        load(rv, a.c.values, 0);
+        for (int j = 0; j < count; ++j, ++n)
+        {
+            const uint32_t stage = n % shape::STAGES;
+            const uint32_t phase = (n / shape::STAGES) & 1U;
+            if (j - base == AHEAD)
             {
-                // ================= issue of the products =================
-                constexpr uint32_t s_idesc = tc::instr_desc(0U, 128U, ROWS);
-                constexpr uint32_t o_idesc = tc::instr_desc(0U, 128U, DIM) | (1U << 16); // second operand along its outputs
-                const uint32_t s_addr = tmem + my_tile * ROWS;
-                const uint32_t o_addr = tmem + shape::O_COL + my_tile * DIM;
-                const uint64_t q_desc = tc::smem_desc_sw128(q_tiles + my_tile * shape::Q_BYTES);
-                for (int j = 0; j < count; ++j)
+                base = j;
+                page_now = page_next;
+                ks_now = ks_next;
+                vs_now = vs_next;
+                page_next = pages_from(j + AHEAD);
+            }
+            if (warp == 0 && j - base == AHEAD / 2)
+            {
+                scales_of(page_next, ks_next, vs_next);
+            }
+            if (!warp_wait(&st.k_empty[stage], phase ^ 1U))
+            {
+                return false;
+            }
+            store(rk, st.k_tiles + stage * shape::KV_BYTES);
+            if (warp == 0 && lane / shape::GROUPS == j - base)
+            {
+                const float vs = fminf(fmaxf(vs_now, pow2_int(E_MIN)), pow2_int(E_MAX));
+                st.scales[(n % RING) * shape::GROUPS + lane % shape::GROUPS] =
+                    make_float4(ks_now, ks_now == 0.0F ? -INFINITY : log2_fast(vs), __fdividef(1.0F, vs), 0.0F);
+            }
+            fence_async_proxy();
+            tc::mbar_arrive(&st.k_full[stage]);
+            load(rk, a.c.keys, j + 1);
+            if (!warp_wait(&st.v_empty[stage], phase ^ 1U))
+            {
+                return false;
+            }
+            if (nearest < furthest && (first_tile + j + 1) * ROWS > nearest)
+            {
+                clean(rv, j);
+            }
+            store(rv, st.v_tiles + stage * shape::KV_BYTES);
+            fence_async_proxy();
+            tc::mbar_arrive(&st.v_full[stage]);
+            load(rv, a.c.values, j + 1);
+        }
+        ++items;
+    } while (w.next(a));
+    return true;
+}
+
+// ================= issue of the products of a query tile: one thread =================
+template <int DIM>
+__device__ __forceinline__ bool issue_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem,
+                                           int my_tile)
+{
+    using shape = tc_shape<DIM>;
+    constexpr uint32_t s_idesc = tc::instr_desc(0U, 128U, shape::ROWS);
+    constexpr uint32_t o_idesc = tc::instr_desc(0U, 128U, DIM) | (1U << 16); // second operand along its outputs
+    const uint32_t s_base = tmem + my_tile * 2 * shape::ROWS;
+    const uint32_t o_addr = tmem + shape::O_COL + my_tile * DIM;
+    const uint64_t q_desc = tc::smem_desc_sw128(st.q_tiles + my_tile * shape::Q_BYTES);
+    uint32_t n = 0;       // tiles of the block so far
+    uint32_t s_tiles = 0; // and of this query tile
+    uint32_t q_items = 0;
+    do
+    {
+        const int count = w.count();
+        if (my_tile >= w.query_tiles())
+        {
+            // no rows in this query tile: give the stages back
+            for (int j = 0; j < count; ++j, ++n)
+            {
+                const uint32_t stage = n % shape::STAGES;
+                const uint32_t phase = (n / shape::STAGES) & 1U;
+                if (!ptx::mbar_wait_bounded_spin(&st.k_full[stage], phase))
                 {
-                    const uint32_t n = kv_tiles + j;
-                    const uint32_t stage = n & 1;
-                    const uint32_t phase = (n >> 1) & 1U;
-                    fine = ptx::mbar_wait_bounded_spin(&k_full[stage], phase);
-                    // the weights that lie over the scores have to be read before
-                    if (fine && my_tile < tiles && j > 0)
-                    {
-                        fine = ptx::mbar_wait_bounded_spin(&o_done[my_tile], (s_tiles - 1) & 1U);
-                    }
-                    if (!fine)
-                    {
-                        break;
-                    }
-                    if (my_tile >= tiles) // no rows in this query tile: give the stages back
-                    {
-                        tc::mbar_arrive(&k_empty[stage]);
-                        fine = ptx::mbar_wait_bounded_spin(&v_full[stage], phase);
-                        if (!fine)
-                        {
-                            break;
-                        }
-                        tc::mbar_arrive(&v_empty[stage]);
-                        continue;
-                    }
-                    tc::fence_after_sync();
-                    const uint64_t k_desc = tc::smem_desc_sw128(k_tiles + stage * shape::KV_BYTES);
-#pragma unroll
-                    for (int k = 0; k < DIM / 16; ++k)
-                    {
-                        tc::mma<true>(s_addr, q_desc + (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2,
-                                      k_desc + (k >> 2) * (ROWS * 128 >> 4) + (k & 3) * 2, s_idesc, k != 0);
-                    }
-                    tc::mbar_arrive(&s_full[my_tile]);
-                    tc::mma_commit(&s_full[my_tile]);
-                    tc::mma_commit(&k_empty[stage]);
-                    fine = ptx::mbar_wait_bounded_spin(&v_full[stage], phase) &&
-                           ptx::mbar_wait_bounded_spin(&p_full[my_tile], s_tiles & 1U);
-                    if (!fine)
-                    {
-                        break;
-                    }
-                    ++s_tiles;
-                    tc::fence_after_sync();
-                    const uint64_t v_desc = values_desc(v_tiles + stage * shape::KV_BYTES, ROWS * 128);
-#pragma unroll
-                    for (int k = 0; k < ROWS / 16; ++k)
-                    {
-                        mma_ts(o_addr, s_addr + k * 8, v_desc + k * (16 * 128 >> 4), o_idesc, j != 0 || k != 0);
-                    }
-                    tc::mbar_arrive(&o_done[my_tile]);
-                    tc::mma_commit(&o_done[my_tile]);
-                    tc::mma_commit(&v_empty[stage]);
+                    return false;
                 }
-            }
-            kv_tiles += count;
-            if (at == it.begin && !whole && t == 0)
-            {
-                a.joins[blockIdx.x] = make_int4(it.first_token, it.head, it.column0, it.columns);
-                a.join_end[blockIdx.x] = static_cast<int>(((it.end * blocks) - 1) / total);
-            }
-            // all of the block leaves together when a wait has expired
-            if (__syncthreads_or(fine ? 0 : 1) != 0)
-            {
-                if (!fine)
+                tc::mbar_arrive(&st.k_empty[stage]);
+                if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], phase))
                 {
-                    atomicOr(status, DEVICE_STATUS_TIMEOUT);
+                    return false;
                 }
-                break;
+                tc::mbar_arrive(&st.v_empty[stage]);
+            }
+            continue;
+        }
+        if (count == 0)
+        {
+            continue;
+        }
+        // scores of tile j into score tile (s_tiles + j) % 2, whose weights the product before last has read
+        auto scores = [&](int j) {
+            const uint32_t stage = (n + j) % shape::STAGES;
+            const uint32_t s = s_tiles + j;
+            if (!ptx::mbar_wait_bounded_spin(&st.k_full[stage], ((n + j) / shape::STAGES) & 1U))
+            {
+                return false;
             }
             tc::fence_after_sync();
-            at = seg_end;
-            if (at >= share_end)
+            const uint64_t k_desc = tc::smem_desc_sw128(st.k_tiles + stage * shape::KV_BYTES);
+#pragma unroll
+            for (int k = 0; k < DIM / 16; ++k)
             {
-                break;
+                tc::mma<true>(s_base + (s & 1) * shape::ROWS, q_desc + (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2,
+                              k_desc + (k >> 2) * (shape::ROWS * 128 >> 4) + (k & 3) * 2, s_idesc, k != 0);
             }
-            it.begin = it.end;
-            it.column0 += shape::COLS;
-            if (it.column0 >= it.columns)
+            tc::mbar_arrive(&st.s_full[my_tile * 2 + (s & 1)]);
+            tc::mma_commit(&st.s_full[my_tile * 2 + (s & 1)]);
+            tc::mma_commit(&st.k_empty[stage]);
+            return true;
+        };
+        // both score tiles are free once the last product of the item before has been through
+        if (!ptx::mbar_wait_bounded_spin(&st.q_full[my_tile], q_items & 1U) ||
+            (s_tiles > 0 && !ptx::mbar_wait_bounded_spin(&st.o_done[my_tile], (s_tiles - 1) & 1U)) || !scores(0))
+        {
+            return false;
+        }
+        ++q_items;
+        for (int j = 0; j < count; ++j)
+        {
+            if (j + 1 < count)
             {
-                it.column0 = 0;
-                if (++it.head == a.c.heads)
+                if ((j > 0 && !ptx::mbar_wait_bounded_spin(&st.o_done[my_tile], (s_tiles + j - 1) & 1U)) || !scores(j + 1))
                 {
-                    it.head = 0;
-                    do
-                    {
-                        ++it.request; // requests without tokens have no units; `at` < total, so one follows
-                        q = request_of(a.b, it.request);
-                    } while (q.count == 0);
-                    it.first_token = q.first;
-                    it.columns = q.count * a.group;
+                    return false;
                 }
             }
-            it.end = it.begin + units_of_block<shape>(a, q, it.column0);
+            const uint32_t stage = (n + j) % shape::STAGES;
+            const uint32_t s = s_tiles + j;
+            if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], ((n + j) / shape::STAGES) & 1U) ||
+                !ptx::mbar_wait_bounded_spin(&st.p_full[my_tile * 2 + (s & 1)], (s >> 1) & 1U))
+            {
+                return false;
+            }
+            tc::fence_after_sync();
+            const uint64_t v_desc = values_desc(st.v_tiles + stage * shape::KV_BYTES, shape::ROWS * 128);
+#pragma unroll
+            for (int k = 0; k < shape::ROWS / 16; ++k)
+            {
+                mma_ts(o_addr, s_base + (s & 1) * shape::ROWS + k * 8, v_desc + k * (16 * 128 >> 4), o_idesc, j != 0 || k != 0);
+            }
+            tc::mbar_arrive(&st.o_done[my_tile]);
+            tc::mma_commit(&st.o_done[my_tile]);
+            tc::mma_commit(&st.v_empty[stage]);
         }
+        n += count;
+        s_tiles += count;
+    } while (w.next(a));
+    return true;
+}
+
+// Warps 0-3 and 4-7: softmax of query tile 0 and 1, one thread per row.  Warps 8-11: converters, codes
+// to halves.  Warps 12 and 13: one thread each issues the products of a query tile.
+//
+// A tile of 64 positions goes round like this.  The converters bring 16 codes per thread and load from
+// the cache a tile ahead, turn them into halves and store them in the swizzled layout the tensor cores
+// read (STAGES tiles each of keys and values).  S = Q K^T lands in one of a query tile's two score tiles
+// in tensor memory; a softmax thread takes its row, and writes the weights as halves over the scores;
+// O += P V takes them from there as its first operand, and the values as they lie, contiguous
+// along the outputs.  The next scores are computed while the softmax runs.  O stays in tensor memory;
+// it is touched only when a row's reference point has to move by more than 2^8 (rarely after the first
+// tile).  The roles meet at mbarriers alone, also from one item to the next, so the next item's first
+// tiles are converted while the last one is being written.
+//   Rings: the converters are at most STAGES tiles ahead of the scores, and scores need the product
+// before last, whose weights their softmax has written: a slot of RING >= STAGES + 2 is read before it is
+// written again.  The first-NaN slots go by items of at least one tile, so the same holds for them.
+//   Barriers that one role completes and another reads the fruits of (scales, NaN) carry an arrival of
+// the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
+//
+// Bound by the exponentials (16 per clock and SM: 1024 clocks for 256 rows x 64 positions) and the
+// tensor cores (4 products of 128 x 64 x 128: about 1200 clocks) alike.
+template <int DIM>
+__global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)
+{
+    using shape = tc_shape<DIM>;
+    constexpr int WARPS_HERE = TC_THREADS / 32;
+    extern __shared__ unsigned char raw[];
+    __shared__ int64_t s_words[WARPS_HERE];
+    __shared__ int s_found;
+    __shared__ uint32_t s_tmem;
+    const int t = threadIdx.x;
+    const int warp = t >> 5;
+    const int lane = t & 31;
+    tc_state st;
+    st.q_tiles = raw + ((1024U - (ptx::smem_addr(raw) & 1023U)) & 1023U);
+    st.k_tiles = st.q_tiles + shape::NQ * shape::Q_BYTES;
+    st.v_tiles = st.k_tiles + shape::STAGES * shape::KV_BYTES;
+    st.scales = reinterpret_cast<float4*>(st.v_tiles + shape::STAGES * shape::KV_BYTES);
+    st.first_nan = reinterpret_cast<uint32_t*>(st.scales + RING * shape::GROUPS);
+    st.k_full = reinterpret_cast<uint64_t*>(st.first_nan + RING * DIM);
+    st.k_empty = st.k_full + 4;
+    st.v_full = st.k_full + 8;
+    st.v_empty = st.k_full + 12;
+    st.s_full = st.k_full + 16;
+    st.p_full = st.k_full + 20;
+    st.o_done = st.k_full + 24;
+    st.q_full = st.k_full + 26;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (t == 0)
+    {
+        a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+        for (int i = 0; i < shape::STAGES; ++i)
+        {
+            ptx::mbar_init(&st.k_full[i], CONVERTERS);
+            ptx::mbar_init(&st.v_full[i], CONVERTERS);
+            ptx::mbar_init(&st.k_empty[i], shape::NQ);
+            ptx::mbar_init(&st.v_empty[i], shape::NQ);
+        }
+        for (int i = 0; i < 4; ++i)
+        {
+            ptx::mbar_init(&st.s_full[i], 2);
+            ptx::mbar_init(&st.p_full[i], 128);
+        }
+        for (int i = 0; i < 2; ++i)
+        {
+            ptx::mbar_init(&st.o_done[i], 2);
+            ptx::mbar_init(&st.q_full[i], 128);
+        }
+        ptx::mbar_init_fence();
+    }
+    for (int d = t; d < RING * DIM; d += TC_THREADS)
+    {
+        st.first_nan[d] = 0U;
+    }
+    if (warp == 0)
+    {
+        tc::tmem_alloc(&s_tmem, shape::TMEM_COLS);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = s_tmem;
+
+    int64_t sum = 0;
+    for (int r = t; r < a.b.requests; r += TC_THREADS)
+    {
+        sum += units_of_head<shape>(a, request_of(a.b, r)) * a.c.heads;
+    }
+    const int64_t total = block_sum<WARPS_HERE>(sum, s_words);
+    const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total);
+    if (blockIdx.x < blocks)
+    {
+        walk<shape> w{};
+        w.at = blockIdx.x * total / blocks;
+        w.share_end = (blockIdx.x + 1) * total / blocks;
+        int64_t first = 0;
+        w.it.request = find_request<shape, WARPS_HERE>(a, w.at, &first, s_words, &s_found);
+        w.q = request_of(a.b, w.it.request);
+        const int64_t per_head = units_of_head<shape>(a, w.q);
+        w.it.head = static_cast<int>((w.at - first) / per_head);
+        w.it.begin = first + w.it.head * per_head;
+        w.it.first_token = w.q.first;
+        w.it.columns = w.q.count * a.group;
+        w.it.end = w.it.begin + units_of_block<shape>(a, w.q, 0);
+        while (w.at >= w.it.end)
+        {
+            w.it.column0 += shape::COLS;
+            w.it.begin = w.it.end;
+            w.it.end += units_of_block<shape>(a, w.q, w.it.column0);
+        }
+        bool fine = true;
+        if (warp < 8)
+        {
+            more_registers<SOFTMAX_REGISTERS>();
+            if (shape::NQ == 2 || warp < 4)
+            {
+                fine = softmax_role<DIM>(a, st, w, tmem);
+            }
+        }
+        else if (warp < 12)
+        {
+            fewer_registers<CONVERT_REGISTERS>();
+            fine = convert_role<DIM>(a, st, w);
+        }
+        else
+        {
+            fewer_registers<ISSUE_REGISTERS>();
+            if (warp < 12 + shape::NQ && lane == 0)
+            {
+                fine = issue_role<DIM>(a, st, w, tmem, warp - 12);
+            }
+            else if (warp == 15 && lane == 0)
+            {
+                // the item that begins here and ends in a later block, if there is one: the last of the share
+                while (w.segment_end() < w.share_end)
+                {
+                    w.next(a);
+                }
+                if (w.at == w.it.begin && w.it.end > w.share_end)
+                {
+                    a.joins[blockIdx.x] = make_int4(w.it.first_token, w.it.head, w.it.column0, w.it.columns);
+                    a.join_end[blockIdx.x] = static_cast<int>((w.it.end * blocks - 1) / total);
+                }
+            }
+        }
+        if (!fine)
+        {
+            atomicOr(status, DEVICE_STATUS_TIMEOUT);
+        }
+        __syncwarp();
     }
     tc::fence_before_sync();
     __syncthreads();
