@@ -38,7 +38,8 @@ struct tc_shape
     static constexpr int O_COL = NQ * 2 * ROWS;  // tensor memory: two score tiles per query tile, then the sums
     static constexpr int USED_COLS = O_COL + NQ * DIM;
     static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
-    static constexpr int TAIL = RING * GROUPS * 16 + RING * DIM * 4 + 32 * 8; // scales, first NaN, barriers
+    static constexpr int NANS = DIM + 4; // words of a first-NaN slot: the dimensions, then the largest of them
+    static constexpr int TAIL = RING * GROUPS * 16 + RING * NANS * 4 + 32 * 8; // scales, first NaN, barriers
     static constexpr int BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + TAIL + 1024;
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(BYTES <= 227 * 1024, "shared memory");
@@ -96,6 +97,35 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Two FP32 numbers in a register pair.
+__device__ __forceinline__ uint64_t pair_of(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+
+__device__ __forceinline__ float2 floats_of_pair(uint64_t r)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+    return f;
+}
+
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // Largest logit of a row of 64 scores, 16 scores to a scale; with CUT only columns below `limit` count.
 template <bool CUT>
 __device__ __forceinline__ float row_top(const uint32_t (&s)[2][32], const float4* scales, float factor, int limit)
@@ -139,23 +169,27 @@ __device__ __forceinline__ float row_weights(const uint32_t (&s)[2][32], uint32_
         const float4 k = scales[g];
         const float f = factor * k.x;
         const float add = k.y + bias;
-        float even = 0.0F;
-        float odd = 0.0F;
+        const uint64_t ff = pair_of(f, f);
+        const uint64_t aa = pair_of(add, add);
+        uint64_t sum = 0;
 #pragma unroll
         for (int i = 0; i < 16; i += 2)
         {
-            float x = exp2_fast(fmaf(__uint_as_float(s[g / 2][g % 2 * 16 + i]), f, add));
-            float y = exp2_fast(fmaf(__uint_as_float(s[g / 2][g % 2 * 16 + i + 1]), f, add));
+            float2 x = floats_of_pair(fma_pair(pair_of(__uint_as_float(s[g / 2][g % 2 * 16 + i]),
+                                                       __uint_as_float(s[g / 2][g % 2 * 16 + i + 1])),
+                                               ff, aa));
+            x.x = exp2_fast(x.x);
+            x.y = exp2_fast(x.y);
             if constexpr (CUT)
             {
-                x = g * 16 + i < limit ? x : 0.0F;
-                y = g * 16 + i + 1 < limit ? y : 0.0F;
+                x.x = g * 16 + i < limit ? x.x : 0.0F;
+                x.y = g * 16 + i + 1 < limit ? x.y : 0.0F;
             }
-            even += x;
-            odd += y;
-            p[g * 8 + i / 2] = pack_half2(x, y);
+            sum = i == 0 ? pair_of(x.x, x.y) : add_pair(sum, pair_of(x.x, x.y));
+            p[g * 8 + i / 2] = pack_half2(x.x, x.y);
         }
-        l = fmaf(even + odd, k.z, l);
+        const float2 total = floats_of_pair(sum);
+        l = fmaf(total.x + total.y, k.z, l);
     }
     return l;
 }
@@ -238,7 +272,7 @@ struct tc_state
     unsigned char* k_tiles;
     unsigned char* v_tiles;
     float4* scales;     // [RING][GROUPS]: key scale, log2 of the value scale, its inverse
-    uint32_t* first_nan; // [RING][DIM]: nan_key
+    uint32_t* first_nan; // [RING][NANS]: nan_key
     uint64_t* k_full;   // [STAGES]
     uint64_t* k_empty;
     uint64_t* v_full;
@@ -288,20 +322,28 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                     }
                     return __half22float2(*reinterpret_cast<const __half2*>(&x));
                 };
-                float top = 0.0F;
+                // both 16-bit types order like their bits once the sign is gone
+                uint32_t most = 0;
 #pragma unroll 8
                 for (int i = 0; i < DIM / 8; ++i)
                 {
                     const uint4 v = real ? __ldg(from + i) : make_uint4(0U, 0U, 0U, 0U);
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffU, v.y & 0x7fff7fffU),
+                                                   __vmaxu2(v.z & 0x7fff7fffU, v.w & 0x7fff7fffU)));
+                }
+                most = max(most & 0xffffU, most >> 16);
+                const uint32_t infinite = a.dtype == BITSKNN_BF16 ? 0x7f80U : 0x7c00U;
+                if (most >= infinite)
+                {
+                    // infinities and NaN set no scale: the largest finite entry
+                    most = 0;
+                    for (int i = 0; i < DIM; ++i)
                     {
-                        const float2 f = floats(x[j]);
-                        top = fabsf(f.x) < INFINITY ? fmaxf(top, fabsf(f.x)) : top;
-                        top = fabsf(f.y) < INFINITY ? fmaxf(top, fabsf(f.y)) : top;
+                        const uint32_t x = reinterpret_cast<const uint16_t*>(from)[i] & 0x7fffU;
+                        most = x < infinite ? max(most, x) : most;
                     }
                 }
+                const float top = floats(most).x;
                 // the same scaling as pack_column: a power of two that puts the largest entry into
                 // [2^14, 2^15); the sign of the scale goes with the query
                 const int e = max(static_cast<int>(__float_as_uint(top) >> 23), 1) - 127;
@@ -393,11 +435,12 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
             tc::fence_after_sync();
             const bool whole = w.at == w.it.begin && w.segment_end() == w.it.end;
             const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (w.at == w.it.begin ? 1 : 0);
-            const uint32_t* const first_nan = st.first_nan + (items % RING) * DIM;
+            const uint32_t* const first_nan = st.first_nan + (items % RING) * shape::NANS;
             // a key of this item at least as large stands for a position below `see`
             const int cut_base = visible_of(a.b, w.q, w.it.column0 / a.group) / shape::ROWS * shape::ROWS;
             const uint32_t seen_nan = see > cut_base ? nan_key(items, see - 1 - cut_base) : 0xffffffffU;
-            const float inverse = l == 0.0F ? 0.0F : 1.0F / l;
+            const bool nan_here = count > 0 && first_nan[DIM] >= seen_nan;
+            const float inverse = l == 0.0F ? 1.0F : 1.0F / l; // l = 0: nothing was seen; a NaN makes the row NaN
             uint16_t* const out =
                 static_cast<uint16_t*>(a.out) + row_token * a.out_stride + static_cast<int64_t>(qhead) * DIM;
             const bool aligned =
@@ -415,10 +458,13 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                 }
                 if (real)
                 {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    if (l == 0.0F || nan_here)
                     {
-                        o[i] = count > 0 ? (first_nan[c + i] >= seen_nan ? 0x7fc00000U : o[i]) : 0U;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                        {
+                            o[i] = l != 0.0F ? (first_nan[c + i] >= seen_nan ? 0x7fc00000U : o[i]) : 0U;
+                        }
                     }
                     if (!whole)
                     {
@@ -430,8 +476,7 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                     }
                     else
                     {
-                        // l = 0: nothing was seen; a NaN in l makes the row NaN
-                        auto result = [&](uint32_t x) { return l == 0.0F ? 0.0F : __uint_as_float(x) * inverse; };
+                        auto result = [&](uint32_t x) { return __uint_as_float(x) * inverse; };
                         auto pair = [&](uint32_t x, uint32_t y) {
                             if (a.dtype == BITSKNN_BF16)
                             {
@@ -512,43 +557,65 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         const int furthest = visible_of(a.b, w.q, w.last_column() / a.group);
         const int nearest = visible_of(a.b, w.q, w.it.column0 / a.group);
         const int32_t* const table = a.b.table + w.it.request * a.b.table_ld;
-        uint32_t* const first_nan = st.first_nan + (items % RING) * DIM;
+        uint32_t* const first_nan = st.first_nan + (items % RING) * shape::NANS;
         const int cut_base = nearest / ROWS * ROWS;
-        auto pages_from = [&](int j) { // page of this lane's 16 positions, AHEAD tiles from tile j on
+        // AHEAD tiles from tile j on, this lane's 16 positions: their page, and where their first row lies
+        auto pages_from = [&](int j) {
             const int pos = (first_tile + j) * ROWS + lane * 16;
             const int p = j < count && pos < furthest ? table[pos >> a.c.page_shift] : -1;
             return p < a.c.pages ? p : -1;
         };
-        int page_now = pages_from(0);
-        int page_next = pages_from(AHEAD);
+        auto offset_of = [&](int page, int j) -> int64_t {
+            const int pos = (first_tile + j) * ROWS + lane * 16;
+            return page < 0 ? -1
+                            : page * a.c.page_stride +
+                                  ((static_cast<int64_t>(w.it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
+        };
         auto scales_of = [&](int page, float& ks, float& vs) {
             ks = page < 0 ? 0.0F : a.c.key_scales[static_cast<int64_t>(page) * a.c.heads + w.it.head];
             vs = page < 0 ? 1.0F : a.c.value_scales[static_cast<int64_t>(page) * a.c.heads + w.it.head];
         };
+        const int page_first = pages_from(0);
+        int page_next = pages_from(AHEAD);
+        int64_t offset_now = offset_of(page_first, 0);
         float ks_now = 0.0F, vs_now = 1.0F, ks_next = 0.0F, vs_next = 1.0F;
         if (warp == 0)
         {
-            scales_of(page_now, ks_now, vs_now);
+            scales_of(page_first, ks_now, vs_now);
         }
-        int base = 0; // first tile of page_now
-        auto load = [&](uint4 (&r)[PIECES], const uint8_t* codes, int j) {
-            const int pages = j - base < AHEAD ? page_now : page_next;
+        int base = 0; // first tile of offset_now
+        const int whole_tiles = furthest / ROWS - first_tile; // tiles before this one have all their rows
+        int64_t from[SLABS]; // of the tile loaded next, this thread's pieces; -1: absent
+        auto locate = [&](int j) {
+            if (j - base == AHEAD)
+            {
+                base = j;
+                offset_now = offset_of(page_next, j);
+                ks_now = ks_next;
+                vs_now = vs_next;
+                page_next = pages_from(j + AHEAD);
+            }
 #pragma unroll
             for (int i = 0; i < SLABS; ++i)
             {
-                const int pos = (first_tile + j) * ROWS + i * 32 + row0;
-                const int p = __shfl_sync(FULL_MASK, pages, (j % AHEAD) * shape::GROUPS + i * 2 + (warp >> 1));
-                const uint8_t* const from = codes + max(p, 0) * a.c.page_stride +
-                                            ((static_cast<int64_t>(w.it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM +
-                                            piece * 16;
-                const bool there = j < count && p >= 0 && pos < furthest;
+                const int64_t o =
+                    __shfl_sync(FULL_MASK, offset_now, (j - base) * shape::GROUPS + i * 2 + (warp >> 1));
+                const bool there = o >= 0 && j < count &&
+                                   (j < whole_tiles || (first_tile + j) * ROWS + i * 32 + row0 < furthest);
+                from[i] = there ? o + (row0 & 15) * DIM + piece * 16 : -1;
+            }
+        };
+        auto load = [&](uint4 (&r)[PIECES], const uint8_t* codes) {
+#pragma unroll
+            for (int i = 0; i < SLABS; ++i)
+            {
 #pragma unroll
                 for (int b = 0; b < BLK; ++b)
                 {
                     r[i * BLK + b] = make_uint4(0U, 0U, 0U, 0U);
-                    if (there && (DIM % 64 == 0 || b * 64 + piece * 16 < DIM))
+                    if (from[i] >= 0 && (DIM % 64 == 0 || b * 64 + piece * 16 < DIM))
                     {
-                        r[i * BLK + b] = __ldg(reinterpret_cast<const uint4*>(from + b * 64));
+                        r[i * BLK + b] = __ldg(reinterpret_cast<const uint4*>(codes + from[i] + b * 64));
                     }
                 }
             }
@@ -595,6 +662,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                             if ((hit >> (8 * z + 7)) & 1U)
                             {
                                 atomicMax(&first_nan[d + z], nan_key(items, pos - cut_base));
+                                atomicMax(&first_nan[DIM], nan_key(items, pos - cut_base));
                                 x[y] &= ~(0xffU << (8 * z));
                             }
                         }
@@ -605,24 +673,13 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         };
         uint4 rk[PIECES];
         uint4 rv[PIECES];
-        load(rk, a.c.keys, 0);
-        load(rv, a.c.values, 0);
+        locate(0);
+        load(rk, a.c.keys);
+        load(rv, a.c.values);
         for (int j = 0; j < count; ++j, ++n)
         {
             const uint32_t stage = n % shape::STAGES;
             const uint32_t phase = (n / shape::STAGES) & 1U;
-            if (j - base == AHEAD)
-            {
-                base = j;
-                page_now = page_next;
-                ks_now = ks_next;
-                vs_now = vs_next;
-                page_next = pages_from(j + AHEAD);
-            }
-            if (warp == 0 && j - base == AHEAD / 2)
-            {
-                scales_of(page_next, ks_next, vs_next);
-            }
             if (!warp_wait(&st.k_empty[stage], phase ^ 1U))
             {
                 return false;
@@ -634,9 +691,14 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 st.scales[(n % RING) * shape::GROUPS + lane % shape::GROUPS] =
                     make_float4(ks_now, ks_now == 0.0F ? -INFINITY : log2_fast(vs), __fdividef(1.0F, vs), 0.0F);
             }
+            if (warp == 0 && j - base == AHEAD / 2)
+            {
+                scales_of(page_next, ks_next, vs_next);
+            }
             fence_async_proxy();
             tc::mbar_arrive(&st.k_full[stage]);
-            load(rk, a.c.keys, j + 1);
+            locate(j + 1);
+            load(rk, a.c.keys);
             if (!warp_wait(&st.v_empty[stage], phase ^ 1U))
             {
                 return false;
@@ -648,7 +710,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
             store(rv, st.v_tiles + stage * shape::KV_BYTES);
             fence_async_proxy();
             tc::mbar_arrive(&st.v_full[stage]);
-            load(rv, a.c.values, j + 1);
+            load(rv, a.c.values);
         }
         ++items;
     } while (w.next(a));
@@ -795,7 +857,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
     st.v_tiles = st.k_tiles + shape::STAGES * shape::KV_BYTES;
     st.scales = reinterpret_cast<float4*>(st.v_tiles + shape::STAGES * shape::KV_BYTES);
     st.first_nan = reinterpret_cast<uint32_t*>(st.scales + RING * shape::GROUPS);
-    st.k_full = reinterpret_cast<uint64_t*>(st.first_nan + RING * DIM);
+    st.k_full = reinterpret_cast<uint64_t*>(st.first_nan + RING * shape::NANS);
     st.k_empty = st.k_full + 4;
     st.v_full = st.k_full + 8;
     st.v_empty = st.k_full + 12;
@@ -827,7 +889,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
         }
         ptx::mbar_init_fence();
     }
-    for (int d = t; d < RING * DIM; d += TC_THREADS)
+    for (int d = t; d < RING * shape::NANS; d += TC_THREADS)
     {
         st.first_nan[d] = 0U;
     }
