@@ -97,6 +97,19 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Waits for this thread's loads from tensor memory.  The registers pass through the wait, so that nothing
+// that uses them can be moved in front of it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+
 // Two FP32 numbers in a register pair.
 __device__ __forceinline__ uint64_t pair_of(float x, float y)
 {
@@ -158,11 +171,13 @@ __device__ __forceinline__ float row_top(const uint32_t (&s)[2][32], const float
     return top;
 }
 
-// Scores to weights 2^(logit + bias) as halves; returns l plus the row's share of the denominator.
+// Scores to weights 2^(logit + bias) as halves.  x: sum of the weights, y: sum of the weights over their
+// value scales (the row's share of the denominator).
 template <bool CUT>
-__device__ __forceinline__ float row_weights(const uint32_t (&s)[2][32], uint32_t (&p)[32], const float4* scales,
-                                             float factor, float bias, int limit, float l)
+__device__ __forceinline__ float2 row_weights(const uint32_t (&s)[2][32], uint32_t (&p)[32], const float4* scales,
+                                              float factor, float bias, int limit)
 {
+    float2 sums = make_float2(0.0F, 0.0F);
 #pragma unroll
     for (int g = 0; g < 4; ++g)
     {
@@ -189,9 +204,10 @@ __device__ __forceinline__ float row_weights(const uint32_t (&s)[2][32], uint32_
             p[g * 8 + i / 2] = pack_half2(x.x, x.y);
         }
         const float2 total = floats_of_pair(sum);
-        l = fmaf(total.x + total.y, k.z, l);
+        sums.x += total.x + total.y;
+        sums.y = fmaf(total.x + total.y, k.z, sums.y);
     }
-    return l;
+    return sums;
 }
 
 template <int N>
@@ -279,7 +295,7 @@ struct tc_state
     uint64_t* v_empty;
     uint64_t* s_full;   // [query tile][score tile]
     uint64_t* p_full;   // [query tile][score tile]
-    uint64_t* o_done;   // [query tile]
+    uint64_t* o_done;   // [query tile][score tile]
     uint64_t* q_full;   // [query tile]
 };
 
@@ -386,19 +402,33 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                 uint32_t s[2][32];
                 tc::tmem_ld_32x32(s_addr, s[0]);
                 tc::tmem_ld_32x32(s_addr + 32, s[1]);
-                tc::tmem_ld_wait();
-                const float top =
-                    cut ? row_top<true>(s, scales, factor, see - pos) : row_top<false>(s, scales, factor, 0);
-                if (__any_sync(FULL_MASK, top > m + WEIGHT_SLACK))
+                tmem_ld_wait(s[0]);
+                tmem_ld_wait(s[1]);
+                // Weights against the reference point as it stands.  They are positive, so a sum of at most
+                // 2^15 says that none is too large for a half and nothing has to be compared; only when the
+                // sum is larger (or NaN, or there is no reference point yet) is the maximum looked for.
+                uint32_t p[32];
+                auto weigh = [&] {
+                    const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
+                    return cut ? row_weights<true>(s, p, scales, factor, bias, see - pos)
+                               : row_weights<false>(s, p, scales, factor, bias, 0);
+                };
+                float2 sums = weigh();
+                if (__any_sync(FULL_MASK, m == -INFINITY || !(sums.x <= 32768.0F)))
                 {
-                    const float raised = fmaxf(top, m);
+                    tc::tmem_ld_32x32(s_addr, s[0]);
+                    tc::tmem_ld_32x32(s_addr + 32, s[1]);
+                    tmem_ld_wait(s[0]);
+                    tmem_ld_wait(s[1]);
+                    const float raised = fmaxf(
+                        cut ? row_top<true>(s, scales, factor, see - pos) : row_top<false>(s, scales, factor, 0), m);
                     const float keep = m == -INFINITY ? 0.0F : exp2_fast(m - raised);
                     m = raised;
                     l *= keep;
                     if (j > 0)
                     {
                         // the product before this one has to be through with the sums
-                        if (!warp_wait(&st.o_done[my_tile], (s_tiles - 1) & 1U))
+                        if (!warp_wait(&st.o_done[my_tile * 2 + ((s_tiles - 1) & 1)], ((s_tiles - 1) >> 1) & 1U))
                         {
                             return false;
                         }
@@ -408,7 +438,7 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                         {
                             uint32_t o[32];
                             tc::tmem_ld_32x32(o_addr + c, o);
-                            tc::tmem_ld_wait();
+                            tmem_ld_wait(o);
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
                             {
@@ -417,18 +447,16 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                             tmem_st_32(o_addr + c, o);
                         }
                     }
+                    sums = weigh();
                 }
-                const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
-                uint32_t p[32];
-                l = cut ? row_weights<true>(s, p, scales, factor, bias, see - pos, l)
-                        : row_weights<false>(s, p, scales, factor, bias, 0, l);
+                l += sums.y;
                 tmem_st_32(s_addr, p); // over the scores
                 tmem_st_wait();
                 tc::fence_before_sync();
                 tc::mbar_arrive(&st.p_full[my_tile * 2 + buffer]);
             }
             // ---- the row's result ----
-            if (count > 0 && !warp_wait(&st.o_done[my_tile], (s_tiles - 1) & 1U))
+            if (count > 0 && !warp_wait(&st.o_done[my_tile * 2 + ((s_tiles - 1) & 1)], ((s_tiles - 1) >> 1) & 1U))
             {
                 return false;
             }
@@ -454,7 +482,7 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                 if (count > 0)
                 {
                     tc::tmem_ld_32x32(o_addr + c, o);
-                    tc::tmem_ld_wait();
+                    tmem_ld_wait(o);
                 }
                 if (real)
                 {
@@ -586,6 +614,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         int base = 0; // first tile of offset_now
         const int whole_tiles = furthest / ROWS - first_tile; // tiles before this one have all their rows
         int64_t from[SLABS]; // of the tile loaded next, this thread's pieces; -1: absent
+        bool all_there = false; // all pieces of the warp's tile exist
         auto locate = [&](int j) {
             if (j - base == AHEAD)
             {
@@ -595,6 +624,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 vs_now = vs_next;
                 page_next = pages_from(j + AHEAD);
             }
+            bool absent = false;
 #pragma unroll
             for (int i = 0; i < SLABS; ++i)
             {
@@ -603,9 +633,24 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 const bool there = o >= 0 && j < count &&
                                    (j < whole_tiles || (first_tile + j) * ROWS + i * 32 + row0 < furthest);
                 from[i] = there ? o + (row0 & 15) * DIM + piece * 16 : -1;
+                absent |= !there;
             }
+            all_there = DIM % 64 == 0 && !__any_sync(FULL_MASK, absent);
         };
         auto load = [&](uint4 (&r)[PIECES], const uint8_t* codes) {
+            if (all_there)
+            {
+#pragma unroll
+                for (int i = 0; i < SLABS; ++i)
+                {
+#pragma unroll
+                    for (int b = 0; b < BLK; ++b)
+                    {
+                        r[i * BLK + b] = __ldg(reinterpret_cast<const uint4*>(codes + from[i] + b * 64));
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < SLABS; ++i)
             {
@@ -779,21 +824,22 @@ __device__ __forceinline__ bool issue_role(const attend_args& a, const tc_state&
             tc::mma_commit(&st.k_empty[stage]);
             return true;
         };
+        auto product_done = [&](uint32_t s) {
+            return ptx::mbar_wait_bounded_spin(&st.o_done[my_tile * 2 + (s & 1)], (s >> 1) & 1U);
+        };
         // both score tiles are free once the last product of the item before has been through
         if (!ptx::mbar_wait_bounded_spin(&st.q_full[my_tile], q_items & 1U) ||
-            (s_tiles > 0 && !ptx::mbar_wait_bounded_spin(&st.o_done[my_tile], (s_tiles - 1) & 1U)) || !scores(0))
+            (s_tiles > 0 && !product_done(s_tiles - 1)) || !scores(0))
         {
             return false;
         }
         ++q_items;
         for (int j = 0; j < count; ++j)
         {
-            if (j + 1 < count)
+            // the product before has read the weights in the score tile of j + 1
+            if ((j > 0 && !product_done(s_tiles + j - 1)) || (j + 1 < count && !scores(j + 1)))
             {
-                if ((j > 0 && !ptx::mbar_wait_bounded_spin(&st.o_done[my_tile], (s_tiles + j - 1) & 1U)) || !scores(j + 1))
-                {
-                    return false;
-                }
+                return false;
             }
             const uint32_t stage = (n + j) % shape::STAGES;
             const uint32_t s = s_tiles + j;
@@ -809,8 +855,8 @@ __device__ __forceinline__ bool issue_role(const attend_args& a, const tc_state&
             {
                 mma_ts(o_addr, s_base + (s & 1) * shape::ROWS + k * 8, v_desc + k * (16 * 128 >> 4), o_idesc, j != 0 || k != 0);
             }
-            tc::mbar_arrive(&st.o_done[my_tile]);
-            tc::mma_commit(&st.o_done[my_tile]);
+            tc::mbar_arrive(&st.o_done[my_tile * 2 + (s & 1)]);
+            tc::mma_commit(&st.o_done[my_tile * 2 + (s & 1)]);
             tc::mma_commit(&st.v_empty[stage]);
         }
         n += count;
@@ -834,6 +880,9 @@ __device__ __forceinline__ bool issue_role(const attend_args& a, const tc_state&
 //   Rings: the converters are at most STAGES tiles ahead of the scores, and scores need the product
 // before last, whose weights their softmax has written: a slot of RING >= STAGES + 2 is read before it is
 // written again.  The first-NaN slots go by items of at least one tile, so the same holds for them.
+//   Score tiles, weights and products have a barrier per score tile: a role may be a tile ahead of the one
+// that waits, and a wait by parity can tell a phase from the next one only while it is at most one phase
+// of the same barrier away.
 //   Barriers that one role completes and another reads the fruits of (scales, NaN) carry an arrival of
 // the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
 //
@@ -864,7 +913,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
     st.s_full = st.k_full + 16;
     st.p_full = st.k_full + 20;
     st.o_done = st.k_full + 24;
-    st.q_full = st.k_full + 26;
+    st.q_full = st.k_full + 28;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (t == 0)
@@ -881,10 +930,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
         {
             ptx::mbar_init(&st.s_full[i], 2);
             ptx::mbar_init(&st.p_full[i], 128);
+            ptx::mbar_init(&st.o_done[i], 2);
         }
         for (int i = 0; i < 2; ++i)
         {
-            ptx::mbar_init(&st.o_done[i], 2);
             ptx::mbar_init(&st.q_full[i], 128);
         }
         ptx::mbar_init_fence();
