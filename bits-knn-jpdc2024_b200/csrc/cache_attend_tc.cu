@@ -11,7 +11,7 @@ namespace bitsknn
 namespace
 {
 
-constexpr int TC_THREADS = 16 * 32; // warps 14 and 15 only complete the warpgroup of the issuers
+constexpr int TC_THREADS = 16 * 32;
 constexpr int CONVERTERS = 128;
 constexpr int RING = 8;             // scale slots (tiles) and first-NaN slots (items): see cache_attend_tc_kernel
 // Registers of a thread after the split of the 512 x 128 the block is launched with: two warpgroups of
@@ -46,15 +46,34 @@ struct tc_shape
     static_assert(RING >= STAGES + 2, "scale slots");
 };
 
-// D[tmem] (+)= A[tmem] * B[smem], halves, FP32 sums; issued by one thread.
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate)
+// D[tmem] (+)= A[smem] * B[smem] and D[tmem] (+)= A[tmem] * B[smem], halves, FP32 sums; issued by one thread.
+// Descriptors come as their low words (start address, leading offset) and the high word they all share.
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc)
 {
     asm volatile("{\n"
                  ".reg .pred p;\n"
-                 "setp.ne.b32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+                 ".reg .b64 da, db;\n"
+                 "setp.ne.b32 p, %5, 0;\n"
+                 "mov.b64 da, {%1, %3};\n"
+                 "mov.b64 db, {%2, %3};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n"
                  "}\n" ::"r"(d_tmem),
-                 "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1U : 0U)
+                 "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                       bool accumulate)
+{
+    asm volatile("{\n"
+                 ".reg .pred p;\n"
+                 ".reg .b64 db;\n"
+                 "setp.ne.b32 p, %5, 0;\n"
+                 "mov.b64 db, {%2, %3};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n"
+                 "}\n" ::"r"(d_tmem),
+                 "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate ? 1U : 0U)
                  : "memory");
 }
 
@@ -222,6 +241,17 @@ __device__ __forceinline__ void fewer_registers()
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// One arrival for a whole warp, after all its threads have come here (arrivals of single threads on one
+// barrier are served one after the other: 512 of them per tile took a third of the shared-memory pipe).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0)
+    {
+        tc::mbar_arrive(bar);
+    }
+}
+
 // A wait of a whole warp: its threads go on, or give up, together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity)
 {
@@ -381,7 +411,7 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                     st_shared16(to + tile_byte(t & 127, i, 128), h[0], h[1], h[2], h[3]);
                 }
                 fence_async_proxy();
-                tc::mbar_arrive(&st.q_full[my_tile]);
+                warp_arrive(&st.q_full[my_tile]);
             }
             const int nearest = visible_of(a.b, w.q, min(w.it.column0 + my_tile * 128, w.last_column()) / a.group);
             float m = -INFINITY;
@@ -453,7 +483,7 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                 tmem_st_32(s_addr, p); // over the scores
                 tmem_st_wait();
                 tc::fence_before_sync();
-                tc::mbar_arrive(&st.p_full[my_tile * 2 + buffer]);
+                warp_arrive(&st.p_full[my_tile * 2 + buffer]);
             }
             // ---- the row's result ----
             if (count > 0 && !warp_wait(&st.o_done[my_tile * 2 + ((s_tiles - 1) & 1)], ((s_tiles - 1) >> 1) & 1U))
@@ -741,7 +771,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 scales_of(page_next, ks_next, vs_next);
             }
             fence_async_proxy();
-            tc::mbar_arrive(&st.k_full[stage]);
+            warp_arrive(&st.k_full[stage]);
             locate(j + 1);
             load(rk, a.c.keys);
             if (!warp_wait(&st.v_empty[stage], phase ^ 1U))
@@ -754,7 +784,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
             }
             store(rv, st.v_tiles + stage * shape::KV_BYTES);
             fence_async_proxy();
-            tc::mbar_arrive(&st.v_full[stage]);
+            warp_arrive(&st.v_full[stage]);
             load(rv, a.c.values);
         }
         ++items;
@@ -762,111 +792,137 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
     return true;
 }
 
-// ================= issue of the products of a query tile: one thread =================
+// ================= issue of the products of a query tile: one thread for each of the two =================
+// A thread is held while its products run, and what it does between them -- waits, commits, address
+// arithmetic -- adds up to as much again; so the scores and the sums of either query tile have a thread of
+// their own, which only meet at barriers.
 template <int DIM>
-__device__ __forceinline__ bool issue_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem,
-                                           int my_tile)
+__device__ __forceinline__ bool scores_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem,
+                                            int my_tile)
 {
     using shape = tc_shape<DIM>;
-    constexpr uint32_t s_idesc = tc::instr_desc(0U, 128U, shape::ROWS);
-    constexpr uint32_t o_idesc = tc::instr_desc(0U, 128U, DIM) | (1U << 16); // second operand along its outputs
+    constexpr uint32_t idesc = tc::instr_desc(0U, 128U, shape::ROWS);
     const uint32_t s_base = tmem + my_tile * 2 * shape::ROWS;
-    const uint32_t o_addr = tmem + shape::O_COL + my_tile * DIM;
     const uint64_t q_desc = tc::smem_desc_sw128(st.q_tiles + my_tile * shape::Q_BYTES);
-    uint32_t n = 0;       // tiles of the block so far
-    uint32_t s_tiles = 0; // and of this query tile
+    const uint32_t q_lo = static_cast<uint32_t>(q_desc);
+    const uint32_t hi = static_cast<uint32_t>(q_desc >> 32);
+    const uint32_t k_lo0 = static_cast<uint32_t>(tc::smem_desc_sw128(st.k_tiles));
+    uint32_t stage = 0;
+    uint32_t phase = 0;
+    uint32_t s = 0; // score tiles of this query tile so far
     uint32_t q_items = 0;
     do
     {
         const int count = w.count();
-        if (my_tile >= w.query_tiles())
+        const bool active = my_tile < w.query_tiles(); // else no rows: give the stages back
+        if (active && count > 0)
         {
-            // no rows in this query tile: give the stages back
-            for (int j = 0; j < count; ++j, ++n)
-            {
-                const uint32_t stage = n % shape::STAGES;
-                const uint32_t phase = (n / shape::STAGES) & 1U;
-                if (!ptx::mbar_wait_bounded_spin(&st.k_full[stage], phase))
-                {
-                    return false;
-                }
-                tc::mbar_arrive(&st.k_empty[stage]);
-                if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], phase))
-                {
-                    return false;
-                }
-                tc::mbar_arrive(&st.v_empty[stage]);
-            }
-            continue;
-        }
-        if (count == 0)
-        {
-            continue;
-        }
-        // scores of tile j into score tile (s_tiles + j) % 2, whose weights the product before last has read
-        auto scores = [&](int j) {
-            const uint32_t stage = (n + j) % shape::STAGES;
-            const uint32_t s = s_tiles + j;
-            if (!ptx::mbar_wait_bounded_spin(&st.k_full[stage], ((n + j) / shape::STAGES) & 1U))
+            if (!ptx::mbar_wait_bounded_spin(&st.q_full[my_tile], q_items & 1U))
             {
                 return false;
             }
-            tc::fence_after_sync();
-            const uint64_t k_desc = tc::smem_desc_sw128(st.k_tiles + stage * shape::KV_BYTES);
-#pragma unroll
-            for (int k = 0; k < DIM / 16; ++k)
-            {
-                tc::mma<true>(s_base + (s & 1) * shape::ROWS, q_desc + (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2,
-                              k_desc + (k >> 2) * (shape::ROWS * 128 >> 4) + (k & 3) * 2, s_idesc, k != 0);
-            }
-            tc::mbar_arrive(&st.s_full[my_tile * 2 + (s & 1)]);
-            tc::mma_commit(&st.s_full[my_tile * 2 + (s & 1)]);
-            tc::mma_commit(&st.k_empty[stage]);
-            return true;
-        };
-        auto product_done = [&](uint32_t s) {
-            return ptx::mbar_wait_bounded_spin(&st.o_done[my_tile * 2 + (s & 1)], (s >> 1) & 1U);
-        };
-        // both score tiles are free once the last product of the item before has been through
-        if (!ptx::mbar_wait_bounded_spin(&st.q_full[my_tile], q_items & 1U) ||
-            (s_tiles > 0 && !product_done(s_tiles - 1)) || !scores(0))
-        {
-            return false;
+            ++q_items;
         }
-        ++q_items;
         for (int j = 0; j < count; ++j)
         {
-            // the product before has read the weights in the score tile of j + 1
-            if ((j > 0 && !product_done(s_tiles + j - 1)) || (j + 1 < count && !scores(j + 1)))
+            if (!ptx::mbar_wait_bounded_spin(&st.k_full[stage], phase))
             {
                 return false;
             }
-            const uint32_t stage = (n + j) % shape::STAGES;
-            const uint32_t s = s_tiles + j;
-            if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], ((n + j) / shape::STAGES) & 1U) ||
-                !ptx::mbar_wait_bounded_spin(&st.p_full[my_tile * 2 + (s & 1)], (s >> 1) & 1U))
+            if (active)
             {
-                return false;
-            }
-            tc::fence_after_sync();
-            const uint64_t v_desc = values_desc(st.v_tiles + stage * shape::KV_BYTES, shape::ROWS * 128);
+                // the product before last has read the weights that lie over this score tile
+                if (s >= 2 && !ptx::mbar_wait_bounded_spin(&st.o_done[my_tile * 2 + (s & 1)], ((s >> 1) - 1) & 1U))
+                {
+                    return false;
+                }
+                tc::fence_after_sync();
+                const uint32_t s_addr = s_base + (s & 1) * shape::ROWS;
+                const uint32_t k_lo = k_lo0 + stage * (shape::KV_BYTES >> 4);
+                mma_ss<false>(s_addr, q_lo, k_lo, hi, idesc);
 #pragma unroll
-            for (int k = 0; k < shape::ROWS / 16; ++k)
-            {
-                mma_ts(o_addr, s_base + (s & 1) * shape::ROWS + k * 8, v_desc + k * (16 * 128 >> 4), o_idesc, j != 0 || k != 0);
+                for (int k = 1; k < DIM / 16; ++k)
+                {
+                    mma_ss<true>(s_addr, q_lo + (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2,
+                                 k_lo + (k >> 2) * (shape::ROWS * 128 >> 4) + (k & 3) * 2, hi, idesc);
+                }
+                tc::mma_commit(&st.s_full[my_tile * 2 + (s & 1)]);
+                tc::mma_commit(&st.k_empty[stage]);
+                tc::mbar_arrive(&st.s_full[my_tile * 2 + (s & 1)]);
+                ++s;
             }
-            tc::mbar_arrive(&st.o_done[my_tile * 2 + (s & 1)]);
-            tc::mma_commit(&st.o_done[my_tile * 2 + (s & 1)]);
-            tc::mma_commit(&st.v_empty[stage]);
+            else
+            {
+                tc::mbar_arrive(&st.k_empty[stage]);
+            }
+            if (++stage == shape::STAGES)
+            {
+                stage = 0;
+                phase ^= 1U;
+            }
         }
-        n += count;
-        s_tiles += count;
+    } while (w.next(a));
+    return true;
+}
+
+template <int DIM>
+__device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem,
+                                          int my_tile)
+{
+    using shape = tc_shape<DIM>;
+    constexpr uint32_t idesc = tc::instr_desc(0U, 128U, DIM) | (1U << 16); // second operand along its outputs
+    const uint32_t s_base = tmem + my_tile * 2 * shape::ROWS;
+    const uint32_t o_addr = tmem + shape::O_COL + my_tile * DIM;
+    const uint64_t v_desc = values_desc(st.v_tiles, shape::ROWS * 128);
+    const uint32_t hi = static_cast<uint32_t>(v_desc >> 32);
+    uint32_t stage = 0;
+    uint32_t phase = 0;
+    uint32_t s = 0; // products of this query tile so far
+    do
+    {
+        const int count = w.count();
+        const bool active = my_tile < w.query_tiles();
+        for (int j = 0; j < count; ++j)
+        {
+            if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], phase))
+            {
+                return false;
+            }
+            if (active)
+            {
+                if (!ptx::mbar_wait_bounded_spin(&st.p_full[my_tile * 2 + (s & 1)], (s >> 1) & 1U))
+                {
+                    return false;
+                }
+                tc::fence_after_sync();
+                const uint32_t p_addr = s_base + (s & 1) * shape::ROWS;
+                const uint32_t v_lo = static_cast<uint32_t>(v_desc) + stage * (shape::KV_BYTES >> 4);
+#pragma unroll
+                for (int k = 0; k < shape::ROWS / 16; ++k)
+                {
+                    mma_ts(o_addr, p_addr + k * 8, v_lo + k * (16 * 128 >> 4), hi, idesc, j != 0 || k != 0);
+                }
+                tc::mma_commit(&st.o_done[my_tile * 2 + (s & 1)]);
+                tc::mma_commit(&st.v_empty[stage]);
+                tc::mbar_arrive(&st.o_done[my_tile * 2 + (s & 1)]);
+                ++s;
+            }
+            else
+            {
+                tc::mbar_arrive(&st.v_empty[stage]);
+            }
+            if (++stage == shape::STAGES)
+            {
+                stage = 0;
+                phase ^= 1U;
+            }
+        }
     } while (w.next(a));
     return true;
 }
 
 // Warps 0-3 and 4-7: softmax of query tile 0 and 1, one thread per row.  Warps 8-11: converters, codes
-// to halves.  Warps 12 and 13: one thread each issues the products of a query tile.
+// to halves.  Warps 12 ... 15: one thread each issues the scores (12, 13) or the sums (14, 15) of a query tile.
 //
 // A tile of 64 positions goes round like this.  The converters bring 16 codes per thread and load from
 // the cache a tile ahead, turn them into halves and store them in the swizzled layout the tensor cores
@@ -921,20 +977,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
         a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
         for (int i = 0; i < shape::STAGES; ++i)
         {
-            ptx::mbar_init(&st.k_full[i], CONVERTERS);
-            ptx::mbar_init(&st.v_full[i], CONVERTERS);
+            ptx::mbar_init(&st.k_full[i], CONVERTERS / 32);
+            ptx::mbar_init(&st.v_full[i], CONVERTERS / 32);
             ptx::mbar_init(&st.k_empty[i], shape::NQ);
             ptx::mbar_init(&st.v_empty[i], shape::NQ);
         }
         for (int i = 0; i < 4; ++i)
         {
             ptx::mbar_init(&st.s_full[i], 2);
-            ptx::mbar_init(&st.p_full[i], 128);
+            ptx::mbar_init(&st.p_full[i], 4);
             ptx::mbar_init(&st.o_done[i], 2);
         }
         for (int i = 0; i < 2; ++i)
         {
-            ptx::mbar_init(&st.q_full[i], 128);
+            ptx::mbar_init(&st.q_full[i], 4);
         }
         ptx::mbar_init_fence();
     }
@@ -995,11 +1051,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
         else
         {
             fewer_registers<ISSUE_REGISTERS>();
-            if (warp < 12 + shape::NQ && lane == 0)
+            const int issuer = warp - 12; // 0, 1: scores of query tile 0, 1; 2, 3: sums
+            if (lane == 0 && (issuer & 1) < shape::NQ)
             {
-                fine = issue_role<DIM>(a, st, w, tmem, warp - 12);
+                fine = issuer < 2 ? scores_role<DIM>(a, st, w, tmem, issuer & 1) : sums_role<DIM>(a, st, w, tmem, issuer & 1);
             }
-            else if (warp == 15 && lane == 0)
+            else if (warp == TC_THREADS / 32 - 1 && lane == 1)
             {
                 // the item that begins here and ends in a later block, if there is one: the last of the share
                 while (w.segment_end() < w.share_end)
