@@ -168,86 +168,109 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
             auto row_of = [&](int j) { return (first_tile + j) * TILE + warp * SUB; };
 
             // ---- the stream ----
-            // page of subtile j (dense), or position and page of this lane's list entry (selected),
-            // fetched one subtile (entries: two) ahead of the copies that need it
-            int next_page = -1;
-            int next_pos = -1;
-            int later_pos = -1;
-            auto entry = [&](int j) {
-                const int e = row_of(j) + lane;
-                int p = lane < SUB && j < count && e < a.k ? list[e] : -1;
+            // Positions and pages are looked up well before the copies that need them.  All positions: one
+            // subtile per lane, 32 subtiles at a time; a subtile lies within one page, so its rows are
+            // contiguous and share their scales.  A list: one entry per lane, two subtiles at a time.
+            constexpr int BATCH = SELECTED ? 2 : 32; // subtiles
+            constexpr int PARTS = DIM / 16;
+            auto where = [&](int j) { // this lane's position in the batch that begins with subtile j; -1: none
+                if constexpr (SELECTED)
+                {
+                    // rows 0 ... 15 of subtile j, then of the next one
+                    const int e = row_of(j + (lane >> 4)) + (lane & 15);
+                    const int p = j + (lane >> 4) < count && e < a.k ? list[e] : -1;
+                    return p < furthest ? p : -1;
+                }
+                const int p = j + lane < count ? row_of(j + lane) : -1;
                 return p < furthest ? p : -1;
             };
             auto page_at = [&](int pos) {
                 const int p = pos >= 0 ? table[pos >> a.c.page_shift] : -1;
                 return p < a.c.pages ? p : -1;
             };
-            if constexpr (SELECTED)
-            {
-                next_pos = entry(0);
-                next_page = page_at(next_pos);
-                later_pos = entry(1);
-            }
-            else
-            {
-                next_page = page_at(row_of(0) < furthest ? row_of(0) : -1);
-            }
+            auto offset_of = [&](int page, int pos) -> int64_t {
+                return page < 0 ? -1
+                                : page * a.c.page_stride +
+                                      ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
+            };
+            // key scale (0: absent), log2 of the value scale, its inverse; value scales at the border of their
+            // range and beyond would leave that of the sums
+            auto scales_of = [&](int page) {
+                float3 r = make_float3(0.0F, 0.0F, 0.0F);
+                if (page >= 0)
+                {
+                    const int64_t at_scale = static_cast<int64_t>(page) * a.c.heads + it.head;
+                    const float vs = fminf(fmaxf(a.c.value_scales[at_scale], pow2_int(E_MIN)), pow2_int(E_MAX));
+                    r = make_float3(a.c.key_scales[at_scale], log2_fast(vs), __fdividef(1.0F, vs));
+                }
+                return r;
+            };
+            int batch = 0; // first subtile of the batch the copies are in
+            int pos_next = where(0);
+            int page_next = page_at(pos_next);
+            int page_now = page_next;
+            int64_t offset_now = offset_of(page_next, pos_next);
+            float3 scales_now = scales_of(page_next);
+            float3 scales_before = scales_now;
+            pos_next = where(BATCH);
+            page_next = page_at(pos_next);
+            int pos_later = SELECTED ? where(2 * BATCH) : 0;
+            int slot_in = 0;
+            int slot_out = 0;
+            const uint32_t stage0 = ptx::smem_addr(mine);
             auto issue = [&](int j) {
                 if (j < count)
                 {
-                    const uint32_t dst = ptx::smem_addr(mine + (j % STAGES) * smem::STAGE);
-                    constexpr int PARTS = DIM / 16;
-                    const int page = next_page;
-                    const int safe = max(page, 0);
+                    if (j - batch == BATCH)
+                    {
+                        batch = j;
+                        page_now = page_next;
+                        offset_now = offset_of(page_next, pos_next);
+                        if constexpr (!SELECTED)
+                        {
+                            scales_before = scales_now;
+                            scales_now = scales_of(page_next);
+                        }
+                        pos_next = SELECTED ? pos_later : where(j + BATCH);
+                        page_next = page_at(pos_next);
+                        pos_later = SELECTED ? where(j + 2 * BATCH) : 0;
+                    }
+                    const uint32_t dst = stage0 + slot_in * smem::STAGE;
                     if constexpr (SELECTED)
                     {
-                        int64_t from = -1;
-                        if (page >= 0)
-                        {
-                            from = page * a.c.page_stride +
-                                   ((static_cast<int64_t>(it.head) << a.c.page_shift) + (next_pos & rows_mask)) * DIM;
-                        }
-                        const uint32_t there = page >= 0 ? 4U : 0U;
-                        next_pos = later_pos;
-                        next_page = page_at(next_pos);
-                        later_pos = entry(j + 2);
 #pragma unroll
                         for (int x = 0; x < DIM / 32; ++x)
                         {
                             const int e = lane + x * 32;
                             const int row = e / PARTS;
-                            const int64_t f = __shfl_sync(FULL_MASK, from, row);
+                            const int64_t f = __shfl_sync(FULL_MASK, offset_now, (j - batch) * SUB + row);
                             const int64_t g = max(f, static_cast<int64_t>(0)) + (e % PARTS) * 16;
                             const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
                             copy16(to, a.c.keys + g, f >= 0 ? 16U : 0U);
                             copy16(to + SUB * PITCH<DIM>, a.c.values + g, f >= 0 ? 16U : 0U);
                         }
-                        if (lane < SUB)
+                        if ((lane >> 4) == j - batch) // the scales of each row go with the rows
                         {
-                            const int64_t s = static_cast<int64_t>(safe) * a.c.heads + it.head;
-                            copy4(dst + smem::SCALES + lane * 4, a.c.key_scales + s, there);
-                            copy4(dst + smem::SCALES + SUB * 4 + lane * 4, a.c.value_scales + s, there);
+                            const int64_t at_scale = static_cast<int64_t>(max(page_now, 0)) * a.c.heads + it.head;
+                            const uint32_t to = dst + smem::SCALES + (lane & 15) * 4;
+                            copy4(to, a.c.key_scales + at_scale, page_now >= 0 ? 4U : 0U);
+                            copy4(to + SUB * 4, a.c.value_scales + at_scale, page_now >= 0 ? 4U : 0U);
                         }
                     }
                     else
                     {
-                        const int pos = row_of(j);
-                        const int there = page < 0 ? 0 : min(SUB, furthest - pos);
-                        next_page = page_at(j + 1 < count && row_of(j + 1) < furthest ? row_of(j + 1) : -1);
-                        // a subtile lies within one page: its rows are contiguous and share a scale
-                        const int64_t from = safe * a.c.page_stride + lane * 16 +
-                                             ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
-                        const uint8_t* const k_from = a.c.keys + from;
-                        const uint8_t* const v_from = a.c.values + from;
-                        if (there == SUB)
+                        const int64_t offset = __shfl_sync(FULL_MASK, offset_now, j - batch);
+                        const int there = offset < 0 ? 0 : min(SUB, furthest - row_of(j));
+                        const uint8_t* const k_from = a.c.keys + max(offset, static_cast<int64_t>(0)) + lane * 16;
+                        const uint8_t* const v_from = a.c.values + max(offset, static_cast<int64_t>(0)) + lane * 16;
+                        if (there == SUB && 32 % PARTS == 0)
                         {
+                            const uint32_t to = dst + lane / PARTS * PITCH<DIM> + (lane % PARTS) * 16;
 #pragma unroll
                             for (int x = 0; x < DIM / 32; ++x)
                             {
-                                const int e = lane + x * 32;
-                                const uint32_t to = dst + e / PARTS * PITCH<DIM> + (e % PARTS) * 16;
-                                copy16(to, k_from + x * 512);
-                                copy16(to + SUB * PITCH<DIM>, v_from + x * 512);
+                                copy16(to + x * (32 / PARTS) * PITCH<DIM>, k_from + x * 512);
+                                copy16(to + (x * (32 / PARTS) + SUB) * PITCH<DIM>, v_from + x * 512);
                             }
                         }
                         else
@@ -262,17 +285,11 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                                 copy16(to + SUB * PITCH<DIM>, v_from + x * 512, row < there ? 16U : 0U);
                             }
                         }
-                        if (lane < 2)
-                        {
-                            const float* scales = lane == 0 ? a.c.key_scales : a.c.value_scales;
-                            copy4(dst + smem::SCALES + lane * 4, scales + static_cast<int64_t>(safe) * a.c.heads + it.head,
-                                  page < 0 ? 0U : 4U);
-                        }
                     }
                 }
                 copy_commit();
+                slot_in = slot_in + 1 == STAGES ? 0 : slot_in + 1;
             };
-
             float o[DIM / 16][NB][4];
             float m[NB][2];
             float l[NB][2];
@@ -307,18 +324,29 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                 const int pos = row_of(j);
                 if (pos < row_end)
                 {
-                    const unsigned char* const stage = mine + (j % STAGES) * smem::STAGE;
-                    const float* const scales = reinterpret_cast<const float*>(stage + smem::SCALES);
+                    const unsigned char* const stage = mine + slot_out * smem::STAGE;
                     float s[NB][4];
                     score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
-                    // value scales at the border of their range and beyond would leave that of the sums
-                    auto fit = [](float vs) { return fminf(fmaxf(vs, pow2_int(E_MIN)), pow2_int(E_MAX)); };
-                    const float ks_lo = SELECTED ? scales[row_lo] : scales[0];
-                    const float ks_hi = SELECTED ? scales[row_lo + 8] : ks_lo;
-                    const float vs_lo = fit(SELECTED ? scales[SUB + row_lo] : scales[1]);
-                    const float vs_hi = SELECTED ? fit(scales[SUB + row_lo + 8]) : vs_lo;
-                    const float lv_lo = log2_fast(vs_lo);
-                    const float lv_hi = SELECTED ? log2_fast(vs_hi) : lv_lo;
+                    float ks_lo, ks_hi, lv_lo, lv_hi, iv_lo, iv_hi;
+                    if constexpr (SELECTED)
+                    {
+                        const float* const scales = reinterpret_cast<const float*>(stage + smem::SCALES);
+                        const float vs_lo = fminf(fmaxf(scales[SUB + row_lo], pow2_int(E_MIN)), pow2_int(E_MAX));
+                        const float vs_hi = fminf(fmaxf(scales[SUB + row_lo + 8], pow2_int(E_MIN)), pow2_int(E_MAX));
+                        ks_lo = scales[row_lo];
+                        ks_hi = scales[row_lo + 8];
+                        lv_lo = log2_fast(vs_lo);
+                        lv_hi = log2_fast(vs_hi);
+                        iv_lo = __fdividef(1.0F, vs_lo);
+                        iv_hi = __fdividef(1.0F, vs_hi);
+                    }
+                    else
+                    {
+                        // the copies may have moved on to the next batch
+                        ks_hi = ks_lo = __shfl_sync(FULL_MASK, j < batch ? scales_before.x : scales_now.x, j & 31);
+                        lv_hi = lv_lo = __shfl_sync(FULL_MASK, j < batch ? scales_before.y : scales_now.y, j & 31);
+                        iv_hi = iv_lo = __shfl_sync(FULL_MASK, j < batch ? scales_before.z : scales_now.z, j & 31);
+                    }
                     // absent rows were copied as zeros, scale included; others are seen below `see`
                     const int at_lo = ks_lo != 0.0F ? pos + row_lo : 0x7fffffff;
                     const int at_hi = ks_hi != 0.0F ? pos + row_lo + 8 : 0x7fffffff;
@@ -377,8 +405,6 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     }
                     uint32_t w_lo[NB];
                     uint32_t w_hi[NB];
-                    const float iv_lo = __fdividef(1.0F, vs_lo);
-                    const float iv_hi = SELECTED ? __fdividef(1.0F, vs_hi) : iv_lo;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
@@ -492,6 +518,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     }
                 }
                 __syncwarp();
+                slot_out = slot_out + 1 == STAGES ? 0 : slot_out + 1;
                 issue(j + STAGES - 1);
             }
             copy_wait<0>();

@@ -39,7 +39,7 @@ __device__ __forceinline__ float max_nan(float a, float b)
 template <int DIM, int NB>
 struct distance_smem
 {
-    static constexpr int STAGE = SUB * PITCH<DIM> + 16; // rows and their scale
+    static constexpr int STAGE = SUB * PITCH<DIM>;
     static constexpr int SCRATCH = 8 * NB * (SUB + 1) * 4;
     static constexpr int IMAGE = NB * 16 * DIM; // 8 NB columns of DIM halves
     static constexpr int BYTES = IMAGE + 8 * NB * 4 + WARPS * (DIST_STAGES * STAGE + SCRATCH);
@@ -114,32 +114,52 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
             const int first = begin / SUB + warp;
             const int count = end > first * SUB ? ((end - 1) / SUB - first) / WARPS + 1 : 0;
             const int loaded = furthest > first * SUB ? min(count, ((furthest - 1) / SUB - first) / WARPS + 1) : 0;
-            auto page_of = [&](int j) { // page of subtile j of this warp
+            // Where the warp's next 32 subtiles lie and their scales, one subtile per lane; looked up a batch
+            // ahead.  A subtile lies within one page, so its rows are contiguous and share a scale.
+            auto page_of = [&](int j) {
                 const int p = j < loaded ? table[((first + j * WARPS) * SUB) >> a.c.page_shift] : -1;
                 return p < a.c.pages ? p : -1;
             };
-            int next_page = page_of(0);
+            auto offset_of = [&](int page, int j) -> int64_t {
+                const int pos = (first + j * WARPS) * SUB;
+                return page < 0 ? -1
+                                : page * a.c.page_stride +
+                                      ((static_cast<int64_t>(head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
+            };
+            auto scale_of = [&](int page) { // 0 marks an absent page
+                return page < 0 ? 0.0F : a.c.key_scales[static_cast<int64_t>(page) * a.c.heads + head];
+            };
+            int batch = 0; // first subtile of the batch the copies are in
+            const int page_first = page_of(lane);
+            int page_next = page_of(32 + lane);
+            int64_t offset_now = offset_of(page_first, lane);
+            float scale_now = scale_of(page_first);
+            float scale_before = 0.0F;
+            int slot_in = 0;
+            int slot_out = 0;
+            const uint32_t stage0 = ptx::smem_addr(mine);
+            constexpr int PARTS = DIM / 16;
             auto issue = [&](int j) {
                 if (j < loaded)
                 {
-                    const int page = next_page;
-                    next_page = page_of(j + 1);
-                    const int pos = (first + j * WARPS) * SUB;
-                    const int there = page < 0 ? 0 : min(SUB, furthest - pos);
-                    const uint32_t dst = ptx::smem_addr(mine + (j % DIST_STAGES) * smem::STAGE);
-                    const int safe = max(page, 0);
-                    const uint8_t* src = a.c.keys + safe * a.c.page_stride +
-                                         ((static_cast<int64_t>(head) << a.c.page_shift) + (pos & rows_mask)) * DIM +
-                                         lane * 16;
-                    // a subtile lies within one page: its rows are contiguous and share a scale
-                    constexpr int PARTS = DIM / 16;
-                    if (there == SUB)
+                    if (j - batch == 32)
+                    {
+                        batch = j;
+                        offset_now = offset_of(page_next, j + lane);
+                        scale_before = scale_now;
+                        scale_now = scale_of(page_next);
+                        page_next = page_of(j + 32 + lane);
+                    }
+                    const int64_t offset = __shfl_sync(FULL_MASK, offset_now, j - batch);
+                    const int there = offset < 0 ? 0 : min(SUB, furthest - (first + j * WARPS) * SUB);
+                    const uint32_t dst = stage0 + slot_in * smem::STAGE + lane / PARTS * PITCH<DIM> + (lane % PARTS) * 16;
+                    const uint8_t* src = a.c.keys + max(offset, static_cast<int64_t>(0)) + lane * 16;
+                    if (there == SUB && 32 % PARTS == 0)
                     {
 #pragma unroll
                         for (int x = 0; x < DIM / 32; ++x)
                         {
-                            const int e = lane + x * 32;
-                            copy16(dst + e / PARTS * PITCH<DIM> + (e % PARTS) * 16, src + x * 512);
+                            copy16(dst + x * (32 / PARTS) * PITCH<DIM>, src + x * 512);
                         }
                     }
                     else
@@ -149,22 +169,21 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                         {
                             const int e = lane + x * 32;
                             const int row = e / PARTS;
-                            copy16(dst + row * PITCH<DIM> + (e % PARTS) * 16, src + x * 512, row < there ? 16U : 0U);
+                            copy16(stage0 + slot_in * smem::STAGE + row * PITCH<DIM> + (e % PARTS) * 16, src + x * 512,
+                                   row < there ? 16U : 0U);
                         }
-                    }
-                    if (lane == 0)
-                    {
-                        copy4(dst + SUB * PITCH<DIM>, a.c.key_scales + static_cast<int64_t>(safe) * a.c.heads + head,
-                              page < 0 ? 0U : 4U);
                     }
                 }
                 copy_commit();
+                slot_in = slot_in + 1 == DIST_STAGES ? 0 : slot_in + 1;
             };
 #pragma unroll
             for (int j = 0; j < DIST_STAGES - 1; ++j)
             {
                 issue(j);
             }
+            // One token whose heads all are columns of this block: the maximum over them stays in registers.
+            const bool simple = many == 1 && columns <= 8 * NB;
             const int row = lane & (SUB - 1);
             const int half = lane >> 4;
             const int cols = min(columns - col0, 8 * NB);
@@ -174,13 +193,48 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                 const int pos = (first + j * WARPS) * SUB;
                 copy_wait<DIST_STAGES - 2>();
                 __syncwarp();
-                float ks = 0.0F; // that of an absent page was copied as zero
+                const unsigned char* const stage = mine + slot_out * smem::STAGE;
+                slot_out = slot_out + 1 == DIST_STAGES ? 0 : slot_out + 1;
+                const float ks = j < loaded ? __shfl_sync(FULL_MASK, j < batch ? scale_before : scale_now, j & 31) : 0.0F;
+                float s[NB][4];
                 if (j < loaded)
                 {
-                    const unsigned char* stage = mine + (j % DIST_STAGES) * smem::STAGE;
-                    ks = *reinterpret_cast<const float*>(stage + SUB * PITCH<DIM>);
-                    float s[NB][4];
                     score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
+                }
+                if (simple)
+                {
+                    float lo = -INFINITY;
+                    float hi = -INFINITY;
+                    if (j < loaded)
+                    {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                        {
+                            const int c = nb * 8 + (lane & 3) * 2;
+                            lo = max_nan(lo, c < columns ? s[nb][0] * factor[nb][0] : -INFINITY);
+                            hi = max_nan(hi, c < columns ? s[nb][2] * factor[nb][0] : -INFINITY);
+                            lo = max_nan(lo, c + 1 < columns ? s[nb][1] * factor[nb][1] : -INFINITY);
+                            hi = max_nan(hi, c + 1 < columns ? s[nb][3] * factor[nb][1] : -INFINITY);
+                        }
+                    }
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1)
+                    {
+                        lo = max_nan(lo, __shfl_xor_sync(FULL_MASK, lo, o));
+                        hi = max_nan(hi, __shfl_xor_sync(FULL_MASK, hi, o));
+                    }
+                    // lanes 0 and 1 of a group of four write its rows row_order and 8 + row_order
+                    const int at = pos + row_order(lane >> 2) + (lane & 1) * 8;
+                    if ((lane & 2) == 0 && at < end)
+                    {
+                        only[at] = ks != 0.0F && at < furthest ? -(((lane & 1) == 0 ? lo : hi) * ks) : INFINITY;
+                    }
+                    __syncwarp();
+                    issue(j + DIST_STAGES - 1);
+                    continue;
+                }
+                if (j < loaded)
+                {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
