@@ -9,6 +9,7 @@ from torch import bfloat16, empty, float16, float32, int32, int64, uint8
 from . import BF16, F16, F32, BatchStruct, BitsKnnError, CacheStruct, last_error, lib
 
 _CODES = {bfloat16: BF16, float16: F16, float32: F32}
+_current_device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream without the object
 
 
@@ -21,7 +22,7 @@ def _run(fn, *args):
 def _current(index, *tensors):
     """The tensors must be CUDA tensors of the current device (`index`): the library has no CPU path and launches on
     the current device."""
-    if index < 0 or index != torch.cuda.current_device():
+    if index < 0 or index != _current_device():
         raise ValueError(f"the tensors must be CUDA tensors of the current device (the library has no CPU path), "
                          f"not of device {index}")
     for t in tensors:
@@ -77,8 +78,8 @@ class Cache:
         return cls(*codes, *scales)
 
 
-def _batch(cache, shape, lengths, table, starts):
-    """bitsknn_cache_batch_t of a call with queries of this shape."""
+def _batch(cache, queries, shape, lengths, table, starts, *more):
+    """bitsknn_cache_batch_t of a call; all its tensors (`more`: further ones) have to be on the current device."""
     if len(shape) != 3 or shape[2] != cache.dim:
         raise ValueError(f"queries of shape {tuple(shape)} do not fit the cache")
     if lengths.dtype is not int32 or table.dtype is not int32:
@@ -92,10 +93,8 @@ def _batch(cache, shape, lengths, table, starts):
         _dense(starts, int32, "starts")
         if starts.shape != (requests + 1,):
             raise ValueError("starts must be (requests + 1,)")
-        _current(cache.index, lengths, table, starts)
         first = starts.data_ptr()
-    else:
-        _current(cache.index, lengths, table)
+    _current(cache.index, queries, lengths, table, *(() if starts is None else (starts,)), *more)
     return BatchStruct(table.data_ptr(), ld if requests > 1 else pages, pages, lengths.data_ptr(), first, requests,
                        shape[0])
 
@@ -122,8 +121,8 @@ def cache_plan(lengths, new, free_pages, table, page_rows, max_tokens, out=None)
         raise ValueError("lengths and new must be (requests,), table (requests, pages)")
     if out is None:
         device = lengths.device
-        out = (empty(requests + 1, dtype=int32, device=device), empty(requests, dtype=int32, device=device),
-               empty(max_tokens, dtype=int64, device=device), empty(3, dtype=int32, device=device))
+        starts, new_lengths, counts = empty(2 * requests + 4, dtype=int32, device=device).split((requests + 1, requests, 3))
+        out = starts, new_lengths, empty(max_tokens, dtype=int64, device=device), counts
     else:
         for t, dtype, size, name in zip(out, (int32, int32, int64, int32), (requests + 1, requests, max_tokens, 3),
                                         ("starts", "new_lengths", "slots", "counts")):
@@ -156,14 +155,13 @@ def cache_append(cache, keys, values, slots):
 def cache_distance(cache, queries, lengths, table, n, starts=None, out=None):
     """(tokens * heads, n) float32 distances for `select`: minus the largest inner product over a head's queries."""
     shape = queries.shape
-    batch = _batch(cache, shape, lengths, table, starts)
+    batch = _batch(cache, queries, shape, lengths, table, starts)
     rows = shape[0] * cache.heads
     if out is None:
-        _current(cache.index, queries)
         out = empty((rows, n), dtype=float32, device=cache.device)
         ld = n
     else:
-        _current(cache.index, queries, out)
+        _current(cache.index, out)
         if out.dim() != 2 or out.dtype is not float32 or out.shape[0] < rows or out.shape[1] < n:
             raise ValueError("out must be float32 and have tokens * heads rows of n distances")
         if out.shape[1] > 1 and out.stride(1) != 1:
@@ -198,16 +196,16 @@ def _attend_buffers(cache, queries, shape, out, lse, workspace):
     if workspace is None:
         workspace = empty(cache_attend_workspace_bytes(cache, shape[1]), dtype=uint8, device=cache.device)
     else:
-        _current(cache.index, workspace)
         _dense(workspace, uint8, "workspace")
+        if workspace.get_device() != cache.index:
+            raise ValueError("workspace must be on the cache's device")
     return out, stride, lse, workspace
 
 
 def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
     """Attention of (tokens, query_heads, dim) queries over everything cached: (out, lse)."""
     shape = queries.shape
-    batch = _batch(cache, shape, lengths, table, starts)
-    _current(cache.index, queries)
+    batch = _batch(cache, queries, shape, lengths, table, starts)
     out, out_stride, lse, workspace = _attend_buffers(cache, queries, shape, out, lse, workspace)
     _run(lib().bitsknn_cache_attend, cache.struct, batch, queries.data_ptr(), _code(queries, "queries"),
          _token_stride("queries", shape, queries.stride()), shape[1], scale, out.data_ptr(), out_stride, lse.data_ptr(),
@@ -218,14 +216,13 @@ def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, l
 def cache_attend_selected(cache, queries, idx, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
     """Attention over listed positions: idx (tokens * heads, k) int32, as `select` returns them.  (out, lse)."""
     shape = queries.shape
-    batch = _batch(cache, shape, lengths, table, starts)
+    batch = _batch(cache, queries, shape, lengths, table, starts, idx)
     rows, k = idx.shape
     ld, inner = idx.stride()
     if rows != shape[0] * cache.heads:
         raise ValueError("idx must be (tokens * heads, k)")
     if idx.dtype is not int32 or (k > 1 and inner != 1):
         raise ValueError("idx must be torch.int32, contiguous in its last dimension")
-    _current(cache.index, queries, idx)
     out, out_stride, lse, workspace = _attend_buffers(cache, queries, shape, out, lse, workspace)
     _run(lib().bitsknn_cache_attend_selected, cache.struct, batch, queries.data_ptr(), _code(queries, "queries"),
          _token_stride("queries", shape, queries.stride()), shape[1], idx.data_ptr(), ld if rows > 1 else k, k, scale,

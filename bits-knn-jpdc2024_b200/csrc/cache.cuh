@@ -198,6 +198,23 @@ __device__ __forceinline__ void copy_wait()
     asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
+// ---- thread-block clusters ----------------------------------------------------------------------
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A float of the shared memory of block `rank` of the cluster, at the place `mine` has in this block.
+__device__ __forceinline__ float cluster_load(const float* mine, int rank)
+{
+    float v;
+    asm volatile("{\n.reg .b32 a;\nmapa.shared::cluster.u32 a, %1, %2;\nld.shared::cluster.f32 %0, [a];\n}\n"
+                 : "=f"(v)
+                 : "r"(ptx::smem_addr(mine)), "r"(rank)
+                 : "memory");
+    return v;
+}
+
 // ---- warp matrix steps -------------------------------------------------------------------------
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1)
@@ -230,13 +247,41 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Row of a 16-row subtile that matrix row r (0 ... 7) stands for.  The order 0 4 1 5 2 6 3 7 puts
-// rows four apart into the same phase of a 128-bit shared-memory load; with a row pitch of an odd
-// number of 16-byte granules the eight lanes of a phase then hit eight different granules.
-__device__ __forceinline__ int row_order(int r) { return (r >> 1) | ((r & 1) << 2); }
+// Staged rows in shared memory, DIM / 16 granules of 16 bytes each.  Eight rows at the same granule have to
+// lie on eight different bank groups.  Padded: a granule is added to every row, which makes the pitch an odd
+// number of them.  Swapped (where DIM is a power of two): the granules of a row change places by the row
+// number.  The attention kernels pad (one long request: 88 us, swapped 103: the addresses of two operands
+// cost more than the space is worth), the distance kernel swaps (74 us, padded 83).
+template <int DIM, bool PADDED>
+constexpr bool SWAPPED = !PADDED && (DIM & (DIM - 1)) == 0;
 
-template <int DIM>
-constexpr int PITCH = DIM + 16; // bytes between staged rows: an odd number of 16-byte granules
+template <int DIM, bool PADDED>
+constexpr int PITCH = SWAPPED<DIM, PADDED> ? DIM : DIM + 16; // bytes between staged rows
+
+template <int DIM, bool PADDED>
+__device__ __forceinline__ int granule_swap(int row)
+{
+    if constexpr (!SWAPPED<DIM, PADDED>)
+    {
+        return 0;
+    }
+    return DIM >= 128 ? row & 7 : DIM == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
+}
+
+template <int DIM, bool PADDED>
+__device__ __forceinline__ int granule_byte(int row, int granule)
+{
+    return row * PITCH<DIM, PADDED> + ((granule ^ granule_swap<DIM, PADDED>(row)) << 4);
+}
+
+// Row of a 16-row subtile that matrix row r (0 ... 7) stands for.  The eight lanes of a phase of a 128-bit
+// load read four granules of two neighbouring matrix rows; unless 32 or 64 numbers are swapped these have
+// to lie four rows apart (order 0 4 1 5 2 6 3 7) to fall on eight different bank groups.
+template <int DIM, bool PADDED>
+__device__ __forceinline__ int row_order(int r)
+{
+    return SWAPPED<DIM, PADDED> && DIM <= 64 ? r : (r >> 1) | ((r & 1) << 2);
+}
 
 // Query columns of a block as halves in the order the matrix step wants them: word pair
 // [kstep][column block][lane] holds, for column lane / 4, the dims base + 0, 1 and base + 2, 3.
@@ -292,14 +337,17 @@ __device__ __forceinline__ float pack_column(uint32_t* image, int col, const voi
 // Scores of 16 staged rows against NB blocks of 8 query columns: s[nb] = rows x columns, where
 // thread (r = lane / 4, c = lane % 4) gets rows row_order(r) and 8 + row_order(r) of columns
 // 8 nb + 2 c and 2 c + 1.  `image` is the packed query image (shared memory).
-template <int DIM, int NB>
+template <int DIM, int NB, bool PADDED>
 __device__ __forceinline__ void score_rows(float (&s)[NB][4], const unsigned char* rows, const uint2* image)
 {
     constexpr int FULL = DIM / 64;
     const int lane = threadIdx.x & 31;
     const int c = lane & 3;
-    const unsigned char* low = rows + row_order(lane >> 2) * PITCH<DIM>;
-    const unsigned char* high = low + 8 * PITCH<DIM>;
+    // this lane's granules: c of every unit of four, moved by the row's swap (rows r and r + 8 share it)
+    const int row = row_order<DIM, PADDED>(lane >> 2);
+    const int swap = granule_swap<DIM, PADDED>(row);
+    const unsigned char* low = rows + row * PITCH<DIM, PADDED> + ((c ^ (swap & 3)) << 4);
+    const int unit_swap = (swap >> 2) * 64;
     // two sums, for even and odd steps, so that a step does not wait for the one before it
     float odd[NB][4];
 #pragma unroll
@@ -322,8 +370,8 @@ __device__ __forceinline__ void score_rows(float (&s)[NB][4], const unsigned cha
 #pragma unroll
     for (int u = 0; u < FULL; ++u)
     {
-        const uint4 x = *reinterpret_cast<const uint4*>(low + u * 64 + c * 16);
-        const uint4 y = *reinterpret_cast<const uint4*>(high + u * 64 + c * 16);
+        const uint4 x = *reinterpret_cast<const uint4*>(low + ((u * 64) ^ unit_swap));
+        const uint4 y = *reinterpret_cast<const uint4*>(low + ((u * 64) ^ unit_swap) + 8 * PITCH<DIM, PADDED>);
         step(u * 4 + 0, x.x, y.x);
         step(u * 4 + 1, x.y, y.y);
         step(u * 4 + 2, x.z, y.z);
@@ -331,8 +379,9 @@ __device__ __forceinline__ void score_rows(float (&s)[NB][4], const unsigned cha
     }
     if constexpr (DIM % 64 != 0)
     {
-        const uint2 x = *reinterpret_cast<const uint2*>(low + FULL * 64 + c * 8);
-        const uint2 y = *reinterpret_cast<const uint2*>(high + FULL * 64 + c * 8);
+        const unsigned char* tail = rows + granule_byte<DIM, PADDED>(row, FULL * 4 + (c >> 1)) + (c & 1) * 8;
+        const uint2 x = *reinterpret_cast<const uint2*>(tail);
+        const uint2 y = *reinterpret_cast<const uint2*>(tail + 8 * PITCH<DIM, PADDED>);
         step(FULL * 4 + 0, x.x, y.x);
         step(FULL * 4 + 1, x.y, y.y);
     }

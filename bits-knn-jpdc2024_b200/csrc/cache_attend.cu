@@ -15,13 +15,18 @@ struct attend_smem
 {
     static constexpr int COLS = 8 * NB;
     static constexpr int ROWS = TILE;
-    static constexpr int COST = 3; // an item's beginning and end take about as long as three tiles
-    static constexpr int SCALES = 2 * SUB * PITCH<DIM>; // offset of the scales in a stage
+    // An item's beginning and end in tiles (ragged decode batch of 64 requests, 150 ... 24000 positions: 141 us
+    // with 1, 131 with 3, 121 with 5 and with 8).  Lists are all of one length; there it only costs.
+    static constexpr int COST = 6;
+    static constexpr int LIST_COST = 1;
+    static constexpr int SCALES = 2 * SUB * PITCH<DIM, true>; // offset of the scales in a stage
     static constexpr int STAGE = SCALES + 2 * SUB * 4;
-    static constexpr int FIT = 18432 / STAGE;
-    static constexpr int STAGES = FIT < 3 ? (NB > 3 ? NB : 3) : FIT > 8 ? 8 : (FIT < NB ? NB : FIT);
     static constexpr int IMAGE = NB * 16 * DIM;
-    static constexpr int SMALL = COLS * (4 + 4 + WARPS * 8); // undo, visible, per-warp (m, l)
+    static constexpr int SMALL = COLS * (4 + 4 + WARPS * 8 + 8); // undo, visible, (m, l) of warps and block
+    // as many stages as three blocks per SM leave room for
+    static constexpr int FIT = 18432 / STAGE;
+    static constexpr int LEAST = NB > 3 ? NB : 3;
+    static constexpr int STAGES = FIT < LEAST ? LEAST : FIT > 8 ? 8 : FIT;
     static constexpr int BYTES = IMAGE + SMALL + WARPS * STAGES * STAGE;
     static constexpr int BY_SMEM = 227 * 1024 / (BYTES + 1024);
     static constexpr int BY_REGS = NB * DIM <= 128 ? 4 : NB * DIM <= 256 ? 3 : 2;
@@ -41,7 +46,7 @@ struct attend_smem
 //                                            dims; the pairs are split when they become halves)
 // The four warps' sums are joined in shared memory when an item ends, those of several blocks by
 // cache_join_kernel.  Bound by the bytes of the cache (HBM) while the columns are few.
-template <int DIM, int NB, bool SELECTED>
+template <int DIM, int NB, bool SELECTED, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_attend_kernel(const attend_args a)
 {
     using smem = attend_smem<DIM, NB>;
@@ -54,19 +59,25 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
     float* const undo = reinterpret_cast<float*>(shared + smem::IMAGE);
     int* const visible = reinterpret_cast<int*>(undo + COLS);
     float2* const warp_ml = reinterpret_cast<float2*>(visible + COLS);
+    float2* const block_ml = warp_ml + WARPS * COLS; // of a cluster's block
     unsigned char* const stages = shared + smem::IMAGE + smem::SMALL;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     unsigned char* const mine = stages + warp * STAGES * smem::STAGE;
     const int rows_mask = (1 << a.c.page_shift) - 1;
     const int c = (lane & 3) * 2;             // this thread's columns: c, c + 1 of every block of 8
-    const int row_lo = row_order(lane >> 2);  // its rows: row_lo, row_lo + 8
+    const int row_lo = row_order<DIM, true>(lane >> 2);  // its rows: row_lo, row_lo + 8
 
     // this block's share, and the item it begins in
-    const int list_units = SELECTED ? (a.k + TILE - 1) / TILE + smem::COST : 0;
+    constexpr int COST = SELECTED ? smem::LIST_COST : smem::COST;
+    const int list_units = SELECTED ? (a.k + TILE - 1) / TILE + COST : 0;
     const int list_blocks = SELECTED ? (a.group + COLS - 1) / COLS : 0;
     int64_t total;
-    if constexpr (SELECTED)
+    if constexpr (CLUSTER)
+    {
+        total = 0; // no shares
+    }
+    else if constexpr (SELECTED)
     {
         total = static_cast<int64_t>(a.b.tokens) * a.c.heads * list_blocks * list_units;
     }
@@ -79,45 +90,63 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
         }
         total = block_sum<WARPS>(sum, s_words);
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (threadIdx.x == 0)
-    {
-        a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-    }
-    const int64_t blocks = min(static_cast<int64_t>(gridDim.x), total); // those that get a share at all
-    if (blockIdx.x >= blocks)
-    {
-        return;
-    }
-    int64_t at = blockIdx.x * total / blocks;
-    const int64_t share_end = (blockIdx.x + 1) * total / blocks;
+    int64_t blocks = 0;
+    int64_t at = 0;
+    int64_t share_end = 0;
     item it{};
-    if constexpr (SELECTED)
+    if constexpr (CLUSTER)
     {
-        const int64_t n = at / list_units;
-        it.begin = n * list_units;
-        it.end = it.begin + list_units;
-        it.column0 = static_cast<int>(n % list_blocks) * COLS;
-        it.head = static_cast<int>(n / list_blocks % a.c.heads);
-        it.first_token = static_cast<int>(n / list_blocks / a.c.heads);
+        // one token per request (or a list per token): the items are known without a look at the lengths
+        const int column_blocks = (a.group + COLS - 1) / COLS;
+        const int n = static_cast<int>(blockIdx.x) / a.cluster;
+        it.column0 = n % column_blocks * COLS;
+        it.head = n / column_blocks % a.c.heads;
+        it.first_token = n / column_blocks / a.c.heads;
+        it.request = it.first_token;
         it.columns = a.group;
+        it.end = share_end = 1;
     }
     else
     {
-        int64_t first = 0;
-        it.request = find_request<smem, WARPS>(a, at, &first, s_words, &s_found);
-        const request q = request_of(a.b, it.request);
-        const int64_t per_head = units_of_head<smem>(a, q);
-        it.head = static_cast<int>((at - first) / per_head);
-        it.begin = first + it.head * per_head;
-        it.first_token = q.first;
-        it.columns = q.count * a.group;
-        it.end = it.begin + units_of_block<smem>(a, q, 0);
-        while (at >= it.end)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        if (threadIdx.x == 0)
         {
-            it.column0 += COLS;
-            it.begin = it.end;
-            it.end += units_of_block<smem>(a, q, it.column0);
+            a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+        }
+        blocks = min(static_cast<int64_t>(gridDim.x), total); // those that get a share at all
+        if (blockIdx.x >= blocks)
+        {
+            return;
+        }
+        at = blockIdx.x * total / blocks;
+        share_end = (blockIdx.x + 1) * total / blocks;
+        if constexpr (SELECTED)
+        {
+            const int64_t n = at / list_units;
+            it.begin = n * list_units;
+            it.end = it.begin + list_units;
+            it.column0 = static_cast<int>(n % list_blocks) * COLS;
+            it.head = static_cast<int>(n / list_blocks % a.c.heads);
+            it.first_token = static_cast<int>(n / list_blocks / a.c.heads);
+            it.columns = a.group;
+        }
+        else
+        {
+            int64_t first = 0;
+            it.request = find_request<smem, WARPS>(a, at, &first, s_words, &s_found);
+            const request q = request_of(a.b, it.request);
+            const int64_t per_head = units_of_head<smem>(a, q);
+            it.head = static_cast<int>((at - first) / per_head);
+            it.begin = first + it.head * per_head;
+            it.first_token = q.first;
+            it.columns = q.count * a.group;
+            it.end = it.begin + units_of_block<smem>(a, q, 0);
+            while (at >= it.end)
+            {
+                it.column0 += COLS;
+                it.begin = it.end;
+                it.end += units_of_block<smem>(a, q, it.column0);
+            }
         }
     }
 
@@ -134,8 +163,148 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
         if (live)
         {
             q = request_of(a.b, it.request);
-            // ---- columns ----
-            __syncthreads();
+            __syncthreads(); // the sums of the item before, which lie over the stages, have been read
+            // columns of a block see ever more positions
+            const int last = min(it.column0 + COLS, it.columns) - 1;
+            const int furthest = visible_of(a.b, q, SELECTED ? it.first_token - q.first : last / a.group);
+            const int nearest = SELECTED ? furthest : visible_of(a.b, q, it.column0 / a.group);
+            const int32_t* const table = a.b.table + it.request * a.b.table_ld;
+            const int32_t* list = nullptr;
+            if constexpr (SELECTED)
+            {
+                list = a.idx + (static_cast<int64_t>(it.first_token) * a.c.heads + it.head) * a.ld_idx;
+            }
+            // tiles of the share; none if it ends within the units of the item's beginning
+            int first_tile = max(static_cast<int>(at - it.begin) - COST, 0);
+            int count = max(static_cast<int>(seg_end - it.begin) - COST, 0) - first_tile;
+            if constexpr (CLUSTER)
+            {
+                const int tiles = ((SELECTED ? a.k : furthest) + TILE - 1) / TILE;
+                const int rank = static_cast<int>(blockIdx.x) % a.cluster;
+                first_tile = rank * tiles / a.cluster;
+                count = (rank + 1) * tiles / a.cluster - first_tile;
+            }
+            const int row_end = SELECTED ? a.k : furthest; // rows behind it are zero
+            auto row_of = [&](int j) { return (first_tile + j) * TILE + warp * SUB; };
+
+            // ---- the stream ----
+            constexpr int PARTS = DIM / 16;
+            int slot_in = 0;
+            int slot_out = 0;
+            const uint32_t stage0 = ptx::smem_addr(mine);
+            auto page_at = [&](int pos) {
+                const int p = pos >= 0 ? table[pos >> a.c.page_shift] : -1;
+                return p < a.c.pages ? p : -1;
+            };
+            // All positions: a subtile lies within one page, so its rows are contiguous and share their
+            // scales; the page is looked up one subtile ahead of the copies.  (Pages of 32 subtiles looked up
+            // at a time, one per lane, cost a ragged batch 7 us of 121: items end before it pays.)
+            auto position = [&](int j) { return j < count && row_of(j) < furthest ? row_of(j) : -1; };
+            // A list: the entries and pages of two subtiles at a time, one row per lane, entries two and
+            // pages one such pair ahead.
+            auto entry = [&](int j) {
+                const int e = row_of(j + (lane >> 4)) + (lane & 15);
+                const int p = j + (lane >> 4) < count && e < a.k ? list[e] : -1;
+                return p < furthest ? p : -1;
+            };
+            int pos_next = SELECTED ? entry(0) : position(0);
+            int page_next = page_at(pos_next);
+            int pos_later = 0;
+            int page_now = -1;
+            int64_t offset_now = -1;
+            if constexpr (SELECTED)
+            {
+                pos_later = entry(2);
+            }
+            auto issue = [&](int j) {
+                if (j < count)
+                {
+                    const uint32_t dst = stage0 + slot_in * smem::STAGE;
+                    if constexpr (SELECTED)
+                    {
+                        if ((j & 1) == 0)
+                        {
+                            page_now = page_next;
+                            offset_now = -1;
+                            if (page_now >= 0)
+                            {
+                                offset_now = page_now * a.c.page_stride +
+                                             ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos_next & rows_mask)) * DIM;
+                            }
+                            pos_next = pos_later;
+                            page_next = page_at(pos_next);
+                            pos_later = entry(j + 4);
+                        }
+#pragma unroll
+                        for (int x = 0; x < DIM / 32; ++x)
+                        {
+                            const int e = lane + x * 32;
+                            const int row = e / PARTS;
+                            const int64_t f = __shfl_sync(FULL_MASK, offset_now, (j & 1) * SUB + row);
+                            const int64_t g = max(f, static_cast<int64_t>(0)) + (e % PARTS) * 16;
+                            const uint32_t to = dst + row * PITCH<DIM, true> + (e % PARTS) * 16;
+                            copy16(to, a.c.keys + g, f >= 0 ? 16U : 0U);
+                            copy16(to + SUB * PITCH<DIM, true>, a.c.values + g, f >= 0 ? 16U : 0U);
+                        }
+                        if ((lane >> 4) == (j & 1)) // the scales of each row go with the rows
+                        {
+                            const int64_t at_scale = static_cast<int64_t>(max(page_now, 0)) * a.c.heads + it.head;
+                            const uint32_t to = dst + smem::SCALES + (lane & 15) * 4;
+                            copy4(to, a.c.key_scales + at_scale, page_now >= 0 ? 4U : 0U);
+                            copy4(to + SUB * 4, a.c.value_scales + at_scale, page_now >= 0 ? 4U : 0U);
+                        }
+                    }
+                    else
+                    {
+                        const int page = page_next;
+                        const int safe = max(page, 0);
+                        const int pos = row_of(j);
+                        const int there = page < 0 ? 0 : min(SUB, furthest - pos);
+                        page_next = page_at(position(j + 1));
+                        const int64_t from = safe * a.c.page_stride + lane * 16 +
+                                             ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
+                        const uint8_t* const k_from = a.c.keys + from;
+                        const uint8_t* const v_from = a.c.values + from;
+                        if (there == SUB)
+                        {
+#pragma unroll
+                            for (int x = 0; x < DIM / 32; ++x)
+                            {
+                                const int e = lane + x * 32;
+                                const uint32_t to = dst + e / PARTS * PITCH<DIM, true> + (e % PARTS) * 16;
+                                copy16(to, k_from + x * 512);
+                                copy16(to + SUB * PITCH<DIM, true>, v_from + x * 512);
+                            }
+                        }
+                        else
+                        {
+#pragma unroll
+                            for (int x = 0; x < DIM / 32; ++x)
+                            {
+                                const int e = lane + x * 32;
+                                const int row = e / PARTS;
+                                const uint32_t to = dst + row * PITCH<DIM, true> + (e % PARTS) * 16;
+                                copy16(to, k_from + x * 512, row < there ? 16U : 0U);
+                                copy16(to + SUB * PITCH<DIM, true>, v_from + x * 512, row < there ? 16U : 0U);
+                            }
+                        }
+                        if (lane < 2)
+                        {
+                            const float* scales = lane == 0 ? a.c.key_scales : a.c.value_scales;
+                            copy4(dst + smem::SCALES + lane * 4, scales + static_cast<int64_t>(safe) * a.c.heads + it.head,
+                                  page < 0 ? 0U : 4U);
+                        }
+                    }
+                }
+                copy_commit();
+                slot_in = slot_in + 1 == STAGES ? 0 : slot_in + 1;
+            };
+#pragma unroll
+            for (int j = 0; j < STAGES - 1; ++j)
+            {
+                issue(j);
+            }
+            // ---- the columns, while the first copies are under way ----
             for (int col = warp; col < COLS; col += WARPS)
             {
                 const int g = it.column0 + col;
@@ -152,144 +321,6 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                 }
             }
             __syncthreads();
-            const int last = min(it.column0 + COLS, it.columns) - 1 - it.column0;
-            const int furthest = visible[last];
-            const int nearest = visible[0]; // columns of a block see ever more positions
-            const int32_t* const table = a.b.table + it.request * a.b.table_ld;
-            const int32_t* list = nullptr;
-            if constexpr (SELECTED)
-            {
-                list = a.idx + (static_cast<int64_t>(it.first_token) * a.c.heads + it.head) * a.ld_idx;
-            }
-            // tiles of the share; none if it ends within the units of the item's beginning
-            const int first_tile = max(static_cast<int>(at - it.begin) - smem::COST, 0);
-            const int count = max(static_cast<int>(seg_end - it.begin) - smem::COST, 0) - first_tile;
-            const int row_end = SELECTED ? a.k : furthest; // rows behind it are zero
-            auto row_of = [&](int j) { return (first_tile + j) * TILE + warp * SUB; };
-
-            // ---- the stream ----
-            // Positions and pages are looked up well before the copies that need them.  All positions: one
-            // subtile per lane, 32 subtiles at a time; a subtile lies within one page, so its rows are
-            // contiguous and share their scales.  A list: one entry per lane, two subtiles at a time.
-            constexpr int BATCH = SELECTED ? 2 : 32; // subtiles
-            constexpr int PARTS = DIM / 16;
-            auto where = [&](int j) { // this lane's position in the batch that begins with subtile j; -1: none
-                if constexpr (SELECTED)
-                {
-                    // rows 0 ... 15 of subtile j, then of the next one
-                    const int e = row_of(j + (lane >> 4)) + (lane & 15);
-                    const int p = j + (lane >> 4) < count && e < a.k ? list[e] : -1;
-                    return p < furthest ? p : -1;
-                }
-                const int p = j + lane < count ? row_of(j + lane) : -1;
-                return p < furthest ? p : -1;
-            };
-            auto page_at = [&](int pos) {
-                const int p = pos >= 0 ? table[pos >> a.c.page_shift] : -1;
-                return p < a.c.pages ? p : -1;
-            };
-            auto offset_of = [&](int page, int pos) -> int64_t {
-                return page < 0 ? -1
-                                : page * a.c.page_stride +
-                                      ((static_cast<int64_t>(it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
-            };
-            // key scale (0: absent), log2 of the value scale, its inverse; value scales at the border of their
-            // range and beyond would leave that of the sums
-            auto scales_of = [&](int page) {
-                float3 r = make_float3(0.0F, 0.0F, 0.0F);
-                if (page >= 0)
-                {
-                    const int64_t at_scale = static_cast<int64_t>(page) * a.c.heads + it.head;
-                    const float vs = fminf(fmaxf(a.c.value_scales[at_scale], pow2_int(E_MIN)), pow2_int(E_MAX));
-                    r = make_float3(a.c.key_scales[at_scale], log2_fast(vs), __fdividef(1.0F, vs));
-                }
-                return r;
-            };
-            int batch = 0; // first subtile of the batch the copies are in
-            int pos_next = where(0);
-            int page_next = page_at(pos_next);
-            int page_now = page_next;
-            int64_t offset_now = offset_of(page_next, pos_next);
-            float3 scales_now = scales_of(page_next);
-            float3 scales_before = scales_now;
-            pos_next = where(BATCH);
-            page_next = page_at(pos_next);
-            int pos_later = SELECTED ? where(2 * BATCH) : 0;
-            int slot_in = 0;
-            int slot_out = 0;
-            const uint32_t stage0 = ptx::smem_addr(mine);
-            auto issue = [&](int j) {
-                if (j < count)
-                {
-                    if (j - batch == BATCH)
-                    {
-                        batch = j;
-                        page_now = page_next;
-                        offset_now = offset_of(page_next, pos_next);
-                        if constexpr (!SELECTED)
-                        {
-                            scales_before = scales_now;
-                            scales_now = scales_of(page_next);
-                        }
-                        pos_next = SELECTED ? pos_later : where(j + BATCH);
-                        page_next = page_at(pos_next);
-                        pos_later = SELECTED ? where(j + 2 * BATCH) : 0;
-                    }
-                    const uint32_t dst = stage0 + slot_in * smem::STAGE;
-                    if constexpr (SELECTED)
-                    {
-#pragma unroll
-                        for (int x = 0; x < DIM / 32; ++x)
-                        {
-                            const int e = lane + x * 32;
-                            const int row = e / PARTS;
-                            const int64_t f = __shfl_sync(FULL_MASK, offset_now, (j - batch) * SUB + row);
-                            const int64_t g = max(f, static_cast<int64_t>(0)) + (e % PARTS) * 16;
-                            const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
-                            copy16(to, a.c.keys + g, f >= 0 ? 16U : 0U);
-                            copy16(to + SUB * PITCH<DIM>, a.c.values + g, f >= 0 ? 16U : 0U);
-                        }
-                        if ((lane >> 4) == j - batch) // the scales of each row go with the rows
-                        {
-                            const int64_t at_scale = static_cast<int64_t>(max(page_now, 0)) * a.c.heads + it.head;
-                            const uint32_t to = dst + smem::SCALES + (lane & 15) * 4;
-                            copy4(to, a.c.key_scales + at_scale, page_now >= 0 ? 4U : 0U);
-                            copy4(to + SUB * 4, a.c.value_scales + at_scale, page_now >= 0 ? 4U : 0U);
-                        }
-                    }
-                    else
-                    {
-                        const int64_t offset = __shfl_sync(FULL_MASK, offset_now, j - batch);
-                        const int there = offset < 0 ? 0 : min(SUB, furthest - row_of(j));
-                        const uint8_t* const k_from = a.c.keys + max(offset, static_cast<int64_t>(0)) + lane * 16;
-                        const uint8_t* const v_from = a.c.values + max(offset, static_cast<int64_t>(0)) + lane * 16;
-                        if (there == SUB && 32 % PARTS == 0)
-                        {
-                            const uint32_t to = dst + lane / PARTS * PITCH<DIM> + (lane % PARTS) * 16;
-#pragma unroll
-                            for (int x = 0; x < DIM / 32; ++x)
-                            {
-                                copy16(to + x * (32 / PARTS) * PITCH<DIM>, k_from + x * 512);
-                                copy16(to + (x * (32 / PARTS) + SUB) * PITCH<DIM>, v_from + x * 512);
-                            }
-                        }
-                        else
-                        {
-#pragma unroll
-                            for (int x = 0; x < DIM / 32; ++x)
-                            {
-                                const int e = lane + x * 32;
-                                const int row = e / PARTS;
-                                const uint32_t to = dst + row * PITCH<DIM> + (e % PARTS) * 16;
-                                copy16(to, k_from + x * 512, row < there ? 16U : 0U);
-                                copy16(to + SUB * PITCH<DIM>, v_from + x * 512, row < there ? 16U : 0U);
-                            }
-                        }
-                    }
-                }
-                copy_commit();
-                slot_in = slot_in + 1 == STAGES ? 0 : slot_in + 1;
-            };
             float o[DIM / 16][NB][4];
             float m[NB][2];
             float l[NB][2];
@@ -312,11 +343,6 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     o[g][nb][0] = o[g][nb][1] = o[g][nb][2] = o[g][nb][3] = 0.0F;
                 }
             }
-#pragma unroll
-            for (int j = 0; j < STAGES - 1; ++j)
-            {
-                issue(j);
-            }
             for (int j = 0; j < count; ++j)
             {
                 copy_wait<STAGES - 2>();
@@ -326,27 +352,19 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                 {
                     const unsigned char* const stage = mine + slot_out * smem::STAGE;
                     float s[NB][4];
-                    score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
-                    float ks_lo, ks_hi, lv_lo, lv_hi, iv_lo, iv_hi;
-                    if constexpr (SELECTED)
-                    {
-                        const float* const scales = reinterpret_cast<const float*>(stage + smem::SCALES);
-                        const float vs_lo = fminf(fmaxf(scales[SUB + row_lo], pow2_int(E_MIN)), pow2_int(E_MAX));
-                        const float vs_hi = fminf(fmaxf(scales[SUB + row_lo + 8], pow2_int(E_MIN)), pow2_int(E_MAX));
-                        ks_lo = scales[row_lo];
-                        ks_hi = scales[row_lo + 8];
-                        lv_lo = log2_fast(vs_lo);
-                        lv_hi = log2_fast(vs_hi);
-                        iv_lo = __fdividef(1.0F, vs_lo);
-                        iv_hi = __fdividef(1.0F, vs_hi);
-                    }
-                    else
-                    {
-                        // the copies may have moved on to the next batch
-                        ks_hi = ks_lo = __shfl_sync(FULL_MASK, j < batch ? scales_before.x : scales_now.x, j & 31);
-                        lv_hi = lv_lo = __shfl_sync(FULL_MASK, j < batch ? scales_before.y : scales_now.y, j & 31);
-                        iv_hi = iv_lo = __shfl_sync(FULL_MASK, j < batch ? scales_before.z : scales_now.z, j & 31);
-                    }
+                    score_rows<DIM, NB, true>(s, stage, reinterpret_cast<const uint2*>(image));
+                    const float* const scales = reinterpret_cast<const float*>(stage + smem::SCALES);
+                    const float ks_lo = SELECTED ? scales[row_lo] : scales[0];
+                    const float ks_hi = SELECTED ? scales[row_lo + 8] : ks_lo;
+                    float vs_lo = SELECTED ? scales[SUB + row_lo] : scales[1];
+                    float vs_hi = SELECTED ? scales[SUB + row_lo + 8] : vs_lo;
+                    // value scales at the border of their range and beyond would leave that of the sums
+                    vs_lo = fminf(fmaxf(vs_lo, pow2_int(E_MIN)), pow2_int(E_MAX));
+                    vs_hi = SELECTED ? fminf(fmaxf(vs_hi, pow2_int(E_MIN)), pow2_int(E_MAX)) : vs_lo;
+                    const float lv_lo = log2_fast(vs_lo);
+                    const float lv_hi = SELECTED ? log2_fast(vs_hi) : lv_lo;
+                    const float iv_lo = __fdividef(1.0F, vs_lo);
+                    const float iv_hi = SELECTED ? __fdividef(1.0F, vs_hi) : iv_lo;
                     // absent rows were copied as zeros, scale included; others are seen below `see`
                     const int at_lo = ks_lo != 0.0F ? pos + row_lo : 0x7fffffff;
                     const int at_hi = ks_hi != 0.0F ? pos + row_lo + 8 : 0x7fffffff;
@@ -431,20 +449,21 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     // Only rows that some columns see and others do not can do that (rows nobody sees
                     // were copied as zeros); if such a subtile holds one, the codes are cleaned, and a
                     // second product of indicators finds the outputs that the NaN belongs to.
-                    const unsigned char* const vrows = stage + SUB * PITCH<DIM>;
+                    const unsigned char* const vrows = stage + SUB * PITCH<DIM, true>;
                     bool nan_here = false;
                     if (!SELECTED && nearest < furthest && pos + SUB > nearest)
                     {
                         for (int e = lane; e < SUB * DIM / 4; e += 32)
                         {
                             const uint32_t w =
-                                *reinterpret_cast<const uint32_t*>(vrows + (e * 4 / DIM) * PITCH<DIM> + e * 4 % DIM);
+                                *reinterpret_cast<const uint32_t*>(vrows + (e * 4 / DIM) * PITCH<DIM, true> + e * 4 % DIM);
                             nan_here |= (((w & 0x7f7f7f7fU) + 0x01010101U) & 0x80808080U) != 0;
                         }
                         nan_here = __any_sync(FULL_MASK, nan_here);
                     }
                     const uint32_t vaddr = ptx::smem_addr(vrows) +
-                                           (((lane >> 3) & 1) * 8 + row_order(lane & 7)) * PITCH<DIM> + (lane >> 4) * 16;
+                                           (((lane >> 3) & 1) * 8 + row_order<DIM, true>(lane & 7)) * PITCH<DIM, true> +
+                                           (lane >> 4) * 16;
                     if (!nan_here)
                     {
 #pragma unroll
@@ -566,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                 }
             }
             __syncthreads();
-            const bool whole = at == it.begin && seg_end == it.end;
+            const bool whole = (!CLUSTER || a.cluster == 1) && at == it.begin && seg_end == it.end;
             // part 1 of a block: an item that begins in it and ends in another one; part 0: one that began before
             const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at == it.begin ? 1 : 0);
             for (int e = threadIdx.x; e < COLS * DIM; e += THREADS)
@@ -593,7 +612,16 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     sum += sums[(w * COLS + col) * DIM + d];
                     den += ml.x == -INFINITY ? ml.y : ml.y * exp2_fast(ml.x - top);
                 }
-                if (whole)
+                if (CLUSTER && a.cluster > 1)
+                {
+                    // over the first warp's sum, which no other thread reads
+                    sums[e] = sum;
+                    if (d == 0)
+                    {
+                        block_ml[col] = make_float2(top, den);
+                    }
+                }
+                else if (whole)
                 {
                     const int64_t token = it.first_token + g / a.group;
                     const int qhead = it.head * a.group + g % a.group;
@@ -614,12 +642,56 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     }
                 }
             }
-            if (at == it.begin && !whole && threadIdx.x == 0)
+            if (CLUSTER && a.cluster > 1)
+            {
+                // the blocks of the cluster have the same item: each joins its part of the numbers
+                cluster_sync();
+                const int rank = static_cast<int>(blockIdx.x) % a.cluster;
+                for (int e = rank * THREADS + static_cast<int>(threadIdx.x); e < COLS * DIM; e += a.cluster * THREADS)
+                {
+                    const int col = e / DIM;
+                    const int d = e % DIM;
+                    const int g = it.column0 + col;
+                    if (g >= it.columns)
+                    {
+                        break;
+                    }
+                    float top = -INFINITY;
+                    for (int b = 0; b < a.cluster; ++b)
+                    {
+                        top = fmaxf(top, cluster_load(&block_ml[col].x, b));
+                    }
+                    float sum = 0.0F;
+                    float den = 0.0F;
+                    for (int b = 0; b < a.cluster; ++b)
+                    {
+                        const float m_b = cluster_load(&block_ml[col].x, b);
+                        const float keep = m_b == -INFINITY ? 1.0F : exp2_fast(m_b - top);
+                        sum = fmaf(keep, cluster_load(&sums[e], b), sum);
+                        den = fmaf(keep, cluster_load(&block_ml[col].y, b), den);
+                    }
+                    const int64_t token = it.first_token + g / a.group;
+                    const int qhead = it.head * a.group + g % a.group;
+                    store_out(a.out, token * a.out_stride + static_cast<int64_t>(qhead) * DIM + d,
+                              den == 0.0F ? 0.0F : sum / den, a.dtype);
+                    if (d == 0 && a.lse != nullptr)
+                    {
+                        a.lse[token * a.group * a.c.heads + qhead] =
+                            den == 0.0F ? -INFINITY : (top - WEIGHT_BIAS + log2f(den)) * LN_2;
+                    }
+                }
+                cluster_sync(); // nobody leaves while its numbers are being read
+            }
+            else if (!CLUSTER && at == it.begin && !whole && threadIdx.x == 0)
             {
                 // the block of the item's last unit: blocks begin at floor(c * total / blocks)
                 a.joins[blockIdx.x] = make_int4(it.first_token, it.head, it.column0, it.columns);
                 a.join_end[blockIdx.x] = static_cast<int>(((it.end * blocks) - 1) / total);
             }
+        }
+        if constexpr (CLUSTER)
+        {
+            return;
         }
         // ---- the next item ----
         at = seg_end;
@@ -680,24 +752,64 @@ template <int DIM, int NB, bool SELECTED>
 int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaStream_t stream)
 {
     using smem = attend_smem<DIM, NB>;
-    const int blocks = blocks_of<DIM, NB>();
-    const int rc = place_parts<DIM, smem::COLS>(a, blocks, workspace, workspace_bytes);
+    int blocks = blocks_of<DIM, NB>();
+    if (SELECTED || a.b.starts == nullptr)
+    {
+        // Few short items: each goes to a cluster of blocks of its own, which joins through its shared
+        // memory, so that there is no second kernel and no search for shares.  Taken while the clusters
+        // all run at once and a block has at most eight tiles; the table's width bounds the lengths.
+        const int64_t items = static_cast<int64_t>(a.b.tokens) * a.c.heads * ((a.group + smem::COLS - 1) / smem::COLS);
+        const int64_t most = ((SELECTED ? a.k : a.b.limit) + TILE - 1) / TILE;
+        int cluster = 1;
+        while (cluster < 8 && cluster < most && items * cluster * 2 <= blocks)
+        {
+            cluster *= 2;
+        }
+        if (items * cluster <= blocks && most <= 8 * cluster)
+        {
+            a.cluster = cluster;
+            blocks = static_cast<int>(items) * cluster;
+        }
+    }
+    const int rc = place_parts<DIM, smem::COLS>(a, blocks_of<DIM, NB>(), workspace, workspace_bytes);
     if (rc != BITSKNN_OK)
     {
         return rc;
     }
-    auto kernel = cache_attend_kernel<DIM, NB, SELECTED>;
-    static cache::device_set prepared;
-    if (!prepared.contains_current())
+    auto kernel = a.cluster > 0 ? cache_attend_kernel<DIM, NB, SELECTED, true> : cache_attend_kernel<DIM, NB, SELECTED, false>;
+    static cache::device_set prepared[2];
+    cache::device_set& ready = prepared[a.cluster > 0 ? 1 : 0];
+    if (!ready.contains_current())
     {
         BITSKNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem::BYTES));
-        prepared.add_current();
+        ready.add_current();
     }
     {
         kernel_scope scope("cache_attend_kernel", stream);
+        if (a.cluster > 1)
+        {
+            cudaLaunchAttribute shape{};
+            shape.id = cudaLaunchAttributeClusterDimension;
+            shape.val.clusterDim.x = static_cast<unsigned>(a.cluster);
+            shape.val.clusterDim.y = 1;
+            shape.val.clusterDim.z = 1;
+            cudaLaunchConfig_t config{};
+            config.gridDim = dim3(static_cast<unsigned>(blocks));
+            config.blockDim = dim3(THREADS);
+            config.dynamicSmemBytes = smem::BYTES;
+            config.stream = stream;
+            config.attrs = &shape;
+            config.numAttrs = 1;
+            BITSKNN_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a));
+            return BITSKNN_OK;
+        }
         kernel<<<blocks, THREADS, smem::BYTES, stream>>>(a);
     }
     BITSKNN_CUDA_TRY(cudaGetLastError());
+    if (a.cluster > 0)
+    {
+        return BITSKNN_OK;
+    }
     return launch_join<DIM, smem::COLS>(a, blocks, stream);
 }
 

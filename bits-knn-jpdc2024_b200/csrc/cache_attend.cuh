@@ -35,6 +35,7 @@ struct attend_args
     float2* part_ml;  // [2 * blocks][columns]
     int4* joins;      // [blocks]
     int* join_end;    // [blocks]
+    int cluster;        // > 0: an item to every cluster of so many blocks, which joins by itself
 };
 
 // What the stream of a block works on: one block of query columns of a request and head.
@@ -178,38 +179,51 @@ __device__ __forceinline__ int find_request(const attend_args& a, int64_t at, in
 // Joins the parts of items that several blocks worked on: block c looks after the item that begins
 // in block c of the main kernel and ends in a later one, whose parts are part 1 of block c and
 // part 0 of the blocks up to its last.  Always in that order, so results do not depend on timing.
-// One warp per column; launched while the main kernel still runs (griddepcontrol), so that its
-// own launch takes no time.
+// SPLIT warps share the parts of a column (many parts of few columns when a long request decodes, few
+// parts of many columns when prompts are attended to).  Launched while the main kernel still runs
+// (griddepcontrol), so that its own launch takes no time.
+constexpr int JOIN_WARPS = 8;
+
 template <int DIM, int COLS>
-__global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
+constexpr int JOIN_SPLIT = COLS <= 32 ? JOIN_WARPS : 1;
+
+template <int DIM, int COLS>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const attend_args a)
 {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 join = a.joins[blockIdx.x];
-    const int col = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (col >= join.w - join.z)
-    {
-        return;
-    }
-    const int64_t first = 2 * static_cast<int64_t>(blockIdx.x) + 1;
-    const int parts = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x) + 1;
-    auto part = [&](int i) { return (first + (i == 0 ? 0 : 2 * i - 1)) * COLS + col; };
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32)
-    {
-        top = fmaxf(top, a.part_ml[part(i)].x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-    {
-        top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
-    }
+    constexpr int SPLIT = JOIN_SPLIT<DIM, COLS>;
     constexpr int PER = DIM / 32;
     constexpr int VEC = PER % 4 == 0 ? 4 : PER % 2 == 0 ? 2 : 1; // numbers per load
     struct alignas(4 * VEC) vec
     {
         float v[VEC];
     };
+    __shared__ float s_sum[SPLIT > 1 ? SPLIT : 1][DIM];
+    __shared__ float2 s_ml[SPLIT > 1 ? SPLIT : 1];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 join = a.joins[blockIdx.x];
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int col = SPLIT > 1 ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * JOIN_WARPS + warp;
+    if (col >= join.w - join.z)
+    {
+        return; // the whole block when warps share a column
+    }
+    const int64_t first = 2 * static_cast<int64_t>(blockIdx.x) + 1;
+    const int all = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x) + 1;
+    auto part = [&](int i) { return (first + (i == 0 ? 0 : 2 * i - 1)) * COLS + col; };
+    // this warp's parts, a run of them so that the order of the sums is that of the positions
+    const int begin = SPLIT > 1 ? warp * all / SPLIT : 0;
+    const int parts = SPLIT > 1 ? (warp + 1) * all / SPLIT - begin : all;
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32)
+    {
+        top = fmaxf(top, a.part_ml[part(begin + i)].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+    }
     float sum[PER];
 #pragma unroll
     for (int x = 0; x < PER; ++x)
@@ -222,7 +236,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
         float keep = 0.0F;
         if (base + lane < parts)
         {
-            const float2 ml = a.part_ml[part(base + lane)];
+            const float2 ml = a.part_ml[part(begin + base + lane)];
             keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
             den = fmaf(keep, ml.y, den);
         }
@@ -231,7 +245,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
         for (int i = 0; i < here; ++i)
         {
             const float f = __shfl_sync(FULL_MASK, keep, i);
-            const vec* from = reinterpret_cast<const vec*>(a.part_o + part(base + i) * DIM) + lane;
+            const vec* from = reinterpret_cast<const vec*>(a.part_o + part(begin + base + i) * DIM) + lane;
 #pragma unroll
             for (int x = 0; x < PER / VEC; ++x)
             {
@@ -248,6 +262,46 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const attend_args a)
     for (int o = 16; o > 0; o >>= 1)
     {
         den += __shfl_xor_sync(FULL_MASK, den, o);
+    }
+    if constexpr (SPLIT > 1)
+    {
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+        {
+            s_sum[warp][(x / VEC * 32 + lane) * VEC + x % VEC] = sum[x];
+        }
+        if (lane == 0)
+        {
+            s_ml[warp] = make_float2(top, den);
+        }
+        __syncthreads();
+        if (warp > 0)
+        {
+            return;
+        }
+#pragma unroll
+        for (int w = 0; w < SPLIT; ++w)
+        {
+            top = fmaxf(top, s_ml[w].x);
+        }
+        den = 0.0F;
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+        {
+            sum[x] = 0.0F;
+        }
+#pragma unroll
+        for (int w = 0; w < SPLIT; ++w)
+        {
+            const float2 ml = s_ml[w];
+            const float keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
+            den = fmaf(keep, ml.y, den);
+#pragma unroll
+            for (int x = 0; x < PER; ++x)
+            {
+                sum[x] = fmaf(keep, s_sum[w][(x / VEC * 32 + lane) * VEC + x % VEC], sum[x]);
+            }
+        }
     }
     const int g = join.z + col;
     const int64_t token = join.x + g / a.group;
@@ -297,8 +351,8 @@ int launch_join(const attend_args& a, int blocks, cudaStream_t stream)
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(blocks), COLS / 8);
-    config.blockDim = dim3(256);
+    config.gridDim = dim3(static_cast<unsigned>(blocks), COLS * JOIN_SPLIT<DIM, COLS> / JOIN_WARPS);
+    config.blockDim = dim3(JOIN_WARPS * 32);
     config.stream = stream;
     config.attrs = &early;
     config.numAttrs = 1;

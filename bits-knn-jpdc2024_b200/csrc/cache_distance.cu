@@ -39,7 +39,7 @@ __device__ __forceinline__ float max_nan(float a, float b)
 template <int DIM, int NB>
 struct distance_smem
 {
-    static constexpr int STAGE = SUB * PITCH<DIM>;
+    static constexpr int STAGE = SUB * PITCH<DIM, false>;
     static constexpr int SCRATCH = 8 * NB * (SUB + 1) * 4;
     static constexpr int IMAGE = NB * 16 * DIM; // 8 NB columns of DIM halves
     static constexpr int BYTES = IMAGE + 8 * NB * 4 + WARPS * (DIST_STAGES * STAGE + SCRATCH);
@@ -152,25 +152,20 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                     }
                     const int64_t offset = __shfl_sync(FULL_MASK, offset_now, j - batch);
                     const int there = offset < 0 ? 0 : min(SUB, furthest - (first + j * WARPS) * SUB);
-                    const uint32_t dst = stage0 + slot_in * smem::STAGE + lane / PARTS * PITCH<DIM> + (lane % PARTS) * 16;
+                    const uint32_t dst = stage0 + slot_in * smem::STAGE;
                     const uint8_t* src = a.c.keys + max(offset, static_cast<int64_t>(0)) + lane * 16;
-                    if (there == SUB && 32 % PARTS == 0)
-                    {
 #pragma unroll
-                        for (int x = 0; x < DIM / 32; ++x)
+                    for (int x = 0; x < DIM / 32; ++x)
+                    {
+                        const int e = lane + x * 32;
+                        const uint32_t to = dst + granule_byte<DIM, false>(e / PARTS, e % PARTS);
+                        if (there == SUB)
                         {
-                            copy16(dst + x * (32 / PARTS) * PITCH<DIM>, src + x * 512);
+                            copy16(to, src + x * 512);
                         }
-                    }
-                    else
-                    {
-#pragma unroll
-                        for (int x = 0; x < DIM / 32; ++x)
+                        else
                         {
-                            const int e = lane + x * 32;
-                            const int row = e / PARTS;
-                            copy16(stage0 + slot_in * smem::STAGE + row * PITCH<DIM> + (e % PARTS) * 16, src + x * 512,
-                                   row < there ? 16U : 0U);
+                            copy16(to, src + x * 512, e / PARTS < there ? 16U : 0U);
                         }
                     }
                 }
@@ -199,7 +194,7 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                 float s[NB][4];
                 if (j < loaded)
                 {
-                    score_rows<DIM, NB>(s, stage, reinterpret_cast<const uint2*>(image));
+                    score_rows<DIM, NB, false>(s, stage, reinterpret_cast<const uint2*>(image));
                 }
                 if (simple)
                 {
@@ -224,7 +219,7 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                         hi = max_nan(hi, __shfl_xor_sync(FULL_MASK, hi, o));
                     }
                     // lanes 0 and 1 of a group of four write its rows row_order and 8 + row_order
-                    const int at = pos + row_order(lane >> 2) + (lane & 1) * 8;
+                    const int at = pos + row_order<DIM, false>(lane >> 2) + (lane & 1) * 8;
                     if ((lane & 2) == 0 && at < end)
                     {
                         only[at] = ks != 0.0F && at < furthest ? -(((lane & 1) == 0 ? lo : hi) * ks) : INFINITY;
@@ -238,7 +233,7 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
-                        float* out = scratch + (nb * 8 + (lane & 3) * 2) * (SUB + 1) + row_order(lane >> 2);
+                        float* out = scratch + (nb * 8 + (lane & 3) * 2) * (SUB + 1) + row_order<DIM, false>(lane >> 2);
                         out[0] = s[nb][0] * factor[nb][0];
                         out[SUB + 1] = s[nb][1] * factor[nb][1];
                         out[8] = s[nb][2] * factor[nb][0];
