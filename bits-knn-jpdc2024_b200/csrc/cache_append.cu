@@ -76,6 +76,57 @@ __device__ __forceinline__ void floats_of(const raw8<DTYPE>& r, float (&v)[8])
     }
 }
 
+// The largest size among the numbers of `r` and `acc`: two packed 16-bit numbers, or one float's bits.  NaN
+// counts for nothing, infinities count.
+template <int DTYPE>
+__device__ __forceinline__ uint32_t larger(uint32_t acc, const raw8<DTYPE>& r)
+{
+#pragma unroll
+    for (int i = 0; i < (DTYPE == BITSKNN_F32 ? 2 : 1); ++i)
+    {
+        const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            if constexpr (DTYPE == BITSKNN_F32)
+            {
+                acc = __float_as_uint(fmaxf(__uint_as_float(acc), fabsf(__uint_as_float(w[j]))));
+            }
+            else if constexpr (DTYPE == BITSKNN_BF16)
+            {
+                const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&acc),
+                                                 __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
+                acc = *reinterpret_cast<const uint32_t*>(&m);
+            }
+            else
+            {
+                const __half2 m =
+                    __hmax2(*reinterpret_cast<const __half2*>(&acc), __habs2(*reinterpret_cast<const __half2*>(&w[j])));
+                acc = *reinterpret_cast<const uint32_t*>(&m);
+            }
+        }
+    }
+    return acc;
+}
+
+template <int DTYPE>
+__device__ __forceinline__ float size_of(uint32_t acc)
+{
+    if constexpr (DTYPE == BITSKNN_F32)
+    {
+        return __uint_as_float(acc);
+    }
+    else if constexpr (DTYPE == BITSKNN_BF16)
+    {
+        return fmaxf(__uint_as_float(acc << 16), __uint_as_float(acc & 0xffff0000U));
+    }
+    else
+    {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&acc));
+        return fmaxf(f.x, f.y);
+    }
+}
+
 // Smallest power of two s in [2^E_MIN, 2^E_MAX] with amax <= 448 s.  448 = 1.75 * 2^8, so the
 // exponent is that of amax less 8, and one more if its fraction is above 1.75.
 __device__ __forceinline__ float scale_of(float amax)
@@ -106,9 +157,11 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
     const int64_t stride = a.stride[which];
     uint8_t* const codes = which == 0 ? a.c.keys : a.c.values;
     float* const scales = which == 0 ? a.c.key_scales : a.c.value_scales;
-    const int vecs = a.dim >> 3; // vectors per row
-    // w / vecs == (w * vec_magic) >> 16 for w < 2^13, the most vectors a run can have (256 rows of 32)
-    const int vec_magic = (65536 + vecs - 1) / vecs;
+    // a thread serves one vector of eight numbers of every row_step-th row
+    const int vecs = a.dim >> 3;
+    const int row_step = APPEND_THREADS / vecs;
+    const int row0 = t < row_step * vecs ? t / vecs : 1 << 20;
+    const int at_vec = t % vecs * 8;
     const int rows_mask = (1 << a.c.page_shift) - 1;
     const int first_token = blockIdx.x * a.window;
     int end_token = min(first_token + a.window, a.tokens);
@@ -176,44 +229,47 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         }
         const int offset0 = static_cast<int>(slot0) & rows_mask;
         const int64_t base = page * a.c.page_stride + (static_cast<int64_t>(head) << a.c.page_shift) * a.dim;
-        const int work = run * vecs;
+        // rows of the page one after the other, as they are unless a caller leaves some out
+        const bool dense = a.slots[i + run - 1] - slot0 == run - 1;
+        const int64_t from = (i + row0) * stride + static_cast<int64_t>(head) * a.dim + at_vec;
         raw8<DTYPE> held[HELD];
-        float top = 0.0F;
-        auto fetch = [&](int w) {
-            const int row = (w * vec_magic) >> 16;
-            const int part = w - row * vecs;
-            return load8<DTYPE>(src, (i + row) * stride + static_cast<int64_t>(head) * a.dim + part * 8);
-        };
-        auto look = [&](const raw8<DTYPE>& x) {
-            float f[8];
-            floats_of<DTYPE>(x, f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                const float v = fabsf(f[e]);
-                top = v < INFINITY ? fmaxf(top, v) : top; // NaN and the infinities set no scale
-            }
-        };
+        auto fetch = [&](int h) { return load8<DTYPE>(src, from + h * row_step * stride); };
+        uint32_t acc = 0;
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
         {
-            const int w = t + h * APPEND_THREADS;
-            if (w < work)
+            if (row0 + h * row_step < run)
             {
-                held[h] = fetch(w);
+                held[h] = fetch(h);
             }
         }
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
         {
-            if (t + h * APPEND_THREADS < work)
+            if (row0 + h * row_step < run)
             {
-                look(held[h]);
+                acc = larger<DTYPE>(acc, held[h]);
             }
         }
-        for (int w = t + HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
+        for (int h = HELD; row0 + h * row_step < run; ++h)
         {
-            look(fetch(w));
+            acc = larger<DTYPE>(acc, fetch(h));
+        }
+        float top = size_of<DTYPE>(acc);
+        if (top == INFINITY)
+        {
+            // infinities set no scale: the largest finite number of this thread
+            top = 0.0F;
+            for (int h = 0; row0 + h * row_step < run; ++h)
+            {
+                float f[8];
+                floats_of<DTYPE>(fetch(h), f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    top = fabsf(f[e]) < INFINITY ? fmaxf(top, fabsf(f[e])) : top;
+                }
+            }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
@@ -237,31 +293,29 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         const float old = stored > 0.0F && stored <= cache::pow2_int(cache::E_MAX) ? stored : cache::pow2_int(cache::E_MIN);
         const float scale = fmaxf(scale_of(top), old);
         const float inverse = 1.0F / scale;
-        auto store = [&](int w, const raw8<DTYPE>& x) {
+        auto store = [&](int h, const raw8<DTYPE>& x) {
             float f[8];
             floats_of<DTYPE>(x, f);
-            const int row = (w * vec_magic) >> 16;
-            const int part = w - row * vecs;
-            const int64_t at = base + static_cast<int64_t>(static_cast<int>(a.slots[i + row]) & rows_mask) * a.dim + part * 8;
+            const int row = row0 + h * row_step;
+            const int offset = dense ? offset0 + row : static_cast<int>(a.slots[i + row]) & rows_mask;
             uint2 out;
             out.x = cache::codes_of_floats(f[0] * inverse, f[1] * inverse) |
                     cache::codes_of_floats(f[2] * inverse, f[3] * inverse) << 16;
             out.y = cache::codes_of_floats(f[4] * inverse, f[5] * inverse) |
                     cache::codes_of_floats(f[6] * inverse, f[7] * inverse) << 16;
-            *reinterpret_cast<uint2*>(codes + at) = out;
+            *reinterpret_cast<uint2*>(codes + base + static_cast<int64_t>(offset) * a.dim + at_vec) = out;
         };
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
         {
-            const int w = t + h * APPEND_THREADS;
-            if (w < work)
+            if (row0 + h * row_step < run)
             {
-                store(w, held[h]);
+                store(h, held[h]);
             }
         }
-        for (int w = t + HELD * APPEND_THREADS; w < work; w += APPEND_THREADS)
+        for (int h = HELD; row0 + h * row_step < run; ++h)
         {
-            store(w, fetch(w));
+            store(h, fetch(h));
         }
         if (offset0 > 0 && scale > old)
         {

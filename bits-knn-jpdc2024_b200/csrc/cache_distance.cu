@@ -87,6 +87,22 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
         const int64_t nearest = static_cast<int64_t>(q.length) - q.count + (token - q.first) + 1; // token i sees i more
         const int32_t* table = a.b.table + r * a.b.table_ld;
         const int columns = many * a.group;
+        float* const only = a.dist + (static_cast<int64_t>(token) * a.c.heads + head) * a.ld;
+        // columns that no token sees, but for those that share a subtile with some that one does
+        const int unseen = max((furthest + SUB - 1) / SUB * SUB, begin);
+        for (int i = 0; i < many; ++i)
+        {
+            float* const out = only + static_cast<int64_t>(i) * a.c.heads * a.ld;
+            for (int col = unseen + static_cast<int>(threadIdx.x); col < end; col += THREADS)
+            {
+                out[col] = INFINITY;
+            }
+        }
+        if (begin >= furthest)
+        {
+            token += many;
+            continue;
+        }
         // blocks of columns: one, unless a head has more query heads than a block has columns
         for (int col0 = 0; col0 < columns; col0 += 8 * NB)
         {
@@ -112,12 +128,12 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                 factor[nb][1] = undo[nb * 8 + (lane & 3) * 2 + 1];
             }
             const int first = begin / SUB + warp;
-            const int count = end > first * SUB ? ((end - 1) / SUB - first) / WARPS + 1 : 0;
-            const int loaded = furthest > first * SUB ? min(count, ((furthest - 1) / SUB - first) / WARPS + 1) : 0;
+            const int seen = min(end, furthest);
+            const int count = seen > first * SUB ? ((seen - 1) / SUB - first) / WARPS + 1 : 0;
             // Where the warp's next 32 subtiles lie and their scales, one subtile per lane; looked up a batch
             // ahead.  A subtile lies within one page, so its rows are contiguous and share a scale.
             auto page_of = [&](int j) {
-                const int p = j < loaded ? table[((first + j * WARPS) * SUB) >> a.c.page_shift] : -1;
+                const int p = j < count ? table[((first + j * WARPS) * SUB) >> a.c.page_shift] : -1;
                 return p < a.c.pages ? p : -1;
             };
             auto offset_of = [&](int page, int j) -> int64_t {
@@ -140,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
             const uint32_t stage0 = ptx::smem_addr(mine);
             constexpr int PARTS = DIM / 16;
             auto issue = [&](int j) {
-                if (j < loaded)
+                if (j < count)
                 {
                     if (j - batch == 32)
                     {
@@ -182,7 +198,6 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
             const int row = lane & (SUB - 1);
             const int half = lane >> 4;
             const int cols = min(columns - col0, 8 * NB);
-            float* const only = a.dist + (static_cast<int64_t>(token) * a.c.heads + head) * a.ld;
             for (int j = 0; j < count; ++j)
             {
                 const int pos = (first + j * WARPS) * SUB;
@@ -190,27 +205,21 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                 __syncwarp();
                 const unsigned char* const stage = mine + slot_out * smem::STAGE;
                 slot_out = slot_out + 1 == DIST_STAGES ? 0 : slot_out + 1;
-                const float ks = j < loaded ? __shfl_sync(FULL_MASK, j < batch ? scale_before : scale_now, j & 31) : 0.0F;
+                const float ks = __shfl_sync(FULL_MASK, j < batch ? scale_before : scale_now, j & 31);
                 float s[NB][4];
-                if (j < loaded)
-                {
-                    score_rows<DIM, NB, false>(s, stage, reinterpret_cast<const uint2*>(image));
-                }
+                score_rows<DIM, NB, false>(s, stage, reinterpret_cast<const uint2*>(image));
                 if (simple)
                 {
                     float lo = -INFINITY;
                     float hi = -INFINITY;
-                    if (j < loaded)
-                    {
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-                        {
-                            const int c = nb * 8 + (lane & 3) * 2;
-                            lo = max_nan(lo, c < columns ? s[nb][0] * factor[nb][0] : -INFINITY);
-                            hi = max_nan(hi, c < columns ? s[nb][2] * factor[nb][0] : -INFINITY);
-                            lo = max_nan(lo, c + 1 < columns ? s[nb][1] * factor[nb][1] : -INFINITY);
-                            hi = max_nan(hi, c + 1 < columns ? s[nb][3] * factor[nb][1] : -INFINITY);
-                        }
+                    for (int nb = 0; nb < NB; ++nb)
+                    {
+                        const int c = nb * 8 + (lane & 3) * 2;
+                        lo = max_nan(lo, c < columns ? s[nb][0] * factor[nb][0] : -INFINITY);
+                        hi = max_nan(hi, c < columns ? s[nb][2] * factor[nb][0] : -INFINITY);
+                        lo = max_nan(lo, c + 1 < columns ? s[nb][1] * factor[nb][1] : -INFINITY);
+                        hi = max_nan(hi, c + 1 < columns ? s[nb][3] * factor[nb][1] : -INFINITY);
                     }
 #pragma unroll
                     for (int o = 1; o < 4; o <<= 1)
@@ -228,7 +237,6 @@ __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_
                     issue(j + DIST_STAGES - 1);
                     continue;
                 }
-                if (j < loaded)
                 {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
