@@ -742,9 +742,6 @@ int blocks_of()
     return device_sm_count() * attend_smem<DIM, NB>::BLOCKS;
 }
 
-// From this many query columns per request and head on the tensor-memory kernel takes over.
-constexpr int TC_COLUMNS = 64;
-
 // Most columns a block can take: the sums of 8 NB columns take NB * DIM / 4 registers of a thread.
 constexpr int most_columns(int dim) { return dim <= 128 ? 4 : 2; }
 
@@ -876,7 +873,10 @@ int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, con
     const int64_t per_request = selected ? 1 : (batch->tokens + batch->requests - 1) / batch->requests;
     const int64_t want = a.group * per_request;
     auto s = static_cast<cudaStream_t>(stream);
-    if (!selected && want >= TC_COLUMNS)
+    // More columns than one stream of the cache can serve: the tensor-memory kernel takes over (16 requests
+    // of 6000 positions, 8 heads of 128: 32 columns 109 us here and 133 there, 48 columns 166 and 134, 128
+    // columns 316 and 144; 256 numbers, 16 columns 72 and 99, 24 columns 105 and 101).
+    if (!selected && want > 8 * most_columns(cache->dim))
     {
         return launch_attend_tc(cache->dim, a, d_workspace, workspace_bytes, s);
     }

@@ -29,7 +29,7 @@ struct tc_shape
     static constexpr int NQ = DIM <= 128 ? 2 : 1;
     static constexpr int COLS = 128 * NQ;
     static constexpr int ROWS = 64;
-    static constexpr int COST = 4;               // an item's beginning and end, in tiles
+    static constexpr int COST = 10;              // an item's beginning and end, in tiles (4: 402 us, 8: 391, 12: 389)
     static constexpr int BLK = (DIM + 63) / 64;  // 128-byte blocks of 64 halves per row
     static constexpr int Q_BYTES = BLK * 128 * 128;
     static constexpr int KV_BYTES = BLK * ROWS * 128;
