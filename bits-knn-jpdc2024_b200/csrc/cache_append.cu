@@ -144,6 +144,9 @@ __device__ __forceinline__ float scale_of(float amax)
 // A page has one scale per head, which is why a run belongs to one block and why a later token
 // that needs a larger scale re-rounds the rows in front of it: with powers of two that only
 // costs bits at the subnormal end, code * 2^(old - new) is exact for every other code.
+//
+// Bound by HBM (numbers in, codes out) for prompts: 27392 tokens x 8 heads x 128 halves, 169 MB, in 37 us
+// = 4.6 TB/s, 0.70 of the measured copy rate; a decode step is one launch of 6 us.
 template <int DTYPE>
 __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const append_args a)
 {
@@ -153,8 +156,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
     const int lane = t & 31;
     const int head = blockIdx.y;
     const int which = blockIdx.z;
-    const void* src = a.src[which];
-    const int64_t stride = a.stride[which];
+    const void* src = which == 0 ? a.src[0] : a.src[1];
+    const int64_t stride = which == 0 ? a.stride[0] : a.stride[1];
     uint8_t* const codes = which == 0 ? a.c.keys : a.c.values;
     float* const scales = which == 0 ? a.c.key_scales : a.c.value_scales;
     // a thread serves one vector of eight numbers of every row_step-th row
@@ -235,20 +238,31 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         raw8<DTYPE> held[HELD];
         auto fetch = [&](int h) { return load8<DTYPE>(src, from + h * row_step * stride); };
         uint32_t acc = 0;
-#pragma unroll
-        for (int h = 0; h < HELD; ++h)
+        // the whole page at once: every thread has all its vectors, and nothing is asked for each of them
+        const bool full = run >= HELD * row_step && row_step * vecs == APPEND_THREADS;
+        if (full)
         {
-            if (row0 + h * row_step < run)
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
             {
                 held[h] = fetch(h);
             }
-        }
 #pragma unroll
-        for (int h = 0; h < HELD; ++h)
-        {
-            if (row0 + h * row_step < run)
+            for (int h = 0; h < HELD; ++h)
             {
                 acc = larger<DTYPE>(acc, held[h]);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+            {
+                if (row0 + h * row_step < run)
+                {
+                    held[h] = fetch(h);
+                    acc = larger<DTYPE>(acc, held[h]);
+                }
             }
         }
         for (int h = HELD; row0 + h * row_step < run; ++h)
@@ -293,29 +307,41 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         const float old = stored > 0.0F && stored <= cache::pow2_int(cache::E_MAX) ? stored : cache::pow2_int(cache::E_MIN);
         const float scale = fmaxf(scale_of(top), old);
         const float inverse = 1.0F / scale;
-        auto store = [&](int h, const raw8<DTYPE>& x) {
+        uint8_t* const to = codes + base + at_vec;
+        auto store = [&](int h, const raw8<DTYPE>& x, bool in_order) {
             float f[8];
             floats_of<DTYPE>(x, f);
             const int row = row0 + h * row_step;
-            const int offset = dense ? offset0 + row : static_cast<int>(a.slots[i + row]) & rows_mask;
+            const int offset = in_order ? offset0 + row : static_cast<int>(a.slots[i + row]) & rows_mask;
             uint2 out;
             out.x = cache::codes_of_floats(f[0] * inverse, f[1] * inverse) |
                     cache::codes_of_floats(f[2] * inverse, f[3] * inverse) << 16;
             out.y = cache::codes_of_floats(f[4] * inverse, f[5] * inverse) |
                     cache::codes_of_floats(f[6] * inverse, f[7] * inverse) << 16;
-            *reinterpret_cast<uint2*>(codes + base + static_cast<int64_t>(offset) * a.dim + at_vec) = out;
+            *reinterpret_cast<uint2*>(to + offset * a.dim) = out;
         };
-#pragma unroll
-        for (int h = 0; h < HELD; ++h)
+        if (full && dense)
         {
-            if (row0 + h * row_step < run)
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
             {
-                store(h, held[h]);
+                store(h, held[h], true);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+            {
+                if (row0 + h * row_step < run)
+                {
+                    store(h, held[h], dense);
+                }
             }
         }
         for (int h = HELD; row0 + h * row_step < run; ++h)
         {
-            store(h, fetch(h));
+            store(h, fetch(h), dense);
         }
         if (offset0 > 0 && scale > old)
         {
@@ -410,9 +436,9 @@ extern "C" int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_
     a.tokens = static_cast<int>(tokens);
     a.dim = cache->dim;
     a.dtype = dtype;
-    // few tokens: one block for each, so that the runs of a decode step (one token long) run side by
-    // side; many: windows, so that the grid stays at some sixteen blocks per SM
-    const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(device_sm_count()) * 16 / (2 * cache->heads));
+    // Few tokens: one block for each, so that the runs of a decode step (one token long) run side by side;
+    // many: windows, as many as run at once (27392 tokens, 8 heads of 128: 8 blocks per SM 37 us, 16 and 32 40).
+    const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(device_sm_count()) * 8 / (2 * cache->heads));
     a.window = static_cast<int>((tokens + target - 1) / target);
     const int64_t windows = (tokens + a.window - 1) / a.window;
     const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(cache->heads), 2U);

@@ -215,15 +215,6 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
     const int begin = SPLIT > 1 ? warp * all / SPLIT : 0;
     const int parts = SPLIT > 1 ? (warp + 1) * all / SPLIT - begin : all;
     float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32)
-    {
-        top = fmaxf(top, a.part_ml[part(begin + i)].x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-    {
-        top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
-    }
     float sum[PER];
 #pragma unroll
     for (int x = 0; x < PER; ++x)
@@ -231,37 +222,90 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
         sum[x] = 0.0F;
     }
     float den = 0.0F;
-    for (int base = 0; base < parts; base += 32)
+    constexpr int FEW = 4;
+    if (SPLIT == 1 && parts <= FEW)
     {
-        float keep = 0.0F;
-        if (base + lane < parts)
-        {
-            const float2 ml = a.part_ml[part(begin + base + lane)];
-            keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
-            den = fmaf(keep, ml.y, den);
-        }
-        const int here = min(parts - base, 32);
-#pragma unroll 8
-        for (int i = 0; i < here; ++i)
-        {
-            const float f = __shfl_sync(FULL_MASK, keep, i);
-            const vec* from = reinterpret_cast<const vec*>(a.part_o + part(begin + base + i) * DIM) + lane;
+        // the usual case of prompts: everything is loaded at once, and every lane weighs for itself
+        float2 ml[FEW];
+        vec w[FEW][PER / VEC];
 #pragma unroll
-            for (int x = 0; x < PER / VEC; ++x)
+        for (int i = 0; i < FEW; ++i)
+        {
+            ml[i] = make_float2(-INFINITY, 0.0F);
+            if (i < parts)
             {
-                const vec w = from[x * 32];
+                ml[i] = a.part_ml[part(i)];
+                const vec* from = reinterpret_cast<const vec*>(a.part_o + part(i) * DIM) + lane;
 #pragma unroll
-                for (int y = 0; y < VEC; ++y)
+                for (int x = 0; x < PER / VEC; ++x)
                 {
-                    sum[x * VEC + y] = fmaf(f, w.v[y], sum[x * VEC + y]);
+                    w[i][x] = from[x * 32];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < FEW; ++i)
+        {
+            top = fmaxf(top, ml[i].x);
+        }
+#pragma unroll
+        for (int i = 0; i < FEW; ++i)
+        {
+            if (i < parts)
+            {
+                const float keep = ml[i].x == -INFINITY ? 1.0F : exp2_fast(ml[i].x - top);
+                den = fmaf(keep, ml[i].y, den);
+#pragma unroll
+                for (int x = 0; x < PER; ++x)
+                {
+                    sum[x] = fmaf(keep, w[i][x / VEC].v[x % VEC], sum[x]);
                 }
             }
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    else
     {
-        den += __shfl_xor_sync(FULL_MASK, den, o);
+        for (int i = lane; i < parts; i += 32)
+        {
+            top = fmaxf(top, a.part_ml[part(begin + i)].x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+        {
+            top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+        }
+        for (int base = 0; base < parts; base += 32)
+        {
+            float keep = 0.0F;
+            if (base + lane < parts)
+            {
+                const float2 ml = a.part_ml[part(begin + base + lane)];
+                keep = ml.x == -INFINITY ? 1.0F : exp2_fast(ml.x - top);
+                den = fmaf(keep, ml.y, den);
+            }
+            const int here = min(parts - base, 32);
+#pragma unroll 8
+            for (int i = 0; i < here; ++i)
+            {
+                const float f = __shfl_sync(FULL_MASK, keep, i);
+                const vec* from = reinterpret_cast<const vec*>(a.part_o + part(begin + base + i) * DIM) + lane;
+#pragma unroll
+                for (int x = 0; x < PER / VEC; ++x)
+                {
+                    const vec w = from[x * 32];
+#pragma unroll
+                    for (int y = 0; y < VEC; ++y)
+                    {
+                        sum[x * VEC + y] = fmaf(f, w.v[y], sum[x * VEC + y]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+        {
+            den += __shfl_xor_sync(FULL_MASK, den, o);
+        }
     }
     if constexpr (SPLIT > 1)
     {

@@ -942,8 +942,15 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 //   Barriers that one role completes and another reads the fruits of (scales, NaN) carry an arrival of
 // the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
 //
-// Bound by the exponentials (16 per clock and SM: 1024 clocks for 256 rows x 64 positions) and the
-// tensor cores (4 products of 128 x 64 x 128: about 1200 clocks) alike.
+// What bounds it: per 256 rows x 64 positions the exponentials need 1024 clocks (16 per clock and SM), the
+// products about 1300 (128 x 64 x 16: some 45 clocks, 128 x 128 x 16: 73), the operands from shared memory
+// about 1300; a tile takes some 2260, because the steps of one tile depend on one another and a warp's
+// 64 weights alone take 1200 with the other warp of its scheduler doing the same.  3 requests of 1500 ... 8000
+// cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 390 us = 0.79 PFLOP/s, 0.48
+// of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two score
+// tiles of 64 511; packed arithmetic and offsets per 16 rows 444; a thread for each kind of product 405.  Tried
+// and slower: two threads per row (520), other register splits (403 ... 417), rows packed by neighbouring
+// lanes (409), the weights' code shared by both paths in a loop (580: the scores then live on across it).
 template <int DIM>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)
 {

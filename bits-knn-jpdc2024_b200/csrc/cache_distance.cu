@@ -50,7 +50,8 @@ struct distance_smem
 // multiplies them with all columns at once on the tensor cores: keys are the 16 rows of the
 // matrix step, the query heads of the tokens its columns, so a code is converted to a half once
 // for all of them.  Products of a key code (4 significant bits) and a query half are exact; the sums
-// are FP32.  Bound by the key bytes and the matrix it writes (HBM) while the columns are few.
+// are FP32.  Bound by the key bytes and the matrix it writes (HBM) while the columns are few: 16 requests of
+// 2000 ... 60000 positions, 8 heads of 128, 294 MB in 60 us = 4.9 TB/s, 0.75 of the measured copy rate.
 template <int DIM, int NB>
 __global__ void __launch_bounds__(THREADS) cache_distance_kernel(const distance_args a)
 {
