@@ -827,7 +827,7 @@ int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, con
     {
         return rc;
     }
-    if (selected && k < 1)
+    if (selected && (k < 1 || k > (1 << 30))) // list positions are int32, with room for a block of them
     {
         return fail(BITSKNN_ERR_UNSUPPORTED_K, "Unsupported k value: %d", k);
     }

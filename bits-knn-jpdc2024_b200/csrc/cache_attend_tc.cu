@@ -943,8 +943,8 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 // the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
 //
 // What bounds it: per 256 rows x 64 positions the exponentials need 1024 clocks (16 per clock and SM), the
-// products about 1300 (128 x 64 x 16: some 45 clocks, 128 x 128 x 16: 73), the operands from shared memory
-// about 1300; a tile takes some 2260, because the steps of one tile depend on one another and a warp's
+// products about 1500 (the 8 + 4 of one query tile hold their threads for 516 + 234 clocks when it is alone in its
+// block), their operands and the converters' stores about 1300 of shared-memory time; a tile takes some 2260, because the steps of one tile depend on one another and a warp's
 // 64 weights alone take 1200 with the other warp of its scheduler doing the same.  3 requests of 1500 ... 8000
 // cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 390 us = 0.79 PFLOP/s, 0.48
 // of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two score

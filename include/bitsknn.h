@@ -434,8 +434,8 @@ int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_bat
  * over the positions j the token sees; zeros (and lse = -inf) if there are none.
  *   d_out   [tokens][query_heads][dim] of `dtype`, out_stride elements between tokens (0 = dense)
  *   d_lse   optional float32[tokens][query_heads]: ln sum_j p_j (joins results over shards)
- * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the batch; its
- * contents on entry do not matter.  Calls that can overlap need workspaces of their own. */
+ * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the
+ * batch; its contents on entry do not matter.  Calls that can overlap need workspaces of their own. */
 size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* cache, int query_heads);
 int bitsknn_cache_attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries,
                          int dtype, int64_t query_stride, int query_heads, float scale, void* d_out,
@@ -445,7 +445,7 @@ int bitsknn_cache_attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch
 /* The same sums over listed positions only: d_idx[token * heads + h][0 ... k), int32 with ld_idx
  * entries between rows, as bitsknn_select writes them (any order).  Entries that the token does
  * not see -- negative, behind its last position, padding, on an absent page -- are skipped; an
- * entry that is listed twice counts twice.  k >= 1. */
+ * entry that is listed twice counts twice.  1 <= k <= 2^30. */
 int bitsknn_cache_attend_selected(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch,
                                   const void* d_queries, int dtype, int64_t query_stride, int query_heads,
                                   const int32_t* d_idx, int64_t ld_idx, int k, float scale, void* d_out,

@@ -753,3 +753,86 @@ def test_attend_sharp_rows_move_the_reference(bk, cuda):
     check(got_lse, lse, lse_tol, "lse")
     one = bk.cache_attend(p.cache, p.d_queries[-1:], p.d_lengths, p.d_table, 0.02)[0]
     check(one, want[-1:], tol[-1:], "decode")
+
+
+def test_many_columns_beyond_the_table_are_cut(bk, cuda):
+    p = Plain(bk, [200], [70], 1, 4, 64, 32, torch.float16, seed=41)
+    p.table = np.ascontiguousarray(p.table[:, :5])                  # 160 positions
+    p.upload()
+    want, lse, tol, lse_tol = p.plain_attend(0.1)
+    out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    check(out, want, tol, "out")
+    check(got_lse, lse, lse_tol, "lse")
+
+
+def test_rows_behind_the_last_request_are_left_alone(bk, cuda):
+    """Padded batches: packed arrays longer than the requests' tokens, in every kernel that writes rows."""
+    for lengths, news, group in (([60, 40], [3, 2], 4), ([90, 300], [40, 60], 4)):
+        p = Plain(bk, lengths, news, 2, group, 64, 16, torch.bfloat16, seed=42).upload()
+        tokens, pad = p.tokens, 7
+        lists = np.stack([np.random.default_rng(i).permutation(max(lengths))[:20] for i in range(tokens * 2)]).astype(np.int32)
+        queries = torch.cat([p.d_queries, torch.full((pad, 2 * group, 64), math.nan, dtype=torch.bfloat16, device="cuda")])
+        wide_lists = torch.cat([torch.from_numpy(lists).cuda(), torch.zeros((pad * 2, 20), dtype=torch.int32, device="cuda")])
+        for which in ("all", "list"):
+            out = torch.full(queries.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+            lse = torch.full(queries.shape[:2], 7.0, device="cuda")
+            args = (p.d_lengths, p.d_table, 0.1)
+            if which == "all":
+                bk.cache_attend(p.cache, queries, *args, starts=p.d_starts, out=out, lse=lse)
+                want, want_lse, tol, lse_tol = p.plain_attend(0.1)
+            else:
+                bk.cache_attend_selected(p.cache, queries, wide_lists, *args, starts=p.d_starts, out=out, lse=lse)
+                want, want_lse, tol, lse_tol = p.plain_attend(0.1, lists)
+            check(out[:tokens], want, tol, which)
+            check(lse[:tokens], want_lse, lse_tol, which)
+            assert bool((out[tokens:] == 7).all()) and bool((lse[tokens:] == 7).all())
+
+
+def test_offsets_beyond_32_bits(bk, cuda):
+    """Pages 2^31 codes apart: the last one begins behind 2^32 bytes."""
+    heads, rows, dim, group = 1, 64, 64, 4
+    stride = (1 << 31) + 64
+    flat = {w: torch.empty(2 * stride + heads * rows * dim, dtype=torch.uint8, device="cuda") for w in "kv"}
+    shape = (3, heads, rows, dim)
+    views = {w: flat[w].as_strided(shape, (stride, rows * dim, dim, 1)) for w in "kv"}
+    scales = {w: torch.ones((3, heads), device="cuda") for w in "kv"}
+    cache = bk.Cache(views["k"], views["v"], scales["k"], scales["v"])
+    order, count = [2, 0, 1], 170
+    table = torch.tensor([order], dtype=torch.int32, device="cuda")
+    rng = np.random.default_rng(51)
+    kv = {w: torch.from_numpy(rng.standard_normal((count, heads, dim))).to(torch.float32).cuda() for w in "kv"}
+    slots = torch.tensor([order[i // rows] * rows + i % rows for i in range(count)], dtype=torch.int64, device="cuda")
+    bk.cache_append(cache, kv["k"], kv["v"], slots)
+    # the same requests in a small cache
+    small = bk.Cache.empty(3, heads, rows, dim)
+    bk.cache_append(small, kv["k"], kv["v"], slots)
+    for i in range(3):
+        used = min(rows, count - order.index(i) * rows)
+        for w, t in (("k", small.keys), ("v", small.values)):
+            assert torch.equal(views[w][i, :, :used], t[i, :, :used])
+    lengths = torch.tensor([count], dtype=torch.int32, device="cuda")
+    for tokens in (1, 3, 90):
+        q = torch.from_numpy(rng.standard_normal((tokens, group, dim))).to(torch.bfloat16).cuda()
+        starts = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+        lists = torch.from_numpy(np.stack([rng.permutation(count) for _ in range(tokens)]).astype(np.int32)).cuda()
+        for f in (lambda c: bk.cache_attend(c, q, lengths, table, 0.1, starts=starts),
+                  lambda c: bk.cache_attend_selected(c, q, lists, lengths, table, 0.1, starts=starts),
+                  lambda c: (bk.cache_distance(c, q, lengths, table, count, starts=starts),)):
+            for x, y in zip(f(cache), f(small)):
+                assert torch.equal(x, y)
+
+
+def test_calls_on_two_streams_with_workspaces_of_their_own(bk, cuda):
+    p = Plain(bk, [3000, 500], [1, 1], 2, 4, 128, 16, torch.bfloat16, seed=61).upload()
+    many = Plain(bk, [400], [90], 2, 4, 128, 16, torch.bfloat16, seed=62).upload()
+    want = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1)[0]
+    want_many = bk.cache_attend(many.cache, many.d_queries, many.d_lengths, many.d_table, 0.1, starts=many.d_starts)[0]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for _ in range(20):
+        for side, q, w in ((sides[0], p, want), (sides[1], many, want_many)):
+            with torch.cuda.stream(side):
+                results.append((bk.cache_attend(q.cache, q.d_queries, q.d_lengths, q.d_table, 0.1, starts=q.d_starts)[0], w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in results)

@@ -94,6 +94,7 @@ def test_selected_lists_that_are_refused(bk):
 
     assert call(k=0) == bk.ERR_UNSUPPORTED_K
     assert "Unsupported k value: 0" in bk.last_error()
+    assert call(k=(1 << 30) + 1, ld=1 << 31) == bk.ERR_UNSUPPORTED_K
     assert call(ld=7) == bk.ERR_INVALID_ARGUMENT
     assert call(idx=None) == bk.ERR_INVALID_ARGUMENT
     assert call(idx=FAKE + 2) == bk.ERR_INVALID_ARGUMENT
