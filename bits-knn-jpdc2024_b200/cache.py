@@ -35,7 +35,11 @@ def _token_stride(name, shape, stride):
     tokens, heads, dim = shape
     if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{name} must be contiguous in its last two dimensions")
-    return stride[0] if tokens > 1 else heads * dim
+    if tokens < 2:
+        return heads * dim
+    if stride[0] < heads * dim:  # 0 (an expanded tensor) would mean dense to the library
+        raise ValueError(f"the tokens of {name} must not overlap")
+    return stride[0]
 
 
 def _dense(t, dtype, name):
@@ -55,6 +59,9 @@ class Cache:
         pages, heads, rows, dim = keys.shape
         if keys.stride()[1:] != (rows * dim, dim, 1):
             raise ValueError("a page must be contiguous")
+        stride = keys.stride(0) if pages > 1 else heads * rows * dim
+        if stride < heads * rows * dim:
+            raise ValueError("pages must not overlap")
         for t, name in ((key_scales, "key_scales"), (value_scales, "value_scales")):
             _dense(t, float32, name)
             if t.shape != (pages, heads):
@@ -65,7 +72,6 @@ class Cache:
         self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
         self.pages, self.heads, self.page_rows, self.dim = pages, heads, rows, dim
         self.device = keys.device
-        stride = keys.stride(0) if pages > 1 else heads * rows * dim
         self.struct = CacheStruct(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
                                   pages, stride, heads, rows, dim)
 

@@ -151,3 +151,19 @@ def test_python_layer_refuses_tensors_that_do_not_fit(bk):
         bk.Cache(codes, codes, torch.zeros(2, 1), torch.zeros(2, 1))
     with pytest.raises(ValueError, match="CUDA tensor"):
         bk.cache_plan(torch.zeros(1, dtype=torch.int32), None, None, None, 16, 1)
+
+
+def test_python_layer_refuses_rows_that_overlap(bk):
+    """An expanded tensor has stride 0, which the library would take for dense rows."""
+    import torch
+    from importlib import import_module
+    token_stride = import_module(bk.__name__ + ".cache")._token_stride
+    wide = torch.zeros((5, 4, 32))
+    assert token_stride("out", wide.shape, wide.stride()) == 128
+    assert token_stride("out", (1, 4, 32), (0, 32, 1)) == 128
+    for x in (wide[:1].expand(5, 4, 32), wide.as_strided((5, 4, 32), (64, 32, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            token_stride("out", x.shape, x.stride())
+    codes = torch.zeros((1, 1, 16, 32), dtype=torch.uint8).expand(3, 1, 16, 32)
+    with pytest.raises(ValueError, match="overlap"):
+        bk.Cache(codes, codes, torch.zeros(3, 1), torch.zeros(3, 1))
