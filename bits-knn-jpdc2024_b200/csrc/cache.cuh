@@ -26,6 +26,7 @@ constexpr int SUB = 16;              // cached rows a warp handles at a time
 constexpr int TILE = WARPS * SUB;    // cached rows a block handles at a time
 constexpr int E_MIN = -60;           // exponents of the scales the append kernel writes
 constexpr int E_MAX = 60;
+constexpr int MOST_ROWS = 1 << 30;   // requests, tokens: their numbers plus a block of them stay below 2^31
 
 // Devices on which a kernel's attributes have been set (they hold for the life of the context; a
 // device beyond the 64th is set up at every call).
@@ -216,8 +217,8 @@ __device__ __forceinline__ float cluster_load(const float* mine, int rank)
 }
 
 // ---- warp matrix steps -------------------------------------------------------------------------
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1)
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"

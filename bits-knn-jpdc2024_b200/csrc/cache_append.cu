@@ -402,7 +402,7 @@ extern "C" int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_
     {
         return fail(BITSKNN_ERR_UNSUPPORTED_MODE, "dtype %d: only F32, F16 and BF16", dtype);
     }
-    if (tokens < 0 || tokens > 0x7ffffffe)
+    if (tokens < 0 || tokens > cache::MOST_ROWS)
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "invalid token count %lld", static_cast<long long>(tokens));
     }

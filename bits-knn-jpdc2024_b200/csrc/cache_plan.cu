@@ -36,8 +36,10 @@ int check_cache(const bitsknn_cache_t* cache, cache::view* out)
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "page_stride=%lld: at least %lld codes and a multiple of 16",
                     static_cast<long long>(stride), static_cast<long long>(dense));
     }
-    if (((reinterpret_cast<uintptr_t>(cache->d_keys) | reinterpret_cast<uintptr_t>(cache->d_values)) & 15) != 0 ||
-        ((reinterpret_cast<uintptr_t>(cache->d_key_scales) | reinterpret_cast<uintptr_t>(cache->d_value_scales)) & 3) != 0)
+    const auto codes = reinterpret_cast<uintptr_t>(cache->d_keys) | reinterpret_cast<uintptr_t>(cache->d_values);
+    const auto scales =
+        reinterpret_cast<uintptr_t>(cache->d_key_scales) | reinterpret_cast<uintptr_t>(cache->d_value_scales);
+    if ((codes & 15) != 0 || (scales & 3) != 0)
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "misaligned cache: codes need 16-byte, scales 4-byte alignment");
     }
@@ -62,7 +64,8 @@ int check_cache_batch(const bitsknn_cache_batch_t* in, int page_rows, cache::bat
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "null pointer argument");
     }
-    if (in->requests < 0 || in->tokens < 0 || in->requests > 0x7ffffffe || in->tokens > 0x7ffffffe)
+    if (in->requests < 0 || in->tokens < 0 || in->requests > cache::MOST_ROWS ||
+        in->tokens > cache::MOST_ROWS)
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "invalid batch sizes requests=%lld tokens=%lld",
                     static_cast<long long>(in->requests), static_cast<long long>(in->tokens));
@@ -78,7 +81,8 @@ int check_cache_batch(const bitsknn_cache_batch_t* in, int page_rows, cache::bat
     }
     if (in->d_starts == nullptr && in->tokens != in->requests)
     {
-        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "without d_starts every request has one token (tokens=%lld requests=%lld)",
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT,
+                    "without d_starts every request has one token (tokens=%lld requests=%lld)",
                     static_cast<long long>(in->tokens), static_cast<long long>(in->requests));
     }
     out->table = in->d_table;
@@ -100,8 +104,8 @@ int check_cache_queries(const void* d_queries, int dtype, int64_t* query_stride,
     }
     if (query_heads < heads || query_heads % heads != 0 || query_heads / heads > 65535)
     {
-        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "query_heads=%d is not a multiple of the cache's %d heads", query_heads,
-                    heads);
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "query_heads=%d is not a multiple of the cache's %d heads",
+                    query_heads, heads);
     }
     const int64_t dense = static_cast<int64_t>(query_heads) * dim;
     if (*query_stride == 0)
@@ -149,6 +153,13 @@ struct plan_args
     int32_t* counts;
 };
 
+// Pages of `rows` positions.  Unsigned: a length and its new tokens together may pass 2^31.
+__device__ __forceinline__ int pages_of(int length, int added, int page_shift)
+{
+    const unsigned mask = (1U << page_shift) - 1;
+    return static_cast<int>((static_cast<unsigned>(length) + static_cast<unsigned>(added) + mask) >> page_shift);
+}
+
 // Inclusive sums of a pair over the block; `totals` gets the block's sums.
 __device__ __forceinline__ int2 block_scan(int2 v, int2* warp_sums, int2* totals)
 {
@@ -190,7 +201,8 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* warp_sums, int2* totals
 // block, then fills its share of the slots: tiles of 512 tokens dealt round robin, each token
 // finding its request by bisection in shared memory.  A token at row 0 of a page is the one that
 // enters the page into the table, so no block reads what another one writes.  Bound by latency:
-// one launch, about four dependent memory round trips (24 requests 3.8 us, 4096 requests with 302 K tokens 9.6 us).
+// one launch, about four dependent memory round trips (24 requests 3.8 us, 4096 requests with
+// 302 K tokens 9.6 us).
 __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_args a)
 {
     __shared__ int s_start[PLAN_CHUNK];  // first token
@@ -214,7 +226,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
             len[i] = j < count ? max(a.lengths[base + j], 0) : 0;
             add[i] = j < count ? max(a.added[base + j], 0) : 0;
             sum.x += add[i];
-            sum.y += ((len[i] + add[i] + rows - 1) >> a.page_shift) - ((len[i] + rows - 1) >> a.page_shift);
+            sum.y += pages_of(len[i], add[i], a.page_shift) - pages_of(len[i], 0, a.page_shift);
         }
         int2 total;
         const int2 upto = block_scan(sum, s_sums, &total);
@@ -223,8 +235,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
         for (int i = 0; i < PLAN_PER; ++i)
         {
             const int j = t * PLAN_PER + i;
-            const int have = (len[i] + rows - 1) >> a.page_shift;
-            const int need = (len[i] + add[i] + rows - 1) >> a.page_shift;
+            const int have = pages_of(len[i], 0, a.page_shift);
+            const int need = pages_of(len[i], add[i], a.page_shift);
+            const int64_t asked = static_cast<int64_t>(len[i]) + add[i];
             if (j < count)
             {
                 s_start[j] = at.x;
@@ -233,12 +246,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
                 if (blockIdx.x == 0)
                 {
                     a.starts[base + j] = at.x;
-                    a.new_lengths[base + j] = len[i] + add[i];
+                    a.new_lengths[base + j] = static_cast<int>(min(asked, static_cast<int64_t>(0x7fffffff)));
                     // rows there is room for: pages held, plus those the free list still has, cut by the table
                     const int64_t left = max(static_cast<int64_t>(0), a.free_count - at.y);
                     const int64_t pages = min(have + min(static_cast<int64_t>(need - have), left), a.table_pages);
                     const int64_t room = max(pages << a.page_shift, static_cast<int64_t>(len[i]));
-                    short_of += static_cast<int>(max(static_cast<int64_t>(0), len[i] + add[i] - room));
+                    short_of += static_cast<int>(max(static_cast<int64_t>(0), asked - room));
                 }
             }
             at.x += add[i];
@@ -251,11 +264,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
         int tile = begin / PLAN_THREADS;
         tile += (static_cast<int>(blockIdx.x) - tile % static_cast<int>(gridDim.x) + static_cast<int>(gridDim.x)) %
                 static_cast<int>(gridDim.x);
+        // sums beyond 2^31, which the caller must not ask for, wrap: nothing is placed then, see the bounds below
         for (int64_t token0 = static_cast<int64_t>(tile) * PLAN_THREADS; token0 < end;
              token0 += static_cast<int64_t>(gridDim.x) * PLAN_THREADS)
         {
             const int64_t token = token0 + t;
-            if (token < begin || token >= end)
+            if (token < begin || token >= end || token < 0)
             {
                 continue;
             }
@@ -274,9 +288,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
                 }
             }
             const int length = s_length[lo];
-            const int position = length + static_cast<int>(token - s_start[lo]);
-            const int column = position >> a.page_shift;
-            const int fresh = column - ((length + rows - 1) >> a.page_shift); // which of the new pages
+            const unsigned position = static_cast<unsigned>(length) + static_cast<unsigned>(token - s_start[lo]);
+            const int column = static_cast<int>(position >> a.page_shift);
+            const int fresh = column - pages_of(length, 0, a.page_shift); // which of the new pages
+            const int row = static_cast<int>(position) & (rows - 1);
             int page = -1;
             if (column < a.table_pages)
             {
@@ -288,8 +303,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
                 else
                 {
                     const int64_t f = static_cast<int64_t>(s_page[lo]) + fresh;
-                    page = f < a.free_count ? a.free_pages[f] : -1;
-                    if ((position & (rows - 1)) == 0)
+                    page = f >= 0 && f < a.free_count ? a.free_pages[f] : -1;
+                    if (row == 0)
                     {
                         *entry = page;
                     }
@@ -297,14 +312,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) cache_plan_kernel(const plan_arg
             }
             if (token < a.max_tokens)
             {
-                a.slots[token] = page < 0 ? -1 : (static_cast<int64_t>(page) << a.page_shift) + (position & (rows - 1));
+                a.slots[token] = page < 0 ? -1 : (static_cast<int64_t>(page) << a.page_shift) + row;
             }
         }
         carry.x += total.x;
         carry.y += total.y;
         __syncthreads();
     }
-    for (int64_t token = carry.x + blockIdx.x * static_cast<int64_t>(PLAN_THREADS) + t; token < a.max_tokens;
+    for (int64_t token = max(carry.x, 0) + blockIdx.x * static_cast<int64_t>(PLAN_THREADS) + t; token < a.max_tokens;
          token += static_cast<int64_t>(gridDim.x) * PLAN_THREADS)
     {
         a.slots[token] = -1;
@@ -333,7 +348,7 @@ extern "C" int bitsknn_cache_plan(const int32_t* d_lengths, const int32_t* d_new
                                   int64_t max_tokens, int32_t* d_counts, bitsknn_stream_t stream)
 {
     using namespace bitsknn;
-    if (requests < 0 || requests > 0x7ffffffe || free_count < 0 || max_tokens < 0)
+    if (requests < 0 || requests > cache::MOST_ROWS || free_count < 0 || max_tokens < 0)
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "invalid plan sizes requests=%lld free_count=%lld max_tokens=%lld",
                     static_cast<long long>(requests), static_cast<long long>(free_count),

@@ -350,7 +350,8 @@ int bitsknn_sharded_drain(bitsknn_sharded_t* handle, bitsknn_stream_t stream);
  * packed token arrays (d_starts == NULL: one token per request, `tokens` == `requests`).
  * d_lengths[r] counts its cached positions INCLUDING those tokens, so token i of m sees the
  * positions below d_lengths[r] - m + i + 1.  Rows of outputs behind the last request's tokens are
- * left as they were.  Lengths beyond the table's table_pages * page_rows are cut there.
+ * left as they were.  Lengths beyond the table's table_pages * page_rows are cut there.  At most 2^30
+ * requests and 2^30 tokens.
  *
  * Query vectors: BITSKNN_F16 or BITSKNN_BF16, [tokens][query_heads][dim] with `query_stride`
  * elements between tokens (0 = query_heads * dim); query head j belongs to cache head
@@ -392,7 +393,8 @@ typedef struct bitsknn_cache_batch
  * ceil(d_lengths[r] / page_rows) it has are taken from the front of d_free_pages in request order.
  *   d_table        int32[requests][table_ld]: entries of the new pages are written, others kept
  *   d_starts       int32[requests + 1] out: sums of d_new (the batch's d_starts)
- *   d_new_lengths  int32[requests] out: d_lengths + d_new (the batch's d_lengths); not d_lengths itself
+ *   d_new_lengths  int32[requests] out: d_lengths + d_new (the batch's d_lengths), at most 2^31 - 1;
+ *                  not d_lengths itself
  *   d_slots        int64[max_tokens] out: page * page_rows + row of every new token, -1 behind the
  *                  last one and for a token that got no place (free list or table row exhausted,
  *                  or its page is absent from the table).  More than max_tokens tokens: the first
@@ -413,8 +415,9 @@ int bitsknn_cache_plan(const int32_t* d_lengths, const int32_t* d_new, int64_t r
  * the new rows (a page that is begun).  When it grows, the rows in front of the new ones are
  * re-rounded to it.  Rounding is to nearest, ties to even; what lies beyond 448 * 2^60 (and the
  * infinities) saturates; NaN is kept.
- * The tokens of one page must follow one another in d_slots (skipped slots may lie between).  Slots that do not ascend inside a page
- * act like appends one after the other.  Calls that write the same page must not overlap. */
+ * The tokens of one page must follow one another in d_slots (skipped slots may lie between).  Slots
+ * that do not ascend inside a page act like appends one after the other.  Calls that write the same
+ * page must not overlap. */
 int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_new_keys, const void* d_new_values, int dtype,
                          int64_t key_stride, int64_t value_stride, const int64_t* d_slots, int64_t tokens,
                          bitsknn_stream_t stream);
@@ -434,6 +437,7 @@ int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_bat
  * over the positions j the token sees; zeros (and lse = -inf) if there are none.
  *   d_out   [tokens][query_heads][dim] of `dtype`, out_stride elements between tokens (0 = dense)
  *   d_lse   optional float32[tokens][query_heads]: ln sum_j p_j (joins results over shards)
+ * Neither may overlap what the call reads.
  * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the
  * batch; its contents on entry do not matter.  Calls that can overlap need workspaces of their own. */
 size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* cache, int query_heads);

@@ -836,3 +836,20 @@ def test_calls_on_two_streams_with_workspaces_of_their_own(bk, cuda):
                 results.append((bk.cache_attend(q.cache, q.d_queries, q.d_lengths, q.d_table, 0.1, starts=q.d_starts)[0], w))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in results)
+
+
+def test_plan_of_lengths_near_the_end_of_int32(bk, cuda):
+    """Positions that pass 2^31 have no page in any table: their tokens get no place, and nothing is read for them."""
+    top = (1 << 31) - 1
+    lengths, new = [top, top - 5, 30], [1, 40, 5]
+    table = torch.full((3, 4), -7, dtype=torch.int32, device="cuda")
+    table[2, :2] = torch.tensor([8, 9], dtype=torch.int32)
+    i32 = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, new, [3, 4, 5, 6, 7])]
+    starts, after, slots, counts = bk.cache_plan(i32[0], i32[1], i32[2], table, 16, 50)
+    assert starts.tolist() == [0, 1, 41, 46]
+    assert after.tolist() == [top, top, 35]
+    # 2^31 - 1 positions fill 2^27 pages but for one row; 2^31 - 6 all but six: 34 more tokens ask for 3 pages
+    want = [-1] * 41 + [9 * 16 + 14, 9 * 16 + 15, 6 * 16, 6 * 16 + 1, 6 * 16 + 2] + [-1] * 4
+    assert slots.tolist() == want
+    assert table.tolist() == [[-7] * 4, [-7] * 4, [8, 9, 6, -7]]
+    assert counts.tolist() == [46, 4, 41]

@@ -167,3 +167,15 @@ def test_python_layer_refuses_rows_that_overlap(bk):
     codes = torch.zeros((1, 1, 16, 32), dtype=torch.uint8).expand(3, 1, 16, 32)
     with pytest.raises(ValueError, match="overlap"):
         bk.Cache(codes, codes, torch.zeros(3, 1), torch.zeros(3, 1))
+
+
+def test_more_rows_than_are_numbered_are_refused(bk):
+    most = 1 << 30
+    assert attend(bk, batch=batch_struct(bk, tokens=most + 1, d_starts=FAKE)) == bk.ERR_INVALID_ARGUMENT
+    assert attend(bk, batch=batch_struct(bk, tokens=most + 1, requests=most + 1)) == bk.ERR_INVALID_ARGUMENT
+    assert bk.lib().bitsknn_cache_append(cache_struct(bk), FAKE, FAKE, bk.F16, 0, 0, FAKE, most + 1,
+                                         None) == bk.ERR_INVALID_ARGUMENT
+    assert "token count" in bk.last_error()
+    p = [ctypes.c_void_p(FAKE * (i + 1)) for i in range(8)]
+    assert bk.lib().bitsknn_cache_plan(p[0], p[1], most + 1, 16, p[2], 5, p[3], 4, 4, p[4], p[5], p[6], 8, p[7],
+                                       None) == bk.ERR_INVALID_ARGUMENT
