@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
 {
     constexpr int HELD = DTYPE == BITSKNN_F32 ? 4 : 8; // vectors of 8 numbers a thread keeps between the passes
     __shared__ float s_top[APPEND_THREADS / 32];
+    __shared__ int s_first[APPEND_THREADS / 32];
     const int t = threadIdx.x;
     const int lane = t & 31;
     const int head = blockIdx.y;
@@ -196,6 +197,40 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
             }
         }
         return limit;
+    };
+    // the same up to the last token.  The padding of a batch may lie there, so the whole block looks
+    // when nothing is near, 512 slots at a time.
+    auto find_far = [&](int from) {
+        const int close = min(from + 128, a.tokens);
+        int first = find(from, close, -1);
+        for (from = close; first == close && from < a.tokens; from += 4 * APPEND_THREADS)
+        {
+            first = a.tokens;
+#pragma unroll
+            for (int x = 3; x >= 0; --x)
+            {
+                const int j = from + x * APPEND_THREADS + t;
+                first = page_of(j < a.tokens ? a.slots[j] : -1) >= 0 ? j : first;
+            }
+            first = __reduce_min_sync(FULL_MASK, first);
+            if (lane == 0)
+            {
+                s_first[t >> 5] = first;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < APPEND_THREADS / 32; ++w)
+            {
+                first = min(first, s_first[w]);
+            }
+            __syncthreads();
+            if (first < a.tokens)
+            {
+                return first;
+            }
+            first = close; // go on
+        }
+        return first == close ? a.tokens : first;
     };
     int i = find(first_token, end_token, -1);
     if (i < end_token && first_token > 0)
@@ -304,7 +339,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         }
         // a page that is begun forgets the scale of its former owner; one that is continued keeps
         // at least its own (anything but a positive number in range counts as the smallest)
-        const float old = stored > 0.0F && stored <= cache::pow2_int(cache::E_MAX) ? stored : cache::pow2_int(cache::E_MIN);
+        const float old =
+            stored > 0.0F && stored <= cache::pow2_int(cache::E_MAX) ? stored : cache::pow2_int(cache::E_MIN);
         const float scale = fmaxf(scale_of(top), old);
         const float inverse = 1.0F / scale;
         uint8_t* const to = codes + base + at_vec;
@@ -373,7 +409,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         if (i >= end_token)
         {
             // the page may go on behind the window, with rows that do not ascend
-            i = find(i, a.tokens, -1);
+            i = find_far(i);
             if (i == a.tokens || page_of(a.slots[i]) != page)
             {
                 return;
@@ -412,7 +448,8 @@ extern "C" int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_
     const int64_t unit = dtype == BITSKNN_F32 ? 4 : 8; // elements in 16 bytes
     if (key_stride < dense || value_stride < dense || key_stride % unit != 0 || value_stride % unit != 0)
     {
-        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "strides %lld and %lld between tokens: at least %lld and a multiple of %lld",
+        return fail(BITSKNN_ERR_INVALID_ARGUMENT,
+                    "strides %lld and %lld between tokens: at least %lld and a multiple of %lld",
                     static_cast<long long>(key_stride), static_cast<long long>(value_stride),
                     static_cast<long long>(dense), static_cast<long long>(unit));
     }

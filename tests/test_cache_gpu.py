@@ -853,3 +853,31 @@ def test_plan_of_lengths_near_the_end_of_int32(bk, cuda):
     assert slots.tolist() == want
     assert table.tolist() == [[-7] * 4, [-7] * 4, [8, 9, 6, -7]]
     assert counts.tolist() == [46, 4, 41]
+
+
+def test_append_of_a_batch_with_long_padding(bk, cuda):
+    """A page whose tokens lie thousands of skipped slots apart, and padding behind the last one."""
+    heads, rows, dim = 2, 16, 64
+    rng = np.random.default_rng(71)
+    order = [(0, 5), (300, 6), (2900, 3), (3100, 9), (9000, 40)]      # token, slot: page 0 four times, then page 2
+    tokens = 12000
+    slots = torch.full((tokens,), -1, dtype=torch.int64)
+    for token, slot in order:
+        slots[token] = slot
+    slots = slots.cuda()
+    new = [torch.from_numpy(rng.standard_normal((tokens, heads, dim))).to(torch.bfloat16) for _ in range(2)]
+    for x in new:
+        x[2900] *= 50                                                   # the page's scale grows
+    new = [x.cuda() for x in new]
+    got, want = (bk.Cache.empty(3, heads, rows, dim) for _ in range(2))
+    bk.cache_append(got, *new, slots)
+    for token, _ in order:                                              # 5, 6 ascend but act alike one by one
+        one = slice(token, token + 1)
+        bk.cache_append(want, new[0][one], new[1][one], slots[one])
+    assert int((want.key_scales > 0).sum()) == 4
+    for name in ("key_scales", "value_scales"):
+        assert torch.equal(getattr(got, name), getattr(want, name))
+    for name in ("keys", "values"):
+        a, b = (getattr(c, name)[0, :, [3, 9]] for c in (got, want))
+        assert torch.equal(a, b)
+        assert torch.equal(getattr(got, name)[2], getattr(want, name)[2])
