@@ -327,11 +327,13 @@ struct tc_state
     uint64_t* p_full;   // [query tile][score tile]
     uint64_t* o_done;   // [query tile][score tile]
     uint64_t* q_full;   // [query tile]
+    uint64_t* row_done; // [query tile]: the item's rows are written
 };
 
 // ================= softmax: one thread per query row =================
 template <int DIM>
-__device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem)
+__device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w,
+                                             uint32_t tmem)
 {
     using shape = tc_shape<DIM>;
     const int t = threadIdx.x;
@@ -575,6 +577,10 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                     l == 0.0F ? -INFINITY : (m - WEIGHT_BIAS + log2f(l)) * LN_2;
             }
             tc::fence_before_sync();
+            if (count > 0)
+            {
+                warp_arrive(&st.row_done[my_tile]);
+            }
         }
         kv_tiles += count;
         items += count > 0 ? 1 : 0;
@@ -789,6 +795,15 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         }
         ++items;
     } while (w.next(a));
+    // the commits of the last tiles arrive before the block gives its shared memory back
+    for (uint32_t i = n < shape::STAGES ? 0 : n - shape::STAGES; i < n; ++i)
+    {
+        const uint32_t phase = (i / shape::STAGES) & 1U;
+        if (!warp_wait(&st.k_empty[i % shape::STAGES], phase) || !warp_wait(&st.v_empty[i % shape::STAGES], phase))
+        {
+            return false;
+        }
+    }
     return true;
 }
 
@@ -797,8 +812,8 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
 // arithmetic -- adds up to as much again; so the scores and the sums of either query tile have a thread of
 // their own, which only meet at barriers.
 template <int DIM>
-__device__ __forceinline__ bool scores_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem,
-                                            int my_tile)
+__device__ __forceinline__ bool scores_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w,
+                                            uint32_t tmem, int my_tile)
 {
     using shape = tc_shape<DIM>;
     constexpr uint32_t idesc = tc::instr_desc(0U, 128U, shape::ROWS);
@@ -866,8 +881,8 @@ __device__ __forceinline__ bool scores_role(const attend_args& a, const tc_state
 }
 
 template <int DIM>
-__device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, uint32_t tmem,
-                                          int my_tile)
+__device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w,
+                                          uint32_t tmem, int my_tile)
 {
     using shape = tc_shape<DIM>;
     constexpr uint32_t idesc = tc::instr_desc(0U, 128U, DIM) | (1U << 16); // second operand along its outputs
@@ -878,10 +893,19 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
     uint32_t stage = 0;
     uint32_t phase = 0;
     uint32_t s = 0; // products of this query tile so far
+    uint32_t written = 0; // items of this query tile whose rows have to be written
     do
     {
         const int count = w.count();
         const bool active = my_tile < w.query_tiles();
+        // Items without rows here could go by while the softmax still reads the first NaN of the last one that
+        // had some, and take its slot.
+        if (!active && count > 0 && written > 0 &&
+            !ptx::mbar_wait_bounded_spin(&st.row_done[my_tile], (written - 1) & 1U))
+        {
+            return false;
+        }
+        written += active && count > 0 ? 1 : 0;
         for (int j = 0; j < count; ++j)
         {
             if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], phase))
@@ -935,7 +959,8 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 // tiles are converted while the last one is being written.
 //   Rings: the converters are at most STAGES tiles ahead of the scores, and scores need the product
 // before last, whose weights their softmax has written: a slot of RING >= STAGES + 2 is read before it is
-// written again.  The first-NaN slots go by items of at least one tile, so the same holds for them.
+// written again.  The first-NaN slots go by items of at least one tile, so the same holds for them while both
+// query tiles have rows; an item without rows for one of them waits until that one's last rows are written.
 //   Score tiles, weights and products have a barrier per score tile: a role may be a tile ahead of the one
 // that waits, and a wait by parity can tell a phase from the next one only while it is at most one phase
 // of the same barrier away.
@@ -943,10 +968,10 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 // the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
 //
 // What bounds it: per 256 rows x 64 positions the exponentials need 1024 clocks (16 per clock and SM), the
-// products about 1500 (the 8 + 4 of one query tile hold their threads for 516 + 234 clocks when it is alone in its
-// block), their operands and the converters' stores about 1300 of shared-memory time; a tile takes some 2260, because the steps of one tile depend on one another and a warp's
-// 64 weights alone take 1200 with the other warp of its scheduler doing the same.  3 requests of 1500 ... 8000
-// cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 390 us = 0.79 PFLOP/s, 0.48
+// products about 1500 (the 8 + 4 of one query tile hold their threads for 516 + 234 clocks when it is alone in
+// its block), their operands and the converters' stores about 1300 of shared-memory time; a tile takes some
+// 2260, because the steps of one tile depend on one another and a warp's 64 weights alone take 1200 with the
+// other warp of its scheduler doing the same.  3 requests of 1500 ... 8000 cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 390 us = 0.79 PFLOP/s, 0.48
 // of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two score
 // tiles of 64 511; packed arithmetic and offsets per 16 rows 444; a thread for each kind of product 405.  Tried
 // and slower: two threads per row (520), other register splits (403 ... 417), rows packed by neighbouring
@@ -977,6 +1002,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
     st.p_full = st.k_full + 20;
     st.o_done = st.k_full + 24;
     st.q_full = st.k_full + 28;
+    st.row_done = st.k_full + 30;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (t == 0)
@@ -998,6 +1024,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
         for (int i = 0; i < 2; ++i)
         {
             ptx::mbar_init(&st.q_full[i], 4);
+            ptx::mbar_init(&st.row_done[i], 4);
         }
         ptx::mbar_init_fence();
     }
@@ -1061,7 +1088,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
             const int issuer = warp - 12; // 0, 1: scores of query tile 0, 1; 2, 3: sums
             if (lane == 0 && (issuer & 1) < shape::NQ)
             {
-                fine = issuer < 2 ? scores_role<DIM>(a, st, w, tmem, issuer & 1) : sums_role<DIM>(a, st, w, tmem, issuer & 1);
+                fine = issuer < 2 ? scores_role<DIM>(a, st, w, tmem, issuer & 1)
+                                  : sums_role<DIM>(a, st, w, tmem, issuer & 1);
             }
             else if (warp == TC_THREADS / 32 - 1 && lane == 1)
             {

@@ -881,3 +881,28 @@ def test_append_of_a_batch_with_long_padding(bk, cuda):
         a, b = (getattr(c, name)[0, :, [3, 9]] for c in (got, want))
         assert torch.equal(a, b)
         assert torch.equal(getattr(got, name)[2], getattr(want, name)[2])
+
+
+def test_items_with_few_rows_between_items_with_many(bk, cuda):
+    """Blocks that alternate between two query tiles and one, with NaN values that only later tokens see."""
+    news, lengths = [], []
+    for i in range(60):
+        news += [50, 9, 8, 10, 9, 11, 10, 9, 8, 9]
+        lengths += [60 + i % 7, 20, 9, 40, 70, 66, 12, 130, 30, 64]
+    p = Plain(bk, lengths, news, 1, 4, 64, 16, torch.float16, seed=81)
+    p.upload()
+    # the last position's value of every third request is NaN: its last token alone sees it
+    for r in range(0, len(lengths), 3):
+        last = lengths[r] - 1
+        p.cache.values[int(p.d_table[r, last // 16]), 0, last % 16, 5] = 0x7f
+    out, _ = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    token = 0
+    want = torch.zeros(out.shape, dtype=torch.bool)
+    for r, m in enumerate(news):
+        token += m
+        if r % 3 == 0:
+            want[token - 1, :, 5] = True
+    assert torch.equal(torch.isnan(out).cpu(), want)
+    for _ in range(20):
+        again, _ = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+        assert torch.equal(again.view(torch.int16), out.view(torch.int16))
