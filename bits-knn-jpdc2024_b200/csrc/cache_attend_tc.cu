@@ -29,7 +29,7 @@ struct tc_shape
     static constexpr int NQ = DIM <= 128 ? 2 : 1;
     static constexpr int COLS = 128 * NQ;
     static constexpr int ROWS = 64;
-    static constexpr int COST = 10;              // an item's beginning and end, in tiles (4: 402 us, 8: 391, 12: 389)
+    static constexpr int COST = 10;              // an item's beginning and end, in tiles (4: 375 us, 6: 370, 8: 367, 10: 365)
     static constexpr int BLK = (DIM + 63) / 64;  // 128-byte blocks of 64 halves per row
     static constexpr int Q_BYTES = BLK * 128 * 128;
     static constexpr int KV_BYTES = BLK * ROWS * 128;
@@ -112,6 +112,16 @@ __device__ __forceinline__ uint32_t tile_byte(int row, int chunk, int rows)
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
 }
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -337,6 +347,7 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
 {
     using shape = tc_shape<DIM>;
     const int t = threadIdx.x;
+    const int lane = t & 31;
     const int my_tile = t >> 7;
     const uint32_t lane_base = static_cast<uint32_t>(((t >> 5) & 3) * 32) << 16;
     const uint32_t s_base = tmem + lane_base + my_tile * 2 * shape::ROWS;
@@ -358,11 +369,16 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
             float factor = 0.0F;
             if (count > 0)
             {
-                // the products that read the query tile's rows before are done: o_done was waited for
+                // The products that read the query tile's rows before are done: o_done was waited for.  A warp
+                // packs its 32 rows together, G lanes to a row, so that its loads and stores are whole lines, and
+                // in short loops, because what runs once an item comes from beyond the instruction cache (8400
+                // clocks an item; a row to a thread 13500, all 16 steps unrolled 19000).
+                constexpr int CHUNKS = DIM / 8; // of 16 bytes in a row
+                constexpr int G = CHUNKS <= 4 ? 4 : CHUNKS <= 8 ? 8 : CHUNKS <= 16 ? 16 : 32;
+                constexpr int TOGETHER = 32 / G;  // rows of a load
                 const uint32_t to = ptx::smem_addr(st.q_tiles + my_tile * shape::Q_BYTES);
-                const uint4* const from = reinterpret_cast<const uint4*>(
-                    static_cast<const uint16_t*>(a.queries) +
-                    (real ? row_token * a.query_stride + static_cast<int64_t>(qhead) * DIM : 0));
+                const int chunk = lane % G;
+                const int64_t mine = real ? row_token * a.query_stride + static_cast<int64_t>(qhead) * DIM : -1;
                 auto floats = [&](uint32_t x) {
                     if (a.dtype == BITSKNN_BF16)
                     {
@@ -370,48 +386,97 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                     }
                     return __half22float2(*reinterpret_cast<const __half2*>(&x));
                 };
-                // both 16-bit types order like their bits once the sign is gone
-                uint32_t most = 0;
-#pragma unroll 8
-                for (int i = 0; i < DIM / 8; ++i)
-                {
-                    const uint4 v = real ? __ldg(from + i) : make_uint4(0U, 0U, 0U, 0U);
-                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffU, v.y & 0x7fff7fffU),
-                                                   __vmaxu2(v.z & 0x7fff7fffU, v.w & 0x7fff7fffU)));
-                }
-                most = max(most & 0xffffU, most >> 16);
+                // The same scaling as pack_column: a power of two that puts the largest entry into [2^14, 2^15).
+                auto shift_of = [&](uint32_t most) {
+                    const float top = floats(most).x;
+                    const int e = max(static_cast<int>(__float_as_uint(top) >> 23), 1) - 127;
+                    return top > 0.0F ? min(max(14 - e, -126), 126) : 0;
+                };
                 const uint32_t infinite = a.dtype == BITSKNN_BF16 ? 0x7f80U : 0x7c00U;
-                if (most >= infinite)
+                // all rows are asked for at once, as they are, and converted where they come to lie
+#pragma unroll 4
+                for (int b = 0; b < G; ++b)
                 {
-                    // infinities and NaN set no scale: the largest finite entry
-                    most = 0;
-                    for (int i = 0; i < DIM; ++i)
+                    const int64_t from = __shfl_sync(FULL_MASK, mine, b * TOGETHER + lane / G);
+                    if (chunk < CHUNKS)
                     {
-                        const uint32_t x = reinterpret_cast<const uint16_t*>(from)[i] & 0x7fffU;
-                        most = x < infinite ? max(most, x) : most;
+                        const int row = (t & 96) + b * TOGETHER + lane / G;
+                        copy16(to + tile_byte(row, chunk, 128),
+                               static_cast<const uint16_t*>(a.queries) + max(from, static_cast<int64_t>(0)) + chunk * 8,
+                               from >= 0 ? 16U : 0U);
                     }
                 }
-                const float top = floats(most).x;
-                // the same scaling as pack_column: a power of two that puts the largest entry into
-                // [2^14, 2^15); the sign of the scale goes with the query
-                const int e = max(static_cast<int>(__float_as_uint(top) >> 23), 1) - 127;
-                const int shift = top > 0.0F ? min(max(14 - e, -126), 126) : 0;
-                const float up = a.scale < 0.0F ? -pow2_int(shift) : pow2_int(shift);
-                factor = pow2_int(-shift) * fabsf(a.scale);
-#pragma unroll 8
-                for (int i = 0; i < DIM / 8; ++i)
+                copy_commit();
+                uint32_t row_most = 0; // of this thread's row
+                copy_wait<0>();
+                constexpr int BATCH = 4; // rows a lane has under way: the steps of one wait for each other
+#pragma unroll 1
+                for (int b = 0; b < G; b += BATCH)
                 {
-                    const uint4 v = real ? __ldg(from + i) : make_uint4(0U, 0U, 0U, 0U);
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                    uint32_t h[4];
+                    uint32_t x[BATCH][4];
+                    uint32_t most[BATCH];
+                    uint32_t at[BATCH];
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int i = 0; i < BATCH; ++i)
                     {
-                        const float2 f = floats(x[j]);
-                        h[j] = pack_half2(f.x * up, f.y * up);
+                        at[i] = to + tile_byte((t & 96) + (b + i) * TOGETHER + lane / G, chunk, 128);
+                        const uint4 v = chunk < CHUNKS ? ld_shared16(at[i]) : make_uint4(0U, 0U, 0U, 0U);
+                        x[i][0] = v.x;
+                        x[i][1] = v.y;
+                        x[i][2] = v.z;
+                        x[i][3] = v.w;
+                        // both 16-bit types order like their bits once the sign is gone
+                        const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffU, v.y & 0x7fff7fffU),
+                                                    __vmaxu2(v.z & 0x7fff7fffU, v.w & 0x7fff7fffU));
+                        most[i] = max(m & 0xffffU, m >> 16);
+                        top = max(top, most[i]);
                     }
-                    st_shared16(to + tile_byte(t & 127, i, 128), h[0], h[1], h[2], h[3]);
+                    if (__any_sync(FULL_MASK, top >= infinite))
+                    {
+                        // infinities and NaN set no scale: the largest finite entry
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i)
+                        {
+                            most[i] = 0;
+#pragma unroll
+                            for (int y = 0; y < 8; ++y)
+                            {
+                                const uint32_t one = x[i][y >> 1] >> (16 * (y & 1)) & 0x7fffU;
+                                most[i] = one < infinite ? max(most[i], one) : most[i];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int o = 1; o < G; o <<= 1)
+                    {
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i)
+                        {
+                            most[i] = max(most[i], __shfl_xor_sync(FULL_MASK, most[i], o));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i)
+                    {
+                        const uint32_t got = __shfl_sync(FULL_MASK, most[i], lane % TOGETHER * G);
+                        row_most = lane / TOGETHER == b + i ? got : row_most;
+                        // the sign of the scale goes with the query
+                        const float up = a.scale < 0.0F ? -pow2_int(shift_of(most[i])) : pow2_int(shift_of(most[i]));
+                        uint32_t h[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                        {
+                            const float2 f = floats(x[i][y]);
+                            h[y] = pack_half2(f.x * up, f.y * up);
+                        }
+                        if (chunk < CHUNKS)
+                        {
+                            st_shared16(at[i], h[0], h[1], h[2], h[3]);
+                        }
+                    }
                 }
+                factor = pow2_int(-shift_of(row_most)) * fabsf(a.scale);
                 fence_async_proxy();
                 warp_arrive(&st.q_full[my_tile]);
             }
@@ -501,11 +566,14 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
             const uint32_t seen_nan = see > cut_base ? nan_key(items, see - 1 - cut_base) : 0xffffffffU;
             const bool nan_here = count > 0 && first_nan[DIM] >= seen_nan;
             const float inverse = l == 0.0F ? 1.0F : 1.0F / l; // l = 0: nothing was seen; a NaN makes the row NaN
-            uint16_t* const out =
-                static_cast<uint16_t*>(a.out) + row_token * a.out_stride + static_cast<int64_t>(qhead) * DIM;
             const bool aligned =
                 ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * 2)) & 15) == 0;
-            float* const part_row = a.part_o + (part * shape::COLS + t) * DIM;
+            // Through shared memory, 32 numbers of each of the warp's rows at a time, so that its stores are
+            // whole lines too (6500 clocks an item; a row to a thread 9200).  The rows' queries have been read.
+            const uint32_t rows_at = ptx::smem_addr(st.q_tiles + my_tile * shape::Q_BYTES + (t & 96) * 128);
+            const int64_t mine = real ? row_token * a.out_stride + static_cast<int64_t>(qhead) * DIM : -1;
+            float* const part_rows = a.part_o + (part * shape::COLS + (t & ~31)) * DIM;
+            auto granule = [&](int row, int g) { return rows_at + row * 128 + ((g ^ (row & 7)) << 4); };
 #pragma unroll 1
             for (int c = 0; c < DIM; c += 32)
             {
@@ -516,52 +584,72 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                     tc::tmem_ld_32x32(o_addr + c, o);
                     tmem_ld_wait(o);
                 }
-                if (real)
+                if (l == 0.0F || nan_here)
                 {
-                    if (l == 0.0F || nan_here)
-                    {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
+                    for (int i = 0; i < 32; ++i)
+                    {
+                        o[i] = l != 0.0F ? (first_nan[c + i] >= seen_nan ? 0x7fc00000U : o[i]) : 0U;
+                    }
+                }
+                if (!whole)
+                {
+#pragma unroll
+                    for (int g = 0; g < 8; ++g)
+                    {
+                        st_shared16(granule(lane, g), o[g * 4], o[g * 4 + 1], o[g * 4 + 2], o[g * 4 + 3]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        const int row = i * 4 + (lane >> 3);
+                        const uint4 x = ld_shared16(granule(row, lane & 7));
+                        if (__shfl_sync(FULL_MASK, real ? 1 : 0, row) != 0)
                         {
-                            o[i] = l != 0.0F ? (first_nan[c + i] >= seen_nan ? 0x7fc00000U : o[i]) : 0U;
+                            *reinterpret_cast<uint4*>(part_rows + row * DIM + c + (lane & 7) * 4) = x;
                         }
                     }
-                    if (!whole)
+                    continue;
+                }
+                auto result = [&](uint32_t x) { return __uint_as_float(x) * inverse; };
+                auto pair = [&](uint32_t x, uint32_t y) {
+                    if (a.dtype == BITSKNN_BF16)
                     {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(result(x), result(y));
+                        return *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                    return pack_half2(result(x), result(y));
+                };
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                        {
-                            *reinterpret_cast<uint4*>(part_row + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        }
+                for (int g = 0; g < 4; ++g)
+                {
+                    st_shared16(granule(lane, g), pair(o[g * 8], o[g * 8 + 1]), pair(o[g * 8 + 2], o[g * 8 + 3]),
+                                pair(o[g * 8 + 4], o[g * 8 + 5]), pair(o[g * 8 + 6], o[g * 8 + 7]));
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const int row = i * 8 + (lane >> 2);
+                    const uint4 v = ld_shared16(granule(row, lane & 3));
+                    const int64_t to = __shfl_sync(FULL_MASK, mine, row);
+                    if (to < 0)
+                    {
+                        continue;
+                    }
+                    uint16_t* const out = static_cast<uint16_t*>(a.out) + to + c + (lane & 3) * 8;
+                    if (aligned)
+                    {
+                        *reinterpret_cast<uint4*>(out) = v;
                     }
                     else
                     {
-                        auto result = [&](uint32_t x) { return __uint_as_float(x) * inverse; };
-                        auto pair = [&](uint32_t x, uint32_t y) {
-                            if (a.dtype == BITSKNN_BF16)
-                            {
-                                const __nv_bfloat162 b = __floats2bfloat162_rn(result(x), result(y));
-                                return *reinterpret_cast<const uint32_t*>(&b);
-                            }
-                            return pack_half2(result(x), result(y));
-                        };
+                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
+                        for (int y = 0; y < 8; ++y)
                         {
-                            const uint32_t x[4] = {pair(o[i], o[i + 1]), pair(o[i + 2], o[i + 3]), pair(o[i + 4], o[i + 5]),
-                                                   pair(o[i + 6], o[i + 7])};
-                            if (aligned)
-                            {
-                                *reinterpret_cast<uint4*>(out + c + i) = make_uint4(x[0], x[1], x[2], x[3]);
-                            }
-                            else
-                            {
-#pragma unroll
-                                for (int y = 0; y < 8; ++y)
-                                {
-                                    out[c + i + y] = static_cast<uint16_t>(x[y >> 1] >> (16 * (y & 1)));
-                                }
-                            }
+                            out[y] = static_cast<uint16_t>(x[y >> 1] >> (16 * (y & 1)));
                         }
                     }
                 }
@@ -970,12 +1058,15 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 // What bounds it: per 256 rows x 64 positions the exponentials need 1024 clocks (16 per clock and SM), the
 // products about 1500 (the 8 + 4 of one query tile hold their threads for 516 + 234 clocks when it is alone in
 // its block), their operands and the converters' stores about 1300 of shared-memory time; a tile takes some
-// 2260, because the steps of one tile depend on one another and a warp's 64 weights alone take 1200 with the
-// other warp of its scheduler doing the same.  3 requests of 1500 ... 8000 cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 390 us = 0.79 PFLOP/s, 0.48
-// of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two score
-// tiles of 64 511; packed arithmetic and offsets per 16 rows 444; a thread for each kind of product 405.  Tried
-// and slower: two threads per row (520), other register splits (403 ... 417), rows packed by neighbouring
-// lanes (409), the weights' code shared by both paths in a loop (580: the scores then live on across it).
+// 2180, because the steps of one tile depend on one another and a warp's 64 weights alone take 1170 with the
+// other warp of its scheduler doing the same; an item's beginning and end take 17000.  3 requests of 1500 ...
+// 8000 cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 365 us = 0.85 PFLOP/s,
+// 0.51 of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two
+// score tiles of 64 511; packed arithmetic and offsets per 16 rows 444; a thread for each kind of product 405;
+// rows packed and written in whole lines 365.  Tried and slower: two threads per row (520), other register
+// splits (403 ... 417), the weights' code shared by both paths in a loop (580: the scores then live on across
+// it), one product of 128 positions for both score tiles of a query tile (502: the 516 clocks serve twice as
+// much, but the softmax then waits 900 of them every time).
 template <int DIM>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)
 {
