@@ -1,10 +1,11 @@
 """Paged cache of keys and values held in 8 bits: the access layer of the `bitsknn_cache_*` entry points.
 
 These calls run once per layer and decode step, where a microsecond on the host counts: every argument is looked at
-once, tensors' devices are compared as integers, and nothing is kept between calls.
+once, tensors' devices are compared as integers, sizes go to the allocation one by one (a torch.Size costs it
+another 1.5 us), and nothing is kept between calls.
 """
 import torch
-from torch import bfloat16, empty, float16, float32, int32, int64, uint8
+from torch import bfloat16, empty, empty_like, float16, float32, int32, int64, uint8
 
 from . import BF16, F16, F32, BatchStruct, BitsKnnError, CacheStruct, last_error, lib
 
@@ -23,7 +24,7 @@ def _current(index, *tensors):
     """The tensors must be CUDA tensors of the current device (`index`): the library has no CPU path and launches on
     the current device."""
     if index < 0 or index != _current_device():
-        raise ValueError(f"the tensors must be CUDA tensors of the current device (the library has no CPU path), "
+        raise ValueError("the tensors must be CUDA tensors of the current device (the library has no CPU path), "
                          f"not of device {index}")
     for t in tensors:
         if t.get_device() != index:
@@ -126,9 +127,8 @@ def cache_plan(lengths, new, free_pages, table, page_rows, max_tokens, out=None)
     if lengths.shape != (requests,) or new.shape != (requests,) or free_pages.dim() != 1:
         raise ValueError("lengths and new must be (requests,), table (requests, pages)")
     if out is None:
-        device = lengths.device
-        starts, new_lengths, counts = empty(2 * requests + 4, dtype=int32, device=device).split((requests + 1, requests, 3))
-        out = starts, new_lengths, empty(max_tokens, dtype=int64, device=device), counts
+        out = (lengths.new_empty(requests + 1), empty_like(lengths),
+               empty(max_tokens, dtype=int64, device=lengths.device), lengths.new_empty(3))
     else:
         for t, dtype, size, name in zip(out, (int32, int32, int64, int32), (requests + 1, requests, max_tokens, 3),
                                         ("starts", "new_lengths", "slots", "counts")):
@@ -164,7 +164,7 @@ def cache_distance(cache, queries, lengths, table, n, starts=None, out=None):
     batch = _batch(cache, queries, shape, lengths, table, starts)
     rows = shape[0] * cache.heads
     if out is None:
-        out = empty((rows, n), dtype=float32, device=cache.device)
+        out = empty(rows, n, dtype=float32, device=cache.device)
         ld = n
     else:
         _current(cache.index, out)
@@ -186,14 +186,14 @@ def _attend_buffers(cache, queries, shape, out, lse, workspace):
     """(out, elements between its tokens, lse, workspace)"""
     stride = 0
     if out is None:
-        out = empty(shape, dtype=queries.dtype, device=cache.device)
+        out = empty_like(queries) if queries.is_contiguous() else empty(*shape, dtype=queries.dtype, device=cache.device)
     else:
         _current(cache.index, out)
         if out.shape != shape or out.dtype is not queries.dtype:
             raise ValueError("out must have the queries' shape and type")
         stride = _token_stride("out", shape, out.stride())
     if lse is None:
-        lse = empty(shape[:2], dtype=float32, device=cache.device)
+        lse = empty(shape[0], shape[1], dtype=float32, device=cache.device)
     else:
         _current(cache.index, lse)
         _dense(lse, float32, "lse")

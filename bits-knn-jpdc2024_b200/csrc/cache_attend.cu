@@ -880,8 +880,8 @@ int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, con
     const int64_t want = a.group * per_request;
     auto s = static_cast<cudaStream_t>(stream);
     // More columns than one stream of the cache can serve: the tensor-memory kernel takes over (16 requests
-    // of 6000 positions, 8 heads of 128: 32 columns 109 us here and 133 there, 48 columns 166 and 134, 128
-    // columns 316 and 144; 256 numbers, 16 columns 72 and 99, 24 columns 105 and 101).
+    // of 6000 positions, 8 heads of 128: 32 columns 109 us here and 129 there, 48 columns 169 and 130, 128
+    // columns 324 and 134; heads of 256: 16 columns 113 and 165, 24 columns 187 and 167).
     if (!selected && want > 8 * most_columns(cache->dim))
     {
         return launch_attend_tc(cache->dim, a, d_workspace, workspace_bytes, s);
