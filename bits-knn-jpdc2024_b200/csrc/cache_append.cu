@@ -47,6 +47,15 @@ __device__ __forceinline__ raw8<DTYPE> load8(const void* src, int64_t at)
     return r;
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* src, int64_t at, int bytes)
+{
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(src) + at * bytes));
+}
+
+// Vectors of eight numbers a thread keeps between the two passes over a run.
+template <int DTYPE>
+constexpr int HELD = DTYPE == BITSKNN_F32 ? 4 : 8;
+
 template <int DTYPE>
 __device__ __forceinline__ void floats_of(const raw8<DTYPE>& r, float (&v)[8])
 {
@@ -136,24 +145,26 @@ __device__ __forceinline__ float scale_of(float amax)
     return cache::pow2_int(min(max(e, cache::E_MIN), cache::E_MAX)); // subnormal amax: far below the border
 }
 
-// One block = one window of tokens, one head, keys or values (gridDim = windows x heads x 2).  It
-// serves the pages whose first token lies in its window, run after run: a run is the longest
+// A team of threads (a warp or a block) = one window of tokens, one head, keys or values (gridDim = windows
+// x heads x 2).  It serves the pages whose first token lies in its window, run after run: a run is the longest
 // stretch of tokens of one page with ascending rows.  Two passes over a run: the largest finite
-// entry (block maximum), then rounding; what fits into HELD vectors per thread stays in
-// registers between them (64 rows of 128 halves, 32 of 128 floats), the rest is read again from L2.
-// A page has one scale per head, which is why a run belongs to one block and why a later token
+// entry (the team's maximum), then rounding; what fits into HELD vectors per thread stays in
+// registers between them (a block: 64 rows of 128 halves, 32 of 128 floats; a warp a quarter of that), the
+// rest is read again from L2.  Where pages are small the teams are warps: four runs are then under way where a
+// block has one.
+// A page has one scale per head, which is why a run belongs to one team and why a later token
 // that needs a larger scale re-rounds the rows in front of it: with powers of two that only
 // costs bits at the subnormal end, code * 2^(old - new) is exact for every other code.
 //
-// Bound by HBM (numbers in, codes out) for prompts: 27392 tokens x 8 heads x 128 halves, 169 MB, in 37 us
-// = 4.6 TB/s, 0.70 of the measured copy rate; a decode step is one launch of 6 us.
-template <int DTYPE>
+// Bound by HBM (numbers in, codes out) for prompts: 27392 tokens x 8 heads x 128 halves in pages of 64 rows,
+// 169 MB, in 37 us = 4.6 TB/s, 0.70 of the measured copy rate; a decode step is one launch of 4 us.
+template <int DTYPE, int TEAM>
 __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const append_args a)
 {
-    constexpr int HELD = DTYPE == BITSKNN_F32 ? 4 : 8; // vectors of 8 numbers a thread keeps between the passes
+    constexpr int KEPT = HELD<DTYPE>;
     __shared__ float s_top[APPEND_THREADS / 32];
     __shared__ int s_first[APPEND_THREADS / 32];
-    const int t = threadIdx.x;
+    const int t = threadIdx.x % TEAM;
     const int lane = t & 31;
     const int head = blockIdx.y;
     const int which = blockIdx.z;
@@ -163,11 +174,17 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
     float* const scales = which == 0 ? a.c.key_scales : a.c.value_scales;
     // a thread serves one vector of eight numbers of every row_step-th row
     const int vecs = a.dim >> 3;
-    const int row_step = APPEND_THREADS / vecs;
+    const int row_step = TEAM / vecs;
     const int row0 = t < row_step * vecs ? t / vecs : 1 << 20;
     const int at_vec = t % vecs * 8;
     const int rows_mask = (1 << a.c.page_shift) - 1;
-    const int first_token = blockIdx.x * a.window;
+    const int64_t window_begin =
+        (static_cast<int64_t>(blockIdx.x) * (APPEND_THREADS / TEAM) + threadIdx.x / TEAM) * a.window;
+    if (window_begin >= a.tokens)
+    {
+        return; // a warp of the last block (blocks as teams have a window each)
+    }
+    const int first_token = static_cast<int>(window_begin);
     int end_token = min(first_token + a.window, a.tokens);
     auto page_of = [&](int64_t slot) -> int64_t {
         const int64_t p = slot < 0 ? -1 : slot >> a.c.page_shift;
@@ -198,32 +215,46 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         }
         return limit;
     };
-    // the same up to the last token.  The padding of a batch may lie there, so the whole block looks
-    // when nothing is near, 512 slots at a time.
+    auto team_sync = [] {
+        if constexpr (TEAM > 32)
+        {
+            __syncthreads();
+        }
+        else
+        {
+            __syncwarp();
+        }
+    };
+    // the same up to the last token.  The padding of a batch may lie there, so the whole team looks
+    // when nothing is near, 512 (a warp: 256) slots at a time.
     auto find_far = [&](int from) {
+        constexpr int LOOKS = TEAM > 32 ? 4 : 8;
         const int close = min(from + 128, a.tokens);
         int first = find(from, close, -1);
-        for (from = close; first == close && from < a.tokens; from += 4 * APPEND_THREADS)
+        for (from = close; first == close && from < a.tokens; from += LOOKS * TEAM)
         {
             first = a.tokens;
 #pragma unroll
-            for (int x = 3; x >= 0; --x)
+            for (int x = LOOKS - 1; x >= 0; --x)
             {
-                const int j = from + x * APPEND_THREADS + t;
+                const int j = from + x * TEAM + t;
                 first = page_of(j < a.tokens ? a.slots[j] : -1) >= 0 ? j : first;
             }
             first = __reduce_min_sync(FULL_MASK, first);
-            if (lane == 0)
+            if constexpr (TEAM > 32)
             {
-                s_first[t >> 5] = first;
-            }
-            __syncthreads();
+                if (lane == 0)
+                {
+                    s_first[t >> 5] = first;
+                }
+                __syncthreads();
 #pragma unroll
-            for (int w = 0; w < APPEND_THREADS / 32; ++w)
-            {
-                first = min(first, s_first[w]);
+                for (int w = 0; w < TEAM / 32; ++w)
+                {
+                    first = min(first, s_first[w]);
+                }
+                __syncthreads();
             }
-            __syncthreads();
             if (first < a.tokens)
             {
                 return first;
@@ -270,28 +301,44 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         // rows of the page one after the other, as they are unless a caller leaves some out
         const bool dense = a.slots[i + run - 1] - slot0 == run - 1;
         const int64_t from = (i + row0) * stride + static_cast<int64_t>(head) * a.dim + at_vec;
-        raw8<DTYPE> held[HELD];
+        raw8<DTYPE> held[KEPT];
         auto fetch = [&](int h) { return load8<DTYPE>(src, from + h * row_step * stride); };
         uint32_t acc = 0;
         // the whole page at once: every thread has all its vectors, and nothing is asked for each of them
-        const bool full = run >= HELD * row_step && row_step * vecs == APPEND_THREADS;
+        const bool full = run >= KEPT * row_step && row_step * vecs == TEAM;
         if (full)
         {
 #pragma unroll
-            for (int h = 0; h < HELD; ++h)
+            for (int h = 0; h < KEPT; ++h)
             {
                 held[h] = fetch(h);
             }
 #pragma unroll
-            for (int h = 0; h < HELD; ++h)
+            for (int h = 0; h < KEPT; ++h)
             {
                 acc = larger<DTYPE>(acc, held[h]);
+            }
+            if constexpr (TEAM > 32)
+            {
+                // the next run's numbers set out for L2 while this one is finished, one lane per 128 bytes
+                // (27392 tokens in pages of 64 rows: 40 -> 36 us; runs of warps are too short for it)
+                if ((t & (DTYPE == BITSKNN_F32 ? 3 : 7)) == 0)
+                {
+#pragma unroll
+                    for (int h = 0; h < KEPT; ++h)
+                    {
+                        if (i + run + row0 + h * row_step < end_token)
+                        {
+                            prefetch_l2(src, from + (run + h * row_step) * stride, DTYPE == BITSKNN_F32 ? 4 : 2);
+                        }
+                    }
+                }
             }
         }
         else
         {
 #pragma unroll
-            for (int h = 0; h < HELD; ++h)
+            for (int h = 0; h < KEPT; ++h)
             {
                 if (row0 + h * row_step < run)
                 {
@@ -300,7 +347,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
                 }
             }
         }
-        for (int h = HELD; row0 + h * row_step < run; ++h)
+        for (int h = KEPT; row0 + h * row_step < run; ++h)
         {
             acc = larger<DTYPE>(acc, fetch(h));
         }
@@ -325,17 +372,20 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         {
             top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
         }
-        if (lane == 0)
-        {
-            s_top[t >> 5] = top;
-        }
         float* const scale_at = scales + page * a.c.heads + head;
         const float stored = offset0 == 0 ? 0.0F : *scale_at;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < APPEND_THREADS / 32; ++w)
+        if constexpr (TEAM > 32)
         {
-            top = fmaxf(top, s_top[w]);
+            if (lane == 0)
+            {
+                s_top[t >> 5] = top;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < TEAM / 32; ++w)
+            {
+                top = fmaxf(top, s_top[w]);
+            }
         }
         // a page that is begun forgets the scale of its former owner; one that is continued keeps
         // at least its own (anything but a positive number in range counts as the smallest)
@@ -359,7 +409,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         if (full && dense)
         {
 #pragma unroll
-            for (int h = 0; h < HELD; ++h)
+            for (int h = 0; h < KEPT; ++h)
             {
                 store(h, held[h], true);
             }
@@ -367,7 +417,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
         else
         {
 #pragma unroll
-            for (int h = 0; h < HELD; ++h)
+            for (int h = 0; h < KEPT; ++h)
             {
                 if (row0 + h * row_step < run)
                 {
@@ -375,32 +425,35 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
                 }
             }
         }
-        for (int h = HELD; row0 + h * row_step < run; ++h)
+        for (int h = KEPT; row0 + h * row_step < run; ++h)
         {
             store(h, fetch(h), dense);
         }
         if (offset0 > 0 && scale > old)
         {
             const float shrink = old / scale;
-            const int words = offset0 * a.dim >> 2;
-            for (int w = t; w < words; w += APPEND_THREADS)
-            {
-                uint32_t* const p = reinterpret_cast<uint32_t*>(codes + base) + w;
-                const uint32_t c = *p;
+            const int granules = offset0 * a.dim >> 4;
+            auto shrunk = [&](uint32_t c) {
                 uint32_t lo, hi;
                 cache::halves_of_codes(c, lo, hi);
                 const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
                 const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                *p = cache::codes_of_floats(x.x * shrink, x.y * shrink) |
-                     cache::codes_of_floats(y.x * shrink, y.y * shrink) << 16;
+                return cache::codes_of_floats(x.x * shrink, x.y * shrink) |
+                       cache::codes_of_floats(y.x * shrink, y.y * shrink) << 16;
+            };
+            for (int g = t; g < granules; g += TEAM)
+            {
+                uint4* const p = reinterpret_cast<uint4*>(codes + base) + g;
+                const uint4 c = *p;
+                *p = make_uint4(shrunk(c.x), shrunk(c.y), shrunk(c.z), shrunk(c.w));
             }
         }
-        __syncthreads(); // the next run may continue this page
+        team_sync(); // the next run may continue this page
         if (t == 0)
         {
             *scale_at = scale;
         }
-        __syncthreads();
+        team_sync();
         i += run;
         if (i < end_token)
         {
@@ -417,6 +470,34 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) cache_append_kernel(const a
             end_token = i + 1;
         }
     }
+}
+
+template <int DTYPE, int TEAM>
+int launch_append_teams(append_args a, cudaStream_t stream)
+{
+    constexpr int TEAMS = APPEND_THREADS / TEAM;
+    // Few tokens: one team for each, so that the runs of a decode step (one token long) run side by side;
+    // many: windows, as many as run at once (27392 tokens, 8 heads of 128: 8 blocks per SM 37 us, 16 and 32 40).
+    const int64_t target =
+        std::max<int64_t>(1, static_cast<int64_t>(device_sm_count()) * 8 * TEAMS / (2 * a.c.heads));
+    a.window = static_cast<int>((a.tokens + target - 1) / target);
+    const int64_t windows = (static_cast<int64_t>(a.tokens) + a.window - 1) / a.window;
+    const dim3 grid(static_cast<unsigned>((windows + TEAMS - 1) / TEAMS), static_cast<unsigned>(a.c.heads), 2U);
+    {
+        kernel_scope scope("cache_append_kernel", stream);
+        cache_append_kernel<DTYPE, TEAM><<<grid, APPEND_THREADS, 0, stream>>>(a);
+    }
+    BITSKNN_CUDA_TRY(cudaGetLastError());
+    return BITSKNN_OK;
+}
+
+template <int DTYPE>
+int launch_append(const append_args& a, int page_rows, cudaStream_t stream)
+{
+    // Warps for pages of up to twice what they keep (8192 tokens, 8 heads of 128: pages of 16 rows 9.5 us, blocks
+    // 24; of 32 rows 11.6 and 18), blocks for larger ones (27392 tokens, 64 rows: 37 us, warps 62).
+    return page_rows * a.dim <= 2 * 32 * HELD<DTYPE> * 8 ? launch_append_teams<DTYPE, 32>(a, stream)
+                                                         : launch_append_teams<DTYPE, APPEND_THREADS>(a, stream);
 }
 
 } // namespace
@@ -473,22 +554,8 @@ extern "C" int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_
     a.tokens = static_cast<int>(tokens);
     a.dim = cache->dim;
     a.dtype = dtype;
-    // Few tokens: one block for each, so that the runs of a decode step (one token long) run side by side;
-    // many: windows, as many as run at once (27392 tokens, 8 heads of 128: 8 blocks per SM 37 us, 16 and 32 40).
-    const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(device_sm_count()) * 8 / (2 * cache->heads));
-    a.window = static_cast<int>((tokens + target - 1) / target);
-    const int64_t windows = (tokens + a.window - 1) / a.window;
-    const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>(cache->heads), 2U);
     auto s = static_cast<cudaStream_t>(stream);
-    {
-        kernel_scope scope("cache_append_kernel", s);
-        switch (dtype)
-        {
-        case BITSKNN_F32: cache_append_kernel<BITSKNN_F32><<<grid, APPEND_THREADS, 0, s>>>(a); break;
-        case BITSKNN_F16: cache_append_kernel<BITSKNN_F16><<<grid, APPEND_THREADS, 0, s>>>(a); break;
-        default: cache_append_kernel<BITSKNN_BF16><<<grid, APPEND_THREADS, 0, s>>>(a); break;
-        }
-    }
-    BITSKNN_CUDA_TRY(cudaGetLastError());
-    return BITSKNN_OK;
+    return dtype == BITSKNN_F32   ? launch_append<BITSKNN_F32>(a, cache->page_rows, s)
+           : dtype == BITSKNN_F16 ? launch_append<BITSKNN_F16>(a, cache->page_rows, s)
+                                  : launch_append<BITSKNN_BF16>(a, cache->page_rows, s);
 }

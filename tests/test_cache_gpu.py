@@ -906,3 +906,24 @@ def test_items_with_few_rows_between_items_with_many(bk, cuda):
     for _ in range(20):
         again, _ = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
         assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+
+
+@pytest.mark.parametrize("rows, dim, dtype", [(16, 128, torch.float16), (32, 128, torch.bfloat16),
+                                              (64, 128, torch.float16), (16, 256, torch.float32),
+                                              (16, 96, torch.bfloat16), (32, 32, torch.float32)])
+def test_append_does_not_depend_on_how_tokens_are_batched(bk, cuda, rows, dim, dtype):
+    """Many pages in one call, teams of warps and of blocks, against the same tokens page by page."""
+    heads, pages = 3, 40
+    rng = np.random.default_rng(rows + dim)
+    order = rng.permutation(pages)[:30]
+    slots = np.concatenate([p * rows + np.arange(rows) for p in order[:-1]] + [order[-1] * rows + np.arange(5)])
+    new = [torch.from_numpy(rng.standard_normal((len(slots), heads, dim)) * np.exp(rng.standard_normal((len(slots), 1, 1))))
+           .to(dtype).cuda() for _ in range(2)]
+    slots = torch.from_numpy(slots).cuda()
+    got, want = (bk.Cache.empty(pages, heads, rows, dim) for _ in range(2))
+    bk.cache_append(got, *new, slots)
+    for i in range(30):
+        one = slice(i * rows, min((i + 1) * rows, len(slots)))
+        bk.cache_append(want, new[0][one], new[1][one], slots[one])
+    for name in ("keys", "values", "key_scales", "value_scales"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
