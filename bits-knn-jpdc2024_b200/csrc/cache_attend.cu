@@ -500,8 +500,10 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
                         {
-                            one_lo[nb] = transpose_8x8(pack_half2(at_lo < see[nb][0] ? 1.0F : 0.0F, at_lo < see[nb][1] ? 1.0F : 0.0F));
-                            one_hi[nb] = transpose_8x8(pack_half2(at_hi < see[nb][0] ? 1.0F : 0.0F, at_hi < see[nb][1] ? 1.0F : 0.0F));
+                            one_lo[nb] = transpose_8x8(
+                                pack_half2(at_lo < see[nb][0] ? 1.0F : 0.0F, at_lo < see[nb][1] ? 1.0F : 0.0F));
+                            one_hi[nb] = transpose_8x8(
+                                pack_half2(at_hi < see[nb][0] ? 1.0F : 0.0F, at_hi < see[nb][1] ? 1.0F : 0.0F));
                         }
 #pragma unroll
                         for (int g = 0; g < DIM / 16; g += 2)
@@ -779,7 +781,8 @@ int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaSt
     {
         return rc;
     }
-    auto kernel = a.cluster > 0 ? cache_attend_kernel<DIM, NB, SELECTED, true> : cache_attend_kernel<DIM, NB, SELECTED, false>;
+    auto kernel =
+        a.cluster > 0 ? cache_attend_kernel<DIM, NB, SELECTED, true> : cache_attend_kernel<DIM, NB, SELECTED, false>;
     static cache::device_set prepared[2];
     cache::device_set& ready = prepared[a.cluster > 0 ? 1 : 0];
     if (!ready.contains_current())
