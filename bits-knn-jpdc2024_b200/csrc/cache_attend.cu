@@ -49,7 +49,7 @@ struct attend_smem
 //
 // Bound by the bytes of the cache (HBM) while the columns are few.  One request with 250001 positions, 8 heads of 128
 // (512 MB): 90 us = 5.7 TB/s, 0.87 of the measured copy rate, and 10 us for the join; 64 requests with 150 ... 24000
-// positions (625 MB): 110 us, 0.87 and 8 us; 2048 listed positions of 32 requests (137 MB in gathers of 128 bytes):
+// positions (625 MB): 108 us, 0.88 and 6 us; 2048 listed positions of 32 requests (137 MB in gathers of 128 bytes):
 // 40 us, 0.52 -- more copies in flight do not help there, single rows are what the memory delivers more slowly.
 // Three stages and three blocks per SM (four stages: 97 us for the long request, two: 92).
 template <int DIM, int NB, bool SELECTED, bool CLUSTER>

@@ -179,8 +179,9 @@ __device__ __forceinline__ int find_request(const attend_args& a, int64_t at, in
 // Joins the parts of items that several blocks worked on: block c looks after the item that begins
 // in block c of the main kernel and ends in a later one, whose parts are part 1 of block c and
 // part 0 of the blocks up to its last.  Always in that order, so results do not depend on timing.
-// SPLIT warps share the parts of a column (many parts of few columns when a long request decodes, few
-// parts of many columns when prompts are attended to).  Launched while the main kernel still runs
+// SPLIT warps share the parts of a column when there are many (few columns of a long request that decodes); few
+// parts are a warp's work, so that most of the grid has nothing to do (64 requests 115 -> 114
+// us, 32 requests with lists 43 -> 41).  Launched while the main kernel still runs
 // (griddepcontrol), so that its own launch takes no time.
 constexpr int JOIN_WARPS = 8;
 
@@ -203,17 +204,19 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
     const int4 join = a.joins[blockIdx.x];
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int col = SPLIT > 1 ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * JOIN_WARPS + warp;
-    if (col >= join.w - join.z)
+    const int all = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x) + 1; // of no meaning without a join
+    constexpr int FEW = 4;
+    const bool alone = SPLIT == 1 || all <= FEW; // a column is one warp's work
+    const int col = static_cast<int>(blockIdx.y) * (alone ? JOIN_WARPS : 1) + (alone ? warp : 0);
+    if (col >= min(join.w - join.z, COLS))
     {
         return; // the whole block when warps share a column
     }
     const int64_t first = 2 * static_cast<int64_t>(blockIdx.x) + 1;
-    const int all = a.join_end[blockIdx.x] - static_cast<int>(blockIdx.x) + 1;
     auto part = [&](int i) { return (first + (i == 0 ? 0 : 2 * i - 1)) * COLS + col; };
     // this warp's parts, a run of them so that the order of the sums is that of the positions
-    const int begin = SPLIT > 1 ? warp * all / SPLIT : 0;
-    const int parts = SPLIT > 1 ? (warp + 1) * all / SPLIT - begin : all;
+    const int begin = alone ? 0 : warp * all / SPLIT;
+    const int parts = alone ? all : (warp + 1) * all / SPLIT - begin;
     float top = -INFINITY;
     float sum[PER];
 #pragma unroll
@@ -222,10 +225,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
         sum[x] = 0.0F;
     }
     float den = 0.0F;
-    constexpr int FEW = 4;
-    if (SPLIT == 1 && parts <= FEW)
+    if (alone && parts <= FEW)
     {
-        // the usual case of prompts: everything is loaded at once, and every lane weighs for itself
+        // the usual case of prompts and of batches: everything is loaded at once, and every lane weighs for itself
         float2 ml[FEW];
         vec w[FEW][PER / VEC];
 #pragma unroll
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
             den += __shfl_xor_sync(FULL_MASK, den, o);
         }
     }
-    if constexpr (SPLIT > 1)
+    if (!alone)
     {
 #pragma unroll
         for (int x = 0; x < PER; ++x)
