@@ -226,6 +226,16 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with operands of BF16.
+__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -246,6 +256,26 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
+{
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Two halves that hold e4m3 numbers to two BF16 numbers; exact.
+__device__ __forceinline__ uint32_t bf16_of_halves(uint32_t h)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return pack_bf16(f.x, f.y);
+}
+
+// Two floats, each as the sum of two BF16 numbers (17 significant bits over the range of floats).
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& high, uint32_t& low)
+{
+    high = pack_bf16(x, y);
+    low = pack_bf16(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xffff0000U));
 }
 
 // Staged rows in shared memory, DIM / 16 granules of 16 bytes each.  Eight rows at the same granule have to

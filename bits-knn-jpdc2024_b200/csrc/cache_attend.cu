@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
             float l[NB][2];
             float f[NB][2];
             int see[NB][2];
+            uint32_t vs_least = 0; // bits of the largest value scale of the warp's rows so far over 2^SCALE_SPREAD
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
             {
@@ -400,61 +401,77 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                         raise |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + WEIGHT_SLACK;
                         raise |= fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + WEIGHT_SLACK;
                     }
-                    if (__any_sync(FULL_MASK, raise))
+                    // a value scale above the largest one so far or far below it; positive floats order like their bits
+                    auto apart = [&](float vs) { return __float_as_uint(vs) - vs_least > SCALE_SPREAD << 23; };
+                    bool careful = false; // weights do not do as halves (cache_attend.cuh), or there is a NaN
+                    if (__any_sync(FULL_MASK, raise || apart(vs_lo) || (SELECTED && apart(vs_hi))))
                     {
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
+                        const uint32_t most_lo = ks_lo != 0.0F ? __float_as_uint(vs_lo) : 0U; // of rows that are there
+                        const uint32_t most_hi = SELECTED && ks_hi != 0.0F ? __float_as_uint(vs_hi) : most_lo;
+                        const uint32_t most = SELECTED ? __reduce_max_sync(FULL_MASK, max(most_lo, most_hi)) : most_lo;
+                        vs_least = max(vs_least, most - min(most, SCALE_SPREAD << 23));
+                        auto far = [&](float ks, float vs) { return ks != 0.0F && __float_as_uint(vs) < vs_least; };
+                        careful = __any_sync(FULL_MASK, far(ks_lo, vs_lo) || (SELECTED && far(ks_hi, vs_hi))) != 0;
+                        if (__any_sync(FULL_MASK, raise))
                         {
 #pragma unroll
-                            for (int x = 0; x < 2; ++x)
+                            for (int nb = 0; nb < NB; ++nb)
                             {
-                                float top = fmaxf(s[nb][x], s[nb][2 + x]);
 #pragma unroll
-                                for (int w = 4; w < 32; w <<= 1)
+                                for (int x = 0; x < 2; ++x)
                                 {
-                                    top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, w));
-                                }
-                                top = fmaxf(top, m[nb][x]);
-                                const float keep = m[nb][x] == -INFINITY ? 0.0F : exp2_fast(m[nb][x] - top);
-                                m[nb][x] = top;
-                                l[nb][x] *= keep;
+                                    float top = fmaxf(s[nb][x], s[nb][2 + x]);
 #pragma unroll
-                                for (int g = 0; g < DIM / 16; ++g)
-                                {
-                                    o[g][nb][x] *= keep;
-                                    o[g][nb][2 + x] *= keep;
+                                    for (int w = 4; w < 32; w <<= 1)
+                                    {
+                                        top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, w));
+                                    }
+                                    top = fmaxf(top, m[nb][x]);
+                                    const float keep = m[nb][x] == -INFINITY ? 0.0F : exp2_fast(m[nb][x] - top);
+                                    m[nb][x] = top;
+                                    l[nb][x] *= keep;
+#pragma unroll
+                                    for (int g = 0; g < DIM / 16; ++g)
+                                    {
+                                        o[g][nb][x] *= keep;
+                                        o[g][nb][2 + x] *= keep;
+                                    }
                                 }
                             }
                         }
                     }
+                    auto weigh = [&](int nb, float (&p)[4]) { // rows lo, lo, hi, hi
+                        const float b0 = WEIGHT_BIAS - (m[nb][0] == -INFINITY ? 0.0F : m[nb][0]);
+                        const float b1 = WEIGHT_BIAS - (m[nb][1] == -INFINITY ? 0.0F : m[nb][1]);
+                        p[0] = exp2_fast(s[nb][0] + b0);
+                        p[1] = exp2_fast(s[nb][1] + b1);
+                        p[2] = exp2_fast(s[nb][2] + b0);
+                        p[3] = exp2_fast(s[nb][3] + b1);
+                    };
                     uint32_t w_lo[NB];
                     uint32_t w_hi[NB];
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                     {
-                        const float b0 = WEIGHT_BIAS - (m[nb][0] == -INFINITY ? 0.0F : m[nb][0]);
-                        const float b1 = WEIGHT_BIAS - (m[nb][1] == -INFINITY ? 0.0F : m[nb][1]);
-                        const float p0 = exp2_fast(s[nb][0] + b0);
-                        const float p1 = exp2_fast(s[nb][1] + b1);
-                        const float p2 = exp2_fast(s[nb][2] + b0);
-                        const float p3 = exp2_fast(s[nb][3] + b1);
+                        float p[4];
+                        weigh(nb, p);
                         if constexpr (SELECTED)
                         {
-                            l[nb][0] = fmaf(p0, iv_lo, fmaf(p2, iv_hi, l[nb][0]));
-                            l[nb][1] = fmaf(p1, iv_lo, fmaf(p3, iv_hi, l[nb][1]));
+                            l[nb][0] = fmaf(p[0], iv_lo, fmaf(p[2], iv_hi, l[nb][0]));
+                            l[nb][1] = fmaf(p[1], iv_lo, fmaf(p[3], iv_hi, l[nb][1]));
                         }
                         else
                         {
-                            l[nb][0] = fmaf(p0 + p2, iv_lo, l[nb][0]);
-                            l[nb][1] = fmaf(p1 + p3, iv_lo, l[nb][1]);
+                            l[nb][0] = fmaf(p[0] + p[2], iv_lo, l[nb][0]);
+                            l[nb][1] = fmaf(p[1] + p[3], iv_lo, l[nb][1]);
                         }
-                        w_lo[nb] = transpose_8x8(pack_half2(p0, p1));
-                        w_hi[nb] = transpose_8x8(pack_half2(p2, p3));
+                        w_lo[nb] = transpose_8x8(pack_half2(p[0], p[1]));
+                        w_hi[nb] = transpose_8x8(pack_half2(p[2], p[3]));
                     }
                     // A NaN code times a weight of zero would spoil the columns that do not see its row.
                     // Only rows that some columns see and others do not can do that (rows nobody sees
                     // were copied as zeros); if such a subtile holds one, the codes are cleaned, and a
-                    // second product of indicators finds the outputs that the NaN belongs to.
+                    // product of indicators finds the outputs that the NaN belongs to.
                     const unsigned char* const vrows = stage + SUB * PITCH<DIM, true>;
                     bool nan_here = false;
                     if (!SELECTED && nearest < furthest && pos + SUB > nearest)
@@ -465,12 +482,12 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                                 *reinterpret_cast<const uint32_t*>(vrows + (e * 4 / DIM) * PITCH<DIM, true> + e * 4 % DIM);
                             nan_here |= (((w & 0x7f7f7f7fU) + 0x01010101U) & 0x80808080U) != 0;
                         }
-                        nan_here = __any_sync(FULL_MASK, nan_here);
+                        careful |= __any_sync(FULL_MASK, nan_here) != 0;
                     }
                     const uint32_t vaddr = ptx::smem_addr(vrows) +
                                            (((lane >> 3) & 1) * 8 + row_order<DIM, true>(lane & 7)) * PITCH<DIM, true> +
                                            (lane >> 4) * 16;
-                    if (!nan_here)
+                    if (!careful)
                     {
 #pragma unroll
                         for (int g = 0; g < DIM / 16; g += 2)
@@ -497,13 +514,28 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                     {
                         uint32_t one_lo[NB];
                         uint32_t one_hi[NB];
+                        uint32_t w_lo[NB][2]; // the weights once more, each the sum of two BF16 numbers
+                        uint32_t w_hi[NB][2];
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
                         {
-                            one_lo[nb] = transpose_8x8(
-                                pack_half2(at_lo < see[nb][0] ? 1.0F : 0.0F, at_lo < see[nb][1] ? 1.0F : 0.0F));
-                            one_hi[nb] = transpose_8x8(
-                                pack_half2(at_hi < see[nb][0] ? 1.0F : 0.0F, at_hi < see[nb][1] ? 1.0F : 0.0F));
+                            float p[4];
+                            weigh(nb, p);
+                            split_bf16(p[0], p[1], w_lo[nb][0], w_lo[nb][1]);
+                            split_bf16(p[2], p[3], w_hi[nb][0], w_hi[nb][1]);
+#pragma unroll
+                            for (int y = 0; y < 2; ++y)
+                            {
+                                w_lo[nb][y] = transpose_8x8(w_lo[nb][y]);
+                                w_hi[nb][y] = transpose_8x8(w_hi[nb][y]);
+                            }
+                            if constexpr (!SELECTED) // there everyone sees all rows
+                            {
+                                one_lo[nb] = transpose_8x8(
+                                    pack_half2(at_lo < see[nb][0] ? 1.0F : 0.0F, at_lo < see[nb][1] ? 1.0F : 0.0F));
+                                one_hi[nb] = transpose_8x8(
+                                    pack_half2(at_hi < see[nb][0] ? 1.0F : 0.0F, at_hi < see[nb][1] ? 1.0F : 0.0F));
+                            }
                         }
 #pragma unroll
                         for (int g = 0; g < DIM / 16; g += 2)
@@ -526,18 +558,25 @@ __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_a
                                     const uint32_t low = (h[y] & 0x7fffU) > 0x7c00U ? 0xffffU : 0U;
                                     const uint32_t high = (h[y] & 0x7fff0000U) > 0x7c000000U ? 0xffff0000U : 0U;
                                     is[y] = (low | high) & 0x3c003c00U; // ones
-                                    h[y] &= ~(low | high);
+                                    h[y] = bf16_of_halves(SELECTED ? h[y] : h[y] & ~(low | high));
                                 }
 #pragma unroll
                                 for (int nb = 0; nb < NB; ++nb)
                                 {
-                                    float hits[4] = {0.0F, 0.0F, 0.0F, 0.0F};
-                                    mma_16816(hits, is[0], is[1], is[2], is[3], one_lo[nb], one_hi[nb]);
-                                    mma_16816(o[g + x][nb], h[0], h[1], h[2], h[3], w_lo[nb], w_hi[nb]);
 #pragma unroll
-                                    for (int y = 0; y < 4; ++y)
+                                    for (int y = 0; y < 2; ++y)
                                     {
-                                        o[g + x][nb][y] = hits[y] > 0.0F ? NAN : o[g + x][nb][y];
+                                        mma_16816_bf16(o[g + x][nb], h[0], h[1], h[2], h[3], w_lo[nb][y], w_hi[nb][y]);
+                                    }
+                                    if constexpr (!SELECTED)
+                                    {
+                                        float hits[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+                                        mma_16816(hits, is[0], is[1], is[2], is[3], one_lo[nb], one_hi[nb]);
+#pragma unroll
+                                        for (int y = 0; y < 4; ++y)
+                                        {
+                                            o[g + x][nb][y] = hits[y] > 0.0F ? NAN : o[g + x][nb][y];
+                                        }
                                     }
                                 }
                             }

@@ -9,6 +9,14 @@
 // Logits, maxima and sums are FP32.  Weights are rounded to halves (11 bits, the codes are exact
 // halves): the reference point m is kept 7 binary orders below the half range's 2^7 ... 2^15, so a
 // weight of 2^-31 of the largest is still not lost, which 10^5 positions of little weight need.
+//
+// Largest means the largest of p_j vs_j.  Where value scales lie far apart that is not the largest p_j:
+// a page of a scale 2^30 times the others' would take the halves of all other positions to zero,
+// though it may hold a single number, and the outputs of the dimensions it has none in would be lost.  So
+// positions whose scale is below 2^-SCALE_SPREAD of the largest one so far get their weights as sums of two
+// BF16 numbers (17 bits, the range of floats) and their codes as BF16 (exact).  For the others a half, off by at most
+// 2^-25 where the largest p vs has 2^7 or more, is off by 2^(SCALE_SPREAD - 32) = 2^-28 of the largest p.  The BF16
+// weights end at the smallest float: p vs below 2^-133 of the largest counts as zero.
 #pragma once
 
 #include "cache.cuh"
@@ -35,6 +43,7 @@ struct attend_args
     float2* part_ml;  // [2 * blocks][columns]
     int4* joins;      // [blocks]
     int* join_end;    // [blocks]
+    int* far_apart;   // [blocks], tensor-memory kernel: the block's share has value scales far apart
     int cluster;        // > 0: an item to every cluster of so many blocks, which joins by itself
 };
 
@@ -62,6 +71,7 @@ using namespace cache;
 
 constexpr float WEIGHT_BIAS = 7.0F;  // the weight of the reference point is 2^7
 constexpr float WEIGHT_SLACK = 8.0F; // a logit may pass the reference point by 8 (weight 2^15) before it moves
+constexpr uint32_t SCALE_SPREAD = 4;  // binary orders of value scales that halves can serve together
 constexpr float LOG2_E = 1.4426950408889634F;
 constexpr float LN_2 = 0.6931471805599453F;
 
@@ -365,9 +375,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
     }
 }
 
-constexpr size_t JOIN_BYTES = sizeof(int4) + sizeof(int);
+constexpr size_t JOIN_BYTES = sizeof(int4) + 2 * sizeof(int);
 
-// Workspace of a launch of `blocks` blocks: two parts per block and its join.
+// Workspace of a launch of `blocks` blocks: two parts per block, its join and its note of scales.
 template <int DIM, int COLS>
 size_t parts_bytes(int blocks)
 {
@@ -386,6 +396,7 @@ int place_parts(attend_args& a, int blocks, void* workspace, size_t workspace_by
     a.joins = reinterpret_cast<int4*>(a.part_o + static_cast<size_t>(blocks) * 2 * COLS * DIM);
     a.part_ml = reinterpret_cast<float2*>(a.joins + blocks);
     a.join_end = reinterpret_cast<int*>(a.part_ml + static_cast<size_t>(blocks) * 2 * COLS);
+    a.far_apart = a.join_end + blocks;
     return BITSKNN_OK;
 }
 

@@ -89,6 +89,15 @@ __device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&v)[3
                  : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Descriptor of the values as second operand of the second product: rows are positions (the
@@ -135,6 +144,15 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[32])
                  "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
                  "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
                  "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                  :
                  : "memory");
 }
@@ -268,6 +286,81 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity)
     return __all_sync(FULL_MASK, ptx::mbar_wait_bounded_spin(bar, parity)) != 0;
 }
 
+// A row's step of the softmax over a tile whose weights become the sums of two BF16 numbers each: of every 16 words, 8
+// for the upper numbers of 16 positions and 8 for the lower ones, over their scores.  Rare, so it is kept out of the way
+// of the others: group after group, maxima first.  Returns the reference point and the sum, which is -inf if the wait for
+// the product before (`done`, if there is one) ran out.
+template <int DIM>
+__device__ __forceinline__ float2 far_tile(uint32_t s_addr, uint32_t o_addr, const float4* scales, float factor, int limit,
+                                           float m, float l, uint64_t* done, uint32_t phase)
+{
+    uint32_t s[16];
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g)
+    {
+        tc::tmem_ld_32x16(s_addr + g * 16, s);
+        tmem_ld_wait(s);
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            most = g * 16 + i < limit ? fmaxf(most, __uint_as_float(s[i])) : most;
+        }
+        top = fmaxf(top, most == -INFINITY ? most : fmaf(most, factor * scales[g].x, scales[g].y));
+    }
+    if (__any_sync(FULL_MASK, m == -INFINITY || top > m + WEIGHT_SLACK))
+    {
+        top = fmaxf(top, m);
+        const float keep = m == -INFINITY ? 0.0F : exp2_fast(m - top);
+        m = top;
+        l *= keep;
+        if (done != nullptr)
+        {
+            if (!warp_wait(done, phase))
+            {
+                return make_float2(m, -INFINITY);
+            }
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < DIM; c += 16)
+            {
+                tc::tmem_ld_32x16(o_addr + c, s);
+                tmem_ld_wait(s);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    s[i] = __float_as_uint(__uint_as_float(s[i]) * keep);
+                }
+                tmem_st_16(o_addr + c, s);
+            }
+        }
+    }
+    const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g)
+    {
+        tc::tmem_ld_32x16(s_addr + g * 16, s);
+        tmem_ld_wait(s);
+        const float4 k = scales[g];
+        float sum = 0.0F;
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2)
+        {
+            float x = exp2_fast(fmaf(__uint_as_float(s[i]), factor * k.x, k.y + bias));
+            float y = exp2_fast(fmaf(__uint_as_float(s[i + 1]), factor * k.x, k.y + bias));
+            x = g * 16 + i < limit ? x : 0.0F;
+            y = g * 16 + i + 1 < limit ? y : 0.0F;
+            sum += x + y;
+            split_bf16(x, y, p[i / 2], p[8 + i / 2]);
+        }
+        l = fmaf(sum, k.z, l);
+        tmem_st_16(s_addr + g * 16, p);
+    }
+    return make_float2(m, l);
+}
+
 // First position of a dimension with a NaN among the tiles that only some rows of item number `items`
 // see wholly, as an offset (below 1024: a block's columns span at most 256 tokens) from the first
 // of these tiles.  The key grows with the item and towards earlier positions, so a maximum keeps
@@ -327,7 +420,7 @@ struct tc_state
     unsigned char* q_tiles;
     unsigned char* k_tiles;
     unsigned char* v_tiles;
-    float4* scales;     // [RING][GROUPS]: key scale, log2 of the value scale, its inverse
+    float4* scales;     // [RING][GROUPS]: key scale, log2 of the value scale, its inverse, 1 if the tile is BF16 (else 0)
     uint32_t* first_nan; // [RING][NANS]: nan_key
     uint64_t* k_full;   // [STAGES]
     uint64_t* k_empty;
@@ -341,7 +434,7 @@ struct tc_state
 };
 
 // ================= softmax: one thread per query row =================
-template <int DIM>
+template <int DIM, bool FAR>
 __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w,
                                              uint32_t tmem)
 {
@@ -501,53 +594,73 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
                 tc::tmem_ld_32x32(s_addr + 32, s[1]);
                 tmem_ld_wait(s[0]);
                 tmem_ld_wait(s[1]);
-                // Weights against the reference point as it stands.  They are positive, so a sum of at most
-                // 2^15 says that none is too large for a half and nothing has to be compared; only when the
-                // sum is larger (or NaN, or there is no reference point yet) is the maximum looked for.
-                uint32_t p[32];
-                auto weigh = [&] {
-                    const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
-                    return cut ? row_weights<true>(s, p, scales, factor, bias, see - pos)
-                               : row_weights<false>(s, p, scales, factor, bias, 0);
-                };
-                float2 sums = weigh();
-                if (__any_sync(FULL_MASK, m == -INFINITY || !(sums.x <= 32768.0F)))
+                bool far = false;
+                if constexpr (FAR)
                 {
-                    tc::tmem_ld_32x32(s_addr, s[0]);
-                    tc::tmem_ld_32x32(s_addr + 32, s[1]);
-                    tmem_ld_wait(s[0]);
-                    tmem_ld_wait(s[1]);
-                    const float raised = fmaxf(
-                        cut ? row_top<true>(s, scales, factor, see - pos) : row_top<false>(s, scales, factor, 0), m);
-                    const float keep = m == -INFINITY ? 0.0F : exp2_fast(m - raised);
-                    m = raised;
-                    l *= keep;
-                    if (j > 0)
-                    {
-                        // the product before this one has to be through with the sums
-                        if (!warp_wait(&st.o_done[my_tile * 2 + ((s_tiles - 1) & 1)], ((s_tiles - 1) >> 1) & 1U))
-                        {
-                            return false;
-                        }
-                        tc::fence_after_sync();
-#pragma unroll 1
-                        for (int c = 0; c < DIM; c += 32)
-                        {
-                            uint32_t o[32];
-                            tc::tmem_ld_32x32(o_addr + c, o);
-                            tmem_ld_wait(o);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                            {
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                            }
-                            tmem_st_32(o_addr + c, o);
-                        }
-                    }
-                    sums = weigh();
+                    far = __any_sync(FULL_MASK, scales->w != 0.0F) != 0;
                 }
-                l += sums.y;
-                tmem_st_32(s_addr, p); // over the scores
+                if (far)
+                {
+                    const float2 now = far_tile<DIM>(s_addr, o_addr, scales, factor, cut ? see - pos : shape::ROWS, m, l,
+                                                     j > 0 ? &st.o_done[my_tile * 2 + ((s_tiles - 1) & 1)] : nullptr,
+                                                     ((s_tiles - 1) >> 1) & 1U);
+                    m = now.x;
+                    l = now.y;
+                    if (l == -INFINITY)
+                    {
+                        return false;
+                    }
+                }
+                else
+                {
+                    // Weights against the reference point as it stands.  They are positive, so a sum of at most
+                    // 2^15 says that none is too large for a half and nothing has to be compared; only when the
+                    // sum is larger (or NaN, or there is no reference point yet) is the maximum looked for.
+                    uint32_t p[32];
+                    auto weigh = [&] {
+                        const float bias = WEIGHT_BIAS - (m == -INFINITY ? 0.0F : m);
+                        return cut ? row_weights<true>(s, p, scales, factor, bias, see - pos)
+                                   : row_weights<false>(s, p, scales, factor, bias, 0);
+                    };
+                    float2 sums = weigh();
+                    if (__any_sync(FULL_MASK, m == -INFINITY || !(sums.x <= 32768.0F)))
+                    {
+                        tc::tmem_ld_32x32(s_addr, s[0]);
+                        tc::tmem_ld_32x32(s_addr + 32, s[1]);
+                        tmem_ld_wait(s[0]);
+                        tmem_ld_wait(s[1]);
+                        const float raised = fmaxf(
+                            cut ? row_top<true>(s, scales, factor, see - pos) : row_top<false>(s, scales, factor, 0), m);
+                        const float keep = m == -INFINITY ? 0.0F : exp2_fast(m - raised);
+                        m = raised;
+                        l *= keep;
+                        if (j > 0)
+                        {
+                            // the product before this one has to be through with the sums
+                            if (!warp_wait(&st.o_done[my_tile * 2 + ((s_tiles - 1) & 1)], ((s_tiles - 1) >> 1) & 1U))
+                            {
+                                return false;
+                            }
+                            tc::fence_after_sync();
+#pragma unroll 1
+                            for (int c = 0; c < DIM; c += 32)
+                            {
+                                uint32_t o[32];
+                                tc::tmem_ld_32x32(o_addr + c, o);
+                                tmem_ld_wait(o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                {
+                                    o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                                }
+                                tmem_st_32(o_addr + c, o);
+                            }
+                        }
+                        sums = weigh();
+                    }
+                    l += sums.y;
+                    tmem_st_32(s_addr, p); // over the scores
+                }
                 tmem_st_wait();
                 tc::fence_before_sync();
                 warp_arrive(&st.p_full[my_tile * 2 + buffer]);
@@ -676,8 +789,46 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
     return true;
 }
 
+// Scales of a page and head; a key scale of 0 stands for an absent page.
+__device__ __forceinline__ void scales_of(const view& c, int page, int head, float& ks, float& vs)
+{
+    const bool there = page >= 0 && page < c.pages;
+    ks = there ? c.key_scales[static_cast<int64_t>(page) * c.heads + head] : 0.0F;
+    vs = there ? c.value_scales[static_cast<int64_t>(page) * c.heads + head] : 1.0F;
+    vs = fminf(fmaxf(vs, pow2_int(E_MIN)), pow2_int(E_MAX));
+}
+
+// A thread's codes of a tile, PIECES of 16, to halves or to BF16 numbers in shared memory (both exact).
+template <bool AS_BF16, int ROWS, int BLK, int PIECES>
+__device__ __forceinline__ void store_codes(const uint4 (&r)[PIECES], unsigned char* tile, uint32_t first_half,
+                                            uint32_t second_half)
+{
+    const uint32_t to = ptx::smem_addr(tile);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+    {
+        const uint4 x = r[i];
+        const uint32_t at_row = to + i % BLK * ROWS * 128 + i / BLK * 32 * 128;
+        uint32_t h[8];
+        halves_of_codes(x.x, h[0], h[1]);
+        halves_of_codes(x.y, h[2], h[3]);
+        halves_of_codes(x.z, h[4], h[5]);
+        halves_of_codes(x.w, h[6], h[7]);
+        if constexpr (AS_BF16)
+        {
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+            {
+                h[y] = bf16_of_halves(h[y]);
+            }
+        }
+        st_shared16(at_row + first_half, h[0], h[1], h[2], h[3]);
+        st_shared16(at_row + second_half, h[4], h[5], h[6], h[7]);
+    }
+}
+
 // ================= converters: codes from the cache to halves in shared memory =================
-template <int DIM>
+template <int DIM, bool FAR>
 __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w)
 {
     using shape = tc_shape<DIM>;
@@ -698,6 +849,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
     const uint32_t second_half = tile_byte(row0, piece * 2 + 1, ROWS);
     uint32_t n = 0; // tiles so far
     uint32_t items = 0;
+    uint32_t far_apart = 0;
     do
     {
         const int count = w.count();
@@ -723,17 +875,29 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                             : page * a.c.page_stride +
                                   ((static_cast<int64_t>(w.it.head) << a.c.page_shift) + (pos & rows_mask)) * DIM;
         };
-        auto scales_of = [&](int page, float& ks, float& vs) {
-            ks = page < 0 ? 0.0F : a.c.key_scales[static_cast<int64_t>(page) * a.c.heads + w.it.head];
-            vs = page < 0 ? 1.0F : a.c.value_scales[static_cast<int64_t>(page) * a.c.heads + w.it.head];
-        };
         const int page_first = pages_from(0);
         int page_next = pages_from(AHEAD);
         int64_t offset_now = offset_of(page_first, 0);
         float ks_now = 0.0F, vs_now = 1.0F, ks_next = 0.0F, vs_next = 1.0F;
-        if (warp == 0)
+        const bool scaling = FAR || warp == 0; // this warp looks the scales up
+        if (scaling)
         {
-            scales_of(page_first, ks_now, vs_now);
+            scales_of(a.c, page_first, w.it.head, ks_now, vs_now);
+        }
+        // Groups of 16 positions of the tiles looked up whose value scale is far below the largest one up to them
+        // (cache_attend.cuh); the values of their tiles become BF16.
+        uint32_t vs_least = 0; // the largest one over 2^SCALE_SPREAD; positive floats order like their bits
+        uint32_t far_groups = 0;
+        auto compare_scales = [&] {
+            const uint32_t bits = __float_as_uint(vs_now);
+            const uint32_t most = __reduce_max_sync(FULL_MASK, ks_now != 0.0F ? bits : 0U);
+            vs_least = max(vs_least, most - min(most, SCALE_SPREAD << 23));
+            far_groups = __ballot_sync(FULL_MASK, ks_now != 0.0F && bits < vs_least);
+            far_apart |= far_groups;
+        };
+        if (scaling)
+        {
+            compare_scales();
         }
         int base = 0; // first tile of offset_now
         const int whole_tiles = furthest / ROWS - first_tile; // tiles before this one have all their rows
@@ -746,6 +910,10 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 offset_now = offset_of(page_next, j);
                 ks_now = ks_next;
                 vs_now = vs_next;
+                if (scaling)
+                {
+                    compare_scales();
+                }
                 page_next = pages_from(j + AHEAD);
             }
             bool absent = false;
@@ -786,26 +954,6 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                     {
                         r[i * BLK + b] = __ldg(reinterpret_cast<const uint4*>(codes + from[i] + b * 64));
                     }
-                }
-            }
-        };
-        auto store = [&](const uint4 (&r)[PIECES], unsigned char* tile) {
-            const uint32_t to = ptx::smem_addr(tile);
-#pragma unroll
-            for (int i = 0; i < SLABS; ++i)
-            {
-#pragma unroll
-                for (int b = 0; b < BLK; ++b)
-                {
-                    const uint4 x = r[i * BLK + b];
-                    const uint32_t at_row = to + b * ROWS * 128 + i * 32 * 128;
-                    uint32_t h[8];
-                    halves_of_codes(x.x, h[0], h[1]);
-                    halves_of_codes(x.y, h[2], h[3]);
-                    halves_of_codes(x.z, h[4], h[5]);
-                    halves_of_codes(x.w, h[6], h[7]);
-                    st_shared16(at_row + first_half, h[0], h[1], h[2], h[3]);
-                    st_shared16(at_row + second_half, h[4], h[5], h[6], h[7]);
                 }
             }
         };
@@ -853,16 +1001,17 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
             {
                 return false;
             }
-            store(rk, st.k_tiles + stage * shape::KV_BYTES);
+            store_codes<false, ROWS, BLK>(rk, st.k_tiles + stage * shape::KV_BYTES, first_half, second_half);
+            const bool as_bf16 = FAR && (far_groups >> ((j - base) * shape::GROUPS) & ((1U << shape::GROUPS) - 1)) != 0;
             if (warp == 0 && lane / shape::GROUPS == j - base)
             {
-                const float vs = fminf(fmaxf(vs_now, pow2_int(E_MIN)), pow2_int(E_MAX));
                 st.scales[(n % RING) * shape::GROUPS + lane % shape::GROUPS] =
-                    make_float4(ks_now, ks_now == 0.0F ? -INFINITY : log2_fast(vs), __fdividef(1.0F, vs), 0.0F);
+                    make_float4(ks_now, ks_now == 0.0F ? -INFINITY : log2_fast(vs_now), __fdividef(1.0F, vs_now),
+                                as_bf16 ? 1.0F : 0.0F);
             }
-            if (warp == 0 && j - base == AHEAD / 2)
+            if (scaling && j - base == AHEAD / 2)
             {
-                scales_of(page_next, ks_next, vs_next);
+                scales_of(a.c, page_next, w.it.head, ks_next, vs_next);
             }
             fence_async_proxy();
             warp_arrive(&st.k_full[stage]);
@@ -876,7 +1025,14 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
             {
                 clean(rv, j);
             }
-            store(rv, st.v_tiles + stage * shape::KV_BYTES);
+            if (as_bf16)
+            {
+                store_codes<true, ROWS, BLK>(rv, st.v_tiles + stage * shape::KV_BYTES, first_half, second_half);
+            }
+            else
+            {
+                store_codes<false, ROWS, BLK>(rv, st.v_tiles + stage * shape::KV_BYTES, first_half, second_half);
+            }
             fence_async_proxy();
             warp_arrive(&st.v_full[stage]);
             load(rv, a.c.values);
@@ -891,6 +1047,10 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         {
             return false;
         }
+    }
+    if (!FAR && warp == 0 && lane == 0 && far_apart != 0)
+    {
+        a.far_apart[blockIdx.x] = 1;
     }
     return true;
 }
@@ -968,18 +1128,21 @@ __device__ __forceinline__ bool scores_role(const attend_args& a, const tc_state
     return true;
 }
 
-template <int DIM>
+template <int DIM, bool FAR>
 __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w,
                                           uint32_t tmem, int my_tile)
 {
     using shape = tc_shape<DIM>;
-    constexpr uint32_t idesc = tc::instr_desc(0U, 128U, DIM) | (1U << 16); // second operand along its outputs
+    constexpr uint32_t along = 1U << 16; // second operand along its outputs
+    constexpr uint32_t idesc = tc::instr_desc(0U, 128U, DIM) | along;
+    constexpr uint32_t idesc_bf16 = tc::instr_desc(1U, 128U, DIM) | along;
     const uint32_t s_base = tmem + my_tile * 2 * shape::ROWS;
     const uint32_t o_addr = tmem + shape::O_COL + my_tile * DIM;
     const uint64_t v_desc = values_desc(st.v_tiles, shape::ROWS * 128);
     const uint32_t hi = static_cast<uint32_t>(v_desc >> 32);
     uint32_t stage = 0;
     uint32_t phase = 0;
+    uint32_t n = 0; // tiles so far
     uint32_t s = 0; // products of this query tile so far
     uint32_t written = 0; // items of this query tile whose rows have to be written
     do
@@ -994,7 +1157,7 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
             return false;
         }
         written += active && count > 0 ? 1 : 0;
-        for (int j = 0; j < count; ++j)
+        for (int j = 0; j < count; ++j, ++n)
         {
             if (!ptx::mbar_wait_bounded_spin(&st.v_full[stage], phase))
             {
@@ -1002,6 +1165,7 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
             }
             if (active)
             {
+                const bool as_bf16 = FAR && st.scales[(n % RING) * shape::GROUPS].w != 0.0F;
                 if (!ptx::mbar_wait_bounded_spin(&st.p_full[my_tile * 2 + (s & 1)], (s >> 1) & 1U))
                 {
                     return false;
@@ -1009,10 +1173,21 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
                 tc::fence_after_sync();
                 const uint32_t p_addr = s_base + (s & 1) * shape::ROWS;
                 const uint32_t v_lo = static_cast<uint32_t>(v_desc) + stage * (shape::KV_BYTES >> 4);
+                // the weights of 16 positions: 8 words of halves, or 8 of their upper parts and 8 of the lower ones
+                const uint32_t words = as_bf16 ? 16U : 8U;
+                const uint32_t form = as_bf16 ? idesc_bf16 : idesc;
 #pragma unroll
                 for (int k = 0; k < shape::ROWS / 16; ++k)
                 {
-                    mma_ts(o_addr, p_addr + k * 8, v_lo + k * (16 * 128 >> 4), hi, idesc, j != 0 || k != 0);
+                    mma_ts(o_addr, p_addr + k * words, v_lo + k * (16 * 128 >> 4), hi, form, j != 0 || k != 0);
+                }
+                if (as_bf16)
+                {
+#pragma unroll
+                    for (int k = 0; k < shape::ROWS / 16; ++k)
+                    {
+                        mma_ts(o_addr, p_addr + 8 + k * words, v_lo + k * (16 * 128 >> 4), hi, form, true);
+                    }
                 }
                 tc::mma_commit(&st.o_done[my_tile * 2 + (s & 1)]);
                 tc::mma_commit(&st.v_empty[stage]);
@@ -1055,6 +1230,11 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 //   Barriers that one role completes and another reads the fruits of (scales, NaN) carry an arrival of
 // the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
 //
+// Value scales far apart (cache_attend.cuh) take weights and values as BF16 numbers.  What that needs in addition costs
+// the loops of the usual case 14 ... 100 us of 376 wherever it stands in them, taken or not; so a block only notes that its
+// share has such scales, and the instantiation with FAR, launched behind and left at once by the other blocks (2 us), does
+// the share again.
+//
 // What bounds it: per 256 rows x 64 positions the exponentials need 1024 clocks (16 per clock and SM), the
 // products about 1500 (the 8 + 4 of one query tile hold their threads for 516 + 234 clocks when it is alone in
 // its block), their operands and the converters' stores about 1300 of shared-memory time; a tile takes some
@@ -1067,7 +1247,7 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 // splits (403 ... 417), the weights' code shared by both paths in a loop (580: the scores then live on across
 // it), one product of 128 positions for both score tiles of a query tile (502: the 516 clocks serve twice as
 // much, but the softmax then waits 900 of them every time).
-template <int DIM>
+template <int DIM, bool FAR>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)
 {
     using shape = tc_shape<DIM>;
@@ -1096,9 +1276,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
     st.row_done = st.k_full + 30;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if constexpr (FAR)
+    {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (a.far_apart[blockIdx.x] == 0)
+        {
+            return;
+        }
+    }
     if (t == 0)
     {
         a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if constexpr (!FAR)
+        {
+            a.far_apart[blockIdx.x] = 0;
+        }
         for (int i = 0; i < shape::STAGES; ++i)
         {
             ptx::mbar_init(&st.k_full[i], CONVERTERS / 32);
@@ -1165,13 +1357,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
             more_registers<SOFTMAX_REGISTERS>();
             if (shape::NQ == 2 || warp < 4)
             {
-                fine = softmax_role<DIM>(a, st, w, tmem);
+                fine = softmax_role<DIM, FAR>(a, st, w, tmem);
             }
         }
         else if (warp < 12)
         {
             fewer_registers<CONVERT_REGISTERS>();
-            fine = convert_role<DIM>(a, st, w);
+            fine = convert_role<DIM, FAR>(a, st, w);
         }
         else
         {
@@ -1180,7 +1372,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
             if (lane == 0 && (issuer & 1) < shape::NQ)
             {
                 fine = issuer < 2 ? scores_role<DIM>(a, st, w, tmem, issuer & 1)
-                                  : sums_role<DIM>(a, st, w, tmem, issuer & 1);
+                                  : sums_role<DIM, FAR>(a, st, w, tmem, issuer & 1);
             }
             else if (warp == TC_THREADS / 32 - 1 && lane == 1)
             {
@@ -1228,15 +1420,28 @@ int launch_tc(attend_args a, void* workspace, size_t workspace_bytes, cudaStream
     static cache::device_set prepared;
     if (!prepared.contains_current())
     {
-        BITSKNN_CUDA_TRY(
-            cudaFuncSetAttribute(cache_attend_tc_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, shape::BYTES));
+        BITSKNN_CUDA_TRY(cudaFuncSetAttribute(cache_attend_tc_kernel<DIM, false>,
+                                              cudaFuncAttributeMaxDynamicSharedMemorySize, shape::BYTES));
+        BITSKNN_CUDA_TRY(cudaFuncSetAttribute(cache_attend_tc_kernel<DIM, true>,
+                                              cudaFuncAttributeMaxDynamicSharedMemorySize, shape::BYTES));
         prepared.add_current();
     }
     {
         kernel_scope scope("cache_attend_kernel", stream);
-        cache_attend_tc_kernel<DIM><<<blocks, TC_THREADS, shape::BYTES, stream>>>(a, status);
+        cache_attend_tc_kernel<DIM, false><<<blocks, TC_THREADS, shape::BYTES, stream>>>(a, status);
     }
     BITSKNN_CUDA_TRY(cudaGetLastError());
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(blocks));
+    config.blockDim = dim3(TC_THREADS);
+    config.dynamicSmemBytes = shape::BYTES;
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    BITSKNN_CUDA_TRY(cudaLaunchKernelEx(&config, cache_attend_tc_kernel<DIM, true>, a, status));
     return launch_join<DIM, shape::COLS>(a, blocks, stream);
 }
 

@@ -437,6 +437,8 @@ int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_bat
  * over the positions j the token sees; zeros (and lse = -inf) if there are none.
  *   d_out   [tokens][query_heads][dim] of `dtype`, out_stride elements between tokens (0 = dense)
  *   d_lse   optional float32[tokens][query_heads]: ln sum_j p_j (joins results over shards)
+ * Weights are held to 11 bits or more and to 2^-28 of the row's largest p_j, whatever the pages' value scales;
+ * a position whose p_j times value scale lies below 2^-133 of the row's largest counts as zero in the sum of values.
  * Neither may overlap what the call reads.
  * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the
  * batch; its contents on entry do not matter.  Calls that can overlap need workspaces of their own. */

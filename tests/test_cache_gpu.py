@@ -927,3 +927,118 @@ def test_append_does_not_depend_on_how_tokens_are_batched(bk, cuda, rows, dim, d
         bk.cache_append(want, new[0][one], new[1][one], slots[one])
     for name in ("keys", "values", "key_scales", "value_scales"):
         assert torch.equal(getattr(got, name), getattr(want, name)), name
+
+
+# ---- value scales far apart ------------------------------------------------------------------------------------
+# A weight is rounded to a half (2^-11 of itself) or to two BF16 numbers (less).  Where halves are subnormal they are off
+# by at most 2^-25, half their spacing, with 2^7 or more for the largest p vs so far; the positions that get halves have a
+# scale of at least 2^-4 of the largest one so far, so that is 2^-32 * 2^4 = 2^-28 of the largest p.  Below the smallest
+# float, 2^-126, weights are zero: 2^-133 of the largest p vs.  Nothing else depends on the other positions' scales.
+def plain_attend_by_dimension(p, scale, lists=None):
+    """plain_attend with a tolerance that is made of each dimension's own values."""
+    out, lse, _, lse_tol = p.plain_attend(scale, lists)
+    tol = np.zeros_like(out)
+    q = p.queries.double().numpy()
+    for t, r, vis in p.token_rows():
+        for h in range(p.heads):
+            k, there = p.matrix("k", r, h, vis)
+            v, _ = p.matrix("v", r, h, vis)
+            use = np.flatnonzero(there)
+            if lists is not None:
+                use = np.array([j for j in lists[t * p.heads + h] if 0 <= j < vis and there[j]], dtype=int)
+            if len(use) == 0:
+                continue
+            k, v = k[use], v[use]
+            most = 448 * np.repeat(p.scales["v"][p.table[r], h], p.rows)[:vis][use].max()
+            for g in range(h * p.group, (h + 1) * p.group):
+                s = scale * (k @ q[t, g])
+                d = abs(scale) * p.dim * 2 * U * (np.abs(k) @ np.abs(q[t, g])).max()
+                w = np.exp(s - s.max())
+                near = 2 * (2 * d + 2.0 ** -17 + len(use) * 2 * U)
+                tol[t, g] = ((2.0 ** -11 + near) * (w @ np.abs(v)) + 2.0 ** -28 * np.abs(v).sum(axis=0)
+                             + 2.0 ** -133 * len(use) * most) / w.sum()
+    least = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}[p.dtype]    # half a step of the smallest numbers
+    return out, lse, tol + HALF_STEP[p.dtype] * (np.abs(out) + tol) + least, lse_tol
+
+
+def pages_apart(bk, lengths, news, heads, group, dim, page_rows, dtype, high, large, low, seed):
+    """Pages `high` of every request hold one dimension alone, at 2^large; the scales of the others are 2^low times theirs."""
+    p = Plain(bk, lengths, news, heads, group, dim, page_rows, dtype, seed)
+    rng = np.random.default_rng(seed + 1)
+    for r, n in enumerate(lengths):
+        for c in range(-(-n // page_rows)):
+            page = p.table[r, c]
+            if c in high:
+                used = min(page_rows, n - c * page_rows)
+                p.codes["v"][page, :, :used] = 0
+                p.codes["v"][page, :, :used, 3] = round_e4m3(rng.uniform(1, 2, (heads, used)))
+                p.scales["v"][page] = 2.0 ** large
+            else:
+                p.scales["v"][page] *= 2.0 ** low
+    return p.upload()
+
+
+@pytest.mark.parametrize("dtype, large, low", [
+    (torch.bfloat16, 26, 0), (torch.float16, 13, -15), (torch.bfloat16, 40, 0), (torch.bfloat16, 60, -30)])
+@pytest.mark.parametrize("lengths, news, heads, group, dim, page_rows, high", [
+    ([200], [1], 1, 4, 128, 16, {2}),                              # a cluster of blocks
+    ([300, 77], [1, 1], 2, 8, 64, 32, {0, 4}),                     # first: all others lie below what was seen
+    ([6000, 250], [1, 1], 1, 4, 128, 64, {5, 40}),                 # parts of several blocks
+    ([120, 60], [3, 5], 1, 4, 32, 16, {1, 3}),                     # several tokens, the last ones see more
+    ([150, 90], [2, 3], 1, 8, 96, 16, {2, 7}),
+    ([420] * 70, [1] * 70, 8, 4, 64, 64, {1}),                     # warps with many subtiles
+    ([300] * 100, [3] * 100, 4, 2, 128, 64, {0, 3}),
+    ([260] * 60, [1] * 60, 8, 9, 256, 256, {0}),
+    ([90], [2], 1, 16, 192, 16, {0, 3}),                           # more than one block of columns
+    ([300], [1], 1, 16, 256, 32, {1}),
+    ([400], [64], 1, 4, 128, 16, {3, 9}),                          # tensor memory: groups of a tile apart
+    ([700, 300], [90, 120], 2, 4, 64, 64, {0, 6}),                 # whole tiles
+    ([500], [150], 1, 3, 32, 128, {1}),
+    ([450], [70], 1, 8, 96, 16, {0, 11, 27}),
+    ([333], [70], 1, 5, 192, 16, {4}),
+    ([3000], [131], 1, 2, 256, 32, {70}),                          # late, parts of several blocks
+])
+def test_weights_of_pages_with_small_scales(bk, cuda, lengths, news, heads, group, dim, page_rows, high, dtype, large, low):
+    p = pages_apart(bk, lengths, news, heads, group, dim, page_rows, dtype, high, large, low, seed=dim + group)
+    want, lse, tol, lse_tol = plain_attend_by_dimension(p, 0.1)
+    calls = [p.d_starts]
+    if p.d_starts is None:                                          # one token each: with starts, too
+        calls.append(torch.arange(len(news) + 1, dtype=torch.int32, device="cuda"))
+    for starts in calls:
+        out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=starts)
+        check(out, want, tol, "out")
+        check(got_lse, lse, lse_tol, "lse")
+    bk.device_status()
+
+
+@pytest.mark.parametrize("dtype, large, low", [(torch.bfloat16, 33, 0), (torch.float16, 13, -15), (torch.bfloat16, 60, -30)])
+@pytest.mark.parametrize("lengths, news, heads, group, dim, page_rows, high, k", [
+    ([200], [1], 1, 4, 128, 16, {2}, 64),
+    ([5000, 3000], [1, 1], 2, 4, 128, 64, {5, 40}, 2000),
+    ([300, 90], [2, 3], 1, 20, 64, 32, {0, 2}, 90),
+    ([400], [2], 1, 9, 256, 16, {3, 9}, 200),
+])
+def test_weights_of_listed_positions_with_small_scales(bk, cuda, lengths, news, heads, group, dim, page_rows, high, k, dtype,
+                                                       large, low):
+    p = pages_apart(bk, lengths, news, heads, group, dim, page_rows, dtype, high, large, low, seed=dim + k)
+    rng = np.random.default_rng(k)
+    lists = np.stack([rng.permutation(max(lengths) + 5)[:k] for _ in range(p.tokens * heads)]).astype(np.int32)
+    want, lse, tol, lse_tol = plain_attend_by_dimension(p, 0.1, lists)
+    out, got_lse = bk.cache_attend_selected(p.cache, p.d_queries, torch.from_numpy(lists).cuda(), p.d_lengths, p.d_table, 0.1,
+                                            starts=p.d_starts)
+    check(out, want, tol, "out")
+    check(got_lse, lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("dim, group, count", [(64, 4, 7), (128, 4, 100), (256, 1, 90)])
+def test_nan_among_scales_far_apart(bk, cuda, dim, group, count):
+    p = pages_apart(bk, [count + 70], [count], 1, group, dim, 16, torch.bfloat16, {1, 5}, 40, 0, seed=dim)
+    for w, pos, d in (("v", 40, 5), ("v", count + 66, 6), ("k", count + 68, 1)):
+        p.codes[w][p.table[0, pos // 16], 0, pos % 16, d] = 0x7f
+    p.upload()
+    with np.errstate(invalid="ignore"):
+        want, lse, tol, lse_tol = plain_attend_by_dimension(p, 0.1)
+    assert 0 < np.isnan(want[:, :, 6]).sum() < want[:, :, 6].size
+    out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    check(out, want, np.nan_to_num(tol), "out")
+    check(got_lse, lse, np.nan_to_num(lse_tol), "lse")
