@@ -38,7 +38,7 @@ struct tc_shape
     static constexpr int O_COL = NQ * 2 * ROWS;  // tensor memory: two score tiles per query tile, then the sums
     static constexpr int USED_COLS = O_COL + NQ * DIM;
     static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
-    static constexpr int NANS = DIM + 4; // words of a first-NaN slot: the dimensions, then the largest of them
+    static constexpr int NANS = DIM + 4; // words of a first-NaN slot: the dimensions, the largest of them, the first position
     static constexpr int TAIL = RING * GROUPS * 16 + RING * NANS * 4 + 32 * 8; // scales, first NaN, barriers
     static constexpr int BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + TAIL + 1024;
     static_assert(USED_COLS <= 512, "tensor memory");
@@ -421,7 +421,7 @@ struct tc_state
     unsigned char* k_tiles;
     unsigned char* v_tiles;
     float4* scales;     // [RING][GROUPS]: key scale, log2 of the value scale, its inverse, 1 if the tile is BF16 (else 0)
-    uint32_t* first_nan; // [RING][NANS]: nan_key
+    uint32_t* first_nan; // [RING][NANS]: nan_key; behind them the first position of the item's share that is there
     uint64_t* k_full;   // [STAGES]
     uint64_t* k_empty;
     uint64_t* v_full;
@@ -678,6 +678,13 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
             const int cut_base = visible_of(a.b, w.q, w.it.column0 / a.group) / shape::ROWS * shape::ROWS;
             const uint32_t seen_nan = see > cut_base ? nan_key(items, see - 1 - cut_base) : 0xffffffffU;
             const bool nan_here = count > 0 && first_nan[DIM] >= seen_nan;
+            if (count > 0 && see <= static_cast<int>(first_nan[DIM + 1]))
+            {
+                // Nothing there was seen.  Positions of absent pages have weight 2^-inf, but for a query that is not finite
+                // their scores, 0 times infinity, are NaN.
+                m = -INFINITY;
+                l = 0.0F;
+            }
             const float inverse = l == 0.0F ? 1.0F : 1.0F / l; // l = 0: nothing was seen; a NaN makes the row NaN
             const bool aligned =
                 ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * 2)) & 15) == 0;
@@ -899,6 +906,20 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         {
             compare_scales();
         }
+        // the first position that is there, kept by the warp that looks the scales up in any case
+        int first_there = 0x7fffffff;
+        auto look_for_first = [&](int j) {
+            const uint32_t there = __ballot_sync(FULL_MASK, ks_now != 0.0F);
+            first_there = there != 0 ? (first_tile + j) * ROWS + (__ffs(there) - 1) * 16 : first_there;
+            if (lane == 0)
+            {
+                first_nan[DIM + 1] = static_cast<uint32_t>(first_there);
+            }
+        };
+        if (warp == 0)
+        {
+            look_for_first(0);
+        }
         int base = 0; // first tile of offset_now
         const int whole_tiles = furthest / ROWS - first_tile; // tiles before this one have all their rows
         int64_t from[SLABS]; // of the tile loaded next, this thread's pieces; -1: absent
@@ -913,6 +934,10 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 if (scaling)
                 {
                     compare_scales();
+                }
+                if (warp == 0 && first_there == 0x7fffffff)
+                {
+                    look_for_first(j);
                 }
                 page_next = pages_from(j + AHEAD);
             }

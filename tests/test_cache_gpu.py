@@ -1042,3 +1042,36 @@ def test_nan_among_scales_far_apart(bk, cuda, dim, group, count):
     out, got_lse = bk.cache_attend(p.cache, p.d_queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
     check(out, want, np.nan_to_num(tol), "out")
     check(got_lse, lse, np.nan_to_num(lse_tol), "lse")
+
+
+@pytest.mark.parametrize("lengths, news, group, dim, page_rows", [
+    ([300, 90], [2, 3], 4, 64, 16),                                # warps
+    ([90, 40], [1, 1], 8, 128, 32),
+    ([300, 90], [200, 80], 4, 64, 16),                             # tensor memory
+    ([4000, 90, 700], [150, 80, 90], 2, 128, 32),                  # shares of several blocks
+    ([500, 200], [450, 180], 1, 256, 64),
+])
+def test_rows_that_see_absent_pages_alone_are_empty_whatever_their_query(bk, cuda, lengths, news, group, dim, page_rows):
+    p = Plain(bk, lengths, news, 1, group, dim, page_rows, torch.bfloat16, seed=dim + 7)
+    hidden = -(-(lengths[0] - news[0] // 2) // page_rows)          # about half of the first request's tokens see none but these
+    p.table[0, :hidden] = -1
+    p.table[1, :] = 10 ** 6
+    p.upload()
+    want, lse, tol, lse_tol = p.plain_attend(0.1)
+    empty = np.isinf(lse)
+    assert empty.any()
+    bad = torch.tensor([math.nan, math.inf, -math.inf], dtype=torch.bfloat16, device="cuda")
+    spoiled = p.d_queries.clone()
+    for n, (t, g) in enumerate(zip(*np.nonzero(empty))):
+        spoiled[t, g, n % dim] = bad[n % 3]
+    out, got_lse = bk.cache_attend(p.cache, spoiled, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    check(out, want, tol, "out")
+    check(got_lse, lse, lse_tol, "lse")
+    lists = torch.arange(max(lengths), dtype=torch.int32, device="cuda").repeat(p.tokens, 1)
+    out, got_lse = bk.cache_attend_selected(p.cache, spoiled, lists, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    check(out, want, tol, "selected out")
+    check(got_lse, lse, lse_tol, "selected lse")
+    dist = bk.cache_distance(p.cache, spoiled, p.d_lengths, p.d_table, max(lengths), starts=p.d_starts)
+    none = torch.from_numpy(empty.all(axis=1)).cuda()
+    assert bool((dist[none] == math.inf).all())
+    bk.device_status()
