@@ -53,13 +53,18 @@ class Cache:
     (pages, heads) scales.  Holds the tensors; pages may lie apart (stride of the first dimension)."""
 
     def __init__(self, keys, values, key_scales, value_scales):
-        if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
-            raise ValueError("keys and values must be (pages, heads, page_rows, dim) tensors of the same strides")
+        if keys.dim() != 4 or values.shape != keys.shape:
+            raise ValueError("keys and values must be (pages, heads, page_rows, dim) tensors of the same shape")
         if keys.dtype is not uint8 or values.dtype is not uint8:
             raise ValueError("keys and values must be uint8 (e4m3 codes)")
         pages, heads, rows, dim = keys.shape
-        if keys.stride()[1:] != (rows * dim, dim, 1):
-            raise ValueError("a page must be contiguous")
+        # strides of dimensions of one entry are never used, and differ between views of the same memory
+        for t in (keys, values):
+            for size, have, want in zip(t.shape[1:], t.stride()[1:], (rows * dim, dim, 1)):
+                if have != want and size > 1:
+                    raise ValueError("a page must be contiguous")
+        if pages > 1 and values.stride(0) != keys.stride(0):
+            raise ValueError("the pages of keys and values must lie equally far apart")
         stride = keys.stride(0) if pages > 1 else heads * rows * dim
         if stride < heads * rows * dim:
             raise ValueError("pages must not overlap")

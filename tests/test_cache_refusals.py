@@ -179,3 +179,27 @@ def test_more_rows_than_are_numbered_are_refused(bk):
     p = [ctypes.c_void_p(FAKE * (i + 1)) for i in range(8)]
     assert bk.lib().bitsknn_cache_plan(p[0], p[1], most + 1, 16, p[2], 5, p[3], 4, 4, p[4], p[5], p[6], 8, p[7],
                                        None) == bk.ERR_INVALID_ARGUMENT
+
+
+def test_strides_of_dimensions_of_one_entry_do_not_matter(bk):
+    """Views of the same memory as (pages, 1, rows, dim) differ in the stride of the head; both fit (and fail for their device)."""
+    import torch
+    flat = torch.zeros((3, 16, 1, 32), dtype=torch.uint8)
+    views = (flat.transpose(1, 2), flat.view(3, 1, 16, 32))
+    assert views[0].stride() != views[1].stride()
+    scales = torch.zeros(3, 1)
+    for keys in views:
+        for values in views:
+            with pytest.raises(ValueError, match="CUDA tensor"):
+                bk.Cache(keys, values, scales, scales)
+    one = torch.zeros((1, 2, 16, 32), dtype=torch.uint8)           # one page: the distance to the next does not matter
+    other = torch.zeros((3, 2, 16, 32), dtype=torch.uint8)[::2][:1]
+    assert one.stride() != other.stride()
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        bk.Cache(one, other, torch.zeros(1, 2), torch.zeros(1, 2))
+    two = torch.zeros((3, 16, 2, 32), dtype=torch.uint8).transpose(1, 2)
+    with pytest.raises(ValueError, match="contiguous"):
+        bk.Cache(two, two, torch.zeros(3, 2), torch.zeros(3, 2))
+    wide = torch.zeros((3, 1, 32, 32), dtype=torch.uint8)[:, :, :16]
+    with pytest.raises(ValueError, match="equally far apart"):
+        bk.Cache(wide, views[1], scales, scales)
