@@ -437,6 +437,40 @@ int check_cache(const bitsknn_cache_t* cache, cache::view* out);
 int check_cache_batch(const bitsknn_cache_batch_t* in, int page_rows, cache::batch* out);
 int check_cache_queries(const void* d_queries, int dtype, int64_t* query_stride, int query_heads, int heads, int dim);
 
+// Rows of an array in memory, for the checks of what a call reads against what it writes.
+struct extent
+{
+    const char* name;
+    const void* data;
+    int64_t rows;
+    int64_t stride; // bytes between rows
+    int64_t width;  // bytes of a row
+};
+
+inline extent dense_extent(const char* name, const void* data, int64_t bytes) { return {name, data, 1, bytes, bytes}; }
+
+// Whether the first row of the array that begins later lies in rows of the other one.  For arrays of one stride that
+// is whether they share memory; arrays that take turns in the rows of a wider one do not.
+inline bool overlap(const extent& x, const extent& y)
+{
+    if (x.data == nullptr || y.data == nullptr || x.rows < 1 || y.rows < 1 || x.width < 1 || y.width < 1)
+    {
+        return false;
+    }
+    const bool ordered = reinterpret_cast<uintptr_t>(x.data) <= reinterpret_cast<uintptr_t>(y.data);
+    const extent& a = ordered ? x : y;
+    const extent& b = ordered ? y : x;
+    const uint64_t apart = reinterpret_cast<uintptr_t>(b.data) - reinterpret_cast<uintptr_t>(a.data);
+    const uint64_t stride = static_cast<uint64_t>(a.stride);
+    const uint64_t row = apart / stride;
+    const uint64_t last = static_cast<uint64_t>(a.rows) - 1;
+    return (row <= last && apart % stride < static_cast<uint64_t>(a.width)) ||
+           (row < last && stride - apart % stride < static_cast<uint64_t>(b.width));
+}
+
+// Refuses arrays a call writes that share memory with one another or with those it reads.
+int check_apart(const extent* writes, int write_count, const extent* reads, int read_count);
+
 // Calls fn with std::integral_constant<int, DIM> for a supported row length (checked before).
 template <typename F>
 int dispatch_cache_dim(int dim, F&& fn)

@@ -384,6 +384,7 @@ size_t parts_bytes(int blocks)
     return static_cast<size_t>(blocks) * (2 * COLS * (DIM * sizeof(float) + sizeof(float2)) + JOIN_BYTES) + 256;
 }
 
+// Checks the workspace and the arrays of a call (none of its writes may lie where it reads) and places the parts.
 template <int DIM, int COLS>
 int place_parts(attend_args& a, int blocks, void* workspace, size_t workspace_bytes)
 {
@@ -391,6 +392,18 @@ int place_parts(attend_args& a, int blocks, void* workspace, size_t workspace_by
     {
         return fail(BITSKNN_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes,
                     parts_bytes<DIM, COLS>(blocks));
+    }
+    // other blocks still read when the first ones write
+    const int64_t heads = static_cast<int64_t>(a.group) * a.c.heads;
+    const extent writes[] = {{"d_out", a.out, a.b.tokens, a.out_stride * 2, heads * DIM * 2},
+                             dense_extent("d_lse", a.lse, a.b.tokens * heads * 4),
+                             dense_extent("the workspace", workspace, static_cast<int64_t>(parts_bytes<DIM, COLS>(blocks)))};
+    const extent reads[] = {{"d_queries", a.queries, a.b.tokens, a.query_stride * 2, heads * DIM * 2},
+                            {"d_idx", a.idx, static_cast<int64_t>(a.b.tokens) * a.c.heads, a.ld_idx * 4, a.k * 4LL}};
+    const int rc = check_apart(writes, 3, reads, 2);
+    if (rc != BITSKNN_OK)
+    {
+        return rc;
     }
     a.part_o = static_cast<float*>(workspace);
     a.joins = reinterpret_cast<int4*>(a.part_o + static_cast<size_t>(blocks) * 2 * COLS * DIM);

@@ -362,6 +362,14 @@ extern "C" int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitskn
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "misaligned matrix: 4-byte alignment needed");
     }
+    const extent write = {"d_dist", d_dist, batch->tokens * cache->heads, ld * 4, n * 4};
+    const extent read = {"d_queries", d_queries, batch->tokens, query_stride * 2,
+                         static_cast<int64_t>(query_heads) * cache->dim * 2};
+    rc = check_apart(&write, 1, &read, 1);
+    if (rc != BITSKNN_OK)
+    {
+        return rc;
+    }
     a.queries = d_queries;
     a.dtype = dtype;
     a.query_stride = query_stride;

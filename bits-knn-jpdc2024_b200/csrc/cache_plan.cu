@@ -96,6 +96,23 @@ int check_cache_batch(const bitsknn_cache_batch_t* in, int page_rows, cache::bat
     return BITSKNN_OK;
 }
 
+int check_apart(const extent* writes, int write_count, const extent* reads, int read_count)
+{
+    for (int i = 0; i < write_count; ++i)
+    {
+        for (int j = 0; j < i + read_count; ++j)
+        {
+            const extent& other = j < i ? writes[j] : reads[j - i];
+            if (overlap(writes[i], other))
+            {
+                return fail(BITSKNN_ERR_INVALID_ARGUMENT, "%s overlaps %s: what the call writes has to lie apart",
+                            writes[i].name, other.name);
+            }
+        }
+    }
+    return BITSKNN_OK;
+}
+
 int check_cache_queries(const void* d_queries, int dtype, int64_t* query_stride, int query_heads, int heads, int dim)
 {
     if (dtype != BITSKNN_F16 && dtype != BITSKNN_BF16)
@@ -369,10 +386,17 @@ extern "C" int bitsknn_cache_plan(const int32_t* d_lengths, const int32_t* d_new
     {
         return fail(BITSKNN_ERR_INVALID_ARGUMENT, "null pointer argument");
     }
-    if (requests > 0 && (d_new_lengths == d_lengths || d_new_lengths == d_new))
+    // every block reads all lengths and its own entries of the others, while other blocks write
+    const extent writes[] = {dense_extent("d_starts", d_starts, (requests + 1) * 4),
+                             dense_extent("d_new_lengths", d_new_lengths, requests * 4),
+                             dense_extent("d_slots", d_slots, max_tokens * 8), dense_extent("d_counts", d_counts, 3 * 4),
+                             {"d_table", d_table, requests, table_ld * 4, table_pages * 4}};
+    const extent reads[] = {dense_extent("d_lengths", d_lengths, requests * 4), dense_extent("d_new", d_new, requests * 4),
+                            dense_extent("d_free_pages", d_free_pages, free_count * 4)};
+    const int rc = check_apart(writes, 5, reads, 3);
+    if (rc != BITSKNN_OK)
     {
-        // every block reads all lengths while the first one writes the new ones
-        return fail(BITSKNN_ERR_INVALID_ARGUMENT, "the new lengths need an array of their own");
+        return rc;
     }
     plan_args a{};
     a.lengths = d_lengths;

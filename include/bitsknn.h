@@ -393,15 +393,15 @@ typedef struct bitsknn_cache_batch
  * ceil(d_lengths[r] / page_rows) it has are taken from the front of d_free_pages in request order.
  *   d_table        int32[requests][table_ld]: entries of the new pages are written, others kept
  *   d_starts       int32[requests + 1] out: sums of d_new (the batch's d_starts)
- *   d_new_lengths  int32[requests] out: d_lengths + d_new (the batch's d_lengths), at most 2^31 - 1;
- *                  not d_lengths itself
+ *   d_new_lengths  int32[requests] out: d_lengths + d_new (the batch's d_lengths), at most 2^31 - 1
  *   d_slots        int64[max_tokens] out: page * page_rows + row of every new token, -1 behind the
  *                  last one and for a token that got no place (free list or table row exhausted,
  *                  or its page is absent from the table).  More than max_tokens tokens: the first
  *                  max_tokens slots are written
  *   d_counts       int32[3] out: new tokens, pages asked of the free list, tokens for which the
  *                  free list or the table row was too short (0: the plan holds)
- * The sum of d_new must stay below 2^31. */
+ * The sum of d_new must stay below 2^31.  The arrays the call writes must not overlap one another or those
+ * it reads (INVALID_ARGUMENT). */
 int bitsknn_cache_plan(const int32_t* d_lengths, const int32_t* d_new, int64_t requests, int page_rows,
                        const int32_t* d_free_pages, int64_t free_count, int32_t* d_table, int64_t table_ld,
                        int64_t table_pages, int32_t* d_starts, int32_t* d_new_lengths, int64_t* d_slots,
@@ -427,7 +427,7 @@ int bitsknn_cache_append(const bitsknn_cache_t* cache, const void* d_new_keys, c
  * for the positions j < n that the token sees, +inf for the others below n.  A smaller value is a
  * nearer key, so bitsknn_select(d_dist, ld, ..., tokens * heads, n, k, ...) lists the k keys with
  * the largest inner products.  NaN products give NaN distances, which are never selected.
- * float32[tokens * heads][ld], ld >= n, 4-byte aligned. */
+ * float32[tokens * heads][ld], ld >= n, 4-byte aligned, apart from the queries. */
 int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries,
                            int dtype, int64_t query_stride, int query_heads, float* d_dist, int64_t ld, int64_t n,
                            bitsknn_stream_t stream);
@@ -439,7 +439,8 @@ int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_bat
  *   d_lse   optional float32[tokens][query_heads]: ln sum_j p_j (joins results over shards)
  * Weights are held to 11 bits or more and to 2^-28 of the row's largest p_j, whatever the pages' value scales;
  * a position whose p_j times value scale lies below 2^-133 of the row's largest counts as zero in the sum of values.
- * Neither may overlap what the call reads.
+ * Neither may overlap the queries (attention in place), the lists, the workspace or the other (INVALID_ARGUMENT);
+ * rows that take turns with those of the queries in a wider array are fine.
  * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the
  * batch; its contents on entry do not matter.  Calls that can overlap need workspaces of their own. */
 size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* cache, int query_heads);

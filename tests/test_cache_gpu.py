@@ -1075,3 +1075,21 @@ def test_rows_that_see_absent_pages_alone_are_empty_whatever_their_query(bk, cud
     none = torch.from_numpy(empty.all(axis=1)).cuda()
     assert bool((dist[none] == math.inf).all())
     bk.device_status()
+
+
+@pytest.mark.parametrize("lengths, news, group", [([300, 90], [1, 1], 4), ([400, 60], [90, 60], 4)])
+def test_outputs_may_take_turns_with_queries_but_not_lie_on_them(bk, cuda, lengths, news, group):
+    p = Plain(bk, lengths, news, 2, group, 64, 16, torch.bfloat16, seed=91).upload()
+    heads = 2 * group
+    rows = torch.full((p.tokens, 2 * heads + 1, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    rows[:, 1:heads + 1] = p.d_queries
+    queries, out = rows[:, 1:heads + 1], rows[:, heads + 1:]
+    want, _, tol, _ = p.plain_attend(0.1)
+    bk.cache_attend(p.cache, queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts, out=out)
+    check(out, want, tol, "out")
+    assert torch.equal(queries, p.d_queries) and bool((rows[:, 0] == 7).all())
+    with pytest.raises(bk.BitsKnnError, match="d_out overlaps d_queries"):
+        bk.cache_attend(p.cache, queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts, out=queries)
+    with pytest.raises(bk.BitsKnnError, match="d_out overlaps d_queries"):
+        bk.cache_attend(p.cache, queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts, out=rows[:, :heads])
+    assert torch.equal(queries, p.d_queries)

@@ -203,3 +203,44 @@ def test_strides_of_dimensions_of_one_entry_do_not_matter(bk):
     wide = torch.zeros((3, 1, 32, 32), dtype=torch.uint8)[:, :, :16]
     with pytest.raises(ValueError, match="equally far apart"):
         bk.Cache(wide, views[1], scales, scales)
+
+
+MIB = 1 << 20
+
+
+def test_outputs_that_lie_where_the_call_reads_are_refused(bk):
+    """3 tokens x 4 heads x 64 halves: rows of 512 bytes; 12 lengths of output per row."""
+    far = dict(queries=64 * MIB, out=65 * MIB, lse=66 * MIB, workspace=4096 * MIB)
+
+    def refused(batch=None, **over):
+        status = attend(bk, batch=batch, **{**far, **over})
+        return status == bk.ERR_INVALID_ARGUMENT and "overlaps" in bk.last_error()
+
+    q = far["queries"]
+    assert refused(out=q) and refused(out=q + 2) and refused(out=q + 1534) and refused(out=q - 1534)
+    assert refused(lse=q) and refused(lse=q + 1532) and refused(lse=q - 44)
+    assert refused(lse=far["out"]) and refused(workspace=q) and refused(workspace=far["out"] - 256)
+    assert refused(stride=512, out_stride=512, out=q + 768)            # turns in wider rows, by half a row only
+    assert refused(stride=512, out=q + 1024)                           # the second row of the queries
+    lib, cache, batch = bk.lib(), cache_struct(bk), batch_struct(bk)
+    assert lib.bitsknn_cache_distance(cache, batch, q, bk.F16, 0, 4, q + 1024, 64, 64, None) == bk.ERR_INVALID_ARGUMENT
+    assert "d_dist overlaps d_queries" in bk.last_error()
+    assert lib.bitsknn_cache_attend_selected(cache, batch, q, bk.F16, 0, 4, far["out"] + 512, 8, 8, 0.1, far["out"], 0, None,
+                                             far["workspace"], 1 << 40, None) == bk.ERR_INVALID_ARGUMENT
+    assert "d_out overlaps d_idx" in bk.last_error()
+
+
+def test_outputs_of_a_plan_that_lie_on_other_arrays_are_refused(bk):
+    names = ("lengths", "new", "free", "table", "starts", "out", "slots", "counts")
+    at = {name: MIB * (i + 1) for i, name in enumerate(names)}
+
+    def refused(**over):
+        p = {**at, **over}
+        status = bk.lib().bitsknn_cache_plan(p["lengths"], p["new"], 3, 16, p["free"], 5, p["table"], 6, 4, p["starts"],
+                                             p["out"], p["slots"], 8, p["counts"], None)
+        return status == bk.ERR_INVALID_ARGUMENT and "overlaps" in bk.last_error()
+
+    assert refused(out=at["lengths"]) and refused(out=at["lengths"] + 8) and refused(out=at["new"])
+    assert refused(starts=at["lengths"]) and refused(starts=at["new"] + 4) and refused(starts=at["free"] + 16)
+    assert refused(counts=at["free"]) and refused(slots=at["lengths"] - 56) and refused(slots=at["starts"])
+    assert refused(counts=at["table"] + 24 * 2 + 12) and refused(lengths=at["table"])
