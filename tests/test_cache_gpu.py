@@ -1093,3 +1093,40 @@ def test_outputs_may_take_turns_with_queries_but_not_lie_on_them(bk, cuda, lengt
     with pytest.raises(bk.BitsKnnError, match="d_out overlaps d_queries"):
         bk.cache_attend(p.cache, queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts, out=rows[:, :heads])
     assert torch.equal(queries, p.d_queries)
+
+
+def test_what_a_workspace_held_does_not_matter(bk, cuda):
+    """One workspace of the least size for kernels, row lengths and column counts in turn, filled with two patterns."""
+    few = Plain(bk, [9000, 300], [1, 1], 2, 4, 128, 16, torch.bfloat16, seed=101).upload()      # shares, joins of warps' items
+    some = Plain(bk, [1500, 700], [4, 4], 2, 4, 128, 16, torch.bfloat16, seed=102).upload()     # two blocks of columns each
+    many = Plain(bk, [900, 100], [150, 90], 2, 4, 128, 16, torch.bfloat16, seed=103).upload()   # tensor memory
+    apart = pages_apart(bk, [900, 100], [150, 90], 2, 4, 128, 16, torch.bfloat16, {2, 9}, 30, 0, seed=104)
+    size = bk.cache_attend_workspace_bytes(few.cache, 8)
+    work = torch.empty(size, dtype=torch.uint8, device="cuda")
+    lists = {id(p): torch.arange(700, dtype=torch.int32, device="cuda").repeat(p.tokens * 2, 1) for p in (few, some)}
+
+    def call(p, listed, workspace):
+        args = (p.d_lengths, p.d_table, 0.1)
+        if listed:
+            return bk.cache_attend_selected(p.cache, p.d_queries, lists[id(p)], *args, starts=p.d_starts, workspace=workspace)
+        return bk.cache_attend(p.cache, p.d_queries, *args, starts=p.d_starts, workspace=workspace)
+
+    calls = [(few, False), (many, False), (some, True), (apart, False), (some, False), (many, False), (few, True)]
+    want = [call(p, listed, torch.zeros(size, dtype=torch.uint8, device="cuda")) for p, listed in calls]
+    for fill in (None, 0xff, 0x7f, 0x01):
+        for (p, listed), w in zip(calls, want):
+            if fill is not None:
+                work.fill_(fill)
+            got = call(p, listed, work)
+            assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1]), (fill, listed)
+    bk.device_status()
+
+
+def test_columns_of_a_matrix_may_be_selected_from(bk, cuda):
+    """A matrix of one column has no stride along its rows that could matter."""
+    wide = torch.randn((5, 7), device="cuda")
+    for dist in (wide[:, 3:4], wide.t()[:, :1]):
+        got_d, got_i = bk.select(dist, 1)
+        assert torch.equal(got_d, dist) and bool((got_i == 0).all())
+    with pytest.raises(ValueError, match="contiguous"):
+        bk.select(wide.t()[:, :2], 1)
