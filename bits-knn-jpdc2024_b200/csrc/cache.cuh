@@ -462,8 +462,12 @@ inline bool overlap(const extent& x, const extent& y)
     const extent& b = ordered ? y : x;
     const uint64_t apart = reinterpret_cast<uintptr_t>(b.data) - reinterpret_cast<uintptr_t>(a.data);
     const uint64_t stride = static_cast<uint64_t>(a.stride);
-    const uint64_t row = apart / stride;
     const uint64_t last = static_cast<uint64_t>(a.rows) - 1;
+    if (apart >= last * stride + static_cast<uint64_t>(a.width))
+    {
+        return false; // behind all of it: the usual case
+    }
+    const uint64_t row = apart / stride;
     return (row <= last && apart % stride < static_cast<uint64_t>(a.width)) ||
            (row < last && stride - apart % stride < static_cast<uint64_t>(b.width));
 }

@@ -1130,3 +1130,25 @@ def test_columns_of_a_matrix_may_be_selected_from(bk, cuda):
         assert torch.equal(got_d, dist) and bool((got_i == 0).all())
     with pytest.raises(ValueError, match="contiguous"):
         bk.select(wide.t()[:, :2], 1)
+
+
+def test_many_columns_in_a_graph(bk, cuda):
+    """Captured and replayed with other queries, lengths and scales than at the capture, next to an eager call."""
+    p = pages_apart(bk, [900, 100], [150, 90], 2, 4, 128, 16, torch.bfloat16, {2, 9}, 0, 0, seed=111)
+    queries = p.d_queries.clone()
+    args = (p.cache, queries, p.d_lengths, p.d_table, 0.1)
+    bk.cache_attend(*args, starts=p.d_starts)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = bk.cache_attend(*args, starts=p.d_starts)
+    for step, (large, first) in enumerate(((0, 900), (40, 777), (0, 900), (60, 400))):
+        queries.copy_(torch.roll(p.d_queries, step, dims=0))
+        p.d_lengths.copy_(torch.tensor([first, 100 - step], dtype=torch.int32))
+        for page in (2, 9):                                         # only at some steps do the scales lie apart
+            p.cache.value_scales[int(p.d_table[0, page])] = 2.0 ** large
+        graph.replay()
+        eager = bk.cache_attend(*args, starts=p.d_starts)
+        assert torch.equal(captured[0], eager[0]) and torch.equal(captured[1], eager[1]), step
+        assert bool(captured[0].isfinite().all())
+    bk.device_status()
