@@ -43,7 +43,6 @@ struct attend_args
     float2* part_ml;  // [2 * blocks][columns]
     int4* joins;      // [blocks]
     int* join_end;    // [blocks]
-    int* far_apart;   // [blocks], tensor-memory kernel: the block's share has value scales far apart
     int cluster;        // > 0: an item to every cluster of so many blocks, which joins by itself
 };
 
@@ -375,9 +374,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) cache_join_kernel(const atten
     }
 }
 
-constexpr size_t JOIN_BYTES = sizeof(int4) + 2 * sizeof(int);
+constexpr size_t JOIN_BYTES = sizeof(int4) + sizeof(int);
 
-// Workspace of a launch of `blocks` blocks: two parts per block, its join and its note of scales.
+// Workspace of a launch of `blocks` blocks: two parts per block and its join.
 template <int DIM, int COLS>
 size_t parts_bytes(int blocks)
 {
@@ -409,7 +408,6 @@ int place_parts(attend_args& a, int blocks, void* workspace, size_t workspace_by
     a.joins = reinterpret_cast<int4*>(a.part_o + static_cast<size_t>(blocks) * 2 * COLS * DIM);
     a.part_ml = reinterpret_cast<float2*>(a.joins + blocks);
     a.join_end = reinterpret_cast<int*>(a.part_ml + static_cast<size_t>(blocks) * 2 * COLS);
-    a.far_apart = a.join_end + blocks;
     return BITSKNN_OK;
 }
 

@@ -14,6 +14,7 @@ namespace
 constexpr int TC_THREADS = 16 * 32;
 constexpr int CONVERTERS = 128;
 constexpr int RING = 8;             // scale slots (tiles) and first-NaN slots (items): see cache_attend_tc_kernel
+constexpr int BARRIERS = 32;        // of a pass over the share
 // Registers of a thread after the split of the 512 x 128 the block is launched with: two warpgroups of
 // softmax, one of converters, one of issuers: 256 * 168 + 128 * 112 + 128 * 56 = 64512 of 65536.
 constexpr int SOFTMAX_REGISTERS = 168;
@@ -39,7 +40,7 @@ struct tc_shape
     static constexpr int USED_COLS = O_COL + NQ * DIM;
     static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
     static constexpr int NANS = DIM + 4; // words of a first-NaN slot: the dimensions, the largest of them, the first position
-    static constexpr int TAIL = RING * GROUPS * 16 + RING * NANS * 4 + 32 * 8; // scales, first NaN, barriers
+    static constexpr int TAIL = RING * GROUPS * 16 + RING * NANS * 4 + 2 * BARRIERS * 8; // scales, first NaN, barriers
     static constexpr int BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + TAIL + 1024;
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(BYTES <= 227 * 1024, "shared memory");
@@ -433,6 +434,29 @@ struct tc_state
     uint64_t* row_done; // [query tile]: the item's rows are written
 };
 
+// Where things lie in shared memory; the barriers of either pass over a share (cache_attend_tc_kernel).
+template <int DIM>
+__device__ __forceinline__ tc_state state_of(unsigned char* raw, int pass)
+{
+    using shape = tc_shape<DIM>;
+    tc_state st;
+    st.q_tiles = raw + ((1024U - (ptx::smem_addr(raw) & 1023U)) & 1023U);
+    st.k_tiles = st.q_tiles + shape::NQ * shape::Q_BYTES;
+    st.v_tiles = st.k_tiles + shape::STAGES * shape::KV_BYTES;
+    st.scales = reinterpret_cast<float4*>(st.v_tiles + shape::STAGES * shape::KV_BYTES);
+    st.first_nan = reinterpret_cast<uint32_t*>(st.scales + RING * shape::GROUPS);
+    st.k_full = reinterpret_cast<uint64_t*>(st.first_nan + RING * shape::NANS) + pass * BARRIERS;
+    st.k_empty = st.k_full + 4;
+    st.v_full = st.k_full + 8;
+    st.v_empty = st.k_full + 12;
+    st.s_full = st.k_full + 16;
+    st.p_full = st.k_full + 20;
+    st.o_done = st.k_full + 24;
+    st.q_full = st.k_full + 28;
+    st.row_done = st.k_full + 30;
+    return st;
+}
+
 // ================= softmax: one thread per query row =================
 template <int DIM, bool FAR>
 __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w,
@@ -796,13 +820,12 @@ __device__ __forceinline__ bool softmax_role(const attend_args& a, const tc_stat
     return true;
 }
 
-// Scales of a page and head; a key scale of 0 stands for an absent page.
+// Scales of a page (-1: absent) and head; a key scale of 0 stands for an absent page.
 __device__ __forceinline__ void scales_of(const view& c, int page, int head, float& ks, float& vs)
 {
-    const bool there = page >= 0 && page < c.pages;
+    const bool there = page >= 0;
     ks = there ? c.key_scales[static_cast<int64_t>(page) * c.heads + head] : 0.0F;
     vs = there ? c.value_scales[static_cast<int64_t>(page) * c.heads + head] : 1.0F;
-    vs = fminf(fmaxf(vs, pow2_int(E_MIN)), pow2_int(E_MAX));
 }
 
 // A thread's codes of a tile, PIECES of 16, to halves or to BF16 numbers in shared memory (both exact).
@@ -836,7 +859,7 @@ __device__ __forceinline__ void store_codes(const uint4 (&r)[PIECES], unsigned c
 
 // ================= converters: codes from the cache to halves in shared memory =================
 template <int DIM, bool FAR>
-__device__ __forceinline__ bool convert_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w)
+__device__ __forceinline__ bool convert_role(const attend_args& a, const tc_state& st, walk<tc_shape<DIM>> w, int* verdict)
 {
     using shape = tc_shape<DIM>;
     constexpr int BLK = shape::BLK;
@@ -892,20 +915,18 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
             scales_of(a.c, page_first, w.it.head, ks_now, vs_now);
         }
         // Groups of 16 positions of the tiles looked up whose value scale is far below the largest one up to them
-        // (cache_attend.cuh); the values of their tiles become BF16.
+        // (cache_attend.cuh); the values of their tiles become BF16.  The scales are first touched here, long after
+        // their loads (touched when they are loaded, 172 -> 182 us for rows of 256 numbers).
         uint32_t vs_least = 0; // the largest one over 2^SCALE_SPREAD; positive floats order like their bits
         uint32_t far_groups = 0;
         auto compare_scales = [&] {
+            vs_now = fminf(fmaxf(vs_now, pow2_int(E_MIN)), pow2_int(E_MAX));
             const uint32_t bits = __float_as_uint(vs_now);
             const uint32_t most = __reduce_max_sync(FULL_MASK, ks_now != 0.0F ? bits : 0U);
             vs_least = max(vs_least, most - min(most, SCALE_SPREAD << 23));
             far_groups = __ballot_sync(FULL_MASK, ks_now != 0.0F && bits < vs_least);
             far_apart |= far_groups;
         };
-        if (scaling)
-        {
-            compare_scales();
-        }
         // the first position that is there, kept by the warp that looks the scales up in any case
         int first_there = 0x7fffffff;
         auto look_for_first = [&](int j) {
@@ -916,10 +937,6 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
                 first_nan[DIM + 1] = static_cast<uint32_t>(first_there);
             }
         };
-        if (warp == 0)
-        {
-            look_for_first(0);
-        }
         int base = 0; // first tile of offset_now
         const int whole_tiles = furthest / ROWS - first_tile; // tiles before this one have all their rows
         int64_t from[SLABS]; // of the tile loaded next, this thread's pieces; -1: absent
@@ -1018,6 +1035,14 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
         locate(0);
         load(rk, a.c.keys);
         load(rv, a.c.values);
+        if (scaling) // behind the first loads, which would wait for the scales otherwise
+        {
+            compare_scales();
+        }
+        if (warp == 0)
+        {
+            look_for_first(0);
+        }
         for (int j = 0; j < count; ++j, ++n)
         {
             const uint32_t stage = n % shape::STAGES;
@@ -1075,7 +1100,7 @@ __device__ __forceinline__ bool convert_role(const attend_args& a, const tc_stat
     }
     if (!FAR && warp == 0 && lane == 0 && far_apart != 0)
     {
-        a.far_apart[blockIdx.x] = 1;
+        verdict[0] = 1;
     }
     return true;
 }
@@ -1233,6 +1258,30 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
     return true;
 }
 
+// Where the roles meet after their way over the share: whether all of them have to go over it again.
+template <class SHAPE>
+__device__ __forceinline__ bool once_more(uint32_t* first_nan, int* verdict, bool fine)
+{
+    if (!fine)
+    {
+        verdict[1] = 1;
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    asm volatile("bar.sync 1, %0;" ::"n"(TC_THREADS) : "memory");
+    if (verdict[0] == 0 || verdict[1] != 0)
+    {
+        return false;
+    }
+    for (int d = threadIdx.x; d < RING * SHAPE::NANS; d += TC_THREADS)
+    {
+        first_nan[d] = 0U;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(TC_THREADS) : "memory");
+    tc::fence_after_sync();
+    return true;
+}
+
 // Warps 0-3 and 4-7: softmax of query tile 0 and 1, one thread per row.  Warps 8-11: converters, codes
 // to halves.  Warps 12 ... 15: one thread each issues the scores (12, 13) or the sums (14, 15) of a query tile.
 //
@@ -1255,10 +1304,10 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 //   Barriers that one role completes and another reads the fruits of (scales, NaN) carry an arrival of
 // the issuing thread beside the products' commit: what it has seen of the converters is then seen too.
 //
-// Value scales far apart (cache_attend.cuh) take weights and values as BF16 numbers.  What that needs in addition costs
-// the loops of the usual case 14 ... 100 us of 376 wherever it stands in them, taken or not; so a block only notes that its
-// share has such scales, and the instantiation with FAR, launched behind and left at once by the other blocks (2 us), does
-// the share again.
+// Value scales far apart (cache_attend.cuh) take weights and values as BF16 numbers.  What that needs in addition cost
+// the loops of the usual case 14 ... 100 us of 376 wherever it stood in them, taken or not.  So the converters only note
+// that the share has such scales, and then the block goes over it again with roles of their own (FAR) and barriers of
+// their own (1000 us; a kernel of its own for this pass cost each call 5 us).
 //
 // What bounds it: per 256 rows x 64 positions the exponentials need 1024 clocks (16 per clock and SM), the
 // products about 1500 (the 8 + 4 of one query tile hold their threads for 516 + 234 clocks when it is alone in
@@ -1272,7 +1321,8 @@ __device__ __forceinline__ bool sums_role(const attend_args& a, const tc_state& 
 // splits (403 ... 417), the weights' code shared by both paths in a loop (580: the scores then live on across
 // it), one product of 128 positions for both score tiles of a query tile (502: the 516 clocks serve twice as
 // much, but the softmax then waits 900 of them every time).
-template <int DIM, bool FAR>
+// Spills (-Xptxas -v: 0.5 KB stored, 0.8 KB loaded per thread) lie in the softmax: without it 16 bytes are left.
+template <int DIM>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)
 {
     using shape = tc_shape<DIM>;
@@ -1281,58 +1331,39 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
     __shared__ int64_t s_words[WARPS_HERE];
     __shared__ int s_found;
     __shared__ uint32_t s_tmem;
+    __shared__ walk<shape> s_walk;
+    __shared__ int s_verdict[2];
     const int t = threadIdx.x;
     const int warp = t >> 5;
     const int lane = t & 31;
-    tc_state st;
-    st.q_tiles = raw + ((1024U - (ptx::smem_addr(raw) & 1023U)) & 1023U);
-    st.k_tiles = st.q_tiles + shape::NQ * shape::Q_BYTES;
-    st.v_tiles = st.k_tiles + shape::STAGES * shape::KV_BYTES;
-    st.scales = reinterpret_cast<float4*>(st.v_tiles + shape::STAGES * shape::KV_BYTES);
-    st.first_nan = reinterpret_cast<uint32_t*>(st.scales + RING * shape::GROUPS);
-    st.k_full = reinterpret_cast<uint64_t*>(st.first_nan + RING * shape::NANS);
-    st.k_empty = st.k_full + 4;
-    st.v_full = st.k_full + 8;
-    st.v_empty = st.k_full + 12;
-    st.s_full = st.k_full + 16;
-    st.p_full = st.k_full + 20;
-    st.o_done = st.k_full + 24;
-    st.q_full = st.k_full + 28;
-    st.row_done = st.k_full + 30;
+    const tc_state st = state_of<DIM>(raw, 0);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if constexpr (FAR)
-    {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        if (a.far_apart[blockIdx.x] == 0)
-        {
-            return;
-        }
-    }
     if (t == 0)
     {
         a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-        if constexpr (!FAR)
+        s_verdict[0] = s_verdict[1] = 0;
+        for (int pass = 0; pass < 2; ++pass)
         {
-            a.far_apart[blockIdx.x] = 0;
-        }
-        for (int i = 0; i < shape::STAGES; ++i)
-        {
-            ptx::mbar_init(&st.k_full[i], CONVERTERS / 32);
-            ptx::mbar_init(&st.v_full[i], CONVERTERS / 32);
-            ptx::mbar_init(&st.k_empty[i], shape::NQ);
-            ptx::mbar_init(&st.v_empty[i], shape::NQ);
-        }
-        for (int i = 0; i < 4; ++i)
-        {
-            ptx::mbar_init(&st.s_full[i], 2);
-            ptx::mbar_init(&st.p_full[i], 4);
-            ptx::mbar_init(&st.o_done[i], 2);
-        }
-        for (int i = 0; i < 2; ++i)
-        {
-            ptx::mbar_init(&st.q_full[i], 4);
-            ptx::mbar_init(&st.row_done[i], 4);
+            const tc_state set = state_of<DIM>(raw, pass);
+            for (int i = 0; i < shape::STAGES; ++i)
+            {
+                ptx::mbar_init(&set.k_full[i], CONVERTERS / 32);
+                ptx::mbar_init(&set.v_full[i], CONVERTERS / 32);
+                ptx::mbar_init(&set.k_empty[i], shape::NQ);
+                ptx::mbar_init(&set.v_empty[i], shape::NQ);
+            }
+            for (int i = 0; i < 4; ++i)
+            {
+                ptx::mbar_init(&set.s_full[i], 2);
+                ptx::mbar_init(&set.p_full[i], 4);
+                ptx::mbar_init(&set.o_done[i], 2);
+            }
+            for (int i = 0; i < 2; ++i)
+            {
+                ptx::mbar_init(&set.q_full[i], 4);
+                ptx::mbar_init(&set.row_done[i], 4);
+            }
         }
         ptx::mbar_init_fence();
     }
@@ -1376,28 +1407,42 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
             w.it.begin = w.it.end;
             w.it.end += units_of_block<shape>(a, w.q, w.it.column0);
         }
+        if (t == 0)
+        {
+            s_walk = w;
+        }
         bool fine = true;
         if (warp < 8)
         {
             more_registers<SOFTMAX_REGISTERS>();
-            if (shape::NQ == 2 || warp < 4)
+            const bool active = shape::NQ == 2 || warp < 4;
+            if (active)
             {
-                fine = softmax_role<DIM, FAR>(a, st, w, tmem);
+                fine = softmax_role<DIM, false>(a, st, w, tmem);
+            }
+            if (once_more<shape>(st.first_nan, s_verdict, fine) && active)
+            {
+                fine = softmax_role<DIM, true>(a, state_of<DIM>(raw, 1), s_walk, tmem);
             }
         }
         else if (warp < 12)
         {
             fewer_registers<CONVERT_REGISTERS>();
-            fine = convert_role<DIM, FAR>(a, st, w);
+            fine = convert_role<DIM, false>(a, st, w, s_verdict);
+            if (once_more<shape>(st.first_nan, s_verdict, fine))
+            {
+                fine = convert_role<DIM, true>(a, state_of<DIM>(raw, 1), s_walk, s_verdict);
+            }
         }
         else
         {
             fewer_registers<ISSUE_REGISTERS>();
             const int issuer = warp - 12; // 0, 1: scores of query tile 0, 1; 2, 3: sums
-            if (lane == 0 && (issuer & 1) < shape::NQ)
+            const bool active = lane == 0 && (issuer & 1) < shape::NQ;
+            if (active)
             {
                 fine = issuer < 2 ? scores_role<DIM>(a, st, w, tmem, issuer & 1)
-                                  : sums_role<DIM, FAR>(a, st, w, tmem, issuer & 1);
+                                  : sums_role<DIM, false>(a, st, w, tmem, issuer & 1);
             }
             else if (warp == TC_THREADS / 32 - 1 && lane == 1)
             {
@@ -1411,6 +1456,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const at
                     a.joins[blockIdx.x] = make_int4(w.it.first_token, w.it.head, w.it.column0, w.it.columns);
                     a.join_end[blockIdx.x] = static_cast<int>((w.it.end * blocks - 1) / total);
                 }
+            }
+            if (once_more<shape>(st.first_nan, s_verdict, fine) && active)
+            {
+                const tc_state again = state_of<DIM>(raw, 1);
+                fine = issuer < 2 ? scores_role<DIM>(a, again, s_walk, tmem, issuer & 1)
+                                  : sums_role<DIM, true>(a, again, s_walk, tmem, issuer & 1);
             }
         }
         if (!fine)
@@ -1445,28 +1496,15 @@ int launch_tc(attend_args a, void* workspace, size_t workspace_bytes, cudaStream
     static cache::device_set prepared;
     if (!prepared.contains_current())
     {
-        BITSKNN_CUDA_TRY(cudaFuncSetAttribute(cache_attend_tc_kernel<DIM, false>,
-                                              cudaFuncAttributeMaxDynamicSharedMemorySize, shape::BYTES));
-        BITSKNN_CUDA_TRY(cudaFuncSetAttribute(cache_attend_tc_kernel<DIM, true>,
-                                              cudaFuncAttributeMaxDynamicSharedMemorySize, shape::BYTES));
+        BITSKNN_CUDA_TRY(
+            cudaFuncSetAttribute(cache_attend_tc_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, shape::BYTES));
         prepared.add_current();
     }
     {
         kernel_scope scope("cache_attend_kernel", stream);
-        cache_attend_tc_kernel<DIM, false><<<blocks, TC_THREADS, shape::BYTES, stream>>>(a, status);
+        cache_attend_tc_kernel<DIM><<<blocks, TC_THREADS, shape::BYTES, stream>>>(a, status);
     }
     BITSKNN_CUDA_TRY(cudaGetLastError());
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(blocks));
-    config.blockDim = dim3(TC_THREADS);
-    config.dynamicSmemBytes = shape::BYTES;
-    config.stream = stream;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    BITSKNN_CUDA_TRY(cudaLaunchKernelEx(&config, cache_attend_tc_kernel<DIM, true>, a, status));
     return launch_join<DIM, shape::COLS>(a, blocks, stream);
 }
 
