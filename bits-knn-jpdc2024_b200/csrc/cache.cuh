@@ -87,12 +87,15 @@ __device__ __forceinline__ request request_of(const batch& b, int r)
     request q;
     q.first = r;
     q.count = 1;
+    q.length = max(b.lengths[r], 0);
     if (b.starts != nullptr)
     {
+        const int end = b.starts[r + 1];
         q.first = min(max(b.starts[r], 0), b.tokens);
-        q.count = min(max(b.starts[r + 1], q.first), b.tokens) - q.first;
+        q.count = min(max(end, q.first), b.tokens) - q.first;
+        // a request whose tokens the arrays hold in part: the others' positions lie behind all that these see
+        q.length -= max(end - b.tokens, 0);
     }
-    q.length = max(b.lengths[r], 0);
     return q;
 }
 

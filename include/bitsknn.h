@@ -348,6 +348,7 @@ int bitsknn_sharded_drain(bitsknn_sharded_t* handle, bitsknn_stream_t stream);
  * [j * page_rows, (j + 1) * page_rows), an entry outside [0, pages) is an absent page whose
  * positions nobody sees.  Its query tokens are the rows [d_starts[r], d_starts[r + 1]) of the
  * packed token arrays (d_starts == NULL: one token per request, `tokens` == `requests`).
+ * Tokens that d_starts puts behind the arrays' `tokens` rows (a plan of more than max_tokens) are left out.
  * d_lengths[r] counts its cached positions INCLUDING those tokens, so token i of m sees the
  * positions below d_lengths[r] - m + i + 1.  Rows of outputs behind the last request's tokens are
  * left as they were.  Lengths beyond the table's table_pages * page_rows are cut there.  At most 2^30

@@ -1152,3 +1152,28 @@ def test_many_columns_in_a_graph(bk, cuda):
         assert torch.equal(captured[0], eager[0]) and torch.equal(captured[1], eager[1]), step
         assert bool(captured[0].isfinite().all())
     bk.device_status()
+
+
+@pytest.mark.parametrize("lengths, news, group, tokens", [
+    ([60, 90, 30], [3, 5, 4], 4, 5),                                # warps; the second request is cut, the third is not there
+    ([60, 90], [3, 5], 4, 3),                                       # cut between requests
+    ([300, 90], [90, 60], 4, 70),                                   # tensor memory
+    ([30, 700], [10, 200], 4, 150),
+])
+def test_arrays_that_end_within_a_request(bk, cuda, lengths, news, group, tokens):
+    """Packed arrays shorter than the starts say: the tokens that are there see what they see in the whole batch."""
+    p = Plain(bk, lengths, news, 2, group, 64, 16, torch.bfloat16, seed=121).upload()
+    want, lse, tol, lse_tol = p.plain_attend(0.1)
+    queries = p.d_queries[:tokens]
+    out, got_lse = bk.cache_attend(p.cache, queries, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    check(out, want[:tokens], tol[:tokens], "out")
+    check(got_lse, lse[:tokens], lse_tol[:tokens], "lse")
+    n = max(lengths)
+    want_d, tol_d = p.plain_distance(n)
+    check(bk.cache_distance(p.cache, queries, p.d_lengths, p.d_table, n, starts=p.d_starts), want_d[:tokens * 2],
+          tol_d[:tokens * 2], "distance")
+    lists = torch.arange(n, dtype=torch.int32, device="cuda").repeat(tokens * 2, 1)
+    out, got_lse = bk.cache_attend_selected(p.cache, queries, lists, p.d_lengths, p.d_table, 0.1, starts=p.d_starts)
+    check(out, want[:tokens], tol[:tokens], "selected out")
+    check(got_lse, lse[:tokens], lse_tol[:tokens], "selected lse")
+    bk.device_status()
