@@ -164,7 +164,8 @@ def cache_append(cache, keys, values, slots):
 
 
 def cache_distance(cache, queries, lengths, table, n, starts=None, out=None):
-    """(tokens * heads, n) float32 distances for `select`: minus the largest inner product over a head's queries."""
+    """(tokens * heads, n) float32 distances for `select`: minus the largest inner product over a head's queries.  Rows of
+    tokens behind the last request are left as they were, which is undefined where the call allocates `out`."""
     shape = queries.shape
     batch = _batch(cache, queries, shape, lengths, table, starts)
     rows = shape[0] * cache.heads
@@ -214,7 +215,9 @@ def _attend_buffers(cache, queries, shape, out, lse, workspace):
 
 
 def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
-    """Attention of (tokens, query_heads, dim) queries over everything cached: (out, lse)."""
+    """Attention of (tokens, query_heads, dim) queries over everything cached: (out, lse).  Rows of tokens behind the last
+    request are left as they were, which is undefined where the call allocates `out` and `lse`.  With one token for each
+    request leave `starts` out: few short requests then take one launch."""
     shape = queries.shape
     batch = _batch(cache, queries, shape, lengths, table, starts)
     out, out_stride, lse, workspace = _attend_buffers(cache, queries, shape, out, lse, workspace)
@@ -225,7 +228,8 @@ def cache_attend(cache, queries, lengths, table, scale, starts=None, out=None, l
 
 
 def cache_attend_selected(cache, queries, idx, lengths, table, scale, starts=None, out=None, lse=None, workspace=None):
-    """Attention over listed positions: idx (tokens * heads, k) int32, as `select` returns them.  (out, lse)."""
+    """Attention over listed positions: idx (tokens * heads, k) int32, as `select` returns them.  (out, lse), as from
+    cache_attend."""
     shape = queries.shape
     batch = _batch(cache, queries, shape, lengths, table, starts, idx)
     rows, k = idx.shape

@@ -15,8 +15,9 @@ struct attend_smem
 {
     static constexpr int COLS = 8 * NB;
     static constexpr int ROWS = TILE;
-    // An item's beginning and end in tiles (ragged decode batch of 64 requests, 150 ... 24000 positions: 141 us
-    // with 1, 131 with 3, 121 with 5 and with 8).  Lists are all of one length; there it only costs.
+    // An item's beginning and end in tiles (ragged decode batch of 64 requests, 150 ... 24000 positions, rows of
+    // 128: 141 us with 1, 131 with 3, 121 with 5 and with 8; other rows not measured).  Lists are all of one length;
+    // there it only costs.
     static constexpr int COST = 6;
     static constexpr int LIST_COST = 1;
     static constexpr int SCALES = 2 * SUB * PITCH<DIM, true>; // offset of the scales in a stage
@@ -48,9 +49,10 @@ struct attend_smem
 // cache_join_kernel, or, for few short items, those of a cluster's blocks through their shared memory.
 //
 // Bound by the bytes of the cache (HBM) while the columns are few.  One request with 250001 positions, 8 heads of 128
-// (512 MB): 90 us = 5.7 TB/s, 0.87 of the measured copy rate, and 10 us for the join; 64 requests with 150 ... 24000
-// positions (625 MB): 108 us, 0.88 and 6 us; 2048 listed positions of 32 requests (137 MB in gathers of 128 bytes):
-// 40 us, 0.52 -- more copies in flight do not help there, single rows are what the memory delivers more slowly.
+// (512 MB): 92 us = 5.6 TB/s, 0.85 of the measured copy rate, and 10 us for the join; 64 requests with 150 ... 24000
+// positions (625 MB): 117 us, 0.82 and 7 us; 2048 listed positions of 32 requests (137 MB in gathers of 128 bytes):
+// 41 us, 0.51 -- more copies in flight do not help there; whether single rows or the look-ups of entries and pages in
+// front of them are the reason has not been told apart.
 // Three stages and three blocks per SM (four stages: 97 us for the long request, two: 92).
 template <int DIM, int NB, bool SELECTED, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, attend_smem<DIM, NB>::BLOCKS) cache_attend_kernel(const attend_args a)
@@ -801,7 +803,8 @@ int launch_attend(attend_args a, void* workspace, size_t workspace_bytes, cudaSt
     {
         // Few short items: each goes to a cluster of blocks of its own, which joins through its shared
         // memory, so that there is no second kernel and no search for shares.  Taken while the clusters
-        // all run at once and a block has at most eight tiles; the table's width bounds the lengths.
+        // all run at once and a block has at most eight tiles; the table's width bounds the lengths, which the host does
+        // not see (one request of 778 positions: 7.6 us, with starts or under a table of 131072 positions 12.4).
         const int64_t items = static_cast<int64_t>(a.b.tokens) * a.c.heads * ((a.group + smem::COLS - 1) / smem::COLS);
         const int64_t most = ((SELECTED ? a.k : a.b.limit) + TILE - 1) / TILE;
         int cluster = 1;
@@ -923,7 +926,8 @@ int attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, con
     auto s = static_cast<cudaStream_t>(stream);
     // More columns than one stream of the cache can serve: the tensor-memory kernel takes over (16 requests
     // of 6000 positions, 8 heads of 128: 32 columns 109 us here and 129 there, 48 columns 169 and 130, 128
-    // columns 324 and 134; heads of 256: 16 columns 113 and 165, 24 columns 187 and 167).
+    // columns 324 and 134; heads of 256: 16 columns 113 and 165, 24 columns 187 and 167; by now the kernel taken
+    // needs 100, 135, 140, 108 and 172).
     if (!selected && want > 8 * most_columns(cache->dim))
     {
         return launch_attend_tc(cache->dim, a, d_workspace, workspace_bytes, s);

@@ -30,7 +30,8 @@ struct tc_shape
     static constexpr int NQ = DIM <= 128 ? 2 : 1;
     static constexpr int COLS = 128 * NQ;
     static constexpr int ROWS = 64;
-    static constexpr int COST = 10;              // an item's beginning and end, in tiles (4: 375 us, 6: 370, 8: 367, 10: 365)
+    // an item's beginning and end, in tiles (rows of 128: 4 375 us, 6 370, 8 367, 10 365; other rows not measured)
+    static constexpr int COST = 10;
     static constexpr int BLK = (DIM + 63) / 64;  // 128-byte blocks of 64 halves per row
     static constexpr int Q_BYTES = BLK * 128 * 128;
     static constexpr int KV_BYTES = BLK * ROWS * 128;
@@ -39,7 +40,7 @@ struct tc_shape
     static constexpr int O_COL = NQ * 2 * ROWS;  // tensor memory: two score tiles per query tile, then the sums
     static constexpr int USED_COLS = O_COL + NQ * DIM;
     static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
-    static constexpr int NANS = DIM + 4; // words of a first-NaN slot: the dimensions, the largest of them, the first position
+    static constexpr int NANS = DIM + 4; // words of a first-NaN slot: the dimensions, their largest, the first position
     static constexpr int TAIL = RING * GROUPS * 16 + RING * NANS * 4 + 2 * BARRIERS * 8; // scales, first NaN, barriers
     static constexpr int BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + TAIL + 1024;
     static_assert(USED_COLS <= 512, "tensor memory");
@@ -1314,13 +1315,13 @@ __device__ __forceinline__ bool once_more(uint32_t* first_nan, int* verdict, boo
 // its block), their operands and the converters' stores about 1300 of shared-memory time; a tile takes some
 // 2180, because the steps of one tile depend on one another and a warp's 64 weights alone take 1170 with the
 // other warp of its scheduler doing the same; an item's beginning and end take 17000.  3 requests of 1500 ...
-// 8000 cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 365 us = 0.85 PFLOP/s,
-// 0.51 of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two
+// 8000 cached and 700 ... 2100 new positions, 8 heads of 4 queries of 128: 309 GFLOP in 376 us = 0.82 PFLOP/s,
+// 0.49 of the measured dense rate.  Steps on the way: tiles of 128 positions with one score tile 620 us; two
 // score tiles of 64 511; packed arithmetic and offsets per 16 rows 444; a thread for each kind of product 405;
-// rows packed and written in whole lines 365.  Tried and slower: two threads per row (520), other register
-// splits (403 ... 417), the weights' code shared by both paths in a loop (580: the scores then live on across
-// it), one product of 128 positions for both score tiles of a query tile (502: the 516 clocks serve twice as
-// much, but the softmax then waits 900 of them every time).
+// rows packed and written in whole lines 365 (376 by now, with inputs that take turns).  Tried and slower: two
+// threads per row (520), other register splits (403 ... 417), the weights' code shared by both paths in a loop (580:
+// the scores then live on across it), one product of 128 positions for both score tiles of a query tile (502: the
+// 516 clocks serve twice as much, but the softmax then waits 900 of them every time).
 // Spills (-Xptxas -v: 0.5 KB stored, 0.8 KB loaded per thread) lie in the softmax: without it 16 bytes are left.
 template <int DIM>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attend_tc_kernel(const attend_args a, int* status)

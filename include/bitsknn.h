@@ -339,7 +339,8 @@ int bitsknn_sharded_drain(bitsknn_sharded_t* handle, bitsknn_stream_t stream);
  *                      p * page_stride codes behind the base; bases 16-byte aligned
  *   d_key_scales, d_value_scales   float32[pages][heads]; a number is code * scale.  The append
  *                      writes powers of two in [2^-60, 2^60]; a reader takes any finite positive
- *                      scale in that range and moves value scales outside it to its border
+ *                      scale in that range and moves value scales outside it to its border; a
+ *                      key scale of 0 (never appended to) makes the page an absent one
  *   page_rows          16, 32, 64, 128 or 256
  *   dim                32, 64, 96, 128, 192 or 256 (BITSKNN_ERR_UNSUPPORTED_DIM otherwise)
  *   page_stride        0 = heads * page_rows * dim, else a multiple of 16 at least as large
@@ -356,7 +357,9 @@ int bitsknn_sharded_drain(bitsknn_sharded_t* handle, bitsknn_stream_t stream);
  *
  * Query vectors: BITSKNN_F16 or BITSKNN_BF16, [tokens][query_heads][dim] with `query_stride`
  * elements between tokens (0 = query_heads * dim); query head j belongs to cache head
- * j / (query_heads / heads).  16-byte aligned, stride a multiple of 8.
+ * j / (query_heads / heads).  16-byte aligned, stride a multiple of 8.  They enter the products as halves times a power
+ * of two for each vector: exact but for BF16 entries below 2^-28 of their vector's largest finite one, which are off by
+ * up to 2^-39 of that.
  * --------------------------------------------------------------------------------------- */
 enum bitsknn_dtype
 {
@@ -443,7 +446,9 @@ int bitsknn_cache_distance(const bitsknn_cache_t* cache, const bitsknn_cache_bat
  * Neither may overlap the queries (attention in place), the lists, the workspace or the other (INVALID_ARGUMENT);
  * rows that take turns with those of the queries in a wider array are fine.
  * The workspace needs bitsknn_cache_attend_workspace_bytes() bytes, 256-byte aligned, whatever the
- * batch; its contents on entry do not matter.  Calls that can overlap need workspaces of their own. */
+ * batch; its contents on entry do not matter.  Calls that can overlap need workspaces of their own.
+ * A step of one token for each request is fastest with d_starts == NULL and table_pages no wider than its
+ * requests need: few short ones then take one launch. */
 size_t bitsknn_cache_attend_workspace_bytes(const bitsknn_cache_t* cache, int query_heads);
 int bitsknn_cache_attend(const bitsknn_cache_t* cache, const bitsknn_cache_batch_t* batch, const void* d_queries,
                          int dtype, int64_t query_stride, int query_heads, float scale, void* d_out,
